@@ -198,6 +198,76 @@ int morpho_soft_backward(const void* grad_out, const void* X, const void* W_phi,
                          const void* forward_workspace, void* workspace, size_t workspace_bytes,
                          morpho_stream_t stream);
 
+/* ------------------------------------------------------------ paged cache
+ * Serving a causal layer token by token: the key codes and values of the
+ * tokens so far are kept in pages, new tokens are appended and attend to them.
+ * No reference counterpart (the reference computes whole sequences only).
+ *
+ * A pool holds `pages` pages of `page_size` tokens in each of `layers` layers:
+ *   codes  [layers, pages, H, page_size, cube_m]              float16
+ *   values [layers, pages, H, page_size / 8, head_dim_v, 8]   float16
+ * Token t of a page has its codes phi contiguous, and value column c at
+ * [t / 8][c][t % 8] (the MFMA operand of the value product: 8 tokens of a
+ * column). cube_m in {16, 32, 64}, head_dim_v in {32, 64, 128}, page_size in
+ * {32, 64, 128, 256}.
+ *
+ * table [B, seq_pages] int32: the pages of each sequence in order. lens [B]
+ * int32: its tokens before the new ones. new_lens [B] int32 (or NULL: n
+ * each): its new tokens; the rows from there to n are padding. All three are
+ * device memory and are read by the kernels, so a captured graph follows
+ * them. The kernels check them: a page outside the pool, or a position past
+ * the table's seq_pages * page_size, is neither read nor written (its key is
+ * left out), negative lengths count as 0. seq_pages * page_size <= 2^30. */
+typedef struct morpho_cache {
+  void* codes;
+  void* values;
+  int64_t layers, pages, H, cube_m, head_dim_v, page_size;
+} morpho_cache;
+
+/* Projects the new tokens X [B, n, D], D = H * head_dim_v, and stores their
+ * codes and values at positions lens[b] .. lens[b] + new_lens[b] - 1. W
+ * [H * cube_m + D, D] float16 is [W_phi | W_V] transposed. phi [B, n, H,
+ * cube_m] float16 receives the codes of every row, padding included, rounded
+ * as they are stored. mode: 0 or one MORPHO_MODE_PROJ_* bit. cache->layers
+ * must be 1. Two sequences must not share a page that is appended to. */
+int morpho_cache_append(const void* X, const void* W, const morpho_cache* cache, const int32_t* table,
+                        const int32_t* lens, const int32_t* new_lens, void* phi, int64_t B, int64_t n,
+                        int64_t seq_pages, int mode, morpho_stream_t stream);
+
+/* Bytes of device workspace morpho_cache_attention needs (0 on invalid sizes,
+ * and where none is needed: then the workspace may be NULL). */
+size_t morpho_cache_attention_workspace_size(const morpho_cache* cache, int64_t B, int64_t n, int64_t seq_pages,
+                                             int64_t max_len);
+
+/* Attention of the new tokens, appended before, over their sequences: out [B,
+ * n, D] float16 and lse [B * H, n] float32 (base 2, as in morpho_forward) from
+ * the codes phi [B, n, H, cube_m]. With MORPHO_MODE_CAUSAL new token i sees the
+ * keys 0 .. lens[b] + i, else all lens[b] + new_lens[b]; MORPHO_MODE_MASK_DIAG
+ * drops its own. tree [B, n] int64 (or NULL), n <= 64, replaces both: the new
+ * tokens are drafts, and i sees the lens[b] keys before them and draft k
+ * where bit k of tree[b][i] is set. A row that sees nothing, and a padding
+ * row, gets out 0 and lse -FLT_MAX. max_len: at least the longest lens[b] +
+ * new_lens[b]; it sets the launch shape only (a longer sequence is still
+ * computed in full). cache->layers must be 1. */
+int morpho_cache_attention(const void* phi, const void* gate_q, const void* gate_k, const morpho_cache* cache,
+                           const int32_t* table, const int32_t* lens, const int32_t* new_lens, const int64_t* tree,
+                           void* out, float* lse, int64_t B, int64_t n, int64_t seq_pages, int64_t max_len,
+                           float scale, int mode, void* workspace, size_t workspace_bytes, morpho_stream_t stream);
+
+/* Copies page src[k] to page dst[k], k < count, in every layer (int32 device
+ * memory). A pair with a page outside the pool is left out. No page may be
+ * written by two pairs, or written by one and read by another. */
+int morpho_cache_copy_pages(const morpho_cache* cache, const int32_t* src, const int32_t* dst, int64_t count,
+                            morpho_stream_t stream);
+
+/* Moves token lens[b] + keep[b][k] of sequence b to position lens[b] + k, k <
+ * keep_lens[b] (NULL: keep_cols), in place and in every layer. keep [B,
+ * keep_cols] int32 has to ascend along a row (then every token is moved before
+ * its place is taken); a negative entry moves nothing. */
+int morpho_cache_compact(const morpho_cache* cache, const int32_t* table, const int32_t* lens, const int32_t* keep,
+                         const int32_t* keep_lens, int64_t B, int64_t keep_cols, int64_t seq_pages,
+                         morpho_stream_t stream);
+
 /* Per-kernel timing for measurement harnesses. No reference counterpart.
  * When enabled (process-wide), every kernel the library launches, from any
  * thread, carries a start and a stop HIP event bound to its dispatch

@@ -24,6 +24,7 @@ from torch import nn
 
 from . import capi
 from ._ops import add_op_namespace_prefix, ops
+from .cache import CacheStep, MorphoCache, morpho_cache_append, morpho_cache_attention, pack_cache_weights
 
 
 @torch.library.register_fake(add_op_namespace_prefix("forward"))
@@ -182,6 +183,37 @@ class MorphoAttention(nn.Module):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         return MorphoAttentionFunction.apply(x, self.W_phi, self.gate_q, self.gate_k, self.W_V, self.num_heads,
                                              self.cube_m, self.scale, self.causal, self.variant)
+
+    def pack_cache_weights(self) -> torch.Tensor:
+        """This layer's weights as :meth:`forward_cached` reads them (see
+        :func:`morphottention_amd.pack_cache_weights`)."""
+        return pack_cache_weights(self.W_phi, self.W_V)
+
+    def forward_cached(self, x: torch.Tensor, weights: torch.Tensor, cache: MorphoCache, step: CacheStep, *,
+                       layer: int = 0, tree: torch.Tensor | None = None) -> torch.Tensor:
+        """New tokens ``x`` ``[B, n, D]`` of the step's sequences: stored in ``cache``,
+        and their attention over the sequences so far. Inference only.
+
+        :param weights: :meth:`pack_cache_weights`, made once.
+        :param step: from ``cache.step``; the caller commits it after the last layer.
+        :param layer: this layer's index in the cache.
+        :param tree: int64 ``[B, n]``, the drafts that each drafted token sees
+            (see :func:`morphottention_amd.morpho_cache_attention`).
+        """
+        if not self.causal:
+            raise ValueError("forward_cached needs a causal layer: later tokens must not change earlier ones")
+        if tree is not None and self.mask_diag:
+            raise ValueError("mask_diag with a tree: leave a draft's own bit out instead")
+        if torch.is_grad_enabled() and x.requires_grad:
+            raise RuntimeError("the cache serves inference and has no gradients: call it under torch.no_grad()")
+        codes, values = cache.codes[layer], cache.values[layer]
+        with torch.no_grad():
+            phi = morpho_cache_append(x.contiguous(), weights, codes, values, step.table, step.lens,
+                                      new_lens=step.new_lens, projection=self.projection)
+            out, _ = morpho_cache_attention(phi, self.gate_q, self.gate_k, codes, values, step.table, step.lens,
+                                            new_lens=step.new_lens, tree=tree, scale=self.scale,
+                                            mask_diag=self.mask_diag, max_len=step.max_len)
+        return out
 
 
 def morpho_attention(x, W_phi, gate_q, gate_k, W_V, num_heads: int, cube_m: int, *, scale: float = 1.0,

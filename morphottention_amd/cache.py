@@ -1,0 +1,372 @@
+"""Serving a causal morpho-attention layer from a paged cache.
+
+No reference counterpart: the reference computes whole sequences only. The
+score of a query and a key is
+
+    s_ij = scale sum_c G_c (2 phi_ic phi_jc - phi_ic - phi_jc),  G = gate_q * gate_k,
+
+so what later tokens need of an earlier one is its codes ``phi`` and its values
+``x W_V``. Both are kept in float16 pages:
+
+* ``codes``  ``[layers, pages, H, page_size, cube_m]``;
+* ``values`` ``[layers, pages, H, page_size // 8, head_dim, 8]``: column ``c`` of
+  token ``t`` of a page at ``[t // 8, c, t % 8]``, the order in which the value
+  product reads them.
+
+The functions work on such tensors directly, with a ``table`` ``[B, seq_pages]``
+(int32, each sequence's pages in order) and ``lens`` ``[B]`` (int32, its tokens
+before the new ones) in device memory, and may be captured in a graph:
+
+* :func:`morpho_cache_append` projects new tokens and stores them;
+* :func:`morpho_cache_attention` lets them attend: one token a sequence, pieces
+  of a prompt, or a tree of drafted tokens;
+* :func:`morpho_cache_copy_pages` and :func:`morpho_cache_compact` copy pages and
+  move kept tokens together, in all layers at once.
+
+:class:`MorphoCache` owns the tensors and keeps account of the pages (sharing
+between forks, copies on write, rollback). ``MorphoAttention.forward_cached``
+runs a layer on it.
+
+The cache serves inference: none of this is differentiable, and a call that
+would need a gradient raises.
+"""
+
+from __future__ import annotations
+
+from dataclasses import dataclass
+
+import torch
+
+from ._ops import add_op_namespace_prefix, ops
+
+
+@torch.library.register_fake(add_op_namespace_prefix("cache_append"))
+def _cache_append_fake(X, weights, codes, values, table, lens, new_lens=None, variant=0):
+    return X.new_empty((X.shape[0], X.shape[1], codes.shape[1], codes.shape[3]))
+
+
+@torch.library.register_fake(add_op_namespace_prefix("cache_attention"))
+def _cache_attention_fake(phi, gate_q, gate_k, codes, values, table, lens, new_lens, tree, scale, causal, variant=0,
+                          max_len=0):
+    B, n, H, _m = phi.shape
+    return [phi.new_empty((B, n, H * values.shape[3])), phi.new_empty((B * H, n), dtype=torch.float32)]
+
+
+@torch.library.register_fake(add_op_namespace_prefix("cache_copy_pages"))
+def _cache_copy_pages_fake(codes, values, src, dst):
+    return None
+
+
+@torch.library.register_fake(add_op_namespace_prefix("cache_compact"))
+def _cache_compact_fake(codes, values, table, lens, keep, keep_lens=None):
+    return None
+
+
+_PROJECTION_BITS = {"sigmoid": 0, "hardtanh01": 4, "identity": 8}
+_MASK_DIAG = 2
+
+
+def _no_grad(*tensors) -> None:
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise RuntimeError("the cache serves inference and has no gradients: call it under torch.no_grad()")
+
+
+def pack_cache_weights(W_phi: torch.Tensor, W_V: torch.Tensor) -> torch.Tensor:
+    """``[W_phi | W_V]`` transposed, ``[H * cube_m + D, D]``: the weights as
+    :func:`morpho_cache_append` reads them. Done once, and again after the
+    weights have changed."""
+    return torch.cat((W_phi.detach(), W_V.detach()), 1).t().contiguous()
+
+
+def morpho_cache_append(x: torch.Tensor, weights: torch.Tensor, codes: torch.Tensor, values: torch.Tensor,
+                        table: torch.Tensor, lens: torch.Tensor, *, new_lens: torch.Tensor | None = None,
+                        projection: str = "sigmoid") -> torch.Tensor:
+    """Project new tokens and store their codes and values in one layer's pages.
+
+    :param x: the new tokens ``[B, n, D]``, float16.
+    :param weights: :func:`pack_cache_weights` of the layer.
+    :param codes: ``[pages, H, page_size, cube_m]``, written.
+    :param values: ``[pages, H, page_size // 8, head_dim, 8]``, written.
+    :param table: int32 ``[B, seq_pages]``, the pages of each sequence. Two
+        sequences must not share a page that is appended to.
+    :param lens: int32 ``[B]``, tokens of each sequence before the new ones; new
+        token ``i`` goes to position ``lens[b] + i``. A position past the table
+        or on a page that the pool does not have is not stored.
+    :param new_lens: int32 ``[B]``, new tokens of each sequence where not all
+        have ``n``; the rows behind them are padding and not stored.
+    :param projection: the layer's cube projection.
+    :returns: the codes ``[B, n, H, cube_m]`` of every row, as they are stored.
+    """
+    if projection not in _PROJECTION_BITS:
+        raise ValueError(f"projection must be one of {sorted(_PROJECTION_BITS)} (got {projection!r})")
+    _no_grad(x, weights)
+    return ops.cache_append(x, weights, codes, values, table, lens, new_lens, _PROJECTION_BITS[projection])
+
+
+def morpho_cache_attention(phi: torch.Tensor, gate_q: torch.Tensor, gate_k: torch.Tensor, codes: torch.Tensor,
+                           values: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, *,
+                           new_lens: torch.Tensor | None = None, tree: torch.Tensor | None = None, scale: float = 1.0,
+                           causal: bool = True, mask_diag: bool = False,
+                           max_len: int | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Attention of new tokens, appended before, over their sequences.
+
+    :param phi: their codes ``[B, n, H, cube_m]``, from :func:`morpho_cache_append`.
+    :param codes, values, table, lens, new_lens: as there (``lens`` still counts
+        the tokens before the new ones). Keys on a page that the pool does not
+        have are left out.
+    :param tree: int64 ``[B, n]``, ``n <= 64``: the new tokens are drafts. Token
+        ``i`` sees the ``lens[b]`` tokens before them and draft ``k`` where bit
+        ``k`` of ``tree[b, i]`` is set (its own bit among them). Replaces
+        ``causal`` and ``mask_diag``.
+    :param causal: new token ``i`` sees positions up to ``lens[b] + i``; else all.
+    :param mask_diag: drop each token's own key.
+    :param max_len: at least the longest ``lens[b] + new_lens[b]``. Sets how the
+        work is split, not what is computed; the table's whole length if not given.
+    :returns: ``out`` ``[B, n, D]`` and the base-2 log-sum-exp of the row scores
+        ``[B * H, n]`` (float32). A row that sees nothing, and a padding row,
+        has 0 and ``-FLT_MAX``.
+    """
+    if max_len is not None and max_len <= 0:
+        raise ValueError(f"max_len must be positive (got {max_len})")
+    if tree is not None and mask_diag:
+        raise ValueError("mask_diag with a tree: leave a draft's own bit out instead")
+    _no_grad(phi, gate_q, gate_k)
+    out, lse = ops.cache_attention(phi, gate_q, gate_k, codes, values, table, lens, new_lens, tree, scale, causal,
+                                   _MASK_DIAG if mask_diag else 0, max_len or 0)
+    return out, lse
+
+
+def morpho_cache_copy_pages(codes: torch.Tensor, values: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> None:
+    """Copy page ``src[k]`` to page ``dst[k]`` (int32 ``[pairs]``), in every layer
+    when ``codes`` and ``values`` have a leading layer dimension. No page may be
+    written twice, or written and read. Pairs with a page that the pool does
+    not have are left out."""
+    ops.cache_copy_pages(codes, values, src, dst)
+
+
+def morpho_cache_compact(codes: torch.Tensor, values: torch.Tensor, table: torch.Tensor, lens: torch.Tensor,
+                         keep: torch.Tensor, *, keep_lens: torch.Tensor | None = None) -> None:
+    """Move token ``lens[b] + keep[b, k]`` to position ``lens[b] + k``, in place and
+    in every layer: the accepted path of a tree to the front of its drafts
+    (``lens``: the tokens before them), or what is left after tokens were
+    evicted (``lens``: 0).
+
+    :param keep: int32 ``[B, kept]``; has to ascend along each row.
+    :param keep_lens: int32 ``[B]``, how many of them count.
+    """
+    ops.cache_compact(codes, values, table, lens, keep, keep_lens)
+
+
+@dataclass
+class CacheStep:
+    """New tokens of some sequences: what one forward pass of all layers needs."""
+
+    seqs: list[int]
+    counts: list[int]
+    n: int
+    table: torch.Tensor
+    lens: torch.Tensor
+    new_lens: torch.Tensor | None
+    max_len: int
+
+
+class MorphoCache:
+    """Pages of key codes and values, and which sequence has which of them.
+
+    :param num_pages: pages of each layer.
+    :param num_heads, cube_m, head_dim: of the layers' ``MorphoAttention``.
+    :param num_layers: layers that share the account of pages.
+    :param page_size: tokens a page: 32, 64, 128 or 256.
+
+    A step appends tokens to some sequences and is then committed::
+
+        seq = cache.new()
+        step = cache.step([seq], x.shape[1])          # pages for the new tokens
+        for i, layer in enumerate(layers):
+            x = layer.forward_cached(x, weights[i], cache, step, layer=i)
+        cache.commit(step)
+
+    Until then the sequences keep their old lengths, so a step that is dropped
+    leaves them as they were. After a tree of drafts :meth:`accept` takes the
+    accepted tokens instead.
+    """
+
+    def __init__(self, num_pages: int, num_heads: int, cube_m: int, head_dim: int, *, num_layers: int = 1,
+                 page_size: int = 64, device: torch.device | str | None = None) -> None:
+        if cube_m not in (16, 32, 64):
+            raise ValueError(f"cube_m must be 16, 32 or 64 (got {cube_m})")
+        if head_dim not in (32, 64, 128):
+            raise ValueError(f"head_dim must be 32, 64 or 128 (got {head_dim})")
+        if page_size not in (32, 64, 128, 256):
+            raise ValueError(f"page_size must be 32, 64, 128 or 256 (got {page_size})")
+        if min(num_pages, num_heads, num_layers) <= 0:
+            raise ValueError("num_pages, num_heads and num_layers must be positive")
+        self.page_size = page_size
+        self.num_pages = num_pages
+        self.codes = torch.zeros((num_layers, num_pages, num_heads, page_size, cube_m), dtype=torch.float16,
+                                 device=device)
+        self.values = torch.zeros((num_layers, num_pages, num_heads, page_size // 8, head_dim, 8), dtype=torch.float16,
+                                  device=device)
+        self._free = list(range(num_pages - 1, -1, -1))
+        self._uses = [0] * num_pages
+        self._pages: dict[int, list[int]] = {}
+        self._lens: dict[int, int] = {}
+        self._next = 0
+
+    # ---- account
+    @property
+    def free_pages(self) -> int:
+        """Pages that no sequence has."""
+        return len(self._free)
+
+    def length(self, seq: int) -> int:
+        """Committed tokens of a sequence."""
+        return self._lens[self._known(seq)]
+
+    def pages(self, seq: int) -> tuple[int, ...]:
+        """The pages of a sequence, in order."""
+        return tuple(self._pages[self._known(seq)])
+
+    def _known(self, seq: int) -> int:
+        if seq not in self._pages:
+            raise KeyError(f"no sequence {seq}")
+        return seq
+
+    def _take(self, count: int) -> list[int]:
+        if count > len(self._free):
+            raise RuntimeError(f"the cache is full: {count} pages needed, {len(self._free)} of {self.num_pages} free")
+        got = [self._free.pop() for _ in range(count)]
+        for p in got:
+            self._uses[p] = 1
+        return got
+
+    def _drop(self, pages) -> None:
+        for p in pages:
+            self._uses[p] -= 1
+            if self._uses[p] == 0:
+                self._free.append(p)
+
+    def new(self) -> int:
+        """A new, empty sequence."""
+        seq, self._next = self._next, self._next + 1
+        self._pages[seq], self._lens[seq] = [], 0
+        return seq
+
+    def free(self, seq: int) -> None:
+        """Give a sequence up; its pages that no fork shares are free again."""
+        self._drop(self._pages.pop(self._known(seq)))
+        del self._lens[seq]
+
+    def _ints(self, rows) -> torch.Tensor:
+        return torch.tensor(rows, dtype=torch.int32, device=self.codes.device)
+
+    def _copy(self, pairs: list[tuple[int, int]]) -> None:
+        if pairs:
+            morpho_cache_copy_pages(self.codes, self.values, self._ints([a for a, _ in pairs]),
+                                    self._ints([b for _, b in pairs]))
+
+    def fork(self, seq: int) -> int:
+        """A new sequence with the same tokens. Full pages are shared; a page
+        that is not full is copied, since both will append to theirs."""
+        length = self._lens[self._known(seq)]
+        full, rest = divmod(length, self.page_size)
+        own = self._take(1) if rest else []
+        if rest:
+            self._copy([(self._pages[seq][full], own[0])])
+        shared = self._pages[seq][:full]
+        for p in shared:
+            self._uses[p] += 1
+        new = self.new()
+        self._pages[new], self._lens[new] = shared + own, length
+        return new
+
+    def truncate(self, seq: int, length: int) -> None:
+        """Forget the tokens of a sequence from position ``length`` on."""
+        if not 0 <= length <= self._lens[self._known(seq)]:
+            raise ValueError(f"length must be 0 .. {self._lens[seq]} (got {length})")
+        keep = -(-length // self.page_size)
+        self._drop(self._pages[seq][keep:])
+        del self._pages[seq][keep:]
+        self._lens[seq] = length
+
+    def _own(self, wanted: list[tuple[int, int, int]]) -> None:
+        """For each (seq, first, end): the pages that hold positions first .. end - 1
+        exist and belong to the sequence alone. Nothing changes when the pool
+        has too few pages left."""
+        P = self.page_size
+        shared, grow = [], []
+        spare: dict[int, int] = {}
+        for seq, first, end in wanted:
+            have = self._pages[seq]
+            # a shared page is copied for all its users but the last: count down
+            for k in range(first // P, min(len(have), -(-end // P))):
+                p = have[k]
+                left = spare.get(p, self._uses[p])
+                if left > 1:
+                    shared.append((seq, k))
+                    spare[p] = left - 1
+            grow.append(max(0, -(-end // P) - len(have)))
+        fresh = self._take(len(shared) + sum(grow))
+        pairs = []
+        for seq, k in shared:
+            page = fresh.pop()
+            pairs.append((self._pages[seq][k], page))
+            self._uses[self._pages[seq][k]] -= 1
+            self._pages[seq][k] = page
+        for (seq, _, _), count in zip(wanted, grow):
+            self._pages[seq] += [fresh.pop() for _ in range(count)]
+        self._copy(pairs)
+
+    # ---- steps
+    def step(self, seqs: list[int], counts: int | list[int]) -> CacheStep:
+        """Pages for new tokens of some sequences: ``counts`` tokens of each, or a
+        list with as many for each."""
+        seqs = list(seqs)
+        if not seqs or len(set(seqs)) != len(seqs):
+            raise ValueError("a step takes one or more different sequences")
+        counts = [counts] * len(seqs) if isinstance(counts, int) else list(counts)
+        if len(counts) != len(seqs) or min(counts) < 0 or max(counts) == 0:
+            raise ValueError("counts must be one number, or one for each sequence, not negative and not all 0")
+        ends = [self._lens[self._known(s)] + c for s, c in zip(seqs, counts)]
+        self._own([(s, self._lens[s], e) for s, e in zip(seqs, ends)])
+        width = max(-(-e // self.page_size) for e in ends)
+        rows = [(self._pages[s] + [-1] * width)[:width] for s in seqs]
+        n = max(counts)
+        return CacheStep(seqs, counts, n, self._ints(rows), self._ints([self._lens[s] for s in seqs]),
+                         self._ints(counts) if min(counts) < n else None, max(ends))
+
+    def commit(self, step: CacheStep) -> None:
+        """The step's tokens belong to their sequences."""
+        for s, c in zip(step.seqs, step.counts):
+            self._lens[self._known(s)] += c
+
+    def accept(self, step: CacheStep, kept: list[list[int]]) -> None:
+        """After a step of drafts: of each sequence the drafts ``kept[b]`` (ascending
+        places among its drafts, e.g. the accepted path) are its next tokens,
+        the others are dropped."""
+        if len(kept) != len(step.seqs):
+            raise ValueError("kept must have a list for each sequence of the step")
+        for k, c in zip(kept, step.counts):
+            if any(a >= b for a, b in zip(k, k[1:])) or (k and not 0 <= k[0] <= k[-1] < c):
+                raise ValueError(f"kept places must ascend within 0 .. {c - 1} (got {k})")
+        if any(k != list(range(len(k))) for k in kept):
+            most = max(len(k) for k in kept)
+            morpho_cache_compact(self.codes, self.values, step.table, step.lens,
+                                 self._ints([list(k) + [0] * (most - len(k)) for k in kept]),
+                                 keep_lens=self._ints([len(k) for k in kept]))
+        for s, k in zip(step.seqs, kept):
+            self._lens[self._known(s)] += len(k)
+            self.truncate(s, self._lens[s])
+
+    def evict(self, seq: int, kept: list[int]) -> None:
+        """Keep only the tokens at positions ``kept`` (ascending) of a sequence; they
+        move together. Pages that forks share are copied first."""
+        length = self._lens[self._known(seq)]
+        if any(a >= b for a, b in zip(kept, kept[1:])) or (kept and not 0 <= kept[0] <= kept[-1] < length):
+            raise ValueError(f"kept positions must ascend within 0 .. {length - 1}")
+        still = next((i for i, k in enumerate(kept) if i != k), len(kept))  # these stay where they are
+        if still < len(kept):
+            self._own([(seq, still, len(kept))])
+            morpho_cache_compact(self.codes, self.values, self._ints([self._pages[seq]]), self._ints([still]),
+                                 self._ints([[k - still for k in kept[still:]]]))
+        self.truncate(seq, len(kept))

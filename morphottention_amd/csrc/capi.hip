@@ -571,6 +571,189 @@ MORPHO_EXPORT int morpho_soft_backward(const void* grad_out, const void* X, cons
   return MORPHO_OK;
 }
 
+// ---------------------------------------------------------------- paged cache
+namespace {
+// Most tokens a table row may address: positions and tile ends stay in int.
+constexpr int64_t kMaxCacheTokens = (int64_t)1 << 30;
+
+// Validates a pool and a call on it; `layers` is whether several are accepted.
+int make_cache_dims(const morpho_cache* c, bool layers, int64_t B, int64_t n, int64_t seq_pages, CacheDims& d) {
+  if (!c) return fail(MORPHO_ERR_INVALID_ARGUMENT, "Null cache pointer");
+  if (c->layers <= 0 || c->pages <= 0 || c->H <= 0 || B <= 0 || n <= 0 || seq_pages <= 0)
+    return fail(MORPHO_ERR_INVALID_ARGUMENT, "Invalid dimensions");
+  if (c->cube_m != 16 && c->cube_m != 32 && c->cube_m != 64)
+    return fail(MORPHO_ERR_UNSUPPORTED, "cube_m must be 16, 32 or 64 (got %lld)", (long long)c->cube_m);
+  if (c->head_dim_v != 32 && c->head_dim_v != 64 && c->head_dim_v != 128)
+    return fail(MORPHO_ERR_UNSUPPORTED, "head_dim_v must be 32, 64 or 128 (got %lld)", (long long)c->head_dim_v);
+  if (c->page_size != 32 && c->page_size != 64 && c->page_size != 128 && c->page_size != 256)
+    return fail(MORPHO_ERR_UNSUPPORTED, "page_size must be 32, 64, 128 or 256 (got %lld)", (long long)c->page_size);
+  if (!layers && c->layers != 1)
+    return fail(MORPHO_ERR_INVALID_ARGUMENT, "this call takes the pool of one layer (got %lld)", (long long)c->layers);
+  // D and H cube_m <= 65536 as elsewhere; a pool's layers sit in a grid
+  // dimension; page numbers and positions are ints. The grids of the kernels
+  // (workgroups of 256 threads) stay below 2^32 work-items.
+  if (c->layers > 65535 || c->pages > INT_MAX || c->H * c->cube_m > 65536 || c->H * c->head_dim_v > 65536 ||
+      c->H > 65536)
+    return fail(MORPHO_ERR_INVALID_ARGUMENT,
+                "cache too large: needs layers <= 65535, H*cube_m and H*head_dim_v <= 65536");
+  if (seq_pages > kMaxCacheTokens / c->page_size)
+    return fail(MORPHO_ERR_INVALID_ARGUMENT, "cache too large: seq_pages * page_size must be at most 2^30");
+  if (B > (1 << 22) || n > (1 << 22) || B * n > (1 << 22) || B * n * c->H > (1 << 23) ||
+      B * c->H * c->layers > (1 << 23))
+    return fail(MORPHO_ERR_INVALID_ARGUMENT,
+                "problem too large: needs B*n <= 2^22, B*n*H <= 2^23 and B*H*layers <= 2^23");
+  d.layers = (int)c->layers;
+  d.pages = (int)c->pages;
+  d.H = (int)c->H;
+  d.M = (int)c->cube_m;
+  d.DV = (int)c->head_dim_v;
+  d.P = (int)c->page_size;
+  d.B = (int)B;
+  d.n = (int)n;
+  d.W = (int)seq_pages;
+  return MORPHO_OK;
+}
+int check_pool(const morpho_cache* c) {
+  if (!c->codes || !c->values) return fail(MORPHO_ERR_INVALID_ARGUMENT, "Null pointer");
+  if (misaligned(c->codes) || misaligned(c->values))
+    return fail(MORPHO_ERR_INVALID_ARGUMENT, "tensor pointers must be 16-byte aligned");
+  return MORPHO_OK;
+}
+bool misaligned_ints(const void* a, const void* b = nullptr, const void* c = nullptr, const void* d = nullptr) {
+  return ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | reinterpret_cast<uintptr_t>(c) |
+           reinterpret_cast<uintptr_t>(d)) & 3) != 0;
+}
+CacheAttnPlan cache_plan(const CacheDims& d, int64_t max_len) {
+  const int64_t cap = (int64_t)d.W * d.P;
+  return cache_attn_plan(d.B, d.H, d.n, max_len < cap ? max_len : cap);
+}
+size_t cache_part_o_bytes(const CacheDims& d, const CacheAttnPlan& p) {
+  return align_up((size_t)d.B * d.H * d.n * p.nsplit * d.DV * 4);
+}
+size_t cache_attn_bytes(const CacheDims& d, const CacheAttnPlan& p) {
+  return p.nsplit == 1 ? 0 : cache_part_o_bytes(d, p) + align_up((size_t)d.B * d.H * d.n * p.nsplit * 16);
+}
+}  // namespace
+
+MORPHO_EXPORT int morpho_cache_append(const void* X, const void* W, const morpho_cache* cache, const int32_t* table,
+                                      const int32_t* lens, const int32_t* new_lens, void* phi, int64_t B, int64_t n,
+                                      int64_t seq_pages, int mode, morpho_stream_t stream) {
+  g_last_error.clear();
+  CacheDims d;
+  int st = make_cache_dims(cache, false, B, n, seq_pages, d);
+  if (st != MORPHO_OK) return st;
+  if (mode != 0 && mode != MORPHO_MODE_PROJ_HARDTANH01 && mode != MORPHO_MODE_PROJ_IDENTITY)
+    return fail(MORPHO_ERR_INVALID_ARGUMENT, "invalid mode bits 0x%x (one projection)", mode);
+  if (!X || !W || !table || !lens || !phi) return fail(MORPHO_ERR_INVALID_ARGUMENT, "Null pointer");
+  if ((st = check_pool(cache)) != MORPHO_OK) return st;
+  if (misaligned(X) || misaligned(W) || misaligned(phi))
+    return fail(MORPHO_ERR_INVALID_ARGUMENT, "tensor pointers must be 16-byte aligned");
+  if (misaligned_ints(table, lens, new_lens))
+    return fail(MORPHO_ERR_INVALID_ARGUMENT, "int32 pointers must be 4-byte aligned");
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  const int proj = mode & MORPHO_MODE_PROJ_HARDTANH01 ? kProjHardTanh01
+                   : mode & MORPHO_MODE_PROJ_IDENTITY ? kProjIdentity
+                                                      : kProjSigmoid;
+  MORPHO_LAUNCH("cache_append",
+                launch_cache_append(d, static_cast<const _Float16*>(X), static_cast<const _Float16*>(W),
+                                    static_cast<_Float16*>(cache->codes), static_cast<_Float16*>(cache->values), table,
+                                    lens, new_lens, static_cast<_Float16*>(phi), proj, s));
+  return MORPHO_OK;
+}
+
+MORPHO_EXPORT size_t morpho_cache_attention_workspace_size(const morpho_cache* cache, int64_t B, int64_t n,
+                                                           int64_t seq_pages, int64_t max_len) {
+  CacheDims d;
+  std::string keep = g_last_error;
+  const int st = make_cache_dims(cache, false, B, n, seq_pages, d);
+  g_last_error = keep;
+  return st == MORPHO_OK && max_len > 0 ? cache_attn_bytes(d, cache_plan(d, max_len)) : 0;
+}
+
+MORPHO_EXPORT int morpho_cache_attention(const void* phi, const void* gate_q, const void* gate_k,
+                                         const morpho_cache* cache, const int32_t* table, const int32_t* lens,
+                                         const int32_t* new_lens, const int64_t* tree, void* out, float* lse,
+                                         int64_t B, int64_t n, int64_t seq_pages, int64_t max_len, float scale,
+                                         int mode, void* workspace, size_t workspace_bytes, morpho_stream_t stream) {
+  g_last_error.clear();
+  CacheDims d;
+  int st = make_cache_dims(cache, false, B, n, seq_pages, d);
+  if (st != MORPHO_OK) return st;
+  if (max_len <= 0) return fail(MORPHO_ERR_INVALID_ARGUMENT, "max_len must be positive");
+  if (!__builtin_isfinite(scale)) return fail(MORPHO_ERR_INVALID_ARGUMENT, "scale must be a finite number");
+  if ((mode & ~(MORPHO_MODE_CAUSAL | MORPHO_MODE_MASK_DIAG)) != 0)
+    return fail(MORPHO_ERR_INVALID_ARGUMENT, "invalid mode bits 0x%x (causal | mask_diag)", mode);
+  if (tree && n > 64) return fail(MORPHO_ERR_UNSUPPORTED, "a tree holds at most 64 drafted tokens (got %lld)", (long long)n);
+  if (tree && (mode & MORPHO_MODE_MASK_DIAG))
+    return fail(MORPHO_ERR_INVALID_ARGUMENT, "MORPHO_MODE_MASK_DIAG with a tree: leave a draft's own bit out instead");
+  if (!phi || !gate_q || !gate_k || !table || !lens || !out || !lse)
+    return fail(MORPHO_ERR_INVALID_ARGUMENT, "Null pointer");
+  if ((st = check_pool(cache)) != MORPHO_OK) return st;
+  if (misaligned(phi) || misaligned(out) || misaligned(lse))
+    return fail(MORPHO_ERR_INVALID_ARGUMENT, "tensor pointers must be 16-byte aligned");
+  if (misaligned_ints(table, lens, new_lens) || (reinterpret_cast<uintptr_t>(tree) & 7) != 0)
+    return fail(MORPHO_ERR_INVALID_ARGUMENT, "int32 pointers must be 4-byte aligned, tree 8-byte");
+  const CacheAttnPlan plan = cache_plan(d, max_len);
+  if ((int64_t)d.B * d.H * plan.qblocks * plan.nsplit > (1 << 23))
+    return fail(MORPHO_ERR_INVALID_ARGUMENT, "problem too large: B*H*pieces must be at most 2^23");
+  const size_t need = cache_attn_bytes(d, plan);
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(MORPHO_ERR_WORKSPACE, "cache attention workspace needs %zu bytes (got %zu)", need, workspace_bytes);
+  if (need && (reinterpret_cast<uintptr_t>(workspace) & 255) != 0)
+    return fail(MORPHO_ERR_WORKSPACE, "workspace must be 256-byte aligned");
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  CacheAttnBuffers part{nullptr, nullptr};
+  if (need) {
+    part.o = static_cast<float*>(workspace);
+    part.st = reinterpret_cast<float4*>(static_cast<char*>(workspace) + cache_part_o_bytes(d, plan));
+  }
+  auto* o = static_cast<_Float16*>(out);
+  MORPHO_LAUNCH("cache_attn",
+                launch_cache_attn(d, plan, static_cast<const _Float16*>(phi), static_cast<const _Float16*>(gate_q),
+                                  static_cast<const _Float16*>(gate_k), static_cast<const _Float16*>(cache->codes),
+                                  static_cast<const _Float16*>(cache->values), table, lens, new_lens, tree, o, lse,
+                                  part, scale, mode & MORPHO_MODE_CAUSAL, mode & MORPHO_MODE_MASK_DIAG, s));
+  if (need) MORPHO_LAUNCH("cache_join", launch_cache_attn_join(d, plan, lens, new_lens, part, o, lse, s));
+  return MORPHO_OK;
+}
+
+MORPHO_EXPORT int morpho_cache_copy_pages(const morpho_cache* cache, const int32_t* src, const int32_t* dst,
+                                          int64_t count, morpho_stream_t stream) {
+  g_last_error.clear();
+  CacheDims d;
+  int st = make_cache_dims(cache, true, 1, 1, 1, d);
+  if (st != MORPHO_OK) return st;
+  if (count < 0 || count > INT_MAX) return fail(MORPHO_ERR_INVALID_ARGUMENT, "Invalid dimensions");
+  if (count == 0) return MORPHO_OK;
+  if (!src || !dst) return fail(MORPHO_ERR_INVALID_ARGUMENT, "Null pointer");
+  if ((st = check_pool(cache)) != MORPHO_OK) return st;
+  if (misaligned_ints(src, dst)) return fail(MORPHO_ERR_INVALID_ARGUMENT, "int32 pointers must be 4-byte aligned");
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  MORPHO_LAUNCH("cache_copy", launch_cache_copy(d, static_cast<_Float16*>(cache->codes),
+                                                static_cast<_Float16*>(cache->values), src, dst, (int)count, s));
+  return MORPHO_OK;
+}
+
+MORPHO_EXPORT int morpho_cache_compact(const morpho_cache* cache, const int32_t* table, const int32_t* lens,
+                                       const int32_t* keep, const int32_t* keep_lens, int64_t B, int64_t keep_cols,
+                                       int64_t seq_pages, morpho_stream_t stream) {
+  g_last_error.clear();
+  CacheDims d;
+  int st = make_cache_dims(cache, true, B, 1, seq_pages, d);
+  if (st != MORPHO_OK) return st;
+  if (keep_cols < 0 || keep_cols > kMaxCacheTokens) return fail(MORPHO_ERR_INVALID_ARGUMENT, "Invalid dimensions");
+  if (keep_cols == 0) return MORPHO_OK;
+  if (!table || !lens || !keep) return fail(MORPHO_ERR_INVALID_ARGUMENT, "Null pointer");
+  if ((st = check_pool(cache)) != MORPHO_OK) return st;
+  if (misaligned_ints(table, lens, keep, keep_lens))
+    return fail(MORPHO_ERR_INVALID_ARGUMENT, "int32 pointers must be 4-byte aligned");
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  MORPHO_LAUNCH("cache_compact", launch_cache_compact(d, static_cast<_Float16*>(cache->codes),
+                                                      static_cast<_Float16*>(cache->values), table, lens, keep,
+                                                      keep_lens, (int)keep_cols, s));
+  return MORPHO_OK;
+}
+
 MORPHO_EXPORT int morpho_timing_enable(int enable) {
   g_timing.store(enable != 0);
   return MORPHO_OK;

@@ -295,4 +295,39 @@ inline BwdGemmPlan bwd_gemm_plan(const Dims& d) {
   return 3 * c128 < 4 * c256 ? p128 : p256;
 }
 
+// ---------------------------------------------------------------- paged cache
+// Sizes of a paged cache of key codes and values and of a call on it.
+struct CacheDims {
+  int layers, pages, H, M, DV, P;  // P tokens a page
+  int B, n, W;                     // sequences, new tokens of each, pages a sequence (table row)
+};
+
+// Launch shape of the attention over the cache. Each wave holds qt tiles of 16
+// query rows. Up to 64 new tokens, the four waves of a workgroup share the
+// rows and divide the keys (rows = 0); more are dealt to the waves, 16 qt
+// each, and every wave walks all keys (rows = 1). The keys of a sequence are
+// cut into pieces of split_keys, one workgroup each; with more than one piece a
+// second kernel joins the partial results.
+struct CacheAttnPlan {
+  int qt, rows, qblocks, nsplit, split_keys;
+};
+inline CacheAttnPlan cache_attn_plan(int B, int H, int n, int64_t max_len) {
+  CacheAttnPlan p;
+  p.qt = n <= 16 ? 1 : n <= 32 ? 2 : 4;
+  p.rows = n > 64;
+  p.qblocks = p.rows ? (n + 255) / 256 : 1;
+  const int64_t wgs = (int64_t)B * H * p.qblocks;
+  int64_t keys = (max_len * wgs + 1023) / 1024;
+  keys = keys < 512 ? 512 : (keys + 127) / 128 * 128;
+  p.nsplit = (int)((max_len + keys - 1) / keys);
+  if (p.nsplit < 1) p.nsplit = 1;
+  p.split_keys = (int)keys;
+  return p;
+}
+
+// Rows of the projection for an append. Up to kCacheSkinnyTokens tokens go
+// through strips of 16 output columns whose waves divide the contraction;
+// more through tiles of 128 x 128.
+constexpr int kCacheSkinnyTokens = 256;
+
 }  // namespace morpho

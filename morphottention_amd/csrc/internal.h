@@ -146,6 +146,26 @@ hipError_t launch_soft_tau_reduce(const float* prep, int nprep, const float* bwd
 int soft_prep_blocks(const Dims& d);  // partial sums written by the prep (one float each)
 int soft_bwd_slots(const Dims& d);    // workgroup slots of both backward kernels (two floats each)
 
+// kernels_cache.hip: the paged cache of key codes and values (CacheDims).
+struct CacheAttnBuffers {
+  float* o;    // [B, H, n, nsplit, DV] unnormalised sums of a piece's weighted values
+  float4* st;  // [B, H, n, nsplit] {reference, sum of weights, row constant, 0}
+};
+hipError_t launch_cache_append(const CacheDims& d, const _Float16* X, const _Float16* W, _Float16* codes,
+                               _Float16* values, const int* table, const int* lens, const int* new_lens,
+                               _Float16* phi, int proj, hipStream_t s);
+hipError_t launch_cache_attn(const CacheDims& d, const CacheAttnPlan& plan, const _Float16* phi,
+                             const _Float16* gate_q, const _Float16* gate_k, const _Float16* codes,
+                             const _Float16* values, const int* table, const int* lens, const int* new_lens,
+                             const int64_t* tree, _Float16* out, float* lse, const CacheAttnBuffers& part, float scale,
+                             int causal, int mask_diag, hipStream_t s);
+hipError_t launch_cache_attn_join(const CacheDims& d, const CacheAttnPlan& plan, const int* lens, const int* new_lens,
+                                  const CacheAttnBuffers& part, _Float16* out, float* lse, hipStream_t s);
+hipError_t launch_cache_copy(const CacheDims& d, _Float16* codes, _Float16* values, const int* src, const int* dst,
+                             int count, hipStream_t s);
+hipError_t launch_cache_compact(const CacheDims& d, _Float16* codes, _Float16* values, const int* table,
+                                const int* lens, const int* keep, const int* keep_lens, int K, hipStream_t s);
+
 // Timing hooks (capi.hip). When timing is enabled, timing_begin opens a
 // record (a name and two events) for the launcher call that follows, and the
 // kernel launches inside it take the record's events through

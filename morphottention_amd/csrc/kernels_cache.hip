@@ -1,0 +1,789 @@
+// Kernels of the paged cache: serving a causal attention layer token by token.
+//
+// The score of a query i and a key j,
+//   s_ij = scale sum_c G_c (2 phi_ic phi_jc - phi_ic - phi_jc),  G = gate_q gate_k,
+// is s_ij = phi_j . u_i - r_i with u_ic = scale G_c (2 phi_ic - 1) and the row
+// constant r_i = scale sum_c G_c phi_ic: what the key adds alone folds into
+// the query. So the cache holds the codes phi_j and the values V_j and nothing
+// else, both rounded to float16 once, and the attention over it is a plain
+// dot product with u_i, exact for these stored numbers to fp32 rounding.
+//
+// Layout of a layer's pool, P tokens a page:
+//   codes  [pages, H, P, M]          a key's codes contiguous
+//   values [pages, H, P / 8, DV, 8]  eight tokens of one value column contiguous
+// In the value product O^T += V^T P^T the contraction runs over the keys, so a
+// lane's MFMA operand is 8 keys of one column: with this layout one 16-byte
+// load from memory, without a transpose through LDS.
+#include "common.h"
+#include "gemm.h"
+#include "internal.h"
+
+namespace morpho {
+
+namespace {
+
+// What a sequence has: ctx tokens before the new ones, nb new ones, total keys.
+struct SeqLen {
+  int ctx, nb, total;
+};
+// Lengths outside their range are cut: a negative one counts as 0, what goes
+// past the table's pages is not there.
+__device__ __forceinline__ SeqLen seq_len(const int* __restrict__ lens, const int* __restrict__ new_lens, int b, int n,
+                                          int cap) {
+  SeqLen q;
+  const int have = max(lens[b], 0);
+  q.nb = new_lens ? min(max(new_lens[b], 0), n) : n;
+  q.total = (int)min((int64_t)have + q.nb, (int64_t)cap);
+  q.ctx = min(have, q.total);
+  return q;
+}
+
+// Bits of an fp16 value: an infinity or a NaN.
+__device__ __forceinline__ bool not_finite(f16 v) {
+  return (__builtin_bit_cast(unsigned short, v) & 0x7c00) == 0x7c00;
+}
+
+}  // namespace
+
+// ---------------------------------------------------------------- attention over the cache
+struct CacheAttnArgs {
+  int n, H, W, pages, lp;  // new tokens, heads, pages a sequence, pages, log2 of the page size
+  int qblocks, nsplit, split_keys;
+  float sl2e;  // scale log2 e
+  int causal, mask_diag;
+};
+
+// One 32-key tile of one head in registers, as MFMA 16x16x32 A operands.
+template <int M, int DV>
+struct CacheTile {
+  static constexpr int KC = M == 64 ? 2 : 1;
+  f16x8 k[2][KC];    // block i: rows are keys 8 (r / 4) + 4 i + r % 4, so that the scores of both blocks
+                     // come out as the value product's B operand (lane group g: keys 8 g .. 8 g + 7)
+  f16x8 v[DV / 16];  // 16 value columns each, keys 8 g .. 8 g + 7
+};
+
+// A workgroup: one (sequence, head), 16 QT query rows (ROWS: 16 QT for each
+// of its four waves), one piece of the keys. S^T = K u^T and O^T += V^T P^T on
+// v_mfma_f32_16x16x32_f16: a lane holds 8 keys of the query lane % 16 in both
+// products, so weights never leave their lane. u is an fp16 hi / lo pair of
+// the row scaled to [2^13, 2^14), the weights are hi / lo pairs too: the
+// result is as exact as fp32 sums.
+//
+// The softmax reference is a maximum seen so far; it moves only when a score
+// passes it by more than 2^3, so most tiles rescale nothing. Weights are
+// 2^(s - reference + 12) <= 2^15: fp16 keeps what is 2^-36 of the largest.
+template <int M, int DV, int QT, bool ROWS>
+__global__ __launch_bounds__(256) void cache_attn_kernel(
+    CacheAttnArgs a, const f16* __restrict__ phi, const f16* __restrict__ gate_q, const f16* __restrict__ gate_k,
+    const f16* __restrict__ codes, const f16* __restrict__ values, const int* __restrict__ table,
+    const int* __restrict__ lens, const int* __restrict__ new_lens, const int64_t* __restrict__ tree,
+    f16* __restrict__ out, float* __restrict__ lse, float* __restrict__ part_o, float4* __restrict__ part_st) {
+  constexpr int KC = CacheTile<M, DV>::KC, NT = DV / 16;
+  constexpr int NU = M == 16 ? 1 : 2 * KC;  // u operands: hi and lo of 32 codes each; at M = 16 one holds both
+  constexpr int STEP = ROWS ? 1 : 4;        // tiles from one of a wave to its next
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c16 = lane & 15, g = lane >> 4;
+  int id = blockIdx.x;
+  const int h = id % a.H;
+  id /= a.H;
+  const int sp = id % a.nsplit;
+  id /= a.nsplit;
+  const int qb = a.qblocks - 1 - id % a.qblocks;  // causal: the longest rows start first
+  const int b = id / a.qblocks;
+
+  const int P = 1 << a.lp;
+  const SeqLen sq = seq_len(lens, new_lens, b, a.n, a.W << a.lp);
+  const int kb = sp * a.split_keys;
+  if (sp > 0 && kb >= sq.total) return;  // not one of this sequence's pieces
+  const int q0 = qb * (ROWS ? 64 * QT : 16 * QT);
+  if (q0 >= sq.nb && a.nsplit > 1) return;  // padding rows: the joining kernel writes them
+  const int qw = q0 + (ROWS ? 16 * QT * w : 0);
+
+  // u_i, its scale and the row constant
+  f16x8 u[QT][NU];
+  float sc[QT], rc[QT];
+  int64_t bits[QT];
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const int row = min(qw + 16 * t + c16, a.n - 1);
+    const f16* pr = phi + (((int64_t)b * a.n + row) * a.H + h) * M;
+    bits[t] = tree ? tree[(int64_t)b * a.n + row] : 0;
+    float x[KC][8], big = 0.f, r = 0.f;
+#pragma unroll
+    for (int c = 0; c < KC; ++c) {
+      const int c0 = M == 16 ? 8 * (g & 1) : 32 * c + 8 * g;
+      const f16x8 p8 = *reinterpret_cast<const f16x8*>(pr + c0);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float G = a.sl2e * ((float)gate_q[h * M + c0 + j] * (float)gate_k[h * M + c0 + j]);
+        x[c][j] = G * (2.f * (float)p8[j] - 1.f);
+        r += G * (float)p8[j];
+        big = fmaxf(big, fabsf(x[c][j]));
+      }
+    }
+    r += __shfl_xor(r, 16);
+    big = fmaxf(big, __shfl_xor(big, 16));
+    if (M != 16) {  // at M = 16 lane groups 2 and 3 hold the codes of 0 and 1 again
+      r += __shfl_xor(r, 32);
+      big = fmaxf(big, __shfl_xor(big, 32));
+    }
+    rc[t] = r;
+    const int e = big > 0.f && big < kFltMax ? max(__builtin_amdgcn_frexp_expf(big), -100) : 14;
+    sc[t] = ldexpf(1.f, e - 14);
+#pragma unroll
+    for (int c = 0; c < KC; ++c)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        f16 hi, lo;
+        split_exact(ldexpf(x[c][j], 14 - e), hi, lo);
+        if (M == 16) {
+          u[t][0][j] = g < 2 ? hi : lo;
+        } else {
+          u[t][c][j] = hi;
+          u[t][KC + c][j] = lo;
+        }
+      }
+  }
+
+  f32x4 O[QT][NT];
+  float ref[QT], sum[QT];
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    ref[t] = -1e30f;  // finite, so that a masked score's weight is 2^-inf
+    sum[t] = 0.f;
+#pragma unroll
+    for (int c = 0; c < NT; ++c) O[t][c] = f32x4{};
+  }
+
+  // keys below `clear` are seen by every row of the wave, none from `end` on by any
+  const int ke = sp == a.nsplit - 1 ? sq.total : min(sq.total, kb + a.split_keys);
+  int clear = sq.ctx, end = sq.total;
+  if (tree == nullptr) {
+    if (a.causal) {
+      clear = sq.ctx + qw + (a.mask_diag ? 0 : 1);
+      end = sq.ctx + min(qw + 16 * QT, sq.nb);
+    } else if (!a.mask_diag) {
+      clear = sq.total;
+    }
+  }
+  clear = min(clear, sq.total);
+  end = qw < sq.nb ? min(end, ke) : 0;
+
+  const int* row = table + (int64_t)b * a.W;
+  const f16* kbase = codes + (int64_t)h * P * M + ((c16 >> 2) * 8 + (c16 & 3)) * M + (M == 16 ? 8 * (g & 1) : 8 * g);
+  const f16* vbase = values + (int64_t)h * P * DV + g * (DV * 8) + c16 * 8;
+  const int64_t kstride = (int64_t)a.H * P * M, vstride = (int64_t)a.H * P * DV;
+  auto page_of = [&](int tile) { return row[(tile * 32) >> a.lp]; };
+  // a page that the pool does not have: its keys are left out
+  auto exists = [&](int page) { return (unsigned)page < (unsigned)a.pages; };
+  auto load = [&](CacheTile<M, DV>& T, int tile, int page) {
+    const int64_t pg = exists(page) ? page : 0;
+    const int slot = (tile * 32) & (P - 1);
+    const f16* kp = kbase + pg * kstride + slot * M;
+    const f16* vp = vbase + pg * vstride + slot * DV;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int c = 0; c < KC; ++c) T.k[i][c] = *reinterpret_cast<const f16x8*>(kp + 4 * i * M + 32 * c);
+#pragma unroll
+    for (int c = 0; c < NT; ++c) T.v[c] = *reinterpret_cast<const f16x8*>(vp + 128 * c);
+  };
+
+  auto work = [&](CacheTile<M, DV>& T, int tile, int page, auto masked) {
+    constexpr bool MASKED = decltype(masked)::value;
+    const int key0 = tile * 32 + 8 * g;
+    bool strange = false;  // an infinity or NaN among the tile's values
+    if constexpr (MASKED) {
+#pragma unroll
+      for (int c = 0; c < NT; ++c)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const bool bad = not_finite(T.v[c][j]);
+          strange |= bad && key0 + j < sq.total;
+          if (bad || key0 + j >= sq.total) T.v[c][j] = (f16)0.f;
+        }
+      strange = __any(strange);
+    }
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      f32x4 s[2] = {f32x4{}, f32x4{}};
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (M == 16) {
+          s[i] = mfma16x16(T.k[i][0], u[t][0], s[i]);
+        } else {
+#pragma unroll
+          for (int c = 0; c < KC; ++c) {
+            s[i] = mfma16x16(T.k[i][c], u[t][c], s[i]);
+            s[i] = mfma16x16(T.k[i][c], u[t][KC + c], s[i]);
+          }
+        }
+      }
+      float x[8];
+      unsigned seen = 0xff;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = s[j >> 2][j & 3] * sc[t];
+      if constexpr (MASKED) {
+        const int i = qw + 16 * t + c16;
+        seen = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int k = key0 + j, d = k - sq.ctx;  // d: which of the new tokens
+          bool v = k < sq.total && i < sq.nb;
+          if (tree)
+            v = v && (d < 0 || ((bits[t] >> min(max(d, 0), 63)) & 1));
+          else
+            v = v && (!a.causal || d <= i) && !(a.mask_diag && d == i);
+          seen |= v ? 1u << j : 0u;
+          x[j] = v ? x[j] : kNegInf;
+        }
+      }
+      float top = x[0];
+#pragma unroll
+      for (int j = 1; j < 8; ++j) top = fmaxf(top, x[j]);
+      if (__any(top > ref[t] + 3.f)) {
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const float nr = fmaxf(ref[t], top), f = fast_exp2(ref[t] - nr);
+        ref[t] = nr;
+        sum[t] *= f;
+#pragma unroll
+        for (int c = 0; c < NT; ++c) O[t][c] *= f;
+      }
+      f16x8 hi, lo;
+      float p[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        p[j] = fast_exp2(x[j] + (12.f - ref[t]));
+        sum[t] += p[j];
+        f16 ph, pl;
+        split_exact(p[j], ph, pl);
+        hi[j] = ph;
+        lo[j] = pl;
+      }
+#pragma unroll
+      for (int c = 0; c < NT; ++c) {
+        O[t][c] = mfma16x16(T.v[c], hi, O[t][c]);
+        O[t][c] = mfma16x16(T.v[c], lo, O[t][c]);
+      }
+      if constexpr (MASKED) {
+        if (strange) {
+          // Such values reach only the rows that see their key: 0 times an
+          // infinity would be NaN in every row of the product above.
+          const f16* vt = values + (int64_t)h * P * DV + page * vstride + ((tile * 32) & (P - 1)) * DV + g * 32;
+#pragma unroll 1
+          for (int k = 0; k < 32; ++k) {
+            const int from = 16 * (k >> 3) + c16;
+            float pk = p[0];
+#pragma unroll
+            for (int j = 1; j < 8; ++j) pk = (k & 7) == j ? p[j] : pk;
+            pk = __shfl(pk, from);
+            const bool sees = (__shfl((int)seen, from) >> (k & 7)) & 1;
+#pragma unroll
+            for (int c = 0; c < NT; ++c)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                const f16 vb = vt[(k >> 3) * DV * 8 + 128 * c + 8 * r + (k & 7)];
+                O[t][c][r] += sees && not_finite(vb) ? pk * (float)vb : 0.f;
+              }
+          }
+        }
+      }
+    }
+  };
+
+  int tile = kb / 32 + (ROWS ? 0 : w);
+  if (tile * 32 < end) {
+    CacheTile<M, DV> A, B;
+    int pa = page_of(tile), pb = 0;
+    load(A, tile, pa);
+    if ((tile + STEP) * 32 < end) pb = page_of(tile + STEP);
+    auto step = [&](CacheTile<M, DV>& cur, CacheTile<M, DV>& nxt, int& pc, int& pn) {
+      const bool more = (tile + STEP) * 32 < end;
+      if (more) load(nxt, tile + STEP, pn);
+      int after = 0;
+      if ((tile + 2 * STEP) * 32 < end) after = page_of(tile + 2 * STEP);
+      if (exists(pc)) {
+        if (tile * 32 + 32 <= clear)
+          work(cur, tile, pc, std::false_type());
+        else
+          work(cur, tile, pc, std::true_type());
+      }
+      pc = after;
+      tile += STEP;
+      return more;
+    };
+    while (step(A, B, pa, pb) && step(B, A, pb, pa)) {
+    }
+  }
+
+  // join the lane groups (each holds its own keys of the same 16 queries)
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    sum[t] += __shfl_xor(sum[t], 16);
+    sum[t] += __shfl_xor(sum[t], 32);
+  }
+  const int64_t orow = (int64_t)b * a.n;
+  // writes a row's 4 columns from c on: the result, or this piece's part
+  auto put = [&](int i, int c, f32x4 o, float m, float l, float r) {
+    if (i >= a.n) return;
+    if (a.nsplit > 1) {
+      if (i >= sq.nb) return;
+      const int64_t at = (((int64_t)b * a.H + h) * a.n + i) * a.nsplit + sp;
+      *reinterpret_cast<f32x4*>(part_o + at * DV + c) = o;
+      if (c == 0) part_st[at] = float4{m, l, r, 0.f};
+      return;
+    }
+    const bool some = i < sq.nb && l != 0.f;  // padding rows and rows that see nothing get 0
+    const float inv = some ? 1.f / l : 0.f;
+    f16x4 y;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) y[k] = some ? (f16)(o[k] * inv) : (f16)0.f;
+    *reinterpret_cast<f16x4*>(out + ((orow + i) * a.H + h) * DV + c) = y;
+    if (c == 0) lse[((int64_t)b * a.H + h) * a.n + i] = some ? m - 12.f + __log2f(l) - r : -kFltMax;
+  };
+  if constexpr (ROWS) {
+#pragma unroll
+    for (int t = 0; t < QT; ++t)
+#pragma unroll
+      for (int c = 0; c < NT; ++c) put(qw + 16 * t + c16, 16 * c + 4 * g, O[t][c], ref[t], sum[t], rc[t]);
+  } else {
+    __shared__ __align__(16) float so[4][16][DV + 4];
+    __shared__ float sm[4][16], sl[4][16], sr[16];
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      if (t) __syncthreads();
+#pragma unroll
+      for (int c = 0; c < NT; ++c) *reinterpret_cast<f32x4*>(&so[w][c16][16 * c + 4 * g]) = O[t][c];
+      if (g == 0) {
+        sm[w][c16] = ref[t];
+        sl[w][c16] = sum[t];
+        if (w == 0) sr[c16] = rc[t];
+      }
+      __syncthreads();
+      for (int e = threadIdx.x; e < 4 * DV; e += 256) {
+        const int q = e / (DV / 4), c = 4 * (e % (DV / 4));
+        float m = sm[0][q];
+#pragma unroll
+        for (int k = 1; k < 4; ++k) m = fmaxf(m, sm[k][q]);
+        float l = 0.f;
+        f32x4 o = {};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float f = fast_exp2(sm[k][q] - m);
+          l += f * sl[k][q];
+          o += f * *reinterpret_cast<const f32x4*>(&so[k][q][c]);
+        }
+        put(q0 + 16 * t + q, c, o, m, l, sr[q]);
+      }
+    }
+  }
+}
+
+// Joins the pieces of a row: one workgroup a (sequence, head, row), its lanes
+// in groups of DV / 4, group k taking pieces k, k + groups, ... in order, then
+// the groups in order.
+template <int DV>
+__global__ __launch_bounds__(256) void cache_join_kernel(CacheAttnArgs a, const int* __restrict__ lens,
+                                                        const int* __restrict__ new_lens,
+                                                        const float* __restrict__ part_o,
+                                                        const float4* __restrict__ part_st, f16* __restrict__ out,
+                                                        float* __restrict__ lse) {
+  constexpr int TC = DV / 4, NG = 256 / TC;
+  const int64_t at = blockIdx.x;  // (b H + h) n + i
+  const int i = (int)(at % a.n);
+  const int64_t bh = at / a.n;
+  const int h = (int)(bh % a.H), b = (int)(bh / a.H);
+  const SeqLen sq = seq_len(lens, new_lens, b, a.n, a.W << a.lp);
+  const int pieces = i < sq.nb ? min(a.nsplit, (sq.total + a.split_keys - 1) / a.split_keys) : 0;
+  const int k = threadIdx.x / TC, c = 4 * (threadIdx.x % TC);
+  float m = -1e30f, l = 0.f;
+  f32x4 o = {};
+  for (int s = k; s < pieces; s += NG) {
+    const float4 st = part_st[at * a.nsplit + s];
+    const f32x4 x = *reinterpret_cast<const f32x4*>(part_o + (at * a.nsplit + s) * DV + c);
+    const float nm = fmaxf(m, st.x), f = fast_exp2(m - nm), fs = fast_exp2(st.x - nm);
+    l = l * f + st.y * fs;
+    o = o * f + x * fs;
+    m = nm;
+  }
+  __shared__ __align__(16) float so[NG][DV];
+  __shared__ float sm[NG], sl[NG];
+  *reinterpret_cast<f32x4*>(&so[k][c]) = o;
+  if (c == 0) {
+    sm[k] = m;
+    sl[k] = l;
+  }
+  __syncthreads();
+  if (k != 0) return;
+#pragma unroll
+  for (int e = 1; e < NG; ++e) m = fmaxf(m, sm[e]);
+  l = 0.f;
+  o = f32x4{};
+#pragma unroll
+  for (int e = 0; e < NG; ++e) {
+    const float f = fast_exp2(sm[e] - m);
+    l += f * sl[e];
+    o += f * *reinterpret_cast<const f32x4*>(&so[e][c]);
+  }
+  const bool some = l != 0.f;
+  const float inv = some ? 1.f / l : 0.f;
+  f16x4 y;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) y[r] = some ? (f16)(o[r] * inv) : (f16)0.f;
+  *reinterpret_cast<f16x4*>(out + (((int64_t)b * a.n + i) * a.H + h) * DV + c) = y;
+  if (c == 0) lse[at] = some ? m - 12.f + __log2f(l) - part_st[at * a.nsplit].z : -kFltMax;
+}
+
+namespace {
+int log2_of(int p) { return __builtin_ctz((unsigned)p); }
+CacheAttnArgs attn_args(const CacheDims& d, const CacheAttnPlan& p) {
+  CacheAttnArgs a{};
+  a.n = d.n;
+  a.H = d.H;
+  a.W = d.W;
+  a.pages = d.pages;
+  a.lp = log2_of(d.P);
+  a.qblocks = p.qblocks;
+  a.nsplit = p.nsplit;
+  a.split_keys = p.split_keys;
+  return a;
+}
+
+template <int M, int DV>
+hipError_t launch_cache_attn_t(const CacheDims& d, const CacheAttnPlan& p, const CacheAttnArgs& a, const f16* phi,
+                               const f16* gate_q, const f16* gate_k, const f16* codes, const f16* values,
+                               const int* table, const int* lens, const int* new_lens, const int64_t* tree, f16* out,
+                               float* lse, const CacheAttnBuffers& part, hipStream_t s) {
+  const dim3 grid((unsigned)((int64_t)d.B * d.H * p.qblocks * p.nsplit)), block(256);
+#define MORPHO_CACHE_ATTN(QT, ROWS)                                                                              \
+  MORPHO_KLAUNCH((cache_attn_kernel<M, DV, QT, ROWS>), grid, block, 0, s, a, phi, gate_q, gate_k, codes, values, \
+                 table, lens, new_lens, tree, out, lse, part.o, part.st)
+  if (p.rows)
+    MORPHO_CACHE_ATTN(4, true);
+  else if (p.qt == 1)
+    MORPHO_CACHE_ATTN(1, false);
+  else if (p.qt == 2)
+    MORPHO_CACHE_ATTN(2, false);
+  else
+    MORPHO_CACHE_ATTN(4, false);
+#undef MORPHO_CACHE_ATTN
+  return hipGetLastError();
+}
+}  // namespace
+
+hipError_t launch_cache_attn(const CacheDims& d, const CacheAttnPlan& plan, const f16* phi, const f16* gate_q,
+                             const f16* gate_k, const f16* codes, const f16* values, const int* table,
+                             const int* lens, const int* new_lens, const int64_t* tree, f16* out, float* lse,
+                             const CacheAttnBuffers& part, float scale, int causal, int mask_diag, hipStream_t s) {
+  CacheAttnArgs a = attn_args(d, plan);
+  a.sl2e = scale * kLog2e;
+  a.causal = causal;
+  a.mask_diag = mask_diag;
+  MORPHO_MDV_DISPATCH(launch_cache_attn_t, d, plan, a, phi, gate_q, gate_k, codes, values, table, lens, new_lens, tree,
+                      out, lse, part, s);
+}
+
+hipError_t launch_cache_attn_join(const CacheDims& d, const CacheAttnPlan& plan, const int* lens, const int* new_lens,
+                                  const CacheAttnBuffers& part, f16* out, float* lse, hipStream_t s) {
+  const CacheAttnArgs a = attn_args(d, plan);
+  const dim3 grid((unsigned)((int64_t)d.B * d.H * d.n)), block(256);
+  if (d.DV == 32)
+    MORPHO_KLAUNCH((cache_join_kernel<32>), grid, block, 0, s, a, lens, new_lens, part.o, part.st, out, lse);
+  else if (d.DV == 64)
+    MORPHO_KLAUNCH((cache_join_kernel<64>), grid, block, 0, s, a, lens, new_lens, part.o, part.st, out, lse);
+  else
+    MORPHO_KLAUNCH((cache_join_kernel<128>), grid, block, 0, s, a, lens, new_lens, part.o, part.st, out, lse);
+  return hipGetLastError();
+}
+
+// ---------------------------------------------------------------- append
+struct CacheAppendArgs {
+  int T, n, D, H, M, DV, C;  // T = B n tokens, C = H (M + DV) columns
+  int W, pages, lp, proj;
+};
+
+// Where a token goes: its page (negative: nowhere) and its place there.
+__device__ __forceinline__ int2 token_slot(const CacheAppendArgs& a, const int* __restrict__ table,
+                                           const int* __restrict__ lens, const int* __restrict__ new_lens, int b,
+                                           int i) {
+  const int have = max(lens[b], 0), nb = new_lens ? new_lens[b] : a.n;
+  const int64_t pos = (int64_t)have + i;
+  if (i >= nb || pos >= ((int64_t)a.W << a.lp)) return int2{-1, 0};
+  const int page = table[(int64_t)b * a.W + (pos >> a.lp)];
+  return int2{(unsigned)page < (unsigned)a.pages ? page : -1, (int)(pos & ((1 << a.lp) - 1))};
+}
+
+// Few tokens: a workgroup of 8 waves per 16 output columns and 16 TT tokens.
+// Each wave contracts every 8th 32-wide step of D, straight from memory (what
+// bounds it is reading the weights once, and latency); the eight partial
+// tiles are added in LDS.
+template <int TT>
+__global__ __launch_bounds__(512) void cache_append_rows_kernel(CacheAppendArgs a, const f16* __restrict__ X,
+                                                               const f16* __restrict__ Wt, f16* __restrict__ codes,
+                                                               f16* __restrict__ values,
+                                                               const int* __restrict__ table,
+                                                               const int* __restrict__ lens,
+                                                               const int* __restrict__ new_lens,
+                                                               f16* __restrict__ phi) {
+  __shared__ __align__(16) float part[8][TT][16][20];  // [wave][token tile][token][column]
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c16 = lane & 15, g = lane >> 4;
+  const int col0 = blockIdx.x * 16, t0 = blockIdx.y * 16 * TT;
+  f32x4 acc[TT];
+#pragma unroll
+  for (int t = 0; t < TT; ++t) acc[t] = f32x4{};
+  const f16* wp = Wt + (int64_t)(col0 + c16) * a.D + 8 * g;
+  const f16* xp[TT];
+#pragma unroll
+  for (int t = 0; t < TT; ++t) xp[t] = X + (int64_t)min(t0 + 16 * t + c16, a.T - 1) * a.D + 8 * g;
+#pragma unroll 4
+  for (int k = 32 * w; k < a.D; k += 256) {
+    const f16x8 wf = *reinterpret_cast<const f16x8*>(wp + k);
+#pragma unroll
+    for (int t = 0; t < TT; ++t) acc[t] = mfma16x16(wf, *reinterpret_cast<const f16x8*>(xp[t] + k), acc[t]);
+  }
+#pragma unroll
+  for (int t = 0; t < TT; ++t) *reinterpret_cast<f32x4*>(&part[w][t][c16][4 * g]) = acc[t];
+  __syncthreads();
+  const bool code = col0 < a.H * a.M;  // M and DV are multiples of 16: a strip lies in one head's codes or values
+  for (int e = threadIdx.x; e < 256 * TT; e += 512) {
+    const int c = e & 15, tok = e >> 4, t = t0 + tok;
+    if (t >= a.T) continue;
+    float z = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) z += part[k][tok >> 4][tok & 15][c];
+    const int b = t / a.n;
+    const int2 at = token_slot(a, table, lens, new_lens, b, t - b * a.n);
+    if (code) {
+      const f16 y = (f16)cube_project(z, a.proj);
+      phi[(int64_t)t * (a.H * a.M) + col0 + c] = y;
+      const int h = (col0 + c) / a.M, cc = (col0 + c) % a.M;
+      if (at.x >= 0) codes[((((int64_t)at.x * a.H + h) << a.lp) + at.y) * a.M + cc] = y;
+    } else {
+      const int v = col0 + c - a.H * a.M, h = v / a.DV, cc = v % a.DV;
+      if (at.x >= 0)
+        values[(((int64_t)at.x * a.H + h) << a.lp) * a.DV + ((at.y >> 3) * a.DV + cc) * 8 + (at.y & 7)] = (f16)z;
+    }
+  }
+}
+
+// Many tokens: 128 x 128 tiles (tokens x columns) of the GEMM main loop.
+using AppendGemm = Gemm<128, 128, 2, true, true, 64, 2>;
+__global__ __launch_bounds__(kGemmThreads) void cache_append_tile_kernel(
+    CacheAppendArgs a, const f16* __restrict__ X, const f16* __restrict__ Wt, f16* __restrict__ codes,
+    f16* __restrict__ values, const int* __restrict__ table, const int* __restrict__ lens,
+    const int* __restrict__ new_lens, f16* __restrict__ phi) {
+  __shared__ __align__(16) char lds[AppendGemm::kLdsBytes];
+  __shared__ int2 slot[128];
+  const int ntm = (a.T + 127) / 128, ntn = (a.C + 127) / 128;
+  int tr, tc;
+  if (!gemm_tile_map(blockIdx.x, ntm, ntn, tr, tc)) return;
+  const int m0 = 128 * tr, n0 = 128 * tc;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (threadIdx.x < 128) {
+    const int t = min(m0 + (int)threadIdx.x, a.T - 1), b = t / a.n;
+    slot[threadIdx.x] = token_slot(a, table, lens, new_lens, b, t - b * a.n);
+  }
+  f32x4 acc[AppendGemm::FI][AppendGemm::FJ];
+  AppendGemm::run(X, a.D, Wt, a.D, a.T, a.C, m0, n0, 0, a.D, lds, acc);
+  __syncthreads();
+  const int wm = w / AppendGemm::WN, wn = w % AppendGemm::WN;
+#pragma unroll
+  for (int j = 0; j < AppendGemm::FJ; ++j) {
+    const int col = n0 + AppendGemm::WTN * wn + 16 * j;  // 16 columns of one head's codes or values
+    if (col >= a.C) continue;
+    const int cl = col + (lane & 15);
+#pragma unroll
+    for (int i = 0; i < AppendGemm::FI; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int rt = AppendGemm::WTM * wm + 16 * i + 4 * (lane >> 4) + r, t = m0 + rt;
+        if (t >= a.T) continue;
+        const int2 at = slot[rt];
+        if (col < a.H * a.M) {
+          const f16 y = (f16)cube_project(acc[i][j][r], a.proj);
+          phi[(int64_t)t * (a.H * a.M) + cl] = y;
+          const int h = cl / a.M, cc = cl % a.M;
+          if (at.x >= 0) codes[((((int64_t)at.x * a.H + h) << a.lp) + at.y) * a.M + cc] = y;
+        } else {
+          const int v = cl - a.H * a.M, h = v / a.DV, cc = v % a.DV;
+          if (at.x >= 0)
+            values[(((int64_t)at.x * a.H + h) << a.lp) * a.DV + ((at.y >> 3) * a.DV + cc) * 8 + (at.y & 7)] =
+                (f16)acc[i][j][r];
+        }
+      }
+  }
+}
+
+hipError_t launch_cache_append(const CacheDims& d, const f16* X, const f16* W, f16* codes, f16* values,
+                               const int* table, const int* lens, const int* new_lens, f16* phi, int proj,
+                               hipStream_t s) {
+  CacheAppendArgs a{};
+  a.T = d.B * d.n;
+  a.n = d.n;
+  a.D = d.H * d.DV;
+  a.H = d.H;
+  a.M = d.M;
+  a.DV = d.DV;
+  a.C = d.H * (d.M + d.DV);
+  a.W = d.W;
+  a.pages = d.pages;
+  a.lp = log2_of(d.P);
+  a.proj = proj;
+  if (a.T <= kCacheSkinnyTokens) {
+    const int tt = a.T <= 16 ? 1 : a.T <= 32 ? 2 : 4;
+    const dim3 grid(a.C / 16, (a.T + 16 * tt - 1) / (16 * tt));
+    if (tt == 1)
+      MORPHO_KLAUNCH((cache_append_rows_kernel<1>), grid, dim3(512), 0, s, a, X, W, codes, values, table, lens,
+                     new_lens, phi);
+    else if (tt == 2)
+      MORPHO_KLAUNCH((cache_append_rows_kernel<2>), grid, dim3(512), 0, s, a, X, W, codes, values, table, lens,
+                     new_lens, phi);
+    else
+      MORPHO_KLAUNCH((cache_append_rows_kernel<4>), grid, dim3(512), 0, s, a, X, W, codes, values, table, lens,
+                     new_lens, phi);
+  } else {
+    const dim3 grid(gemm_tile_grid((a.T + 127) / 128, (a.C + 127) / 128));
+    MORPHO_KLAUNCH(cache_append_tile_kernel, grid, dim3(kGemmThreads), 0, s, a, X, W, codes, values, table, lens,
+                   new_lens, phi);
+  }
+  return hipGetLastError();
+}
+
+// ---------------------------------------------------------------- page copies
+// One launch for all layers: 16 KiB of a page's codes or values a workgroup.
+constexpr int kCopyBytes = 16384;
+__global__ __launch_bounds__(256) void cache_copy_kernel(char* __restrict__ codes, char* __restrict__ values,
+                                                        const int* __restrict__ src, const int* __restrict__ dst,
+                                                        int pages, int64_t cbytes, int64_t vbytes, int nc, int nv) {
+  const int64_t id = blockIdx.x;
+  const int piece = (int)(id % (nc + nv));
+  const int pair = blockIdx.y, layer = blockIdx.z;
+  const int from = src[pair], to = dst[pair];
+  if ((unsigned)from >= (unsigned)pages || (unsigned)to >= (unsigned)pages) return;
+  const bool val = piece >= nc;
+  const int64_t size = val ? vbytes : cbytes, off = (int64_t)(val ? piece - nc : piece) * kCopyBytes;
+  char* pool = (val ? values : codes) + (int64_t)layer * pages * size;
+  const char* p = pool + from * size + off;
+  char* q = pool + to * size + off;
+  const int64_t left = size - off;  // a multiple of 16
+  i32x4 x[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int o = 16 * ((int)threadIdx.x + 256 * i);
+    if (o < left) x[i] = *reinterpret_cast<const i32x4*>(p + o);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int o = 16 * ((int)threadIdx.x + 256 * i);
+    if (o < left) *reinterpret_cast<i32x4*>(q + o) = x[i];
+  }
+}
+
+hipError_t launch_cache_copy(const CacheDims& d, f16* codes, f16* values, const int* src, const int* dst, int count,
+                             hipStream_t s) {
+  const int64_t cb = (int64_t)d.H * d.P * d.M * 2, vb = (int64_t)d.H * d.P * d.DV * 2;
+  const int nc = (int)((cb + kCopyBytes - 1) / kCopyBytes), nv = (int)((vb + kCopyBytes - 1) / kCopyBytes);
+  // grid y and z hold 65535 each
+  for (int at = 0; at < count; at += 65535) {
+    const dim3 grid(nc + nv, count - at < 65535 ? count - at : 65535, d.layers);
+    MORPHO_KLAUNCH(cache_copy_kernel, grid, dim3(256), 0, s, reinterpret_cast<char*>(codes),
+                   reinterpret_cast<char*>(values), src + at, dst + at, d.pages, cb, vb, nc, nv);
+  }
+  return hipGetLastError();
+}
+
+// ---------------------------------------------------------------- compaction
+// One workgroup a (layer, sequence, head) moves its kept tokens in order, 8
+// TB target tokens of one value column a lane and batch. keep ascends, so a
+// token never moves back over one that has yet to move (its place is at most
+// its source), and each batch is read whole before it is written.
+template <int DV>
+__global__ __launch_bounds__(256) void cache_compact_kernel(f16* codes, f16* values, const int* __restrict__ table,
+                                                           const int* __restrict__ lens,
+                                                           const int* __restrict__ keep,
+                                                           const int* __restrict__ keep_lens, int B, int H, int M,
+                                                           int pages, int W, int lp, int K) {
+  constexpr int BT = 64;  // target tokens of a batch
+  constexpr int PER = BT * DV / 256;
+  __shared__ int64_t from[BT], to[BT];  // token's place: page * P + slot, negative: none
+  int id = blockIdx.x;
+  const int h = id % H;
+  id /= H;
+  const int b = id % B, layer = id / B;
+  const int count = keep_lens ? min(max(keep_lens[b], 0), K) : K;
+  const int64_t base = max(lens[b], 0), cap = (int64_t)W << lp;
+  codes += (int64_t)layer * pages * H * ((int64_t)M << lp);
+  values += (int64_t)layer * pages * H * ((int64_t)DV << lp);
+  const int64_t mask = (1 << lp) - 1;
+  auto place = [&](int64_t pos) -> int64_t {
+    if (pos < 0 || pos >= cap) return -1;
+    const int page = table[(int64_t)b * W + (pos >> lp)];
+    return (unsigned)page < (unsigned)pages ? ((int64_t)page << lp) + (pos & mask) : -1;
+  };
+  auto code_at = [&](int64_t pl) { return ((((pl >> lp) * H + h) << lp) + (pl & mask)) * M; };
+  auto value_at = [&](int64_t pl) {
+    return ((((pl >> lp) * H + h) << lp) + (pl & mask & ~(int64_t)7)) * DV + (pl & 7);
+  };
+  for (int k0 = 0; k0 < count; k0 += BT) {
+    const int nk = min(BT, count - k0);
+    if (threadIdx.x < BT) {
+      int64_t f = -1, t = -1;
+      if ((int)threadIdx.x < nk) {
+        const int64_t rel = keep[(int64_t)b * K + k0 + threadIdx.x];
+        f = rel < 0 ? -1 : place(base + rel);
+        t = place(base + k0 + threadIdx.x);
+        if (f < 0 || f == t) t = -1;  // nothing to move
+      }
+      from[threadIdx.x] = f;
+      to[threadIdx.x] = t;
+    }
+    __syncthreads();
+    f16x8 cv[BT * 8 / 256];  // up to 8 pieces of 8 codes a token
+    f16 vv[PER];
+    const int mc = M / 8;
+#pragma unroll
+    for (int i = 0; i < BT * 8 / 256; ++i) {
+      const int e = threadIdx.x + 256 * i, k = e / mc;
+      if (k < nk && to[k] >= 0) cv[i] = *reinterpret_cast<const f16x8*>(codes + code_at(from[k]) + 8 * (e % mc));
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int e = threadIdx.x + 256 * i, k = e / DV, c = e % DV;
+      if (k < nk && to[k] >= 0) vv[i] = values[value_at(from[k]) + 8 * c];
+    }
+    wait_vmcnt<0>();
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < BT * 8 / 256; ++i) {
+      const int e = threadIdx.x + 256 * i, k = e / mc;
+      if (k < nk && to[k] >= 0) *reinterpret_cast<f16x8*>(codes + code_at(to[k]) + 8 * (e % mc)) = cv[i];
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int e = threadIdx.x + 256 * i, k = e / DV, c = e % DV;
+      if (k < nk && to[k] >= 0) values[value_at(to[k]) + 8 * c] = vv[i];
+    }
+    __syncthreads();  // the places are read before the next batch's are written
+  }
+}
+
+hipError_t launch_cache_compact(const CacheDims& d, f16* codes, f16* values, const int* table, const int* lens,
+                                const int* keep, const int* keep_lens, int K, hipStream_t s) {
+  const dim3 grid((unsigned)((int64_t)d.layers * d.B * d.H)), block(256);
+  const int lp = log2_of(d.P);
+#define MORPHO_CACHE_COMPACT(DV)                                                                               \
+  MORPHO_KLAUNCH((cache_compact_kernel<DV>), grid, block, 0, s, codes, values, table, lens, keep, keep_lens,   \
+                 d.B, d.H, d.M, d.pages, d.W, lp, K)
+  if (d.DV == 32)
+    MORPHO_CACHE_COMPACT(32);
+  else if (d.DV == 64)
+    MORPHO_CACHE_COMPACT(64);
+  else
+    MORPHO_CACHE_COMPACT(128);
+#undef MORPHO_CACHE_COMPACT
+  return hipGetLastError();
+}
+
+}  // namespace morpho

@@ -12,6 +12,7 @@
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <torch/library.h>
 
+#include <optional>
 #include <vector>
 
 #include "../../include/morphottention.h"
@@ -247,6 +248,143 @@ std::vector<at::Tensor> op_soft_backward(const at::Tensor& grad_out, const at::T
   return {dX, dW_phi, d_gate_q, d_gate_k, dW_V, dtau};
 }
 
+// ---- paged cache (no reference op: the reference computes whole sequences only)
+void check_ints(const at::Tensor& t, const char* name, const at::Tensor& codes) {
+  TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
+  TORCH_CHECK(t.scalar_type() == at::kInt, name, " must be int32");
+  TORCH_CHECK(t.is_contiguous(), name, " must be contiguous");
+  TORCH_CHECK(t.device() == codes.device(), "all tensors must be on the same device as codes");
+}
+
+// The pool of one layer, or of several (codes then have 5 dimensions).
+morpho_cache check_pool(const at::Tensor& codes, const at::Tensor& values, bool layers) {
+  check(codes, "codes");
+  check(values, "values");
+  TORCH_CHECK(values.device() == codes.device(), "all tensors must be on the same device as codes");
+  const int64_t k = codes.dim() - 4;
+  if (layers) {
+    TORCH_CHECK(k == 0 || k == 1, "codes must be [pages, H, page_size, cube_m] or [layers, pages, H, page_size, cube_m]");
+  } else {
+    TORCH_CHECK(k == 0, "codes must be [pages, H, page_size, cube_m]");
+  }
+  const int64_t L = k ? codes.size(0) : 1, pages = codes.size(k), H = codes.size(k + 1), P = codes.size(k + 2),
+                M = codes.size(k + 3);
+  TORCH_CHECK(values.dim() == k + 5 && (k == 0 || values.size(0) == L) && values.size(k) == pages &&
+                  values.size(k + 1) == H && P % 8 == 0 && values.size(k + 2) == P / 8 && values.size(k + 4) == 8,
+              "values must be [pages, H, page_size / 8, head_dim_v, 8] (with the layers of codes before)");
+  return morpho_cache{codes.data_ptr(), values.data_ptr(), L, pages, H, M, values.size(k + 3), P};
+}
+
+struct CacheCall {
+  const int32_t *table, *lens, *new_lens;
+  int64_t seq_pages;
+};
+CacheCall check_cache_call(const at::Tensor& codes, const at::Tensor& table, const at::Tensor& lens,
+                           const std::optional<at::Tensor>& new_lens, int64_t B) {
+  check_ints(table, "table", codes);
+  check_ints(lens, "lens", codes);
+  TORCH_CHECK(table.dim() == 2 && table.size(0) == B, "table must be [B, seq_pages]");
+  TORCH_CHECK(lens.dim() == 1 && lens.size(0) == B, "lens must be [B]");
+  if (new_lens) {
+    check_ints(*new_lens, "new_lens", codes);
+    TORCH_CHECK(new_lens->dim() == 1 && new_lens->size(0) == B, "new_lens must be [B]");
+  }
+  return {table.data_ptr<int32_t>(), lens.data_ptr<int32_t>(), new_lens ? new_lens->data_ptr<int32_t>() : nullptr,
+          table.size(1)};
+}
+
+at::Tensor op_cache_append(const at::Tensor& X, const at::Tensor& weights, const at::Tensor& codes,
+                           const at::Tensor& values, const at::Tensor& table, const at::Tensor& lens,
+                           const std::optional<at::Tensor>& new_lens, int64_t variant) {
+  const int mode = mode_of(false, variant);
+  const morpho_cache c = check_pool(codes, values, false);
+  check(X, "X");
+  check(weights, "weights");
+  TORCH_CHECK(X.dim() == 3, "X must be [B, n, D]");
+  const int64_t B = X.size(0), n = X.size(1), D = c.H * c.head_dim_v;
+  TORCH_CHECK(X.size(2) == D, "X must be [B, n, D] with D = H*head_dim_v of the cache (", D, ")");
+  TORCH_CHECK(weights.dim() == 2 && weights.size(0) == c.H * c.cube_m + D && weights.size(1) == D,
+              "weights must be [H*cube_m + D, D]");
+  TORCH_CHECK(X.device() == codes.device() && weights.device() == codes.device(),
+              "all tensors must be on the same device as codes");
+  const CacheCall k = check_cache_call(codes, table, lens, new_lens, B);
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(codes.device());
+  auto phi = at::empty({B, n, c.H, c.cube_m}, X.options());
+  raise_on(morpho_cache_append(X.data_ptr(), weights.data_ptr(), &c, k.table, k.lens, k.new_lens, phi.data_ptr(), B, n,
+                               k.seq_pages, mode, current_stream(codes)),
+           "cache_append");
+  return phi;
+}
+
+std::vector<at::Tensor> op_cache_attention(const at::Tensor& phi, const at::Tensor& gate_q, const at::Tensor& gate_k,
+                                           const at::Tensor& codes, const at::Tensor& values, const at::Tensor& table,
+                                           const at::Tensor& lens, const std::optional<at::Tensor>& new_lens,
+                                           const std::optional<at::Tensor>& tree, double scale, bool causal,
+                                           int64_t variant, int64_t max_len) {
+  const int mode = mode_of(causal, variant);
+  const morpho_cache c = check_pool(codes, values, false);
+  check(phi, "phi");
+  check(gate_q, "gate_q");
+  check(gate_k, "gate_k");
+  TORCH_CHECK(phi.dim() == 4 && phi.size(2) == c.H && phi.size(3) == c.cube_m,
+              "phi must be [B, n, H, cube_m] with H and cube_m of the cache");
+  const int64_t B = phi.size(0), n = phi.size(1);
+  TORCH_CHECK(gate_q.dim() == 2 && gate_q.size(0) == c.H && gate_q.size(1) == c.cube_m, "gate_q must be [H, cube_m]");
+  TORCH_CHECK(gate_k.dim() == 2 && gate_k.size(0) == c.H && gate_k.size(1) == c.cube_m, "gate_k must be [H, cube_m]");
+  TORCH_CHECK(phi.device() == codes.device() && gate_q.device() == codes.device() && gate_k.device() == codes.device(),
+              "all tensors must be on the same device as codes");
+  const CacheCall k = check_cache_call(codes, table, lens, new_lens, B);
+  if (tree) {
+    TORCH_CHECK(tree->is_cuda() && tree->scalar_type() == at::kLong && tree->is_contiguous() && tree->dim() == 2 &&
+                    tree->size(0) == B && tree->size(1) == n && tree->device() == codes.device(),
+                "tree must be a contiguous int64 [B, n] CUDA tensor on the device of codes");
+  }
+  TORCH_CHECK(max_len >= 0, "max_len must not be negative (0: the table's length), got ", max_len);
+  if (max_len == 0) max_len = k.seq_pages * c.page_size;
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(codes.device());
+  auto out = at::empty({B, n, c.H * c.head_dim_v}, phi.options());
+  auto lse = at::empty({B * c.H, n}, phi.options().dtype(at::kFloat));
+  const size_t ws_bytes = morpho_cache_attention_workspace_size(&c, B, n, k.seq_pages, max_len);
+  at::Tensor ws;
+  if (ws_bytes) ws = at::empty({(int64_t)ws_bytes}, phi.options().dtype(at::kByte));
+  raise_on(morpho_cache_attention(phi.data_ptr(), gate_q.data_ptr(), gate_k.data_ptr(), &c, k.table, k.lens,
+                                  k.new_lens, tree ? tree->data_ptr<int64_t>() : nullptr, out.data_ptr(),
+                                  lse.data_ptr<float>(), B, n, k.seq_pages, max_len, (float)scale, mode,
+                                  ws_bytes ? ws.data_ptr() : nullptr, ws_bytes, current_stream(codes)),
+           "cache_attention");
+  return {out, lse};
+}
+
+void op_cache_copy_pages(const at::Tensor& codes, const at::Tensor& values, const at::Tensor& src,
+                         const at::Tensor& dst) {
+  const morpho_cache c = check_pool(codes, values, true);
+  check_ints(src, "src", codes);
+  check_ints(dst, "dst", codes);
+  TORCH_CHECK(src.dim() == 1 && dst.dim() == 1 && src.size(0) == dst.size(0), "src and dst must be [pairs]");
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(codes.device());
+  raise_on(morpho_cache_copy_pages(&c, src.data_ptr<int32_t>(), dst.data_ptr<int32_t>(), src.size(0),
+                                   current_stream(codes)),
+           "cache_copy_pages");
+}
+
+void op_cache_compact(const at::Tensor& codes, const at::Tensor& values, const at::Tensor& table,
+                      const at::Tensor& lens, const at::Tensor& keep, const std::optional<at::Tensor>& keep_lens) {
+  const morpho_cache c = check_pool(codes, values, true);
+  check_ints(keep, "keep", codes);
+  TORCH_CHECK(keep.dim() == 2, "keep must be [B, kept]");
+  const int64_t B = keep.size(0);
+  if (keep_lens) {
+    check_ints(*keep_lens, "keep_lens", codes);
+    TORCH_CHECK(keep_lens->dim() == 1 && keep_lens->size(0) == B, "keep_lens must be [B]");
+  }
+  const CacheCall k = check_cache_call(codes, table, lens, std::nullopt, B);
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(codes.device());
+  raise_on(morpho_cache_compact(&c, k.table, k.lens, keep.data_ptr<int32_t>(),
+                                keep_lens ? keep_lens->data_ptr<int32_t>() : nullptr, B, keep.size(1), k.seq_pages,
+                                current_stream(codes)),
+           "cache_compact");
+}
+
 }  // namespace
 
 TORCH_LIBRARY(morphottention, m) {
@@ -264,6 +402,14 @@ TORCH_LIBRARY(morphottention, m) {
   m.def("soft_backward(Tensor grad_out, Tensor X, Tensor W_phi, Tensor gate_q, Tensor gate_k, Tensor W_V, "
         "Tensor tau, Tensor zb, Tensor workspace, int H, int cube_m, float scale, bool causal, int sgn, "
         "int variant=0) -> Tensor[]");
+  m.def("cache_append(Tensor X, Tensor weights, Tensor(a!) codes, Tensor(b!) values, Tensor table, Tensor lens, "
+        "Tensor? new_lens=None, int variant=0) -> Tensor");
+  m.def("cache_attention(Tensor phi, Tensor gate_q, Tensor gate_k, Tensor codes, Tensor values, Tensor table, "
+        "Tensor lens, Tensor? new_lens, Tensor? tree, float scale, bool causal, int variant=0, int max_len=0) "
+        "-> Tensor[]");
+  m.def("cache_copy_pages(Tensor(a!) codes, Tensor(b!) values, Tensor src, Tensor dst) -> ()");
+  m.def("cache_compact(Tensor(a!) codes, Tensor(b!) values, Tensor table, Tensor lens, Tensor keep, "
+        "Tensor? keep_lens=None) -> ()");
 }
 
 TORCH_LIBRARY_IMPL(morphottention, CUDA, m) {
@@ -273,4 +419,8 @@ TORCH_LIBRARY_IMPL(morphottention, CUDA, m) {
   m.impl("backward_train", &op_backward_train);
   m.impl("soft_forward", &op_soft_forward);
   m.impl("soft_backward", &op_soft_backward);
+  m.impl("cache_append", &op_cache_append);
+  m.impl("cache_attention", &op_cache_attention);
+  m.impl("cache_copy_pages", &op_cache_copy_pages);
+  m.impl("cache_compact", &op_cache_compact);
 }
