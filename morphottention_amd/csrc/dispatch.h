@@ -302,22 +302,20 @@ struct CacheDims {
   int B, n, W;                     // sequences, new tokens of each, pages a sequence (table row)
 };
 
-// Launch shape of the attention over the cache. Each wave holds qt tiles of 16
-// query rows. Up to 64 new tokens, the four waves of a workgroup share the
-// rows and divide the keys (rows = 0); more are dealt to the waves, 16 qt
-// each, and every wave walks all keys (rows = 1). The keys of a sequence are
-// cut into pieces of split_keys, one workgroup each; with more than one piece a
-// second kernel joins the partial results.
+// Launch shape of the attention over the cache. qt = 0: up to 16 new tokens,
+// which the four waves of a workgroup share while they divide the keys. qt >
+// 0: 64 qt of them a workgroup (row block), 16 qt for each wave. The keys of a
+// sequence are cut into pieces of split_keys, one workgroup each; with more
+// than one piece a second kernel joins the partial results.
 struct CacheAttnPlan {
-  int qt, rows, qblocks, nsplit, split_keys;
+  int qt, qblocks, nsplit, split_keys;
 };
 inline CacheAttnPlan cache_attn_plan(int B, int H, int n, int64_t max_len) {
   CacheAttnPlan p;
-  p.qt = n <= 16 ? 1 : n <= 32 ? 2 : 4;
-  p.rows = n > 64;
-  p.qblocks = p.rows ? (n + 255) / 256 : 1;
-  const int64_t wgs = (int64_t)B * H * p.qblocks;
-  int64_t keys = (max_len * wgs + 1023) / 1024;
+  p.qt = n <= 16 ? 0 : n <= 64 ? 1 : 2;
+  p.qblocks = p.qt ? (n + 64 * p.qt - 1) / (64 * p.qt) : 1;
+  const int64_t wgs = (int64_t)B * H * p.qblocks, most = p.qt == 2 ? 512 : 1024;
+  int64_t keys = (max_len * wgs + most - 1) / most;
   keys = keys < 512 ? 512 : (keys + 127) / 128 * 128;
   p.nsplit = (int)((max_len + keys - 1) / keys);
   if (p.nsplit < 1) p.nsplit = 1;

@@ -56,383 +56,579 @@ struct CacheAttnArgs {
 // One 32-key tile of one head in registers, as MFMA 16x16x32 A operands.
 template <int M, int DV>
 struct CacheTile {
-  static constexpr int KC = M == 64 ? 2 : 1;
-  f16x8 k[2][KC];    // block i: rows are keys 8 (r / 4) + 4 i + r % 4, so that the scores of both blocks
-                     // come out as the value product's B operand (lane group g: keys 8 g .. 8 g + 7)
-  f16x8 v[DV / 16];  // 16 value columns each, keys 8 g .. 8 g + 7
+  static constexpr int KC = M == 64 ? 2 : 1, NT = DV / 16;
+  static constexpr int kFrags = 2 * KC + NT;  // 16 bytes a lane each
+  f16x8 k[2][KC];  // block i: rows are keys 8 (r / 4) + 4 i + r % 4, so that the scores of both blocks
+                   // come out as the value product's B operand (lane group g: keys 8 g .. 8 g + 7)
+  f16x8 v[NT];     // 16 value columns each, keys 8 g .. 8 g + 7
 };
 
-// A workgroup: one (sequence, head), 16 QT query rows (ROWS: 16 QT for each
-// of its four waves), one piece of the keys. S^T = K u^T and O^T += V^T P^T on
-// v_mfma_f32_16x16x32_f16: a lane holds 8 keys of the query lane % 16 in both
-// products, so weights never leave their lane. u is an fp16 hi / lo pair of
-// the row scaled to [2^13, 2^14), the weights are hi / lo pairs too: the
-// result is as exact as fp32 sums.
+// Where a wave reads a tile's operands from.
+template <int M, int DV>
+struct CacheSource {
+  static constexpr int KC = CacheTile<M, DV>::KC, NT = CacheTile<M, DV>::NT;
+  const f16 *kbase, *vbase;  // of this head and lane, page 0
+  const int* row;            // the sequence's pages
+  int64_t kstride, vstride;  // of a page
+  int pages, lp;
+  __device__ __forceinline__ CacheSource(const CacheAttnArgs& a, const f16* codes, const f16* values,
+                                         const int* table, int b, int h, int lane)
+      : row(table + (int64_t)b * a.W), pages(a.pages), lp(a.lp) {
+    const int c16 = lane & 15, g = lane >> 4, P = 1 << a.lp;
+    kbase = codes + (int64_t)h * P * M + ((c16 >> 2) * 8 + (c16 & 3)) * M + (M == 16 ? 8 * (g & 1) : 8 * g);
+    vbase = values + (int64_t)h * P * DV + g * (DV * 8) + c16 * 8;
+    kstride = (int64_t)a.H * P * M;
+    vstride = (int64_t)a.H * P * DV;
+  }
+  __device__ __forceinline__ int page_of(int tile) const { return row[(tile * 32) >> lp]; }
+  // a page that the pool does not have: its keys are left out
+  __device__ __forceinline__ bool exists(int page) const { return (unsigned)page < (unsigned)pages; }
+  __device__ __forceinline__ int slot(int tile) const { return (tile * 32) & ((1 << lp) - 1); }
+  // operand f of the tile: k[f / KC][f % KC], then v[f - 2 KC]
+  __device__ __forceinline__ const f16* frag(int f, int tile, int page) const {
+    const int64_t pg = exists(page) ? page : 0;
+    if (f < 2 * KC) return kbase + pg * kstride + slot(tile) * M + 4 * (f / KC) * M + 32 * (f % KC);
+    return vbase + pg * vstride + slot(tile) * DV + 128 * (f - 2 * KC);
+  }
+  __device__ __forceinline__ void load(CacheTile<M, DV>& T, int tile, int page) const {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int c = 0; c < KC; ++c) T.k[i][c] = *reinterpret_cast<const f16x8*>(frag(i * KC + c, tile, page));
+#pragma unroll
+    for (int c = 0; c < NT; ++c) T.v[c] = *reinterpret_cast<const f16x8*>(frag(2 * KC + c, tile, page));
+  }
+};
+
+// 16 QT query rows of one (sequence, head) in a wave: the queries, and what
+// they have summed. S^T = K u^T and O^T += V^T P^T on v_mfma_f32_16x16x32_f16:
+// a lane holds 8 keys of the query lane % 16 in both products, so weights
+// never leave their lane. u is an fp16 hi / lo pair of the row scaled to
+// [2^13, 2^14), so scores are as exact as fp32 sums.
 //
 // The softmax reference is a maximum seen so far; it moves only when a score
 // passes it by more than 2^3, so most tiles rescale nothing. Weights are
 // 2^(s - reference + 12) <= 2^15: fp16 keeps what is 2^-36 of the largest.
-template <int M, int DV, int QT, bool ROWS>
-__global__ __launch_bounds__(256) void cache_attn_kernel(
-    CacheAttnArgs a, const f16* __restrict__ phi, const f16* __restrict__ gate_q, const f16* __restrict__ gate_k,
-    const f16* __restrict__ codes, const f16* __restrict__ values, const int* __restrict__ table,
-    const int* __restrict__ lens, const int* __restrict__ new_lens, const int64_t* __restrict__ tree,
-    f16* __restrict__ out, float* __restrict__ lse, float* __restrict__ part_o, float4* __restrict__ part_st) {
-  constexpr int KC = CacheTile<M, DV>::KC, NT = DV / 16;
-  constexpr int NU = M == 16 ? 1 : 2 * KC;  // u operands: hi and lo of 32 codes each; at M = 16 one holds both
-  constexpr int STEP = ROWS ? 1 : 4;        // tiles from one of a wave to its next
-  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int c16 = lane & 15, g = lane >> 4;
-  int id = blockIdx.x;
-  const int h = id % a.H;
-  id /= a.H;
-  const int sp = id % a.nsplit;
-  id /= a.nsplit;
-  const int qb = a.qblocks - 1 - id % a.qblocks;  // causal: the longest rows start first
-  const int b = id / a.qblocks;
-
-  const int P = 1 << a.lp;
-  const SeqLen sq = seq_len(lens, new_lens, b, a.n, a.W << a.lp);
-  const int kb = sp * a.split_keys;
-  if (sp > 0 && kb >= sq.total) return;  // not one of this sequence's pieces
-  const int q0 = qb * (ROWS ? 64 * QT : 16 * QT);
-  if (q0 >= sq.nb && a.nsplit > 1) return;  // padding rows: the joining kernel writes them
-  const int qw = q0 + (ROWS ? 16 * QT * w : 0);
-
-  // u_i, its scale and the row constant
+// LO: the weights enter the value product as hi / lo pairs, and the output is
+// exact to fp32 rounding too (where reading the keys is the bound, the second
+// product is free). Without, they are rounded to fp16 once, and the normaliser
+// sums the rounded ones (a product with ones: no VALU work).
+template <int M, int DV, int QT, bool LO>
+struct CacheRows {
+  static constexpr int KC = CacheTile<M, DV>::KC, NT = CacheTile<M, DV>::NT;
+  static constexpr int NU = M == 16 ? 1 : 2 * KC;  // u operands: hi and lo of 32 codes each; at M = 16 one holds both
   f16x8 u[QT][NU];
-  float sc[QT], rc[QT];
-  int64_t bits[QT];
-#pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    const int row = min(qw + 16 * t + c16, a.n - 1);
-    const f16* pr = phi + (((int64_t)b * a.n + row) * a.H + h) * M;
-    bits[t] = tree ? tree[(int64_t)b * a.n + row] : 0;
-    float x[KC][8], big = 0.f, r = 0.f;
-#pragma unroll
-    for (int c = 0; c < KC; ++c) {
-      const int c0 = M == 16 ? 8 * (g & 1) : 32 * c + 8 * g;
-      const f16x8 p8 = *reinterpret_cast<const f16x8*>(pr + c0);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float G = a.sl2e * ((float)gate_q[h * M + c0 + j] * (float)gate_k[h * M + c0 + j]);
-        x[c][j] = G * (2.f * (float)p8[j] - 1.f);
-        r += G * (float)p8[j];
-        big = fmaxf(big, fabsf(x[c][j]));
-      }
-    }
-    r += __shfl_xor(r, 16);
-    big = fmaxf(big, __shfl_xor(big, 16));
-    if (M != 16) {  // at M = 16 lane groups 2 and 3 hold the codes of 0 and 1 again
-      r += __shfl_xor(r, 32);
-      big = fmaxf(big, __shfl_xor(big, 32));
-    }
-    rc[t] = r;
-    const int e = big > 0.f && big < kFltMax ? max(__builtin_amdgcn_frexp_expf(big), -100) : 14;
-    sc[t] = ldexpf(1.f, e - 14);
-#pragma unroll
-    for (int c = 0; c < KC; ++c)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        f16 hi, lo;
-        split_exact(ldexpf(x[c][j], 14 - e), hi, lo);
-        if (M == 16) {
-          u[t][0][j] = g < 2 ? hi : lo;
-        } else {
-          u[t][c][j] = hi;
-          u[t][KC + c][j] = lo;
-        }
-      }
-  }
-
+  float sc[QT];   // scores = sc S, a power of two
+  float off[QT];  // 12 - reference
+  float thr[QT];  // S from which the reference moves
+  float sum[QT];  // of this lane's weights
+  f32x4 l16[QT];  // !LO: sum of all rounded weights, in every register
   f32x4 O[QT][NT];
-  float ref[QT], sum[QT];
-#pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    ref[t] = -1e30f;  // finite, so that a masked score's weight is 2^-inf
-    sum[t] = 0.f;
-#pragma unroll
-    for (int c = 0; c < NT; ++c) O[t][c] = f32x4{};
-  }
 
-  // keys below `clear` are seen by every row of the wave, none from `end` on by any
-  const int ke = sp == a.nsplit - 1 ? sq.total : min(sq.total, kb + a.split_keys);
-  int clear = sq.ctx, end = sq.total;
-  if (tree == nullptr) {
-    if (a.causal) {
-      clear = sq.ctx + qw + (a.mask_diag ? 0 : 1);
-      end = sq.ctx + min(qw + 16 * QT, sq.nb);
-    } else if (!a.mask_diag) {
-      clear = sq.total;
-    }
-  }
-  clear = min(clear, sq.total);
-  end = qw < sq.nb ? min(end, ke) : 0;
-
-  const int* row = table + (int64_t)b * a.W;
-  const f16* kbase = codes + (int64_t)h * P * M + ((c16 >> 2) * 8 + (c16 & 3)) * M + (M == 16 ? 8 * (g & 1) : 8 * g);
-  const f16* vbase = values + (int64_t)h * P * DV + g * (DV * 8) + c16 * 8;
-  const int64_t kstride = (int64_t)a.H * P * M, vstride = (int64_t)a.H * P * DV;
-  auto page_of = [&](int tile) { return row[(tile * 32) >> a.lp]; };
-  // a page that the pool does not have: its keys are left out
-  auto exists = [&](int page) { return (unsigned)page < (unsigned)a.pages; };
-  auto load = [&](CacheTile<M, DV>& T, int tile, int page) {
-    const int64_t pg = exists(page) ? page : 0;
-    const int slot = (tile * 32) & (P - 1);
-    const f16* kp = kbase + pg * kstride + slot * M;
-    const f16* vp = vbase + pg * vstride + slot * DV;
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int c = 0; c < KC; ++c) T.k[i][c] = *reinterpret_cast<const f16x8*>(kp + 4 * i * M + 32 * c);
-#pragma unroll
-    for (int c = 0; c < NT; ++c) T.v[c] = *reinterpret_cast<const f16x8*>(vp + 128 * c);
-  };
-
-  auto work = [&](CacheTile<M, DV>& T, int tile, int page, auto masked) {
-    constexpr bool MASKED = decltype(masked)::value;
-    const int key0 = tile * 32 + 8 * g;
-    bool strange = false;  // an infinity or NaN among the tile's values
-    if constexpr (MASKED) {
-#pragma unroll
-      for (int c = 0; c < NT; ++c)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const bool bad = not_finite(T.v[c][j]);
-          strange |= bad && key0 + j < sq.total;
-          if (bad || key0 + j >= sq.total) T.v[c][j] = (f16)0.f;
-        }
-      strange = __any(strange);
-    }
+  // Rows first .. first + 16 QT - 1, those from n on repeating the last; rc: the rows' constants.
+  __device__ __forceinline__ void start(const CacheAttnArgs& a, const f16* phi, const f16* gate_q, const f16* gate_k,
+                                        int b, int h, int first, int lane, float (&rc)[QT]) {
+    const int c16 = lane & 15, g = lane >> 4;
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
-      f32x4 s[2] = {f32x4{}, f32x4{}};
+      const int row = min(first + 16 * t + c16, a.n - 1);
+      const f16* pr = phi + (((int64_t)b * a.n + row) * a.H + h) * M;
+      float x[KC][8], big = 0.f, r = 0.f;
+#pragma unroll
+      for (int c = 0; c < KC; ++c) {
+        const int c0 = M == 16 ? 8 * (g & 1) : 32 * c + 8 * g;
+        const f16x8 p8 = *reinterpret_cast<const f16x8*>(pr + c0);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float G = a.sl2e * ((float)gate_q[h * M + c0 + j] * (float)gate_k[h * M + c0 + j]);
+          x[c][j] = G * (2.f * (float)p8[j] - 1.f);
+          r += G * (float)p8[j];
+          big = fmaxf(big, fabsf(x[c][j]));
+        }
+      }
+      r += __shfl_xor(r, 16);
+      big = fmaxf(big, __shfl_xor(big, 16));
+      if (M != 16) {  // at M = 16 lane groups 2 and 3 hold the codes of 0 and 1 again
+        r += __shfl_xor(r, 32);
+        big = fmaxf(big, __shfl_xor(big, 32));
+      }
+      rc[t] = r;
+      const int e = big > 0.f && big < kFltMax ? max(__builtin_amdgcn_frexp_expf(big), -100) : 14;
+      sc[t] = ldexpf(1.f, e - 14);
+#pragma unroll
+      for (int c = 0; c < KC; ++c)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          f16 hi, lo;
+          split_exact(ldexpf(x[c][j], 14 - e), hi, lo);
+          if (M == 16) {
+            u[t][0][j] = g < 2 ? hi : lo;
+          } else {
+            u[t][c][j] = hi;
+            u[t][KC + c][j] = lo;
+          }
+        }
+      off[t] = 1e30f;  // a reference below every score, finite so that a masked one's weight is 2^-inf
+      thr[t] = kNegInf;
+      sum[t] = 0.f;
+      l16[t] = f32x4{};
+#pragma unroll
+      for (int c = 0; c < NT; ++c) O[t][c] = f32x4{};
+    }
+  }
+
+  // Adds a tile. seen(t): bit j: row t of this lane sees key j of its 8; read
+  // only if MASKED. again(t, p, seen): see below.
+  template <bool MASKED, class Seen, class Again>
+  __device__ __forceinline__ void add(const CacheTile<M, DV>& T, const Seen& seen, const Again& again) {
+    f32x4 s[QT][2];
+    float top[QT];
+    bool move = false;
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
+        s[t][i] = f32x4{};
         if (M == 16) {
-          s[i] = mfma16x16(T.k[i][0], u[t][0], s[i]);
+          s[t][i] = mfma16x16(T.k[i][0], u[t][0], s[t][i]);
         } else {
 #pragma unroll
           for (int c = 0; c < KC; ++c) {
-            s[i] = mfma16x16(T.k[i][c], u[t][c], s[i]);
-            s[i] = mfma16x16(T.k[i][c], u[t][KC + c], s[i]);
+            s[t][i] = mfma16x16(T.k[i][c], u[t][c], s[t][i]);
+            s[t][i] = mfma16x16(T.k[i][c], u[t][KC + c], s[t][i]);
           }
         }
       }
-      float x[8];
-      unsigned seen = 0xff;
+    }
+    unsigned vis[QT];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = s[j >> 2][j & 3] * sc[t];
+    for (int t = 0; t < QT; ++t) {
       if constexpr (MASKED) {
-        const int i = qw + 16 * t + c16;
-        seen = 0;
+        vis[t] = seen(t);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int k = key0 + j, d = k - sq.ctx;  // d: which of the new tokens
-          bool v = k < sq.total && i < sq.nb;
-          if (tree)
-            v = v && (d < 0 || ((bits[t] >> min(max(d, 0), 63)) & 1));
-          else
-            v = v && (!a.causal || d <= i) && !(a.mask_diag && d == i);
-          seen |= v ? 1u << j : 0u;
-          x[j] = v ? x[j] : kNegInf;
-        }
+        for (int j = 0; j < 8; ++j) s[t][j >> 2][j & 3] = (vis[t] >> j) & 1 ? s[t][j >> 2][j & 3] : kNegInf;
       }
-      float top = x[0];
+      top[t] = s[t][0][0];
 #pragma unroll
-      for (int j = 1; j < 8; ++j) top = fmaxf(top, x[j]);
-      if (__any(top > ref[t] + 3.f)) {
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
-        const float nr = fmaxf(ref[t], top), f = fast_exp2(ref[t] - nr);
-        ref[t] = nr;
+      for (int j = 1; j < 8; ++j) top[t] = fmaxf(top[t], s[t][j >> 2][j & 3]);
+      move |= top[t] > thr[t];
+    }
+    if (__any(move)) {
+#pragma unroll
+      for (int t = 0; t < QT; ++t) {
+        float m = fmaxf(top[t], __shfl_xor(top[t], 16));
+        m = fmaxf(m, __shfl_xor(m, 32)) * sc[t];
+        const float ref = 12.f - off[t], nr = fmaxf(ref, m), f = fast_exp2(ref - nr);
+        off[t] = 12.f - nr;
+        thr[t] = nr > -1e29f ? (nr + 3.f) / sc[t] : kNegInf;
         sum[t] *= f;
+        l16[t] *= f;
 #pragma unroll
         for (int c = 0; c < NT; ++c) O[t][c] *= f;
       }
+    }
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
       f16x8 hi, lo;
       float p[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        p[j] = fast_exp2(x[j] + (12.f - ref[t]));
+        p[j] = fast_exp2(fmaf(s[t][j >> 2][j & 3], sc[t], off[t]));
         sum[t] += p[j];
-        f16 ph, pl;
-        split_exact(p[j], ph, pl);
-        hi[j] = ph;
-        lo[j] = pl;
+        if constexpr (LO) {
+          f16 ph, pl;
+          split_exact(p[j], ph, pl);
+          hi[j] = ph;
+          lo[j] = pl;
+        } else {
+          hi[j] = (f16)p[j];
+        }
+      }
+      if constexpr (!LO) {
+        const f16 one = (f16)1.f;
+        l16[t] = mfma16x16(f16x8{one, one, one, one, one, one, one, one}, hi, l16[t]);
       }
 #pragma unroll
       for (int c = 0; c < NT; ++c) {
         O[t][c] = mfma16x16(T.v[c], hi, O[t][c]);
-        O[t][c] = mfma16x16(T.v[c], lo, O[t][c]);
+        if constexpr (LO) O[t][c] = mfma16x16(T.v[c], lo, O[t][c]);
       }
-      if constexpr (MASKED) {
-        if (strange) {
-          // Such values reach only the rows that see their key: 0 times an
-          // infinity would be NaN in every row of the product above.
-          const f16* vt = values + (int64_t)h * P * DV + page * vstride + ((tile * 32) & (P - 1)) * DV + g * 32;
-#pragma unroll 1
-          for (int k = 0; k < 32; ++k) {
-            const int from = 16 * (k >> 3) + c16;
-            float pk = p[0];
-#pragma unroll
-            for (int j = 1; j < 8; ++j) pk = (k & 7) == j ? p[j] : pk;
-            pk = __shfl(pk, from);
-            const bool sees = (__shfl((int)seen, from) >> (k & 7)) & 1;
-#pragma unroll
-            for (int c = 0; c < NT; ++c)
-#pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                const f16 vb = vt[(k >> 3) * DV * 8 + 128 * c + 8 * r + (k & 7)];
-                O[t][c][r] += sees && not_finite(vb) ? pk * (float)vb : 0.f;
-              }
-          }
-        }
-      }
+      if constexpr (MASKED) again(t, p, vis[t]);
     }
-  };
+  }
 
-  int tile = kb / 32 + (ROWS ? 0 : w);
+  // After the last tile: the reference, the sum of the weights for the
+  // log-sum-exp and the one that the output is divided by.
+  __device__ __forceinline__ void finish(int t, float& ref, float& l, float& div) {
+    ref = 12.f - off[t];
+    l = sum[t] + __shfl_xor(sum[t], 16);  // the lane groups hold their own keys of the same 16 queries
+    l += __shfl_xor(l, 32);
+    div = LO ? l : l16[t][0];
+  }
+};
+
+// What a wave's rows see of a tile near or past the end of what all see.
+struct CacheMask {
+  int ctx, nb, total, causal, mask_diag;
+  bool tree;
+  // row i (of the new tokens; bits: its drafts), keys key0 .. key0 + 7
+  __device__ __forceinline__ unsigned operator()(int i, int64_t bits, int key0) const {
+    unsigned seen = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int k = key0 + j, d = k - ctx;  // d: which of the new tokens
+      bool v = k < total && i < nb;
+      if (tree)
+        v = v && (d < 0 || ((bits >> min(max(d, 0), 63)) & 1));
+      else
+        v = v && (!causal || d <= i) && !(mask_diag && d == i);
+      seen |= v ? 1u << j : 0u;
+    }
+    return seen;
+  }
+};
+
+// A tile that some row does not see all of. A place behind the last key may
+// hold anything, and 0 times an infinity or a NaN is NaN in every row of the
+// value product: such values are taken out of it and added by themselves, to
+// the rows that see their key.
+template <int M, int DV, int QT, bool LO>
+__device__ __forceinline__ void add_masked(CacheRows<M, DV, QT, LO>& R, CacheTile<M, DV>& T,
+                                           const CacheSource<M, DV>& src, const CacheMask& mask, int first,
+                                           const int64_t (&bits)[QT], int tile, int page, int lane) {
+  constexpr int NT = CacheTile<M, DV>::NT;
+  const int c16 = lane & 15, g = lane >> 4, key0 = tile * 32 + 8 * g;
+  bool strange = false;
+#pragma unroll
+  for (int c = 0; c < NT; ++c)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const bool bad = not_finite(T.v[c][j]);
+      strange |= bad && key0 + j < mask.total;
+      if (bad || key0 + j >= mask.total) T.v[c][j] = (f16)0.f;
+    }
+  const bool any = __any(strange);
+  R.template add<true>(
+      T, [&](int t) { return mask(first + 16 * t + c16, bits[t], key0); },
+      [&](int t, const float(&p)[8], unsigned seen) {
+        if (!any) return;
+        // column 16 c + 4 g + r of key k
+        const f16* v = src.vbase - (g * (DV * 8) + c16 * 8) + page * src.vstride + src.slot(tile) * DV + g * 32;
+#pragma unroll 1
+        for (int k = 0; k < 32; ++k) {
+          const int from = 16 * (k >> 3) + c16;
+          float pk = p[0];
+#pragma unroll
+          for (int j = 1; j < 8; ++j) pk = (k & 7) == j ? p[j] : pk;
+          pk = __shfl(pk, from);
+          const bool sees = (__shfl((int)seen, from) >> (k & 7)) & 1;
+#pragma unroll
+          for (int c = 0; c < NT; ++c)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const f16 x = v[(k >> 3) * DV * 8 + 128 * c + 8 * r + (k & 7)];
+              R.O[t][c][r] += sees && not_finite(x) ? pk * (float)x : 0.f;
+            }
+        }
+      });
+}
+
+// Writes 4 columns from c on of a row: the result, or one piece's part of it.
+template <int DV>
+struct CacheOut {
+  f16* out;
+  float* lse;
+  float* part_o;
+  float4* part_st;
+  int n, H, b, h, nb, nsplit, sp;
+  // m, l: reference and sum of the weights; div: what the output is divided by; r: the row constant
+  __device__ __forceinline__ void operator()(int i, int c, f32x4 o, float m, float l, float div, float r) const {
+    if (i >= n) return;
+    const int64_t at = ((int64_t)b * H + h) * n + i;
+    if (nsplit > 1) {
+      if (i >= nb) return;  // the joining kernel writes padding rows
+      *reinterpret_cast<f32x4*>(part_o + (at * nsplit + sp) * DV + c) = o;
+      if (c == 0) part_st[at * nsplit + sp] = float4{m, l, div, r};
+      return;
+    }
+    const bool some = i < nb && l != 0.f;  // padding rows and rows that see nothing get 0
+    const float inv = some ? 1.f / div : 0.f;
+    f16x4 y;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) y[k] = some ? (f16)(o[k] * inv) : (f16)0.f;
+    *reinterpret_cast<f16x4*>(out + (((int64_t)b * n + i) * H + h) * DV + c) = y;
+    if (c == 0) lse[at] = some ? m - 12.f + __log2f(l) - r : -kFltMax;
+  }
+};
+
+// What a workgroup works on: heads fastest (a page's heads are neighbours in
+// memory, and with a multiple of 8 heads all row blocks of a head share an
+// XCD's L2), then pieces, then row blocks from the last (under a causal mask
+// the longest), then sequences.
+struct CacheBlock {
+  int b, h, sp, qb;
+  __device__ __forceinline__ explicit CacheBlock(const CacheAttnArgs& a) {
+    int id = blockIdx.x;
+    h = id % a.H;
+    id /= a.H;
+    sp = id % a.nsplit;
+    id /= a.nsplit;
+    qb = a.qblocks - 1 - id % a.qblocks;
+    b = id / a.qblocks;
+  }
+};
+
+// Up to 16 rows: the four waves of a workgroup share them and take every
+// fourth tile of the piece's keys, straight into registers, one tile ahead.
+template <int M, int DV>
+__global__ __launch_bounds__(256) void cache_attn_few_kernel(
+    CacheAttnArgs a, const f16* __restrict__ phi, const f16* __restrict__ gate_q, const f16* __restrict__ gate_k,
+    const f16* __restrict__ codes, const f16* __restrict__ values, const int* __restrict__ table,
+    const int* __restrict__ lens, const int* __restrict__ new_lens, const int64_t* __restrict__ tree,
+    f16* __restrict__ out, float* __restrict__ lse, float* __restrict__ part_o, float4* __restrict__ part_st) {
+  constexpr int NT = DV / 16;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c16 = lane & 15, g = lane >> 4;
+  const CacheBlock blk(a);
+  const int b = blk.b, h = blk.h;
+  const SeqLen sq = seq_len(lens, new_lens, b, a.n, a.W << a.lp);
+  const int kb = blk.sp * a.split_keys;
+  if (blk.sp > 0 && kb >= sq.total) return;  // not one of this sequence's pieces
+  if (sq.nb == 0 && a.nsplit > 1) return;    // padding: the joining kernel writes it
+
+  CacheRows<M, DV, 1, true> R;
+  float rc[1];
+  R.start(a, phi, gate_q, gate_k, b, h, 0, lane, rc);
+  const int64_t bits[1] = {tree ? tree[(int64_t)b * a.n + min(c16, a.n - 1)] : 0};
+
+  // keys below `clear` are seen by every row, none from `end` on by any
+  const int ke = blk.sp == a.nsplit - 1 ? sq.total : min(sq.total, kb + a.split_keys);
+  const bool chunk = tree == nullptr;
+  int clear = chunk ? (a.causal ? sq.ctx + (a.mask_diag ? 0 : 1) : a.mask_diag ? sq.ctx : sq.total) : sq.ctx;
+  clear = min(clear, sq.total);
+  const int end = sq.nb > 0 ? ke : 0;
+  const CacheMask mask{sq.ctx, sq.nb, sq.total, a.causal, a.mask_diag, !chunk};
+  const CacheSource<M, DV> src(a, codes, values, table, b, h, lane);
+
+  int tile = kb / 32 + w;
   if (tile * 32 < end) {
     CacheTile<M, DV> A, B;
-    int pa = page_of(tile), pb = 0;
-    load(A, tile, pa);
-    if ((tile + STEP) * 32 < end) pb = page_of(tile + STEP);
+    int pa = src.page_of(tile), pb = 0;
+    src.load(A, tile, pa);
+    if ((tile + 4) * 32 < end) pb = src.page_of(tile + 4);
     auto step = [&](CacheTile<M, DV>& cur, CacheTile<M, DV>& nxt, int& pc, int& pn) {
-      const bool more = (tile + STEP) * 32 < end;
-      if (more) load(nxt, tile + STEP, pn);
+      const bool more = (tile + 4) * 32 < end;
+      if (more) src.load(nxt, tile + 4, pn);
       int after = 0;
-      if ((tile + 2 * STEP) * 32 < end) after = page_of(tile + 2 * STEP);
-      if (exists(pc)) {
+      if ((tile + 8) * 32 < end) after = src.page_of(tile + 8);
+      if (src.exists(pc)) {
         if (tile * 32 + 32 <= clear)
-          work(cur, tile, pc, std::false_type());
+          R.template add<false>(cur, [](int) { return 0u; }, [](int, const float(&)[8], unsigned) {});
         else
-          work(cur, tile, pc, std::true_type());
+          add_masked(R, cur, src, mask, 0, bits, tile, pc, lane);
       }
       pc = after;
-      tile += STEP;
+      tile += 4;
       return more;
     };
     while (step(A, B, pa, pb) && step(B, A, pb, pa)) {
     }
   }
 
-  // join the lane groups (each holds its own keys of the same 16 queries)
+  __shared__ __align__(16) float so[4][16][DV + 4];
+  __shared__ float sm[4][16], sl[4][16], sr[16];
+  float ref, l, div;
+  R.finish(0, ref, l, div);
 #pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    sum[t] += __shfl_xor(sum[t], 16);
-    sum[t] += __shfl_xor(sum[t], 32);
+  for (int c = 0; c < NT; ++c) *reinterpret_cast<f32x4*>(&so[w][c16][16 * c + 4 * g]) = R.O[0][c];
+  if (g == 0) {
+    sm[w][c16] = ref;
+    sl[w][c16] = l;
+    if (w == 0) sr[c16] = rc[0];
   }
-  const int64_t orow = (int64_t)b * a.n;
-  // writes a row's 4 columns from c on: the result, or this piece's part
-  auto put = [&](int i, int c, f32x4 o, float m, float l, float r) {
-    if (i >= a.n) return;
-    if (a.nsplit > 1) {
-      if (i >= sq.nb) return;
-      const int64_t at = (((int64_t)b * a.H + h) * a.n + i) * a.nsplit + sp;
-      *reinterpret_cast<f32x4*>(part_o + at * DV + c) = o;
-      if (c == 0) part_st[at] = float4{m, l, r, 0.f};
-      return;
+  __syncthreads();
+  const CacheOut<DV> put{out, lse, part_o, part_st, a.n, a.H, b, h, sq.nb, a.nsplit, blk.sp};
+  for (int e = threadIdx.x; e < 4 * DV; e += 256) {
+    const int q = e / (DV / 4), c = 4 * (e % (DV / 4));
+    if (q >= a.n) break;
+    float m = sm[0][q];
+#pragma unroll
+    for (int k = 1; k < 4; ++k) m = fmaxf(m, sm[k][q]);
+    l = 0.f;
+    f32x4 o = {};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float f = fast_exp2(sm[k][q] - m);
+      l += f * sl[k][q];
+      o += f * *reinterpret_cast<const f32x4*>(&so[k][q][c]);
     }
-    const bool some = i < sq.nb && l != 0.f;  // padding rows and rows that see nothing get 0
-    const float inv = some ? 1.f / l : 0.f;
-    f16x4 y;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) y[k] = some ? (f16)(o[k] * inv) : (f16)0.f;
-    *reinterpret_cast<f16x4*>(out + ((orow + i) * a.H + h) * DV + c) = y;
-    if (c == 0) lse[((int64_t)b * a.H + h) * a.n + i] = some ? m - 12.f + __log2f(l) - r : -kFltMax;
-  };
-  if constexpr (ROWS) {
-#pragma unroll
-    for (int t = 0; t < QT; ++t)
-#pragma unroll
-      for (int c = 0; c < NT; ++c) put(qw + 16 * t + c16, 16 * c + 4 * g, O[t][c], ref[t], sum[t], rc[t]);
-  } else {
-    __shared__ __align__(16) float so[4][16][DV + 4];
-    __shared__ float sm[4][16], sl[4][16], sr[16];
-#pragma unroll
-    for (int t = 0; t < QT; ++t) {
-      if (t) __syncthreads();
-#pragma unroll
-      for (int c = 0; c < NT; ++c) *reinterpret_cast<f32x4*>(&so[w][c16][16 * c + 4 * g]) = O[t][c];
-      if (g == 0) {
-        sm[w][c16] = ref[t];
-        sl[w][c16] = sum[t];
-        if (w == 0) sr[c16] = rc[t];
-      }
-      __syncthreads();
-      for (int e = threadIdx.x; e < 4 * DV; e += 256) {
-        const int q = e / (DV / 4), c = 4 * (e % (DV / 4));
-        float m = sm[0][q];
-#pragma unroll
-        for (int k = 1; k < 4; ++k) m = fmaxf(m, sm[k][q]);
-        float l = 0.f;
-        f32x4 o = {};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float f = fast_exp2(sm[k][q] - m);
-          l += f * sl[k][q];
-          o += f * *reinterpret_cast<const f32x4*>(&so[k][q][c]);
-        }
-        put(q0 + 16 * t + q, c, o, m, l, sr[q]);
-      }
-    }
+    put(q, c, o, m, l, l, sr[q]);
   }
 }
 
-// Joins the pieces of a row: one workgroup a (sequence, head, row), its lanes
-// in groups of DV / 4, group k taking pieces k, k + groups, ... in order, then
-// the groups in order.
-template <int DV>
-__global__ __launch_bounds__(256) void cache_join_kernel(CacheAttnArgs a, const int* __restrict__ lens,
+// More rows: each of the four waves of a workgroup has 16 QT of its own, and
+// the keys pass through LDS, 64 a stage and three stages, filled by DMA in the
+// order in which the lanes read them as operands (a wave fetches every fourth
+// operand; 1 KiB each, conflict-free both ways).
+template <int M, int DV, int QT>
+__global__ __launch_bounds__(256, 2) void cache_attn_rows_kernel(
+    CacheAttnArgs a, const f16* __restrict__ phi, const f16* __restrict__ gate_q, const f16* __restrict__ gate_k,
+    const f16* __restrict__ codes, const f16* __restrict__ values, const int* __restrict__ table,
+    const int* __restrict__ lens, const int* __restrict__ new_lens, const int64_t* __restrict__ tree,
+    f16* __restrict__ out, float* __restrict__ lse, float* __restrict__ part_o, float4* __restrict__ part_st) {
+  constexpr bool LO = QT == 1;
+  constexpr int NT = DV / 16, NF = CacheTile<M, DV>::kFrags, PER = NF / 2;  // DMA pieces of a wave and stage
+  static_assert(NF % 2 == 0, "a stage's operands divide evenly among four waves");
+  __shared__ __align__(1024) char lds[3][2 * NF * 1024];
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c16 = lane & 15, g = lane >> 4;
+  const CacheBlock blk(a);
+  const int b = blk.b, h = blk.h, q0 = blk.qb * 64 * QT, qw = q0 + 16 * QT * w;
+  const SeqLen sq = seq_len(lens, new_lens, b, a.n, a.W << a.lp);
+  const int kb = blk.sp * a.split_keys;
+  if (blk.sp > 0 && kb >= sq.total) return;
+  if (q0 >= sq.nb && a.nsplit > 1) return;
+
+  CacheRows<M, DV, QT, LO> R;
+  float rc[QT];
+  R.start(a, phi, gate_q, gate_k, b, h, qw, lane, rc);
+  int64_t bits[QT];
+#pragma unroll
+  for (int t = 0; t < QT; ++t)
+    bits[t] = tree ? tree[(int64_t)b * a.n + min(qw + 16 * t + c16, a.n - 1)] : 0;
+
+  const int ke = blk.sp == a.nsplit - 1 ? sq.total : min(sq.total, kb + a.split_keys);
+  // what the rows from `first` on, `count` of them, see: all of them the keys
+  // below clear, none a key from end on
+  const bool chunk = tree == nullptr;
+  auto clear_of = [&](int first) {
+    const int c = chunk ? (a.causal ? sq.ctx + first + (a.mask_diag ? 0 : 1) : a.mask_diag ? sq.ctx : sq.total) : sq.ctx;
+    return min(c, sq.total);
+  };
+  auto end_of = [&](int first, int count) {
+    const int e = chunk && a.causal ? sq.ctx + min(first + count, sq.nb) : sq.total;
+    return first < sq.nb ? min(e, ke) : 0;
+  };
+  const int clear = clear_of(qw), end = end_of(qw, 16 * QT), endw = end_of(q0, 64 * QT);  // endw: of the workgroup
+  const CacheMask mask{sq.ctx, sq.nb, sq.total, a.causal, a.mask_diag, !chunk};
+  const CacheSource<M, DV> src(a, codes, values, table, b, h, lane);
+  const unsigned base = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+
+  const int tile0 = kb / 32, tiles = endw > kb ? (endw - kb + 31) / 32 : 0, stages = (tiles + 1) / 2;
+  auto page = [&](int st, int i) { return src.page_of(tile0 + min(2 * st + i, tiles - 1)); };
+  auto issue = [&](int st, int p0, int p1) {
+    const unsigned to = base + (unsigned)(st % 3) * (2 * NF * 1024);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int f = w + 4 * i;  // of the stage's 2 NF
+      const bool second = f >= NF;
+      const int tile = tile0 + min(2 * st + (second ? 1 : 0), tiles - 1);
+      lds_dma16(src.frag(second ? f - NF : f, tile, second ? p1 : p0), to + 1024u * (unsigned)f);
+    }
+  };
+  int pg[3][2];
+#pragma unroll
+  for (int st = 0; st < 2; ++st)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) pg[st][i] = st < stages ? page(st, i) : -1;
+  pg[2][0] = pg[2][1] = -1;
+  if (stages > 0) issue(0, pg[0][0], pg[0][1]);
+  if (stages > 1) issue(1, pg[1][0], pg[1][1]);
+  for (int st = 0; st < stages; ++st) {
+    // this wave's part of the stage has landed (the next stage's may not have)
+    if (st + 1 < stages)
+      wait_vmcnt_lgkm0<PER>();
+    else
+      wait_vmcnt_lgkm0<0>();
+    asm volatile("s_barrier" ::: "memory");  // ... and every wave's; the stage before is free
+    if (st + 2 < stages) {
+      pg[2][0] = page(st + 2, 0);
+      pg[2][1] = page(st + 2, 1);
+      issue(st + 2, pg[2][0], pg[2][1]);
+    }
+    const char* from = lds[st % 3] + 16 * lane;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int tile = tile0 + 2 * st + i;
+      if (tile * 32 >= end || !src.exists(pg[0][i])) continue;  // uniform in the wave
+      CacheTile<M, DV> T;
+      auto at = [&](int f) { return *reinterpret_cast<const f16x8*>(from + 1024 * (NF * i + f)); };
+#pragma unroll
+      for (int f = 0; f < NF - NT; ++f) T.k[f / T.KC][f % T.KC] = at(f);
+#pragma unroll
+      for (int c = 0; c < NT; ++c) T.v[c] = at(NF - NT + c);
+      if (tile * 32 + 32 <= clear)
+        R.template add<false>(T, [](int) { return 0u; }, [](int, const float(&)[8], unsigned) {});
+      else
+        add_masked(R, T, src, mask, qw, bits, tile, pg[0][i], lane);
+    }
+    pg[0][0] = pg[1][0];
+    pg[0][1] = pg[1][1];
+    pg[1][0] = pg[2][0];
+    pg[1][1] = pg[2][1];
+  }
+  const CacheOut<DV> put{out, lse, part_o, part_st, a.n, a.H, b, h, sq.nb, a.nsplit, blk.sp};
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    float ref, l, div;
+    R.finish(t, ref, l, div);
+#pragma unroll
+    for (int c = 0; c < NT; ++c) put(qw + 16 * t + c16, 16 * c + 4 * g, R.O[t][c], ref, l, div, rc[t]);
+  }
+}
+
+// Joins the pieces of the rows: DV / 4 lanes hold a row's columns, NG such
+// groups take its pieces in turn, and the groups are added in order.
+template <int DV, int NG>
+__global__ __launch_bounds__(256) void cache_join_kernel(CacheAttnArgs a, int64_t rows, const int* __restrict__ lens,
                                                         const int* __restrict__ new_lens,
                                                         const float* __restrict__ part_o,
                                                         const float4* __restrict__ part_st, f16* __restrict__ out,
                                                         float* __restrict__ lse) {
-  constexpr int TC = DV / 4, NG = 256 / TC;
-  const int64_t at = blockIdx.x;  // (b H + h) n + i
+  constexpr int TC = DV / 4, ROWS = 256 / (TC * NG);
+  const int k = threadIdx.x / TC % NG, c = 4 * (threadIdx.x % TC), rl = threadIdx.x / (TC * NG);
+  const int64_t at = (int64_t)blockIdx.x * ROWS + rl;  // (b H + h) n + i
   const int i = (int)(at % a.n);
   const int64_t bh = at / a.n;
-  const int h = (int)(bh % a.H), b = (int)(bh / a.H);
+  const int h = (int)(bh % a.H), b = (int)min(bh / a.H, rows / ((int64_t)a.n * a.H) - 1);
   const SeqLen sq = seq_len(lens, new_lens, b, a.n, a.W << a.lp);
-  const int pieces = i < sq.nb ? min(a.nsplit, (sq.total + a.split_keys - 1) / a.split_keys) : 0;
-  const int k = threadIdx.x / TC, c = 4 * (threadIdx.x % TC);
-  float m = -1e30f, l = 0.f;
+  const int pieces =
+      at < rows && i < sq.nb ? min(a.nsplit, (sq.total + a.split_keys - 1) / a.split_keys) : 0;
+  float m = -1e30f, l = 0.f, div = 0.f, r = 0.f;
   f32x4 o = {};
   for (int s = k; s < pieces; s += NG) {
     const float4 st = part_st[at * a.nsplit + s];
     const f32x4 x = *reinterpret_cast<const f32x4*>(part_o + (at * a.nsplit + s) * DV + c);
     const float nm = fmaxf(m, st.x), f = fast_exp2(m - nm), fs = fast_exp2(st.x - nm);
     l = l * f + st.y * fs;
+    div = div * f + st.z * fs;
     o = o * f + x * fs;
+    r = st.w;  // the same in every piece
     m = nm;
   }
-  __shared__ __align__(16) float so[NG][DV];
-  __shared__ float sm[NG], sl[NG];
-  *reinterpret_cast<f32x4*>(&so[k][c]) = o;
-  if (c == 0) {
-    sm[k] = m;
-    sl[k] = l;
+  if constexpr (NG > 1) {
+    __shared__ __align__(16) float so[ROWS][NG][DV];
+    __shared__ float4 ss[ROWS][NG];
+    *reinterpret_cast<f32x4*>(&so[rl][k][c]) = o;
+    if (c == 0) ss[rl][k] = float4{m, l, div, 0.f};
+    __syncthreads();
+    if (k != 0) return;
+#pragma unroll
+    for (int e = 1; e < NG; ++e) m = fmaxf(m, ss[rl][e].x);
+    l = div = 0.f;
+    o = f32x4{};
+#pragma unroll
+    for (int e = 0; e < NG; ++e) {
+      const float4 st = ss[rl][e];
+      const float f = fast_exp2(st.x - m);
+      l += f * st.y;
+      div += f * st.z;
+      o += f * *reinterpret_cast<const f32x4*>(&so[rl][e][c]);
+    }
   }
-  __syncthreads();
-  if (k != 0) return;
-#pragma unroll
-  for (int e = 1; e < NG; ++e) m = fmaxf(m, sm[e]);
-  l = 0.f;
-  o = f32x4{};
-#pragma unroll
-  for (int e = 0; e < NG; ++e) {
-    const float f = fast_exp2(sm[e] - m);
-    l += f * sl[e];
-    o += f * *reinterpret_cast<const f32x4*>(&so[e][c]);
-  }
-  const bool some = l != 0.f;
-  const float inv = some ? 1.f / l : 0.f;
-  f16x4 y;
-#pragma unroll
-  for (int r = 0; r < 4; ++r) y[r] = some ? (f16)(o[r] * inv) : (f16)0.f;
-  *reinterpret_cast<f16x4*>(out + (((int64_t)b * a.n + i) * a.H + h) * DV + c) = y;
-  if (c == 0) lse[at] = some ? m - 12.f + __log2f(l) - part_st[at * a.nsplit].z : -kFltMax;
+  if (at >= rows) return;
+  const CacheOut<DV> put{out, lse, nullptr, nullptr, a.n, a.H, b, h, sq.nb, 1, 0};
+  put(i, c, o, m, l, div, r);
 }
 
 namespace {
@@ -456,17 +652,15 @@ hipError_t launch_cache_attn_t(const CacheDims& d, const CacheAttnPlan& p, const
                                const int* table, const int* lens, const int* new_lens, const int64_t* tree, f16* out,
                                float* lse, const CacheAttnBuffers& part, hipStream_t s) {
   const dim3 grid((unsigned)((int64_t)d.B * d.H * p.qblocks * p.nsplit)), block(256);
-#define MORPHO_CACHE_ATTN(QT, ROWS)                                                                              \
-  MORPHO_KLAUNCH((cache_attn_kernel<M, DV, QT, ROWS>), grid, block, 0, s, a, phi, gate_q, gate_k, codes, values, \
-                 table, lens, new_lens, tree, out, lse, part.o, part.st)
-  if (p.rows)
-    MORPHO_CACHE_ATTN(4, true);
+#define MORPHO_CACHE_ATTN(...)                                                                                     \
+  MORPHO_KLAUNCH((__VA_ARGS__), grid, block, 0, s, a, phi, gate_q, gate_k, codes, values, table, lens, new_lens, \
+                 tree, out, lse, part.o, part.st)
+  if (p.qt == 0)
+    MORPHO_CACHE_ATTN(cache_attn_few_kernel<M, DV>);
   else if (p.qt == 1)
-    MORPHO_CACHE_ATTN(1, false);
-  else if (p.qt == 2)
-    MORPHO_CACHE_ATTN(2, false);
+    MORPHO_CACHE_ATTN(cache_attn_rows_kernel<M, DV, 1>);
   else
-    MORPHO_CACHE_ATTN(4, false);
+    MORPHO_CACHE_ATTN(cache_attn_rows_kernel<M, DV, 2>);
 #undef MORPHO_CACHE_ATTN
   return hipGetLastError();
 }
@@ -487,13 +681,25 @@ hipError_t launch_cache_attn(const CacheDims& d, const CacheAttnPlan& plan, cons
 hipError_t launch_cache_attn_join(const CacheDims& d, const CacheAttnPlan& plan, const int* lens, const int* new_lens,
                                   const CacheAttnBuffers& part, f16* out, float* lse, hipStream_t s) {
   const CacheAttnArgs a = attn_args(d, plan);
-  const dim3 grid((unsigned)((int64_t)d.B * d.H * d.n)), block(256);
-  if (d.DV == 32)
-    MORPHO_KLAUNCH((cache_join_kernel<32>), grid, block, 0, s, a, lens, new_lens, part.o, part.st, out, lse);
+  const int64_t rows = (int64_t)d.B * d.H * d.n;
+  // few pieces: one group a row, its loads all independent; many: groups that share them
+#define MORPHO_CACHE_JOIN(DV, NG)                                                                            \
+  MORPHO_KLAUNCH((cache_join_kernel<DV, NG>), dim3((unsigned)((rows * (DV / 4) * NG + 255) / 256)), dim3(256), 0, s, \
+                 a, rows, lens, new_lens, part.o, part.st, out, lse)
+  const bool many = plan.nsplit > 8;
+  if (d.DV == 32 && many)
+    MORPHO_CACHE_JOIN(32, 32);
+  else if (d.DV == 32)
+    MORPHO_CACHE_JOIN(32, 1);
+  else if (d.DV == 64 && many)
+    MORPHO_CACHE_JOIN(64, 16);
   else if (d.DV == 64)
-    MORPHO_KLAUNCH((cache_join_kernel<64>), grid, block, 0, s, a, lens, new_lens, part.o, part.st, out, lse);
+    MORPHO_CACHE_JOIN(64, 1);
+  else if (many)
+    MORPHO_CACHE_JOIN(128, 8);
   else
-    MORPHO_KLAUNCH((cache_join_kernel<128>), grid, block, 0, s, a, lens, new_lens, part.o, part.st, out, lse);
+    MORPHO_CACHE_JOIN(128, 1);
+#undef MORPHO_CACHE_JOIN
   return hipGetLastError();
 }
 
