@@ -314,9 +314,23 @@ inline CacheAttnPlan cache_attn_plan(int B, int H, int n, int64_t max_len) {
   CacheAttnPlan p;
   p.qt = n <= 16 ? 0 : n <= 64 ? 1 : 2;
   p.qblocks = p.qt ? (n + 64 * p.qt - 1) / (64 * p.qt) : 1;
-  const int64_t wgs = (int64_t)B * H * p.qblocks, most = p.qt == 2 ? 512 : 1024;
-  int64_t keys = (max_len * wgs + most - 1) / most;
-  keys = keys < 512 ? 512 : (keys + 127) / 128 * 128;
+  const int64_t wgs = (int64_t)B * H * p.qblocks;
+  // Short pieces balance sequences of different lengths and fill the chip with
+  // few of them; each costs a partial result. B64 n1 H16, 1 to 8191 tokens, us
+  // with the join: one piece 58, of 2048 48, 1024 44, 512 42, 256 56; B1 n1 H16
+  // m32, 131071 tokens: of 512 84, 2048 79, 4096 75; trees of 48, B16 H32 m64,
+  // 300 to 4000 tokens: of 2048 70, 512 54, 256 76. From 128 rows a workgroup on, the partial results
+  // cost more than they gain once every CU has two workgroups (B4 n1000 H16
+  // m16 over 4096: of 1024 174, one piece 162).
+  int64_t keys;
+  if (p.qt < 2) {
+    keys = (max_len + 63) / 64;
+    if (keys < (wgs < 1024 ? 512 : 1024)) keys = wgs < 1024 ? 512 : 1024;
+  } else {
+    keys = (max_len * wgs + 511) / 512;
+    if (keys < 512) keys = 512;
+  }
+  keys = (keys + 127) / 128 * 128;
   p.nsplit = (int)((max_len + keys - 1) / keys);
   if (p.nsplit < 1) p.nsplit = 1;
   p.split_keys = (int)keys;

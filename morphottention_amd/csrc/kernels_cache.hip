@@ -177,40 +177,44 @@ struct CacheRows {
     }
   }
 
-  // Adds a tile. seen(t): bit j: row t of this lane sees key j of its 8; read
-  // only if MASKED. again(t, p, seen): see below.
-  template <bool MASKED, class Seen, class Again>
-  __device__ __forceinline__ void add(const CacheTile<M, DV>& T, const Seen& seen, const Again& again) {
-    f32x4 s[QT][2];
+  // Adds NK tiles. seen(t): bit j: row t of this lane sees key j of its 8; read
+  // only if MASKED. again(t, p, seen): called with the weights if MASKED.
+  template <bool MASKED, int NK, class Seen, class Again>
+  __device__ __forceinline__ void add(const CacheTile<M, DV> (&T)[NK], const Seen& seen, const Again& again) {
+    static_assert(!MASKED || NK == 1, "one masked tile at a time");
+    f32x4 s[NK][QT][2];
     float top[QT];
     bool move = false;
 #pragma unroll
-    for (int t = 0; t < QT; ++t) {
+    for (int n = 0; n < NK; ++n)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        s[t][i] = f32x4{};
-        if (M == 16) {
-          s[t][i] = mfma16x16(T.k[i][0], u[t][0], s[t][i]);
-        } else {
+      for (int t = 0; t < QT; ++t)
 #pragma unroll
-          for (int c = 0; c < KC; ++c) {
-            s[t][i] = mfma16x16(T.k[i][c], u[t][c], s[t][i]);
-            s[t][i] = mfma16x16(T.k[i][c], u[t][KC + c], s[t][i]);
+        for (int i = 0; i < 2; ++i) {
+          s[n][t][i] = f32x4{};
+          if (M == 16) {
+            s[n][t][i] = mfma16x16(T[n].k[i][0], u[t][0], s[n][t][i]);
+          } else {
+#pragma unroll
+            for (int c = 0; c < KC; ++c) {
+              s[n][t][i] = mfma16x16(T[n].k[i][c], u[t][c], s[n][t][i]);
+              s[n][t][i] = mfma16x16(T[n].k[i][c], u[t][KC + c], s[n][t][i]);
+            }
           }
         }
-      }
-    }
     unsigned vis[QT];
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
       if constexpr (MASKED) {
         vis[t] = seen(t);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) s[t][j >> 2][j & 3] = (vis[t] >> j) & 1 ? s[t][j >> 2][j & 3] : kNegInf;
+        for (int j = 0; j < 8; ++j) s[0][t][j >> 2][j & 3] = (vis[t] >> j) & 1 ? s[0][t][j >> 2][j & 3] : kNegInf;
       }
-      top[t] = s[t][0][0];
+      top[t] = s[0][t][0][0];
 #pragma unroll
-      for (int j = 1; j < 8; ++j) top[t] = fmaxf(top[t], s[t][j >> 2][j & 3]);
+      for (int n = 0; n < NK; ++n)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top[t] = fmaxf(top[t], s[n][t][j >> 2][j & 3]);
       move |= top[t] > thr[t];
     }
     if (__any(move)) {
@@ -220,7 +224,8 @@ struct CacheRows {
         m = fmaxf(m, __shfl_xor(m, 32)) * sc[t];
         const float ref = 12.f - off[t], nr = fmaxf(ref, m), f = fast_exp2(ref - nr);
         off[t] = 12.f - nr;
-        thr[t] = nr > -1e29f ? (nr + 3.f) / sc[t] : kNegInf;
+        const float next = ldexpf(nr + 3.f, 1 - __builtin_amdgcn_frexp_expf(sc[t]));  // divided by sc
+        thr[t] = nr > -1e29f ? next : kNegInf;
         sum[t] *= f;
         l16[t] *= f;
 #pragma unroll
@@ -228,33 +233,40 @@ struct CacheRows {
       }
     }
 #pragma unroll
-    for (int t = 0; t < QT; ++t) {
-      f16x8 hi, lo;
-      float p[8];
+    for (int n = 0; n < NK; ++n)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        p[j] = fast_exp2(fmaf(s[t][j >> 2][j & 3], sc[t], off[t]));
-        sum[t] += p[j];
-        if constexpr (LO) {
-          f16 ph, pl;
-          split_exact(p[j], ph, pl);
-          hi[j] = ph;
-          lo[j] = pl;
-        } else {
-          hi[j] = (f16)p[j];
+      for (int t = 0; t < QT; ++t) {
+        f16x8 hi, lo;
+        float p[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          p[j] = fast_exp2(fmaf(s[n][t][j >> 2][j & 3], sc[t], off[t]));
+          sum[t] += p[j];
+          if constexpr (LO) {
+            f16 ph, pl;
+            split_exact(p[j], ph, pl);
+            hi[j] = ph;
+            lo[j] = pl;
+          } else {
+            hi[j] = (f16)p[j];
+          }
         }
-      }
-      if constexpr (!LO) {
-        const f16 one = (f16)1.f;
-        l16[t] = mfma16x16(f16x8{one, one, one, one, one, one, one, one}, hi, l16[t]);
-      }
+        if constexpr (!LO) {
+          const f16 one = (f16)1.f;
+          l16[t] = mfma16x16(f16x8{one, one, one, one, one, one, one, one}, hi, l16[t]);
+        }
 #pragma unroll
-      for (int c = 0; c < NT; ++c) {
-        O[t][c] = mfma16x16(T.v[c], hi, O[t][c]);
-        if constexpr (LO) O[t][c] = mfma16x16(T.v[c], lo, O[t][c]);
+        for (int c = 0; c < NT; ++c) {
+          O[t][c] = mfma16x16(T[n].v[c], hi, O[t][c]);
+          if constexpr (LO) O[t][c] = mfma16x16(T[n].v[c], lo, O[t][c]);
+        }
+        if constexpr (MASKED) again(t, p, vis[t]);
       }
-      if constexpr (MASKED) again(t, p, vis[t]);
-    }
+  }
+  // Adds tiles that every row sees all of.
+  template <int NK>
+  __device__ __forceinline__ void add_clear(const CacheTile<M, DV> (&T)[NK]) {
+    add<false>(T, [](int) { return 0u; }, [](int, const float(&)[8], unsigned) {});
   }
 
   // After the last tile: the reference, the sum of the weights for the
@@ -293,11 +305,12 @@ struct CacheMask {
 // value product: such values are taken out of it and added by themselves, to
 // the rows that see their key.
 template <int M, int DV, int QT, bool LO>
-__device__ __forceinline__ void add_masked(CacheRows<M, DV, QT, LO>& R, CacheTile<M, DV>& T,
+__device__ __forceinline__ void add_masked(CacheRows<M, DV, QT, LO>& R, CacheTile<M, DV> (&Ts)[1],
                                            const CacheSource<M, DV>& src, const CacheMask& mask, int first,
                                            const int64_t (&bits)[QT], int tile, int page, int lane) {
   constexpr int NT = CacheTile<M, DV>::NT;
   const int c16 = lane & 15, g = lane >> 4, key0 = tile * 32 + 8 * g;
+  CacheTile<M, DV>& T = Ts[0];
   bool strange = false;
 #pragma unroll
   for (int c = 0; c < NT; ++c)
@@ -309,7 +322,7 @@ __device__ __forceinline__ void add_masked(CacheRows<M, DV, QT, LO>& R, CacheTil
     }
   const bool any = __any(strange);
   R.template add<true>(
-      T, [&](int t) { return mask(first + 16 * t + c16, bits[t], key0); },
+      Ts, [&](int t) { return mask(first + 16 * t + c16, bits[t], key0); },
       [&](int t, const float(&p)[8], unsigned seen) {
         if (!any) return;
         // column 16 c + 4 g + r of key k
@@ -396,43 +409,56 @@ __global__ __launch_bounds__(256) void cache_attn_few_kernel(
   if (blk.sp > 0 && kb >= sq.total) return;  // not one of this sequence's pieces
   if (sq.nb == 0 && a.nsplit > 1) return;    // padding: the joining kernel writes it
 
-  CacheRows<M, DV, 1, true> R;
-  float rc[1];
-  R.start(a, phi, gate_q, gate_k, b, h, 0, lane, rc);
-  const int64_t bits[1] = {tree ? tree[(int64_t)b * a.n + min(c16, a.n - 1)] : 0};
-
   // keys below `clear` are seen by every row, none from `end` on by any
   const int ke = blk.sp == a.nsplit - 1 ? sq.total : min(sq.total, kb + a.split_keys);
   const bool chunk = tree == nullptr;
   int clear = chunk ? (a.causal ? sq.ctx + (a.mask_diag ? 0 : 1) : a.mask_diag ? sq.ctx : sq.total) : sq.ctx;
   clear = min(clear, sq.total);
   const int end = sq.nb > 0 ? ke : 0;
-  const CacheMask mask{sq.ctx, sq.nb, sq.total, a.causal, a.mask_diag, !chunk};
   const CacheSource<M, DV> src(a, codes, values, table, b, h, lane);
 
-  int tile = kb / 32 + w;
-  if (tile * 32 < end) {
-    CacheTile<M, DV> A, B;
-    int pa = src.page_of(tile), pb = 0;
-    src.load(A, tile, pa);
-    if ((tile + 4) * 32 < end) pb = src.page_of(tile + 4);
-    auto step = [&](CacheTile<M, DV>& cur, CacheTile<M, DV>& nxt, int& pc, int& pn) {
-      const bool more = (tile + 4) * 32 < end;
-      if (more) src.load(nxt, tile + 4, pn);
-      int after = 0;
-      if ((tile + 8) * 32 < end) after = src.page_of(tile + 8);
-      if (src.exists(pc)) {
-        if (tile * 32 + 32 <= clear)
-          R.template add<false>(cur, [](int) { return 0u; }, [](int, const float(&)[8], unsigned) {});
-        else
-          add_masked(R, cur, src, mask, 0, bits, tile, pc, lane);
-      }
-      pc = after;
-      tile += 4;
-      return more;
-    };
-    while (step(A, B, pa, pb) && step(B, A, pb, pa)) {
+  // the first tile is on its way while the queries are prepared
+  CacheTile<M, DV> A[1], B[1];
+  int tile = kb / 32 + w, pa = 0, pb = 0;
+  auto within = [&](int t) { return t * 32 < end; };
+  auto clean = [&](int t, int page) { return t * 32 + 32 <= min(clear, end) && src.exists(page); };
+  if (within(tile)) {
+    pa = src.page_of(tile);
+    src.load(A[0], tile, pa);
+  }
+  if (within(tile + 4)) pb = src.page_of(tile + 4);
+
+  CacheRows<M, DV, 1, true> R;
+  float rc[1];
+  R.start(a, phi, gate_q, gate_k, b, h, 0, lane, rc);
+  const int64_t bits[1] = {tree ? tree[(int64_t)b * a.n + min(c16, a.n - 1)] : 0};
+
+  // adds cur, with the next tile's loads in flight
+  auto step = [&](CacheTile<M, DV>(&cur)[1], CacheTile<M, DV>(&nxt)[1], int& pc, int pn) {
+    if (within(tile + 4)) src.load(nxt[0], tile + 4, pn);
+    if (within(tile + 8)) pc = src.page_of(tile + 8);
+    R.add_clear(cur);
+    tile += 4;
+  };
+  while (clean(tile, pa)) {
+    step(A, B, pa, pb);
+    if (!clean(tile, pb)) {
+      A[0] = B[0];
+      const int p = pa;
+      pa = pb;
+      pb = p;
+      break;
     }
+    step(B, A, pb, pa);
+  }
+  const CacheMask mask{sq.ctx, sq.nb, sq.total, a.causal, a.mask_diag, !chunk};
+  while (within(tile)) {
+    if (within(tile + 4)) src.load(B[0], tile + 4, pb);
+    if (src.exists(pa)) add_masked(R, A, src, mask, 0, bits, tile, pa, lane);
+    A[0] = B[0];
+    pa = pb;
+    tile += 4;
+    if (within(tile + 4)) pb = src.page_of(tile + 4);
   }
 
   __shared__ __align__(16) float so[4][16][DV + 4];
@@ -489,14 +515,6 @@ __global__ __launch_bounds__(256, 2) void cache_attn_rows_kernel(
   if (blk.sp > 0 && kb >= sq.total) return;
   if (q0 >= sq.nb && a.nsplit > 1) return;
 
-  CacheRows<M, DV, QT, LO> R;
-  float rc[QT];
-  R.start(a, phi, gate_q, gate_k, b, h, qw, lane, rc);
-  int64_t bits[QT];
-#pragma unroll
-  for (int t = 0; t < QT; ++t)
-    bits[t] = tree ? tree[(int64_t)b * a.n + min(qw + 16 * t + c16, a.n - 1)] : 0;
-
   const int ke = blk.sp == a.nsplit - 1 ? sq.total : min(sq.total, kb + a.split_keys);
   // what the rows from `first` on, `count` of them, see: all of them the keys
   // below clear, none a key from end on
@@ -526,7 +544,7 @@ __global__ __launch_bounds__(256, 2) void cache_attn_rows_kernel(
       lds_dma16(src.frag(second ? f - NF : f, tile, second ? p1 : p0), to + 1024u * (unsigned)f);
     }
   };
-  int pg[3][2];
+  int pg[3][2];  // pages of the stage at hand and the next two
 #pragma unroll
   for (int st = 0; st < 2; ++st)
 #pragma unroll
@@ -534,7 +552,18 @@ __global__ __launch_bounds__(256, 2) void cache_attn_rows_kernel(
   pg[2][0] = pg[2][1] = -1;
   if (stages > 0) issue(0, pg[0][0], pg[0][1]);
   if (stages > 1) issue(1, pg[1][0], pg[1][1]);
-  for (int st = 0; st < stages; ++st) {
+
+  CacheRows<M, DV, QT, LO> R;
+  float rc[QT];
+  R.start(a, phi, gate_q, gate_k, b, h, qw, lane, rc);
+  int64_t bits[QT];
+#pragma unroll
+  for (int t = 0; t < QT; ++t)
+    bits[t] = tree ? tree[(int64_t)b * a.n + min(qw + 16 * t + c16, a.n - 1)] : 0;
+
+  int st = 0;
+  // opens stage st: its keys are in LDS, those of stage st + 2 on their way
+  auto open = [&]() {
     // this wave's part of the stage has landed (the next stage's may not have)
     if (st + 1 < stages)
       wait_vmcnt_lgkm0<PER>();
@@ -546,26 +575,44 @@ __global__ __launch_bounds__(256, 2) void cache_attn_rows_kernel(
       pg[2][1] = page(st + 2, 1);
       issue(st + 2, pg[2][0], pg[2][1]);
     }
-    const char* from = lds[st % 3] + 16 * lane;
+  };
+  auto close = [&]() {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int tile = tile0 + 2 * st + i;
-      if (tile * 32 >= end || !src.exists(pg[0][i])) continue;  // uniform in the wave
-      CacheTile<M, DV> T;
-      auto at = [&](int f) { return *reinterpret_cast<const f16x8*>(from + 1024 * (NF * i + f)); };
-#pragma unroll
-      for (int f = 0; f < NF - NT; ++f) T.k[f / T.KC][f % T.KC] = at(f);
-#pragma unroll
-      for (int c = 0; c < NT; ++c) T.v[c] = at(NF - NT + c);
-      if (tile * 32 + 32 <= clear)
-        R.template add<false>(T, [](int) { return 0u; }, [](int, const float(&)[8], unsigned) {});
-      else
-        add_masked(R, T, src, mask, qw, bits, tile, pg[0][i], lane);
+      pg[0][i] = pg[1][i];
+      pg[1][i] = pg[2][i];
     }
-    pg[0][0] = pg[1][0];
-    pg[0][1] = pg[1][1];
-    pg[1][0] = pg[2][0];
-    pg[1][1] = pg[2][1];
+    ++st;
+  };
+  auto get = [&](CacheTile<M, DV>& T, int i) {
+    const char* from = lds[st % 3] + 16 * lane + 1024 * NF * i;
+#pragma unroll
+    for (int f = 0; f < NF - NT; ++f) T.k[f / T.KC][f % T.KC] = *reinterpret_cast<const f16x8*>(from + 1024 * f);
+#pragma unroll
+    for (int c = 0; c < NT; ++c) T.v[c] = *reinterpret_cast<const f16x8*>(from + 1024 * (NF - NT + c));
+  };
+  // whole stages that all of the wave's rows see, then the rest (every wave
+  // opens every stage, so they meet at its barrier from either loop)
+  const int whole = (min(clear, end) - kb) / 64;
+  while (st < whole && src.exists(pg[0][0]) && src.exists(pg[0][1])) {
+    open();
+    CacheTile<M, DV> T[2];
+    get(T[0], 0);
+    get(T[1], 1);
+    R.add_clear(T);
+    close();
+  }
+  while (st < stages) {
+    open();
+#pragma unroll 1
+    for (int i = 0; i < 2; ++i) {
+      const int tile = tile0 + 2 * st + i, pc = i ? pg[0][1] : pg[0][0];
+      if (tile * 32 >= end || !src.exists(pc)) continue;  // uniform in the wave
+      CacheTile<M, DV> T[1];
+      get(T[0], i);
+      add_masked(R, T, src, mask, qw, bits, tile, pc, lane);
+    }
+    close();
   }
   const CacheOut<DV> put{out, lse, part_o, part_st, a.n, a.H, b, h, sq.nb, a.nsplit, blk.sp};
 #pragma unroll
