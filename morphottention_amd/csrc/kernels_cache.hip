@@ -279,23 +279,23 @@ struct CacheRows {
   }
 };
 
-// What a wave's rows see of a tile near or past the end of what all see.
+// What a wave's rows see of a tile near or past the end of what all see. In
+// integer arithmetic on 8 bits a lane: 8 compares would take 8 register pairs.
 struct CacheMask {
   int ctx, nb, total, causal, mask_diag;
   bool tree;
+  __device__ __forceinline__ static unsigned first(int count) { return (1u << min(max(count, 0), 8)) - 1; }
   // row i (of the new tokens; bits: its drafts), keys key0 .. key0 + 7
-  __device__ __forceinline__ unsigned operator()(int i, int64_t bits, int key0) const {
-    unsigned seen = 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int k = key0 + j, d = k - ctx;  // d: which of the new tokens
-      bool v = k < total && i < nb;
-      if (tree)
-        v = v && (d < 0 || ((bits >> min(max(d, 0), 63)) & 1));
-      else
-        v = v && (!causal || d <= i) && !(mask_diag && d == i);
-      seen |= v ? 1u << j : 0u;
+  __device__ __forceinline__ unsigned operator()(int i, uint64_t bits, int key0) const {
+    const int d = key0 - ctx;  // which of the new tokens the first key is
+    unsigned seen = first(i < nb ? total - key0 : 0);
+    if (tree) {
+      const unsigned drafts = d >= 0 ? (unsigned)(d < 64 ? bits >> d : 0)
+                                     : (d > -8 ? (unsigned)(bits << -d) | first(-d) : 0xffu);
+      return seen & drafts;
     }
+    if (causal) seen &= first(i + 1 - d);
+    if (mask_diag && (unsigned)(i - d) < 8u) seen &= ~(1u << (i - d));
     return seen;
   }
 };
@@ -307,20 +307,29 @@ struct CacheMask {
 template <int M, int DV, int QT, bool LO>
 __device__ __forceinline__ void add_masked(CacheRows<M, DV, QT, LO>& R, CacheTile<M, DV> (&Ts)[1],
                                            const CacheSource<M, DV>& src, const CacheMask& mask, int first,
-                                           const int64_t (&bits)[QT], int tile, int page, int lane) {
+                                           const uint64_t (&bits)[QT], int tile, int page, int lane) {
   constexpr int NT = CacheTile<M, DV>::NT;
   const int c16 = lane & 15, g = lane >> 4, key0 = tile * 32 + 8 * g;
   CacheTile<M, DV>& T = Ts[0];
-  bool strange = false;
+  unsigned there[4], strange = 0;  // halves of the keys that exist
 #pragma unroll
-  for (int c = 0; c < NT; ++c)
+  for (int j = 0; j < 4; ++j) {
+    const int n = mask.total - key0 - 2 * j;
+    there[j] = n >= 2 ? ~0u : n == 1 ? 0xffffu : 0u;
+  }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const bool bad = not_finite(T.v[c][j]);
-      strange |= bad && key0 + j < mask.total;
-      if (bad || key0 + j >= mask.total) T.v[c][j] = (f16)0.f;
+  for (int c = 0; c < NT; ++c) {
+    i32x4 x = __builtin_bit_cast(i32x4, T.v[c]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      // an exponent of all ones carries into bit 15 of its half
+      const unsigned bad = ((((unsigned)x[j] & 0x7c007c00u) + 0x04000400u) >> 15 & 0x00010001u) * 0xffffu;
+      strange |= bad & there[j];
+      x[j] = (int)((unsigned)x[j] & ~bad & there[j]);
     }
-  const bool any = __any(strange);
+    T.v[c] = __builtin_bit_cast(f16x8, x);
+  }
+  const bool any = __any(strange != 0);
   R.template add<true>(
       Ts, [&](int t) { return mask(first + 16 * t + c16, bits[t], key0); },
       [&](int t, const float(&p)[8], unsigned seen) {
@@ -431,7 +440,7 @@ __global__ __launch_bounds__(256) void cache_attn_few_kernel(
   CacheRows<M, DV, 1, true> R;
   float rc[1];
   R.start(a, phi, gate_q, gate_k, b, h, 0, lane, rc);
-  const int64_t bits[1] = {tree ? tree[(int64_t)b * a.n + min(c16, a.n - 1)] : 0};
+  const uint64_t bits[1] = {tree ? (uint64_t)tree[(int64_t)b * a.n + min(c16, a.n - 1)] : 0};
 
   // adds cur, with the next tile's loads in flight
   auto step = [&](CacheTile<M, DV>(&cur)[1], CacheTile<M, DV>(&nxt)[1], int& pc, int pn) {
@@ -534,29 +543,49 @@ __global__ __launch_bounds__(256, 2) void cache_attn_rows_kernel(
 
   const int tile0 = kb / 32, tiles = endw > kb ? (endw - kb + 31) / 32 : 0, stages = (tiles + 1) / 2;
   auto page = [&](int st, int i) { return src.page_of(tile0 + min(2 * st + i, tiles - 1)); };
-  auto issue = [&](int st, int p0, int p1) {
+  // this wave's pieces w, w + 4, ... of a stage's 2 NF operands: where they
+  // lie for a lane, in bytes from the page's codes or values of the tile
+  unsigned off[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int f = (w + 4 * i) % NF;
+    off[i] = 2u * (unsigned)(f < NF - NT
+                                 ? ((c16 >> 2) * 8 + (c16 & 3) + 4 * (f / src.KC)) * M + 32 * (f % src.KC) +
+                                       (M == 16 ? 8 * (g & 1) : 8 * g)
+                                 : g * (DV * 8) + c16 * 8 + 128 * (f - (NF - NT)));
+  }
+  const f16* const kh = codes + (((int64_t)h * M) << a.lp);
+  const f16* const vh = values + (((int64_t)h * DV) << a.lp);
+  auto issue = [&](int st, const int(&p)[2]) {
+    const f16 *kt[2], *vt[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int slot = src.slot(tile0 + min(2 * st + i, tiles - 1));
+      const int64_t pg = src.exists(p[i]) ? p[i] : 0;
+      kt[i] = kh + pg * src.kstride + slot * M;
+      vt[i] = vh + pg * src.vstride + slot * DV;
+    }
     const unsigned to = base + (unsigned)(st % 3) * (2 * NF * 1024);
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int f = w + 4 * i;  // of the stage's 2 NF
-      const bool second = f >= NF;
-      const int tile = tile0 + min(2 * st + (second ? 1 : 0), tiles - 1);
-      lds_dma16(src.frag(second ? f - NF : f, tile, second ? p1 : p0), to + 1024u * (unsigned)f);
+      const int f = w + 4 * i, t = f >= NF, fk = f - (t ? NF : 0);
+      const f16* from = fk < NF - NT ? (t ? kt[1] : kt[0]) : (t ? vt[1] : vt[0]);
+      lds_dma16_so(from, off[i], to + 1024u * (unsigned)f);
     }
   };
-  int pg[3][2];  // pages of the stage at hand and the next two
+  int pg[4][2];  // pages of the stage at hand and the next three
 #pragma unroll
-  for (int st = 0; st < 2; ++st)
+  for (int st = 0; st < 3; ++st)
 #pragma unroll
     for (int i = 0; i < 2; ++i) pg[st][i] = st < stages ? page(st, i) : -1;
-  pg[2][0] = pg[2][1] = -1;
-  if (stages > 0) issue(0, pg[0][0], pg[0][1]);
-  if (stages > 1) issue(1, pg[1][0], pg[1][1]);
+  pg[3][0] = pg[3][1] = -1;
+  if (stages > 0) issue(0, pg[0]);
+  if (stages > 1) issue(1, pg[1]);
 
   CacheRows<M, DV, QT, LO> R;
   float rc[QT];
   R.start(a, phi, gate_q, gate_k, b, h, qw, lane, rc);
-  int64_t bits[QT];
+  uint64_t bits[QT];
 #pragma unroll
   for (int t = 0; t < QT; ++t)
     bits[t] = tree ? tree[(int64_t)b * a.n + min(qw + 16 * t + c16, a.n - 1)] : 0;
@@ -570,10 +599,10 @@ __global__ __launch_bounds__(256, 2) void cache_attn_rows_kernel(
     else
       wait_vmcnt_lgkm0<0>();
     asm volatile("s_barrier" ::: "memory");  // ... and every wave's; the stage before is free
-    if (st + 2 < stages) {
-      pg[2][0] = page(st + 2, 0);
-      pg[2][1] = page(st + 2, 1);
-      issue(st + 2, pg[2][0], pg[2][1]);
+    if (st + 2 < stages) issue(st + 2, pg[2]);
+    if (st + 3 < stages) {
+      pg[3][0] = page(st + 3, 0);
+      pg[3][1] = page(st + 3, 1);
     }
   };
   auto close = [&]() {
@@ -581,6 +610,7 @@ __global__ __launch_bounds__(256, 2) void cache_attn_rows_kernel(
     for (int i = 0; i < 2; ++i) {
       pg[0][i] = pg[1][i];
       pg[1][i] = pg[2][i];
+      pg[2][i] = pg[3][i];
     }
     ++st;
   };
