@@ -542,45 +542,66 @@ __global__ __launch_bounds__(256, 2) void cache_attn_rows_kernel(
   const unsigned base = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
 
   const int tile0 = kb / 32, tiles = endw > kb ? (endw - kb + 31) / 32 : 0, stages = (tiles + 1) / 2;
-  auto page = [&](int st, int i) { return src.page_of(tile0 + min(2 * st + i, tiles - 1)); };
-  // this wave's pieces w, w + 4, ... of a stage's 2 NF operands: where they
-  // lie for a lane, in bytes from the page's codes or values of the tile
-  unsigned off[PER];
+  // A stage lies in one page, or in two of 32 tokens (then `two`, and the
+  // second one of the last stage may not be in the table any more).
+  const bool two = a.lp == 5;
+  auto page = [&](int st, int i) {
+    return src.row[two ? tile0 + min(2 * st + i, tiles - 1) : (32 * tile0 + 64 * st) >> a.lp];
+  };
+  // This wave's operands of a stage: KC of its 4 KC of codes, NT / 2 of its 2
+  // NT of values, every fourth of each. Operand f of a kind with n a tile is
+  // f % n of tile f / n. A lane's place in them in bytes from the stage's
+  // first token (or its own page's, if there are two), and theirs in LDS.
+  constexpr int KC = CacheTile<M, DV>::KC;
+  unsigned koff[KC], voff[NT / 2], kto[KC], vto[NT / 2];
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int f = (w + 4 * i) % NF;
-    off[i] = 2u * (unsigned)(f < NF - NT
-                                 ? ((c16 >> 2) * 8 + (c16 & 3) + 4 * (f / src.KC)) * M + 32 * (f % src.KC) +
-                                       (M == 16 ? 8 * (g & 1) : 8 * g)
-                                 : g * (DV * 8) + c16 * 8 + 128 * (f - (NF - NT)));
+  for (int i = 0; i < KC; ++i) {
+    const int f = w + 4 * i, t = f / (2 * KC), o = f % (2 * KC);
+    koff[i] = 2u * (unsigned)(((c16 >> 2) * 8 + (c16 & 3) + 4 * (o / KC) + (two ? 0 : 32 * t)) * M + 32 * (o % KC) +
+                              (M == 16 ? 8 * (g & 1) : 8 * g));
+    kto[i] = base + 1024u * (unsigned)(NF * t + o);
   }
-  const f16* const kh = codes + (((int64_t)h * M) << a.lp);
-  const f16* const vh = values + (((int64_t)h * DV) << a.lp);
-  auto issue = [&](int st, const int(&p)[2]) {
-    const f16 *kt[2], *vt[2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int slot = src.slot(tile0 + min(2 * st + i, tiles - 1));
-      const int64_t pg = src.exists(p[i]) ? p[i] : 0;
-      kt[i] = kh + pg * src.kstride + slot * M;
-      vt[i] = vh + pg * src.vstride + slot * DV;
+  for (int i = 0; i < NT / 2; ++i) {
+    const int f = w + 4 * i, t = f / NT, o = f % NT;
+    voff[i] = 2u * (unsigned)((g + (two ? 0 : 4 * t)) * (DV * 8) + c16 * 8 + 128 * o);
+    vto[i] = base + 1024u * (unsigned)(NF * t + 2 * KC + o);
+  }
+  const char* const kh = reinterpret_cast<const char*>(codes + (((int64_t)h * M) << a.lp));
+  const char* const vh = reinterpret_cast<const char*>(values + (((int64_t)h * DV) << a.lp));
+  const unsigned kpage = (unsigned)(a.H * M * 2) << a.lp, vpage = (unsigned)(a.H * DV * 2) << a.lp;  // bytes, <= 2^25
+  constexpr unsigned kStage = 2 * NF * 1024;
+  unsigned fill = 0;  // where the next stage goes
+  int slot = (32 * tile0) & ((1 << a.lp) - 1);
+  auto issue = [&](const int(&p)[2]) {
+    const unsigned pg = src.exists(p[0]) ? (unsigned)p[0] : 0u;
+    const char *k[2], *v[2];
+    k[0] = k[1] = kh + ((uint64_t)pg * kpage + (unsigned)(slot * M * 2));
+    v[0] = v[1] = vh + ((uint64_t)pg * vpage + (unsigned)(slot * DV * 2));
+    if (two) {
+      const unsigned p1 = src.exists(p[1]) ? (unsigned)p[1] : 0u;
+      k[1] = kh + (uint64_t)p1 * kpage;
+      v[1] = vh + (uint64_t)p1 * vpage;
     }
-    const unsigned to = base + (unsigned)(st % 3) * (2 * NF * 1024);
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int f = w + 4 * i, t = f >= NF, fk = f - (t ? NF : 0);
-      const f16* from = fk < NF - NT ? (t ? kt[1] : kt[0]) : (t ? vt[1] : vt[0]);
-      lds_dma16_so(from, off[i], to + 1024u * (unsigned)f);
-    }
+    for (int i = 0; i < KC; ++i) lds_dma16_so(k[(w + 4 * i) / (2 * KC)], koff[i], kto[i] + fill);
+#pragma unroll
+    for (int i = 0; i < NT / 2; ++i) lds_dma16_so(v[(w + 4 * i) / NT], voff[i], vto[i] + fill);
+    fill = fill == 2 * kStage ? 0 : fill + kStage;
+    slot = (slot + 64) & ((1 << a.lp) - 1) & ~63;  // 0 with pages of 32
   };
   int pg[4][2];  // pages of the stage at hand and the next three
+  auto pages_of = [&](int st, int(&p)[2]) {
+    p[0] = p[1] = page(st, 0);
+    if (two) p[1] = page(st, 1);
+  };
+#pragma unroll
+  for (int st = 0; st < 4; ++st) pg[st][0] = pg[st][1] = -1;
 #pragma unroll
   for (int st = 0; st < 3; ++st)
-#pragma unroll
-    for (int i = 0; i < 2; ++i) pg[st][i] = st < stages ? page(st, i) : -1;
-  pg[3][0] = pg[3][1] = -1;
-  if (stages > 0) issue(0, pg[0]);
-  if (stages > 1) issue(1, pg[1]);
+    if (st < stages) pages_of(st, pg[st]);
+  if (stages > 0) issue(pg[0]);
+  if (stages > 1) issue(pg[1]);
 
   CacheRows<M, DV, QT, LO> R;
   float rc[QT];
@@ -599,12 +620,10 @@ __global__ __launch_bounds__(256, 2) void cache_attn_rows_kernel(
     else
       wait_vmcnt_lgkm0<0>();
     asm volatile("s_barrier" ::: "memory");  // ... and every wave's; the stage before is free
-    if (st + 2 < stages) issue(st + 2, pg[2]);
-    if (st + 3 < stages) {
-      pg[3][0] = page(st + 3, 0);
-      pg[3][1] = page(st + 3, 1);
-    }
+    if (st + 2 < stages) issue(pg[2]);
+    if (st + 3 < stages) pages_of(st + 3, pg[3]);
   };
+  unsigned read = 0;  // where the stage at hand is
   auto close = [&]() {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -613,9 +632,10 @@ __global__ __launch_bounds__(256, 2) void cache_attn_rows_kernel(
       pg[2][i] = pg[3][i];
     }
     ++st;
+    read = read == 2 * kStage ? 0 : read + kStage;
   };
   auto get = [&](CacheTile<M, DV>& T, int i) {
-    const char* from = lds[st % 3] + 16 * lane + 1024 * NF * i;
+    const char* from = &lds[0][0] + read + 16 * lane + 1024 * NF * i;
 #pragma unroll
     for (int f = 0; f < NF - NT; ++f) T.k[f / T.KC][f % T.KC] = *reinterpret_cast<const f16x8*>(from + 1024 * f);
 #pragma unroll
