@@ -337,9 +337,16 @@ inline CacheAttnPlan cache_attn_plan(int B, int H, int n, int64_t max_len) {
   return p;
 }
 
-// Rows of the projection for an append. Up to kCacheSkinnyTokens tokens go
-// through strips of 16 output columns whose waves divide the contraction;
-// more through tiles of 128 x 128.
-constexpr int kCacheSkinnyTokens = 256;
+// Shape of an append's projection of T tokens to C columns: 16 x tokens rows
+// and 16 x columns columns a workgroup, or (tokens = 0) tiles of 128 x 128.
+struct CacheAppendShape {
+  int tokens, columns;
+};
+inline CacheAppendShape cache_append_shape(int T, int C) {
+  if (T > 256) return {0, 0};
+  if (T <= 32) return {T <= 16 ? 1 : 2, 1};
+  const int strips = (C / 16) * ((T + 63) / 64);
+  return {4, strips >= 640 ? 4 : strips >= 320 ? 2 : 1};
+}
 
 }  // namespace morpho

@@ -818,11 +818,33 @@ __device__ __forceinline__ int2 token_slot(const CacheAppendArgs& a, const int* 
   return int2{(unsigned)page < (unsigned)a.pages ? page : -1, (int)(pos & ((1 << a.lp) - 1))};
 }
 
-// Few tokens: a workgroup of 8 waves per 16 output columns and 16 TT tokens.
-// Each wave contracts every 8th 32-wide step of D, straight from memory (what
-// bounds it is reading the weights once, and latency); the eight partial
-// tiles are added in LDS.
-template <int TT>
+// Column c of token t: its code, to phi and to the token's place, or its value.
+__device__ __forceinline__ void store_column(const CacheAppendArgs& a, float z, int c, int t, int2 at,
+                                             f16* __restrict__ codes, f16* __restrict__ values,
+                                             f16* __restrict__ phi) {
+  const int HM = a.H * a.M;
+  if (c < HM) {
+    const f16 y = (f16)cube_project(z, a.proj);
+    phi[(int64_t)t * HM + c] = y;
+    const int h = c / a.M;
+    if (at.x >= 0) codes[((((int64_t)at.x * a.H + h) << a.lp) + at.y) * a.M + (c - h * a.M)] = y;
+  } else if (at.x >= 0) {
+    const int v = c - HM, h = v / a.DV;
+    values[(((int64_t)at.x * a.H + h) << a.lp) * a.DV + ((at.y >> 3) * a.DV + (v - h * a.DV)) * 8 + (at.y & 7)] = (f16)z;
+  }
+}
+
+// Few tokens: a workgroup of 8 waves per 16 CT output columns and 16 TT
+// tokens. Each wave contracts an eighth of D, 32 wide steps that it brings to
+// LDS for itself (no barriers), and the partial tiles are added in LDS, the
+// upper four waves' first.
+// The operands go through LDS because a lane of the MFMA holds 16 bytes of the
+// row lane % 16: loaded so from row-major memory, neighbouring lanes are rows
+// apart, and the address unit takes them one at a time. Here four neighbours
+// fetch 64 bytes of a row (chunk p of row r holds k chunk p ^ (r / 4 % 4), so
+// that the reads of 8 rows of one chunk hit all banks). T 192, D 2048, C 4096:
+// 19.4 us loaded directly.
+template <int CT, int TT>
 __global__ __launch_bounds__(512) void cache_append_rows_kernel(CacheAppendArgs a, const f16* __restrict__ X,
                                                                const f16* __restrict__ Wt, f16* __restrict__ codes,
                                                                f16* __restrict__ values,
@@ -830,45 +852,91 @@ __global__ __launch_bounds__(512) void cache_append_rows_kernel(CacheAppendArgs 
                                                                const int* __restrict__ lens,
                                                                const int* __restrict__ new_lens,
                                                                f16* __restrict__ phi) {
-  __shared__ __align__(16) float part[8][TT][16][20];  // [wave][token tile][token][column]
+  constexpr int NF = CT + TT, NS = CT == 4 ? 2 : 3;  // operands of a step, 1 KiB each; steps in LDS
+  constexpr int kStage = NF * 1024, kSum = 4 * 16 * TT * (16 * CT + 4) * 4;
+  __shared__ __align__(1024) char smem[8 * NS * kStage > kSum ? 8 * NS * kStage : kSum];
+  auto part = reinterpret_cast<float(*)[16 * TT][16 * CT + 4]>(smem);  // [wave][token][column]
+  __shared__ int2 slot[16 * TT];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c16 = lane & 15, g = lane >> 4;
-  const int col0 = blockIdx.x * 16, t0 = blockIdx.y * 16 * TT;
-  f32x4 acc[TT];
+  const int col0 = blockIdx.x * 16 * CT, t0 = blockIdx.y * 16 * TT;
+  f32x4 acc[CT][TT];
 #pragma unroll
-  for (int t = 0; t < TT; ++t) acc[t] = f32x4{};
-  const f16* wp = Wt + (int64_t)(col0 + c16) * a.D + 8 * g;
-  const f16* xp[TT];
+  for (int c = 0; c < CT; ++c)
 #pragma unroll
-  for (int t = 0; t < TT; ++t) xp[t] = X + (int64_t)min(t0 + 16 * t + c16, a.T - 1) * a.D + 8 * g;
-#pragma unroll 4
-  for (int k = 32 * w; k < a.D; k += 256) {
-    const f16x8 wf = *reinterpret_cast<const f16x8*>(wp + k);
+    for (int t = 0; t < TT; ++t) acc[c][t] = f32x4{};
+  const int s0 = a.D / 32 * w / 8, ns = a.D / 32 * (w + 1) / 8 - s0;  // this wave's steps
+  // a lane's byte offsets from the step's first k of row 0 of the tile; rows
+  // past the end repeat the last
+  unsigned off[NF];
+  {
+    const int r = lane >> 2, chunk = (lane & 3) ^ ((lane >> 4) & 3);
 #pragma unroll
-    for (int t = 0; t < TT; ++t) acc[t] = mfma16x16(wf, *reinterpret_cast<const f16x8*>(xp[t] + k), acc[t]);
+    for (int c = 0; c < CT; ++c) off[c] = (unsigned)(min(16 * c + r, a.C - 1 - col0) * a.D + 8 * chunk) * 2u;
+#pragma unroll
+    for (int t = 0; t < TT; ++t) off[CT + t] = (unsigned)(min(16 * t + r, a.T - 1 - t0) * a.D + 8 * chunk) * 2u;
   }
+  const char* wp = reinterpret_cast<const char*>(Wt + (int64_t)col0 * a.D + 32 * s0);
+  const char* xp = reinterpret_cast<const char*>(X + (int64_t)t0 * a.D + 32 * s0);
+  const unsigned mine = (unsigned)(w * NS * kStage);
+  const unsigned base = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)smem + mine;
+  unsigned fill = 0, read = 0;  // the next step's place, that of the step at hand
+  auto issue = [&]() {
 #pragma unroll
-  for (int t = 0; t < TT; ++t) *reinterpret_cast<f32x4*>(&part[w][t][c16][4 * g]) = acc[t];
+    for (int f = 0; f < NF; ++f) lds_dma16_so(f < CT ? wp : xp, off[f], base + fill + 1024u * (unsigned)f);
+    wp += 64;
+    xp += 64;
+    fill = fill == (NS - 1) * kStage ? 0 : fill + kStage;
+  };
+#pragma unroll
+  for (int i = 0; i < NS - 1; ++i)
+    if (i < ns) issue();
+  if (threadIdx.x < 16 * TT) {
+    const int t = min(t0 + (int)threadIdx.x, a.T - 1), b = t / a.n;
+    slot[threadIdx.x] = token_slot(a, table, lens, new_lens, b, t - b * a.n);
+  }
+  const char* from = smem + mine + 16 * (4 * c16 + (g ^ ((c16 >> 2) & 3)));
+  for (int i = 0; i < ns; ++i) {
+    // the step has landed, those behind it may not have; the reads of the one
+    // before, whose place the next issue takes, are done
+    if (i + NS - 2 < ns && NS > 2)
+      wait_vmcnt_lgkm0<(NS - 2) * NF>();
+    else
+      wait_vmcnt_lgkm0<0>();
+    asm volatile("" ::: "memory");
+    if (i + NS - 1 < ns) issue();
+    f16x8 fr[NF];
+#pragma unroll
+    for (int f = 0; f < NF; ++f) fr[f] = *reinterpret_cast<const f16x8*>(from + read + 1024 * f);
+    read = read == (NS - 1) * kStage ? 0 : read + kStage;
+#pragma unroll
+    for (int c = 0; c < CT; ++c)
+#pragma unroll
+      for (int t = 0; t < TT; ++t) acc[c][t] = mfma16x16(fr[c], fr[CT + t], acc[c][t]);
+  }
+  __syncthreads();  // the sums take the steps' place
+  auto place = [&](int c, int t) { return reinterpret_cast<f32x4*>(&part[w & 3][16 * t + c16][16 * c + 4 * g]); };
+  if (w >= 4) {
+#pragma unroll
+    for (int c = 0; c < CT; ++c)
+#pragma unroll
+      for (int t = 0; t < TT; ++t) *place(c, t) = acc[c][t];
+  }
   __syncthreads();
-  const bool code = col0 < a.H * a.M;  // M and DV are multiples of 16: a strip lies in one head's codes or values
-  for (int e = threadIdx.x; e < 256 * TT; e += 512) {
-    const int c = e & 15, tok = e >> 4, t = t0 + tok;
-    if (t >= a.T) continue;
+  if (w < 4) {  // each place is read and written by one lane
+#pragma unroll
+    for (int c = 0; c < CT; ++c)
+#pragma unroll
+      for (int t = 0; t < TT; ++t) *place(c, t) += acc[c][t];
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < 256 * CT * TT; e += 512) {
+    const int c = col0 + e % (16 * CT), tok = e / (16 * CT), t = t0 + tok;
+    if (t >= a.T || c >= a.C) continue;
     float z = 0.f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) z += part[k][tok >> 4][tok & 15][c];
-    const int b = t / a.n;
-    const int2 at = token_slot(a, table, lens, new_lens, b, t - b * a.n);
-    if (code) {
-      const f16 y = (f16)cube_project(z, a.proj);
-      phi[(int64_t)t * (a.H * a.M) + col0 + c] = y;
-      const int h = (col0 + c) / a.M, cc = (col0 + c) % a.M;
-      if (at.x >= 0) codes[((((int64_t)at.x * a.H + h) << a.lp) + at.y) * a.M + cc] = y;
-    } else {
-      const int v = col0 + c - a.H * a.M, h = v / a.DV, cc = v % a.DV;
-      if (at.x >= 0)
-        values[(((int64_t)at.x * a.H + h) << a.lp) * a.DV + ((at.y >> 3) * a.DV + cc) * 8 + (at.y & 7)] = (f16)z;
-    }
+    for (int k = 0; k < 4; ++k) z += part[k][tok][e % (16 * CT)];
+    store_column(a, z, c, t, slot[tok], codes, values, phi);
   }
 }
 
@@ -903,19 +971,7 @@ __global__ __launch_bounds__(kGemmThreads) void cache_append_tile_kernel(
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int rt = AppendGemm::WTM * wm + 16 * i + 4 * (lane >> 4) + r, t = m0 + rt;
-        if (t >= a.T) continue;
-        const int2 at = slot[rt];
-        if (col < a.H * a.M) {
-          const f16 y = (f16)cube_project(acc[i][j][r], a.proj);
-          phi[(int64_t)t * (a.H * a.M) + cl] = y;
-          const int h = cl / a.M, cc = cl % a.M;
-          if (at.x >= 0) codes[((((int64_t)at.x * a.H + h) << a.lp) + at.y) * a.M + cc] = y;
-        } else {
-          const int v = cl - a.H * a.M, h = v / a.DV, cc = v % a.DV;
-          if (at.x >= 0)
-            values[(((int64_t)at.x * a.H + h) << a.lp) * a.DV + ((at.y >> 3) * a.DV + cc) * 8 + (at.y & 7)] =
-                (f16)acc[i][j][r];
-        }
+        if (t < a.T) store_column(a, acc[i][j][r], cl, t, slot[rt], codes, values, phi);
       }
   }
 }
@@ -935,18 +991,23 @@ hipError_t launch_cache_append(const CacheDims& d, const f16* X, const f16* W, f
   a.pages = d.pages;
   a.lp = log2_of(d.P);
   a.proj = proj;
-  if (a.T <= kCacheSkinnyTokens) {
-    const int tt = a.T <= 16 ? 1 : a.T <= 32 ? 2 : 4;
-    const dim3 grid(a.C / 16, (a.T + 16 * tt - 1) / (16 * tt));
-    if (tt == 1)
-      MORPHO_KLAUNCH((cache_append_rows_kernel<1>), grid, dim3(512), 0, s, a, X, W, codes, values, table, lens,
-                     new_lens, phi);
-    else if (tt == 2)
-      MORPHO_KLAUNCH((cache_append_rows_kernel<2>), grid, dim3(512), 0, s, a, X, W, codes, values, table, lens,
-                     new_lens, phi);
+  const CacheAppendShape p = cache_append_shape(a.T, a.C);
+  if (p.tokens) {
+    const dim3 grid((a.C + 16 * p.columns - 1) / (16 * p.columns), (a.T + 16 * p.tokens - 1) / (16 * p.tokens));
+#define MORPHO_CACHE_APPEND(CT, TT)                                                                               \
+  MORPHO_KLAUNCH((cache_append_rows_kernel<CT, TT>), grid, dim3(512), 0, s, a, X, W, codes, values, table, lens, \
+                 new_lens, phi)
+    if (p.tokens == 1)
+      MORPHO_CACHE_APPEND(1, 1);
+    else if (p.tokens == 2)
+      MORPHO_CACHE_APPEND(1, 2);
+    else if (p.columns == 1)
+      MORPHO_CACHE_APPEND(1, 4);
+    else if (p.columns == 2)
+      MORPHO_CACHE_APPEND(2, 4);
     else
-      MORPHO_KLAUNCH((cache_append_rows_kernel<4>), grid, dim3(512), 0, s, a, X, W, codes, values, table, lens,
-                     new_lens, phi);
+      MORPHO_CACHE_APPEND(4, 4);
+#undef MORPHO_CACHE_APPEND
   } else {
     const dim3 grid(gemm_tile_grid((a.T + 127) / 128, (a.C + 127) / 128));
     MORPHO_KLAUNCH(cache_append_tile_kernel, grid, dim3(kGemmThreads), 0, s, a, X, W, codes, values, table, lens,
