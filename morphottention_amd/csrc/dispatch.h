@@ -338,15 +338,22 @@ inline CacheAttnPlan cache_attn_plan(int B, int H, int n, int64_t max_len) {
 }
 
 // Shape of an append's projection of T tokens to C columns: 16 x tokens rows
-// and 16 x columns columns a workgroup, or (tokens = 0) tiles of 128 x 128.
+// and 16 x columns columns a workgroup that divides the contraction among its
+// waves, or (tokens = 0) tiles of columns x columns. us by shape (tokens x
+// columns), D 2048 C 4096: T 16 1x1 4.5, 2x1 4.8; T 64 2x2 8.3, 4x2 10.3, 4x1
+// 10.1; T 128 4x2 11.6, 4x4 13.0; T 256 4x2 20.2, 4x4 15.4; D 1024 C 1280: T
+// 128 2x2 4.4, 4x2 5.5; T 256 4x2 5.8, 2x2 7.3, 4x4 7.3; T 512 4x4 8.4, 4x2
+// 10.7: the widest tile that still gives about a workgroup to every second CU.
 struct CacheAppendShape {
   int tokens, columns;
 };
 inline CacheAppendShape cache_append_shape(int T, int C) {
-  if (T > 256) return {0, 0};
-  if (T <= 32) return {T <= 16 ? 1 : 2, 1};
-  const int strips = (C / 16) * ((T + 63) / 64);
-  return {4, strips >= 640 ? 4 : strips >= 320 ? 2 : 1};
+  const int64_t blocks = (int64_t)((T + 15) / 16) * (C / 16);  // of 16 x 16 outputs
+  if (blocks > 16 * 512) return {0, 128};
+  if (T <= 16) return {1, 1};
+  if (T <= 32) return {2, 1};
+  if (blocks <= 4 * 256) return {2, 2};
+  return {4, blocks <= 8 * 256 ? 2 : 4};
 }
 
 }  // namespace morpho

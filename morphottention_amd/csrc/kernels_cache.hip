@@ -803,35 +803,31 @@ hipError_t launch_cache_attn_join(const CacheDims& d, const CacheAttnPlan& plan,
 
 // ---------------------------------------------------------------- append
 struct CacheAppendArgs {
-  int T, n, D, H, M, DV, C;  // T = B n tokens, C = H (M + DV) columns
+  int T, n, D, H, C, HM;  // T = B n tokens, C = H (M + DV) columns, the first HM of them codes
+  int lm, ldv;            // log2 of M and DV
   int W, pages, lp, proj;
+  int NR, TR;  // rows of a sequence in the tile kernel's row space, rows in all
 };
 
-// Where a token goes: its page (negative: nowhere) and its place there.
-__device__ __forceinline__ int2 token_slot(const CacheAppendArgs& a, const int* __restrict__ table,
-                                           const int* __restrict__ lens, const int* __restrict__ new_lens, int b,
-                                           int i) {
+// Where new token i of sequence b goes: the row of its page's head 0 in the
+// pool's rows of tokens, [page][head][slot]; -1: nowhere.
+__device__ __forceinline__ int64_t token_row(const CacheAppendArgs& a, const int* __restrict__ table,
+                                             const int* __restrict__ lens, const int* __restrict__ new_lens, int b,
+                                             int i) {
   const int have = max(lens[b], 0), nb = new_lens ? new_lens[b] : a.n;
   const int64_t pos = (int64_t)have + i;
-  if (i >= nb || pos >= ((int64_t)a.W << a.lp)) return int2{-1, 0};
+  if (i >= nb || pos >= ((int64_t)a.W << a.lp)) return -1;
   const int page = table[(int64_t)b * a.W + (pos >> a.lp)];
-  return int2{(unsigned)page < (unsigned)a.pages ? page : -1, (int)(pos & ((1 << a.lp) - 1))};
+  return (unsigned)page < (unsigned)a.pages ? (((int64_t)page * a.H) << a.lp) + (pos & ((1 << a.lp) - 1)) : -1;
 }
-
-// Column c of token t: its code, to phi and to the token's place, or its value.
-__device__ __forceinline__ void store_column(const CacheAppendArgs& a, float z, int c, int t, int2 at,
-                                             f16* __restrict__ codes, f16* __restrict__ values,
-                                             f16* __restrict__ phi) {
-  const int HM = a.H * a.M;
-  if (c < HM) {
-    const f16 y = (f16)cube_project(z, a.proj);
-    phi[(int64_t)t * HM + c] = y;
-    const int h = c / a.M;
-    if (at.x >= 0) codes[((((int64_t)at.x * a.H + h) << a.lp) + at.y) * a.M + (c - h * a.M)] = y;
-  } else if (at.x >= 0) {
-    const int v = c - HM, h = v / a.DV;
-    values[(((int64_t)at.x * a.H + h) << a.lp) * a.DV + ((at.y >> 3) * a.DV + (v - h * a.DV)) * 8 + (at.y & 7)] = (f16)z;
-  }
+// Columns of the projection in the pool: a code, a value (of 8-token groups).
+__device__ __forceinline__ f16* code_place(const CacheAppendArgs& a, f16* codes, int64_t row, int c) {
+  return codes + ((row + ((int64_t)(c >> a.lm) << a.lp)) << a.lm) + (c & ((1 << a.lm) - 1));
+}
+__device__ __forceinline__ f16* value_place(const CacheAppendArgs& a, f16* values, int64_t row, int c) {
+  const int v = c - a.HM;
+  return values + (((row & ~(int64_t)7) + ((int64_t)(v >> a.ldv) << a.lp)) << a.ldv) +
+         8 * (v & ((1 << a.ldv) - 1)) + (row & 7);
 }
 
 // Few tokens: a workgroup of 8 waves per 16 CT output columns and 16 TT
@@ -856,7 +852,7 @@ __global__ __launch_bounds__(512) void cache_append_rows_kernel(CacheAppendArgs 
   constexpr int kStage = NF * 1024, kSum = 4 * 16 * TT * (16 * CT + 4) * 4;
   __shared__ __align__(1024) char smem[8 * NS * kStage > kSum ? 8 * NS * kStage : kSum];
   auto part = reinterpret_cast<float(*)[16 * TT][16 * CT + 4]>(smem);  // [wave][token][column]
-  __shared__ int2 slot[16 * TT];
+  __shared__ int64_t slot[16 * TT];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c16 = lane & 15, g = lane >> 4;
   const int col0 = blockIdx.x * 16 * CT, t0 = blockIdx.y * 16 * TT;
@@ -893,7 +889,7 @@ __global__ __launch_bounds__(512) void cache_append_rows_kernel(CacheAppendArgs 
     if (i < ns) issue();
   if (threadIdx.x < 16 * TT) {
     const int t = min(t0 + (int)threadIdx.x, a.T - 1), b = t / a.n;
-    slot[threadIdx.x] = token_slot(a, table, lens, new_lens, b, t - b * a.n);
+    slot[threadIdx.x] = token_row(a, table, lens, new_lens, b, t - b * a.n);
   }
   const char* from = smem + mine + 16 * (4 * c16 + (g ^ ((c16 >> 2) & 3)));
   for (int i = 0; i < ns; ++i) {
@@ -936,43 +932,143 @@ __global__ __launch_bounds__(512) void cache_append_rows_kernel(CacheAppendArgs 
     float z = 0.f;
 #pragma unroll
     for (int k = 0; k < 4; ++k) z += part[k][tok][e % (16 * CT)];
-    store_column(a, z, c, t, slot[tok], codes, values, phi);
+    const int64_t row = slot[tok];
+    if (c < a.HM) {
+      const f16 y = (f16)cube_project(z, a.proj);
+      phi[(int64_t)t * a.HM + c] = y;
+      if (row >= 0) *code_place(a, codes, row, c) = y;
+    } else if (row >= 0) {
+      *value_place(a, values, row, c) = (f16)z;
+    }
   }
 }
 
-// Many tokens: 128 x 128 tiles (tokens x columns) of the GEMM main loop.
-using AppendGemm = Gemm<128, 128, 2, true, true, 64, 2>;
+// Many tokens: tiles (tokens x columns) of the GEMM main loop. Its row space
+// gives each sequence NR rows. Where sequences are long (SHIFT), its row r is
+// position lens % 8 back from the first new one, + r, so that 8 rows of a tile
+// are the 8 tokens of a value group and are stored as one; a few rows at both
+// ends of a sequence repeat a token and are not stored.
+struct AppendRows {
+  const int* lens;  // null: no shift
+  int NR, n;
+  __device__ __forceinline__ int shift(int b) const { return lens ? max(lens[b], 0) & 7 : 0; }
+  __device__ __forceinline__ int operator()(int r) const {
+    const int b = r / NR;
+    return b * n + min(max(r - b * NR - shift(b), 0), n - 1);
+  }
+};
+
+// 4 x 4 halves among the four lanes of a quad: lane q has column q's rows 0 ..
+// 3 and gets row q's columns 0 .. 3.
+__device__ __forceinline__ f16x4 quad_transpose(f16x4 x, int lane) {
+  typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+  const u32x2 d = __builtin_bit_cast(u32x2, x);
+  const bool up = lane & 2, odd = lane & 1;
+  const unsigned far = (unsigned)__builtin_amdgcn_mov_dpp((int)(up ? d[0] : d[1]), 0x4e /* lane ^ 2 */, 0xf, 0xf, false);
+  const unsigned lo = up ? far : d[0], hi = up ? d[1] : far;  // rows 0, 1 (up: 2, 3) of columns q & 1, (q & 1) + 2
+  const unsigned l = __builtin_amdgcn_perm(hi, lo, 0x05040100), h = __builtin_amdgcn_perm(hi, lo, 0x07060302);
+  const unsigned mine = odd ? h : l;  // row q of the two columns
+  const unsigned near = (unsigned)__builtin_amdgcn_mov_dpp((int)(odd ? l : h), 0xb1 /* lane ^ 1 */, 0xf, 0xf, false);
+  const unsigned c0 = odd ? near : mine, c1 = odd ? mine : near;
+  return __builtin_bit_cast(f16x4, u32x2{__builtin_amdgcn_perm(c1, c0, 0x05040100),
+                                         __builtin_amdgcn_perm(c1, c0, 0x07060302)});
+}
+// v_permlane16_swap: the odd 16-lane rows of a change places with the even
+// ones of b (a' = a0 b0 a2 b2, b' = a1 b1 a3 b3).
+__device__ __forceinline__ void swap_rows16(f16x4& a, f16x4& b) {
+  typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+  u32x2 x = __builtin_bit_cast(u32x2, a), y = __builtin_bit_cast(u32x2, b);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const auto r = __builtin_amdgcn_permlane16_swap(x[i], y[i], false, false);
+    x[i] = r[0];
+    y[i] = r[1];
+  }
+  a = __builtin_bit_cast(f16x4, x);
+  b = __builtin_bit_cast(f16x4, y);
+}
+
+template <int BM, int BN, int STAGES, bool SHIFT>
 __global__ __launch_bounds__(kGemmThreads) void cache_append_tile_kernel(
     CacheAppendArgs a, const f16* __restrict__ X, const f16* __restrict__ Wt, f16* __restrict__ codes,
     f16* __restrict__ values, const int* __restrict__ table, const int* __restrict__ lens,
     const int* __restrict__ new_lens, f16* __restrict__ phi) {
-  __shared__ __align__(16) char lds[AppendGemm::kLdsBytes];
-  __shared__ int2 slot[128];
-  const int ntm = (a.T + 127) / 128, ntn = (a.C + 127) / 128;
+  using G = Gemm<BM, BN, 2, true, true, 64, STAGES>;
+  static_assert(G::FJ % 2 == 0, "column blocks in pairs");
+  __shared__ __align__(16) char lds[G::kLdsBytes];
+  const int ntm = (a.TR + BM - 1) / BM, ntn = (a.C + BN - 1) / BN;
   int tr, tc;
   if (!gemm_tile_map(blockIdx.x, ntm, ntn, tr, tc)) return;
-  const int m0 = 128 * tr, n0 = 128 * tc;
+  const int m0 = BM * tr, n0 = BN * tc;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (threadIdx.x < 128) {
-    const int t = min(m0 + (int)threadIdx.x, a.T - 1), b = t / a.n;
-    slot[threadIdx.x] = token_slot(a, table, lens, new_lens, b, t - b * a.n);
+  const AppendRows rows{SHIFT ? lens : nullptr, a.NR, a.n};
+  f32x4 acc[G::FI][G::FJ];
+  G::run(X, a.D, Wt, a.D, a.TR, a.C, m0, n0, 0, a.D, lds, acc, rows);
+  // the tile's rows: token (-1: none) and place in the pool (-1: not stored)
+  auto token = reinterpret_cast<int*>(lds);
+  auto place = reinterpret_cast<int64_t*>(lds + BM * 4);
+  if (threadIdx.x < BM) {
+    const int r = m0 + threadIdx.x;
+    int t = -1;
+    int64_t p = -1;
+    if (r < a.TR) {
+      const int b = r / a.NR, i = r - b * a.NR - rows.shift(b);
+      if (i >= 0 && i < a.n) {
+        t = b * a.n + i;
+        p = token_row(a, table, lens, new_lens, b, i);
+      }
+    }
+    token[threadIdx.x] = t;
+    place[threadIdx.x] = p;
   }
-  f32x4 acc[AppendGemm::FI][AppendGemm::FJ];
-  AppendGemm::run(X, a.D, Wt, a.D, a.T, a.C, m0, n0, 0, a.D, lds, acc);
   __syncthreads();
-  const int wm = w / AppendGemm::WN, wn = w % AppendGemm::WN;
+  const int wm = w / G::WN, wn = w % G::WN, c16 = lane & 15, g = lane >> 4;
 #pragma unroll
-  for (int j = 0; j < AppendGemm::FJ; ++j) {
-    const int col = n0 + AppendGemm::WTN * wn + 16 * j;  // 16 columns of one head's codes or values
-    if (col >= a.C) continue;
-    const int cl = col + (lane & 15);
+  for (int j = 0; j < G::FJ; ++j) {
+    const int col = n0 + G::WTN * wn + 16 * j;  // 16 columns of one head's codes or values
+    if (col >= a.HM) continue;
 #pragma unroll
-    for (int i = 0; i < AppendGemm::FI; ++i)
+    for (int i = 0; i < G::FI; ++i) {
+      f16x4 y;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) y[r] = (f16)cube_project(acc[i][j][r], a.proj);
+      y = quad_transpose(y, lane);
+      const int rt = G::WTM * wm + 16 * i + 4 * g + (c16 & 3), c = col + (c16 & ~3);
+      if (token[rt] >= 0) *reinterpret_cast<f16x4*>(phi + (int64_t)token[rt] * a.HM + c) = y;
+      if (place[rt] >= 0) *reinterpret_cast<f16x4*>(code_place(a, codes, place[rt], c)) = y;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < G::FJ; j += 2) {
+    const int col = n0 + G::WTN * wn + 16 * j;
+    if (col + 16 < a.HM || col >= a.C) continue;
+    // lane rows 0 and 2: column block j, 1 and 3: block j + 1; 8 rows of each
+    const int c = col + 16 * (g & 1) + c16;
+    const bool mine = c >= a.HM && c < a.C;
+#pragma unroll
+    for (int i = 0; i < G::FI; ++i) {
+      f16x4 lo, hi;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int rt = AppendGemm::WTM * wm + 16 * i + 4 * (lane >> 4) + r, t = m0 + rt;
-        if (t < a.T) store_column(a, acc[i][j][r], cl, t, slot[rt], codes, values, phi);
+        lo[r] = (f16)acc[i][j][r];
+        hi[r] = (f16)acc[i][j + 1][r];
       }
+      swap_rows16(lo, hi);
+      const f16x8 y = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+      const int rt = G::WTM * wm + 16 * i + 8 * (g >> 1);
+      const int64_t first = place[rt], last = place[rt + 7];
+      if (!mine) continue;
+      // 8 tokens of one group: stored tokens of a sequence follow each other
+      if (SHIFT && first >= 0 && (first & 7) == 0 && last == first + 7) {
+        *reinterpret_cast<f16x8*>(value_place(a, values, first, c)) = y;
+      } else {
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          const int64_t p = place[rt + r];
+          if (p >= 0) *value_place(a, values, p, c) = y[r];
+        }
+      }
+    }
   }
 }
 
@@ -984,13 +1080,17 @@ hipError_t launch_cache_append(const CacheDims& d, const f16* X, const f16* W, f
   a.n = d.n;
   a.D = d.H * d.DV;
   a.H = d.H;
-  a.M = d.M;
-  a.DV = d.DV;
   a.C = d.H * (d.M + d.DV);
+  a.HM = d.H * d.M;
+  a.lm = log2_of(d.M);
+  a.ldv = log2_of(d.DV);
   a.W = d.W;
   a.pages = d.pages;
   a.lp = log2_of(d.P);
   a.proj = proj;
+  const bool shift = d.n >= 64;  // up to 14 rows more a sequence
+  a.NR = shift ? (d.n + 14) / 8 * 8 : d.n;
+  a.TR = d.B * a.NR;
   const CacheAppendShape p = cache_append_shape(a.T, a.C);
   if (p.tokens) {
     const dim3 grid((a.C + 16 * p.columns - 1) / (16 * p.columns), (a.T + 16 * p.tokens - 1) / (16 * p.tokens));
@@ -999,19 +1099,29 @@ hipError_t launch_cache_append(const CacheDims& d, const f16* X, const f16* W, f
                  new_lens, phi)
     if (p.tokens == 1)
       MORPHO_CACHE_APPEND(1, 1);
-    else if (p.tokens == 2)
+    else if (p.tokens == 2 && p.columns == 1)
       MORPHO_CACHE_APPEND(1, 2);
-    else if (p.columns == 1)
-      MORPHO_CACHE_APPEND(1, 4);
+    else if (p.tokens == 2)
+      MORPHO_CACHE_APPEND(2, 2);
     else if (p.columns == 2)
       MORPHO_CACHE_APPEND(2, 4);
     else
       MORPHO_CACHE_APPEND(4, 4);
 #undef MORPHO_CACHE_APPEND
   } else {
-    const dim3 grid(gemm_tile_grid((a.T + 127) / 128, (a.C + 127) / 128));
-    MORPHO_KLAUNCH(cache_append_tile_kernel, grid, dim3(kGemmThreads), 0, s, a, X, W, codes, values, table, lens,
-                   new_lens, phi);
+#define MORPHO_CACHE_APPEND(BM, BN, STAGES, SHIFT)                                                          \
+  MORPHO_KLAUNCH((cache_append_tile_kernel<BM, BN, STAGES, SHIFT>),                                       \
+                 dim3(gemm_tile_grid((a.TR + BM - 1) / BM, (a.C + BN - 1) / BN)), dim3(kGemmThreads), 0, s, a, X, W, \
+                 codes, values, table, lens, new_lens, phi)
+    if (shift && p.columns == 256)
+      MORPHO_CACHE_APPEND(256, 256, 2, true);
+    else if (shift)
+      MORPHO_CACHE_APPEND(128, 128, 2, true);
+    else if (p.columns == 256)
+      MORPHO_CACHE_APPEND(256, 256, 2, false);
+    else
+      MORPHO_CACHE_APPEND(128, 128, 2, false);
+#undef MORPHO_CACHE_APPEND
   }
   return hipGetLastError();
 }

@@ -288,38 +288,51 @@ def _append_reference(x, w, H, m, projection):
     return phi, tol, v, tv + v.abs() * 2.0 ** -11 + 2.0 ** -25
 
 
+def _check_append(B, n, H, m, dv, lens, news, projection, P=64):
+    g = torch.Generator().manual_seed(m + dv + n)
+    D = H * dv
+    p = Problem(B, n, H, m, dv, lens, P=P, news=news, seed=n)
+    x = torch.randn((B, n, D), generator=g).half()
+    w = (torch.randn((H * m + D, D), generator=g) * D ** -0.5).half()
+    d = p.device()
+    codes, values = d["codes"].cpu(), d["values"].cpu()
+    phi = ma.morpho_cache_append(x.to(DEV), w.to(DEV), d["codes"], d["values"], d["table"], d["lens"],
+                                 new_lens=d["new_lens"], projection=projection).cpu()
+    ref, tol, v, tv = _append_reference(x, w, H, m, projection)
+    assert ((phi.double().reshape(B, n, H * m) - ref).abs() <= tol).all()
+    dc, dval = d["codes"].cpu(), d["values"].cpu()
+    for b in range(B):
+        t = lens[b] + torch.arange(p.news[b])
+        page, s = p.table[b].long()[t // P], t % P
+        codes[page, :, s] = phi[b, : p.news[b]]
+        got = dval[page, :, s // 8, :, s % 8]
+        assert ((got.double().reshape(-1, D) - v[b, : p.news[b]]).abs() <= tv[b, : p.news[b]]).all()
+        values[page, :, s // 8, :, s % 8] = got
+    # what was not appended to is as it was, NaN included
+    assert torch.equal(dc.view(torch.int16), codes.view(torch.int16))
+    assert torch.equal(dval.view(torch.int16), values.view(torch.int16))
+
+
 @pytest.mark.parametrize("m,dv,H", [(16, 32, 8), (16, 64, 3), (32, 64, 4), (64, 32, 5), (64, 128, 2), (32, 128, 1), (16, 32, 1)])
 @pytest.mark.parametrize("B,n,lens,news", [(1, 1, [37], None), (5, 1, [0, 63, 64, 65, 128], [1, 0, 1, 1, 1]),
                                            (3, 13, [0, 60, 127], [13, 2, 0]), (2, 40, [5, 30], None),
                                            (3, 150, [0, 3, 61], [150, 149, 7])])
 def test_append(m, dv, H, B, n, lens, news):
-    g = torch.Generator().manual_seed(m + dv + n)
-    D, P = H * dv, 64
     for projection in ("sigmoid", "hardtanh01", "identity") if n == 13 else ("sigmoid",):
-        p = Problem(B, n, H, m, dv, lens, P=P, news=news, seed=n)
-        x = torch.randn((B, n, D), generator=g).half()
-        w = (torch.randn((H * m + D, D), generator=g) * D ** -0.5).half()
-        d = p.device()
-        before = d["codes"].clone(), d["values"].clone()
-        phi = ma.morpho_cache_append(x.to(DEV), w.to(DEV), d["codes"], d["values"], d["table"], d["lens"],
-                                     new_lens=d["new_lens"], projection=projection)
-        ref, tol, v, tv = _append_reference(x, w, H, m, projection)
-        got = phi.double().cpu().reshape(B, n, H * m)
-        assert ((got - ref).abs() <= tol).all(), (got - ref).abs().max()
-        codes, values = before[0].cpu(), before[1].cpu()
-        new_v = torch.empty((B, n, H, dv), dtype=torch.float16)
-        dc, dval = d["codes"].cpu(), d["values"].cpu()
-        for b in range(B):
-            for i in range(p.news[b]):
-                t = lens[b] + i
-                page, s = int(p.table[b, t // P]), t % P
-                codes[page, :, s] = phi[b, i].cpu()
-                new_v[b, i] = dval[page, :, s // 8, :, s % 8]
-                assert ((new_v[b, i].double().reshape(-1) - v[b, i]).abs() <= tv[b, i]).all()
-                values[page, :, s // 8, :, s % 8] = new_v[b, i]
-        # what was not appended to is as it was, NaN included
-        assert torch.equal(dc.view(torch.int16), codes.view(torch.int16))
-        assert torch.equal(dval.view(torch.int16), values.view(torch.int16))
+        _check_append(B, n, H, m, dv, lens, news, projection)
+
+
+@pytest.mark.parametrize("m,dv,H", [(64, 64, 8), (16, 128, 3), (16, 64, 16)])
+@pytest.mark.parametrize("T,B", [(200, 5), (500, 20), (1100, 1), (5000, 3), (5000, 100)])
+def test_append_many(m, dv, H, T, B):
+    """Every launch shape: the widest strips and the tiles, with sequences longer and
+    shorter than 64 new tokens, starting anywhere in a group of 8."""
+    n = T // B
+    g = torch.Generator().manual_seed(T + B)
+    lens = torch.randint(0, 70, (B,), generator=g).tolist()
+    news = torch.randint(0, n + 1, (B,), generator=g).tolist()
+    news[0] = n
+    _check_append(B, n, H, m, dv, lens, news if B > 1 else None, "hardtanh01" if T == 500 else "sigmoid")
 
 
 @pytest.mark.parametrize("n", [1, 200])
