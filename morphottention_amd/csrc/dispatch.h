@@ -339,7 +339,7 @@ inline CacheAttnPlan cache_attn_plan(int B, int H, int n, int64_t max_len) {
 
 // Shape of an append's projection of T tokens to C columns: 16 x tokens rows
 // and 16 x columns columns a workgroup that divides the contraction among its
-// waves, or (tokens = 0) tiles of columns x columns. us by shape (tokens x
+// waves, or (tokens = 0) tiles of 128 x 128. us by shape (tokens x
 // columns), D 2048 C 4096: T 16 1x1 4.5, 2x1 4.8; T 64 2x2 8.3, 4x2 10.3, 4x1
 // 10.1; T 128 4x2 11.6, 4x4 13.0; T 256 4x2 20.2, 4x4 15.4; D 1024 C 1280: T
 // 128 2x2 4.4, 4x2 5.5; T 256 4x2 5.8, 2x2 7.3, 4x4 7.3; T 512 4x4 8.4, 4x2
@@ -354,6 +354,24 @@ inline CacheAppendShape cache_append_shape(int T, int C) {
   if (T <= 32) return {2, 1};
   if (blocks <= 4 * 256) return {2, 2};
   return {4, blocks <= 8 * 256 ? 2 : 4};
+}
+// Rows of a sequence in the tiles' row space: n, or (the tokens then shifted to
+// whole groups of 8) up to 14 more. Storing whole groups saves 1 to 5 us of 20
+// to 60, but an extra round of tiles costs more: B8 n256 D 2048 C 4096 44 us
+// unshifted, 62 shifted (512 and 544 tiles); with many rounds it does not show.
+inline int cache_append_rows(int B, int n, int C) {
+  if (n < 64) return n;
+  const int shifted = (n + 14) / 8 * 8;
+  auto rounds = [&](int rows) { return (((int64_t)B * rows + 127) / 128 * ((C + 127) / 128) + 255) / 256; };
+  return rounds(n) > 6 || rounds(shifted) == rounds(n) ? shifted : n;
+}
+
+// Heads of a compaction's workgroup, a power of two: as many as leave four
+// tokens a batch (4096 values) and 512 workgroups.
+inline int cache_compact_heads(int64_t sequences, int H, int DV) {
+  int hg = 1;
+  while (2 * hg * DV <= 1024 && hg < H && sequences * ((H + 2 * hg - 1) / (2 * hg)) >= 512) hg *= 2;
+  return hg;
 }
 
 }  // namespace morpho

@@ -806,7 +806,7 @@ struct CacheAppendArgs {
   int T, n, D, H, C, HM;  // T = B n tokens, C = H (M + DV) columns, the first HM of them codes
   int lm, ldv;            // log2 of M and DV
   int W, pages, lp, proj;
-  int NR, TR;  // rows of a sequence in the tile kernel's row space, rows in all
+  int NR, TR, shift;  // rows of a sequence in the tile kernel's row space, rows in all, whether shifted
 };
 
 // Where new token i of sequence b goes: the row of its page's head 0 in the
@@ -943,11 +943,15 @@ __global__ __launch_bounds__(512) void cache_append_rows_kernel(CacheAppendArgs 
   }
 }
 
-// Many tokens: tiles (tokens x columns) of the GEMM main loop. Its row space
-// gives each sequence NR rows. Where sequences are long (SHIFT), its row r is
-// position lens % 8 back from the first new one, + r, so that 8 rows of a tile
-// are the 8 tokens of a value group and are stored as one; a few rows at both
-// ends of a sequence repeat a token and are not stored.
+// Many tokens: 128 x 128 tiles (tokens x columns) of the GEMM main loop. Its
+// row space gives each sequence NR rows. With shift, row r of a sequence is
+// the position lens % 8 back from the first new one, + r, so that 8 rows of a
+// tile are the 8 tokens of a value group and are stored as one; a few rows at
+// both ends of a sequence repeat a token and are not stored. What bounds it:
+// the main loop's LDS reads and the latency of its two stages (one round of
+// tiles 15 us at D 1024, 28 at 2048; three or four stages, one workgroup to a
+// CU: 1 us less there and up to 25 % more for more rounds; 256 x 256 tiles: 10 %
+// less at T 16384 D 2048 C 4096, up to twice as much for fewer).
 struct AppendRows {
   const int* lens;  // null: no shift
   int NR, n;
@@ -988,12 +992,12 @@ __device__ __forceinline__ void swap_rows16(f16x4& a, f16x4& b) {
   b = __builtin_bit_cast(f16x4, y);
 }
 
-template <int BM, int BN, int STAGES, bool SHIFT>
 __global__ __launch_bounds__(kGemmThreads) void cache_append_tile_kernel(
     CacheAppendArgs a, const f16* __restrict__ X, const f16* __restrict__ Wt, f16* __restrict__ codes,
     f16* __restrict__ values, const int* __restrict__ table, const int* __restrict__ lens,
     const int* __restrict__ new_lens, f16* __restrict__ phi) {
-  using G = Gemm<BM, BN, 2, true, true, 64, STAGES>;
+  constexpr int BM = 128, BN = 128;
+  using G = Gemm<BM, BN, 2, true, true, 64, 2>;
   static_assert(G::FJ % 2 == 0, "column blocks in pairs");
   __shared__ __align__(16) char lds[G::kLdsBytes];
   const int ntm = (a.TR + BM - 1) / BM, ntn = (a.C + BN - 1) / BN;
@@ -1001,7 +1005,7 @@ __global__ __launch_bounds__(kGemmThreads) void cache_append_tile_kernel(
   if (!gemm_tile_map(blockIdx.x, ntm, ntn, tr, tc)) return;
   const int m0 = BM * tr, n0 = BN * tc;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const AppendRows rows{SHIFT ? lens : nullptr, a.NR, a.n};
+  const AppendRows rows{a.shift ? lens : nullptr, a.NR, a.n};
   f32x4 acc[G::FI][G::FJ];
   G::run(X, a.D, Wt, a.D, a.TR, a.C, m0, n0, 0, a.D, lds, acc, rows);
   // the tile's rows: token (-1: none) and place in the pool (-1: not stored)
@@ -1058,8 +1062,9 @@ __global__ __launch_bounds__(kGemmThreads) void cache_append_tile_kernel(
       const int rt = G::WTM * wm + 16 * i + 8 * (g >> 1);
       const int64_t first = place[rt], last = place[rt + 7];
       if (!mine) continue;
-      // 8 tokens of one group: stored tokens of a sequence follow each other
-      if (SHIFT && first >= 0 && (first & 7) == 0 && last == first + 7) {
+      // 8 tokens of one group: no two sequences store to one page, and the
+      // stored tokens of a sequence follow each other
+      if (first >= 0 && (first & 7) == 0 && last == first + 7) {
         *reinterpret_cast<f16x8*>(value_place(a, values, first, c)) = y;
       } else {
 #pragma unroll
@@ -1088,9 +1093,9 @@ hipError_t launch_cache_append(const CacheDims& d, const f16* X, const f16* W, f
   a.pages = d.pages;
   a.lp = log2_of(d.P);
   a.proj = proj;
-  const bool shift = d.n >= 64;  // up to 14 rows more a sequence
-  a.NR = shift ? (d.n + 14) / 8 * 8 : d.n;
+  a.NR = cache_append_rows(d.B, d.n, a.C);
   a.TR = d.B * a.NR;
+  a.shift = a.NR != d.n;
   const CacheAppendShape p = cache_append_shape(a.T, a.C);
   if (p.tokens) {
     const dim3 grid((a.C + 16 * p.columns - 1) / (16 * p.columns), (a.T + 16 * p.tokens - 1) / (16 * p.tokens));
@@ -1109,19 +1114,9 @@ hipError_t launch_cache_append(const CacheDims& d, const f16* X, const f16* W, f
       MORPHO_CACHE_APPEND(4, 4);
 #undef MORPHO_CACHE_APPEND
   } else {
-#define MORPHO_CACHE_APPEND(BM, BN, STAGES, SHIFT)                                                          \
-  MORPHO_KLAUNCH((cache_append_tile_kernel<BM, BN, STAGES, SHIFT>),                                       \
-                 dim3(gemm_tile_grid((a.TR + BM - 1) / BM, (a.C + BN - 1) / BN)), dim3(kGemmThreads), 0, s, a, X, W, \
-                 codes, values, table, lens, new_lens, phi)
-    if (shift && p.columns == 256)
-      MORPHO_CACHE_APPEND(256, 256, 2, true);
-    else if (shift)
-      MORPHO_CACHE_APPEND(128, 128, 2, true);
-    else if (p.columns == 256)
-      MORPHO_CACHE_APPEND(256, 256, 2, false);
-    else
-      MORPHO_CACHE_APPEND(128, 128, 2, false);
-#undef MORPHO_CACHE_APPEND
+    const dim3 grid(gemm_tile_grid((a.TR + 127) / 128, (a.C + 127) / 128));
+    MORPHO_KLAUNCH(cache_append_tile_kernel, grid, dim3(kGemmThreads), 0, s, a, X, W, codes, values, table, lens,
+                   new_lens, phi);
   }
   return hipGetLastError();
 }
@@ -1170,75 +1165,85 @@ hipError_t launch_cache_copy(const CacheDims& d, f16* codes, f16* values, const 
 }
 
 // ---------------------------------------------------------------- compaction
-// One workgroup a (layer, sequence, head) moves its kept tokens in order, 8
-// TB target tokens of one value column a lane and batch. keep ascends, so a
-// token never moves back over one that has yet to move (its place is at most
-// its source), and each batch is read whole before it is written.
+// One workgroup a (layer, sequence, group of 2^lh heads) moves its kept tokens
+// in order, 2^lk a batch, 16 values a lane. keep ascends, so a token never moves
+// back over one that has yet to move (its place is at most its source), and
+// each batch is read whole before it is written. Few tokens (an accepted path)
+// are bound by the chain of loads up to the first value: more heads a workgroup
+// and fewer workgroups take it fewer times (12 layers B32 H16 dv64, up to 9
+// tokens: 14.6 us with one head, 8 heads see cache_compact_heads).
+constexpr int kCompactValues = 4096;  // of a batch
 template <int DV>
 __global__ __launch_bounds__(256) void cache_compact_kernel(f16* codes, f16* values, const int* __restrict__ table,
                                                            const int* __restrict__ lens,
                                                            const int* __restrict__ keep,
-                                                           const int* __restrict__ keep_lens, int B, int H, int M,
-                                                           int pages, int W, int lp, int K) {
-  constexpr int BT = 64;  // target tokens of a batch
-  constexpr int PER = BT * DV / 256;
-  __shared__ int64_t from[BT], to[BT];  // token's place: page * P + slot, negative: none
+                                                           const int* __restrict__ keep_lens, int B, int H, int lm,
+                                                           int pages, int W, int lp, int K, int lh) {
+  constexpr int TH = kCompactValues / DV;           // (token, head) pairs of a batch
+  constexpr int VPER = kCompactValues / 256;        // values of a lane
+  constexpr int CPER = (TH * 8 + 255) / 256;        // 8-code pieces of a lane, at most (cube_m 64)
+  __shared__ int64_t from[TH], to[TH];              // a token's row of head 0 in the pool; to < 0: nothing to move
+  const int groups = (H + (1 << lh) - 1) >> lh;
   int id = blockIdx.x;
-  const int h = id % H;
-  id /= H;
+  const int h0 = (id % groups) << lh;
+  id /= groups;
   const int b = id % B, layer = id / B;
   const int count = keep_lens ? min(max(keep_lens[b], 0), K) : K;
   const int64_t base = max(lens[b], 0), cap = (int64_t)W << lp;
-  codes += (int64_t)layer * pages * H * ((int64_t)M << lp);
-  values += (int64_t)layer * pages * H * ((int64_t)DV << lp);
-  const int64_t mask = (1 << lp) - 1;
+  codes += ((int64_t)layer * pages * H) << (lm + lp);
+  values += ((int64_t)layer * pages * H * DV) << lp;
+  // row of head 0, [page][head][slot]
   auto place = [&](int64_t pos) -> int64_t {
     if (pos < 0 || pos >= cap) return -1;
     const int page = table[(int64_t)b * W + (pos >> lp)];
-    return (unsigned)page < (unsigned)pages ? ((int64_t)page << lp) + (pos & mask) : -1;
+    return (unsigned)page < (unsigned)pages ? (((int64_t)page * H) << lp) + (pos & ((1 << lp) - 1)) : -1;
   };
-  auto code_at = [&](int64_t pl) { return ((((pl >> lp) * H + h) << lp) + (pl & mask)) * M; };
-  auto value_at = [&](int64_t pl) {
-    return ((((pl >> lp) * H + h) << lp) + (pl & mask & ~(int64_t)7)) * DV + (pl & 7);
-  };
-  for (int k0 = 0; k0 < count; k0 += BT) {
-    const int nk = min(BT, count - k0);
-    if (threadIdx.x < BT) {
-      int64_t f = -1, t = -1;
-      if ((int)threadIdx.x < nk) {
-        const int64_t rel = keep[(int64_t)b * K + k0 + threadIdx.x];
-        f = rel < 0 ? -1 : place(base + rel);
-        t = place(base + k0 + threadIdx.x);
-        if (f < 0 || f == t) t = -1;  // nothing to move
-      }
+  const int batch = TH >> lh, heads = min(1 << lh, H - h0), lc = lm - 3;
+  for (int k0 = 0; k0 < count; k0 += batch) {
+    const int nk = min(batch, count - k0);
+    if ((int)threadIdx.x < nk) {
+      const int64_t rel = keep[(int64_t)b * K + k0 + threadIdx.x];
+      const int64_t f = rel < 0 ? -1 : place(base + rel), t = place(base + k0 + threadIdx.x);
       from[threadIdx.x] = f;
-      to[threadIdx.x] = t;
+      to[threadIdx.x] = f < 0 || f == t ? -1 : t;
     }
     __syncthreads();
-    f16x8 cv[BT * 8 / 256];  // up to 8 pieces of 8 codes a token
-    f16 vv[PER];
-    const int mc = M / 8;
+    f16x8 cv[CPER];
+    f16 vv[VPER];
+    // lane's i-th piece of codes: 2^lc of a (token, head) pair, and value
+    auto code = [&](int i, const int64_t* at, bool& ok) {
+      const int e = threadIdx.x + 256 * i, pair = e >> lc, k = pair >> lh, h = pair & ((1 << lh) - 1);
+      ok = k < nk && h < heads && to[k] >= 0;
+      return codes + (((ok ? at[k] : 0) + ((int64_t)(h0 + h) << lp)) << lm) + 8 * (e & ((1 << lc) - 1));
+    };
+    auto value = [&](int i, const int64_t* at, bool& ok) {
+      const int e = threadIdx.x + 256 * i, pair = e / DV, k = pair >> lh, h = pair & ((1 << lh) - 1);
+      ok = k < nk && h < heads && to[k] >= 0;
+      const int64_t row = ok ? at[k] : 0;
+      return values + ((row & ~(int64_t)7) + ((int64_t)(h0 + h) << lp)) * DV + 8 * (e % DV) + (row & 7);
+    };
+    bool ok;
 #pragma unroll
-    for (int i = 0; i < BT * 8 / 256; ++i) {
-      const int e = threadIdx.x + 256 * i, k = e / mc;
-      if (k < nk && to[k] >= 0) cv[i] = *reinterpret_cast<const f16x8*>(codes + code_at(from[k]) + 8 * (e % mc));
+    for (int i = 0; i < CPER; ++i) {
+      const f16* p = code(i, from, ok);
+      if (ok) cv[i] = *reinterpret_cast<const f16x8*>(p);
     }
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int e = threadIdx.x + 256 * i, k = e / DV, c = e % DV;
-      if (k < nk && to[k] >= 0) vv[i] = values[value_at(from[k]) + 8 * c];
+    for (int i = 0; i < VPER; ++i) {
+      const f16* p = value(i, from, ok);
+      if (ok) vv[i] = *p;
     }
     wait_vmcnt<0>();
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < BT * 8 / 256; ++i) {
-      const int e = threadIdx.x + 256 * i, k = e / mc;
-      if (k < nk && to[k] >= 0) *reinterpret_cast<f16x8*>(codes + code_at(to[k]) + 8 * (e % mc)) = cv[i];
+    for (int i = 0; i < CPER; ++i) {
+      f16* p = code(i, to, ok);
+      if (ok) *reinterpret_cast<f16x8*>(p) = cv[i];
     }
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int e = threadIdx.x + 256 * i, k = e / DV, c = e % DV;
-      if (k < nk && to[k] >= 0) values[value_at(to[k]) + 8 * c] = vv[i];
+    for (int i = 0; i < VPER; ++i) {
+      f16* p = value(i, to, ok);
+      if (ok) *p = vv[i];
     }
     __syncthreads();  // the places are read before the next batch's are written
   }
@@ -1246,11 +1251,12 @@ __global__ __launch_bounds__(256) void cache_compact_kernel(f16* codes, f16* val
 
 hipError_t launch_cache_compact(const CacheDims& d, f16* codes, f16* values, const int* table, const int* lens,
                                 const int* keep, const int* keep_lens, int K, hipStream_t s) {
-  const dim3 grid((unsigned)((int64_t)d.layers * d.B * d.H)), block(256);
-  const int lp = log2_of(d.P);
+  const int lh = log2_of(cache_compact_heads(d.layers * (int64_t)d.B, d.H, d.DV)), groups = (d.H + (1 << lh) - 1) >> lh;
+  const dim3 grid((unsigned)((int64_t)d.layers * d.B * groups)), block(256);
+  const int lp = log2_of(d.P), lm = log2_of(d.M);
 #define MORPHO_CACHE_COMPACT(DV)                                                                               \
   MORPHO_KLAUNCH((cache_compact_kernel<DV>), grid, block, 0, s, codes, values, table, lens, keep, keep_lens,   \
-                 d.B, d.H, d.M, d.pages, d.W, lp, K)
+                 d.B, d.H, lm, d.pages, d.W, lp, K, lh)
   if (d.DV == 32)
     MORPHO_CACHE_COMPACT(32);
   else if (d.DV == 64)
