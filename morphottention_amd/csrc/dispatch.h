@@ -330,6 +330,7 @@ inline CacheAttnPlan cache_attn_plan(int B, int H, int n, int64_t max_len) {
     keys = (max_len * wgs + 511) / 512;
     if (keys < 512) keys = 512;
   }
+  if (max_len <= keys + keys / 2) keys = max_len;  // half a piece is not worth the join
   keys = (keys + 127) / 128 * 128;
   p.nsplit = (int)((max_len + keys - 1) / keys);
   if (p.nsplit < 1) p.nsplit = 1;

@@ -525,18 +525,18 @@ __global__ __launch_bounds__(256, 2) void cache_attn_rows_kernel(
   if (q0 >= sq.nb && a.nsplit > 1) return;
 
   const int ke = blk.sp == a.nsplit - 1 ? sq.total : min(sq.total, kb + a.split_keys);
-  // what the rows from `first` on, `count` of them, see: all of them the keys
-  // below clear, none a key from end on
+  // what the wave's rows see: all of them the keys below clear and, where only
+  // their own keys are dropped, those from `beyond` on; none a key from end on
   const bool chunk = tree == nullptr;
-  auto clear_of = [&](int first) {
-    const int c = chunk ? (a.causal ? sq.ctx + first + (a.mask_diag ? 0 : 1) : a.mask_diag ? sq.ctx : sq.total) : sq.ctx;
-    return min(c, sq.total);
-  };
+  const int own = sq.ctx + qw;
+  int clear = chunk ? (a.causal ? own + (a.mask_diag ? 0 : 1) : a.mask_diag ? own : sq.total) : sq.ctx;
+  clear = min(clear, sq.total);
+  const int beyond = chunk && !a.causal && a.mask_diag ? own + 16 * QT : sq.total;
   auto end_of = [&](int first, int count) {
     const int e = chunk && a.causal ? sq.ctx + min(first + count, sq.nb) : sq.total;
     return first < sq.nb ? min(e, ke) : 0;
   };
-  const int clear = clear_of(qw), end = end_of(qw, 16 * QT), endw = end_of(q0, 64 * QT);  // endw: of the workgroup
+  const int end = end_of(qw, 16 * QT), endw = end_of(q0, 64 * QT);  // endw: of the workgroup
   const CacheMask mask{sq.ctx, sq.nb, sq.total, a.causal, a.mask_diag, !chunk};
   const CacheSource<M, DV> src(a, codes, values, table, b, h, lane);
   const unsigned base = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
@@ -641,18 +641,22 @@ __global__ __launch_bounds__(256, 2) void cache_attn_rows_kernel(
 #pragma unroll
     for (int c = 0; c < NT; ++c) T.v[c] = *reinterpret_cast<const f16x8*>(from + 1024 * (NF - NT + c));
   };
-  // whole stages that all of the wave's rows see, then the rest (every wave
+  // stages that all of the wave's rows see whole, and the others (every wave
   // opens every stage, so they meet at its barrier from either loop)
-  const int whole = (min(clear, end) - kb) / 64;
-  while (st < whole && src.exists(pg[0][0]) && src.exists(pg[0][1])) {
-    open();
-    CacheTile<M, DV> T[2];
-    get(T[0], 0);
-    get(T[1], 1);
-    R.add_clear(T);
-    close();
-  }
+  auto clean = [&]() {
+    const int from = kb + 64 * st, to = from + 64;
+    return to <= end && (to <= clear || from >= beyond) && src.exists(pg[0][0]) && src.exists(pg[0][1]);
+  };
   while (st < stages) {
+    while (clean()) {
+      open();
+      CacheTile<M, DV> T[2];
+      get(T[0], 0);
+      get(T[1], 1);
+      R.add_clear(T);
+      close();
+    }
+    if (st == stages) break;
     open();
 #pragma unroll 1
     for (int i = 0; i < 2; ++i) {
