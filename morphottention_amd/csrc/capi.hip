@@ -599,9 +599,9 @@ int make_cache_dims(const morpho_cache* c, bool layers, int64_t B, int64_t n, in
   if (seq_pages > kMaxCacheTokens / c->page_size)
     return fail(MORPHO_ERR_INVALID_ARGUMENT, "cache too large: seq_pages * page_size must be at most 2^30");
   if (B > (1 << 22) || n > (1 << 22) || B * n > (1 << 22) || B * n * c->H > (1 << 23) ||
-      B * c->H * c->layers > (1 << 23))
+      B * c->H * c->layers * c->head_dim_v > (1 << 25))
     return fail(MORPHO_ERR_INVALID_ARGUMENT,
-                "problem too large: needs B*n <= 2^22, B*n*H <= 2^23 and B*H*layers <= 2^23");
+                "problem too large: needs B*n <= 2^22, B*n*H <= 2^23 and B*H*layers*head_dim_v <= 2^25");
   d.layers = (int)c->layers;
   d.pages = (int)c->pages;
   d.H = (int)c->H;

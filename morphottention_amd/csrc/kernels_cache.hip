@@ -1169,47 +1169,67 @@ hipError_t launch_cache_copy(const CacheDims& d, f16* codes, f16* values, const 
 }
 
 // ---------------------------------------------------------------- compaction
-// One workgroup a (layer, sequence, group of 2^lh heads) moves its kept tokens
-// in order, 2^lk a batch, 16 values a lane. keep ascends, so a token never moves
-// back over one that has yet to move (its place is at most its source), and
-// each batch is read whole before it is written. Few tokens (an accepted path)
-// are bound by the chain of loads up to the first value: more heads a workgroup
-// and fewer workgroups take it fewer times (12 layers B32 H16 dv64, up to 9
-// tokens: 14.6 us with one head, 8 heads see cache_compact_heads).
+// keep ascends, so a token never moves back over one that has yet to move (its
+// place is at most its source): a workgroup that moves its share of a
+// sequence's tokens in order, each batch read whole before it is written, needs
+// no other memory. A value's line holds 8 tokens of 8 columns, so a lone token
+// touches 8 times its bytes; that bounds a tree's accepted path.
+struct CompactArgs {
+  int B, H, lm, pages, W, lp, K;
+};
+// A sequence's place in the pool.
+struct CompactSeq {
+  const int* table;
+  int64_t base, cap;
+  int H, pages, lp, count;
+  __device__ __forceinline__ CompactSeq(const CompactArgs& a, const int* tables, const int* lens,
+                                        const int* keep_lens, int b)
+      : table(tables + (int64_t)b * a.W), base(max(lens[b], 0)), cap((int64_t)a.W << a.lp), H(a.H), pages(a.pages),
+        lp(a.lp), count(keep_lens ? min(max(keep_lens[b], 0), a.K) : a.K) {}
+  // row of head 0 of a position, [page][head][slot]; -1: there is none
+  __device__ __forceinline__ int64_t place(int64_t pos) const {
+    if (pos < 0 || pos >= cap) return -1;
+    const int page = table[pos >> lp];
+    return (unsigned)page < (unsigned)pages ? (((int64_t)page * H) << lp) + (pos & ((1 << lp) - 1)) : -1;
+  }
+  // where the k-th kept token, rel behind base, comes from; -1: it stays or is not there
+  __device__ __forceinline__ void move(int k, int rel, int64_t& from, int64_t& to) const {
+    from = rel < 0 ? -1 : place(base + rel);
+    to = place(base + k);
+    if (from < 0 || from == to) to = -1;
+  }
+};
+
+// Few tokens a sequence: one workgroup a (layer, sequence, group of 2^lh
+// heads), 16 values a lane and batch. More heads a workgroup take the chain of
+// loads up to the first value fewer times (12 layers B32 H16 dv64, up to 9
+// tokens: one head 14.6 us, 8 12.6).
 constexpr int kCompactValues = 4096;  // of a batch
 template <int DV>
-__global__ __launch_bounds__(256) void cache_compact_kernel(f16* codes, f16* values, const int* __restrict__ table,
+__global__ __launch_bounds__(256) void cache_compact_kernel(CompactArgs a, f16* codes, f16* values,
+                                                           const int* __restrict__ table,
                                                            const int* __restrict__ lens,
                                                            const int* __restrict__ keep,
-                                                           const int* __restrict__ keep_lens, int B, int H, int lm,
-                                                           int pages, int W, int lp, int K, int lh) {
-  constexpr int TH = kCompactValues / DV;           // (token, head) pairs of a batch
-  constexpr int VPER = kCompactValues / 256;        // values of a lane
-  constexpr int CPER = (TH * 8 + 255) / 256;        // 8-code pieces of a lane, at most (cube_m 64)
-  __shared__ int64_t from[TH], to[TH];              // a token's row of head 0 in the pool; to < 0: nothing to move
-  const int groups = (H + (1 << lh) - 1) >> lh;
+                                                           const int* __restrict__ keep_lens, int lh) {
+  constexpr int TH = kCompactValues / DV;     // (token, head) pairs of a batch
+  constexpr int VPER = kCompactValues / 256;  // values of a lane
+  constexpr int CPER = (TH * 8 + 255) / 256;  // 8-code pieces of a lane, at most (cube_m 64)
+  __shared__ int64_t from[TH], to[TH];
+  const int H = a.H, lm = a.lm, lp = a.lp, groups = (H + (1 << lh) - 1) >> lh;
   int id = blockIdx.x;
   const int h0 = (id % groups) << lh;
   id /= groups;
-  const int b = id % B, layer = id / B;
-  const int count = keep_lens ? min(max(keep_lens[b], 0), K) : K;
-  const int64_t base = max(lens[b], 0), cap = (int64_t)W << lp;
-  codes += ((int64_t)layer * pages * H) << (lm + lp);
-  values += ((int64_t)layer * pages * H * DV) << lp;
-  // row of head 0, [page][head][slot]
-  auto place = [&](int64_t pos) -> int64_t {
-    if (pos < 0 || pos >= cap) return -1;
-    const int page = table[(int64_t)b * W + (pos >> lp)];
-    return (unsigned)page < (unsigned)pages ? (((int64_t)page * H) << lp) + (pos & ((1 << lp) - 1)) : -1;
-  };
+  const int b = id % a.B, layer = id / a.B;
+  const CompactSeq sq(a, table, lens, keep_lens, b);
+  const int count = sq.count;
+  codes += ((int64_t)layer * a.pages * H) << (lm + lp);
+  values += ((int64_t)layer * a.pages * H * DV) << lp;
   const int batch = TH >> lh, heads = min(1 << lh, H - h0), lc = lm - 3;
   for (int k0 = 0; k0 < count; k0 += batch) {
     const int nk = min(batch, count - k0);
     if ((int)threadIdx.x < nk) {
-      const int64_t rel = keep[(int64_t)b * K + k0 + threadIdx.x];
-      const int64_t f = rel < 0 ? -1 : place(base + rel), t = place(base + k0 + threadIdx.x);
-      from[threadIdx.x] = f;
-      to[threadIdx.x] = f < 0 || f == t ? -1 : t;
+      const int k = k0 + threadIdx.x;
+      sq.move(k, keep[(int64_t)b * a.K + k], from[threadIdx.x], to[threadIdx.x]);
     }
     __syncthreads();
     f16x8 cv[CPER];
@@ -1253,14 +1273,117 @@ __global__ __launch_bounds__(256) void cache_compact_kernel(f16* codes, f16* val
   }
 }
 
+// Many tokens a sequence: one workgroup a (layer, sequence, head, 8 value
+// columns) and one a (layer, sequence, head) for the codes, 512 tokens a
+// batch, from a whole group of 8 places on. A lane gathers the 8 values of a
+// group and column and stores them as one; the next batch's places are found
+// while this one's values come.
+template <int DV>
+__global__ __launch_bounds__(256) void cache_compact_long_kernel(CompactArgs a, f16* codes, f16* values,
+                                                                const int* __restrict__ table,
+                                                                const int* __restrict__ lens,
+                                                                const int* __restrict__ keep,
+                                                                const int* __restrict__ keep_lens) {
+  constexpr int BT = 512, SL = DV / 8 + 1;
+  // three batches' places: one is written while a slower wave still reads the one before last
+  __shared__ int64_t from[3][BT], to[3][BT];
+  const int H = a.H, lm = a.lm, lp = a.lp;
+  int id = blockIdx.x;
+  const int slice = id % SL;  // 0: codes
+  id /= SL;
+  const int h = id % H;
+  id /= H;
+  const int b = id % a.B, layer = id / a.B;
+  const CompactSeq sq(a, table, lens, keep_lens, b);
+  codes += (((int64_t)layer * a.pages * H) << (lm + lp)) + ((int64_t)h << (lm + lp));
+  values += (((int64_t)layer * a.pages * H * DV) << lp) + (((int64_t)h * DV) << lp) + 64 * (slice - 1);
+  const int begin = -(int)(sq.base & 7);  // kept token of the first place of a group, mostly not one
+  auto find = [&](int k0, int buf) {
+#pragma unroll
+    for (int i = 0; i < BT / 256; ++i) {
+      const int at = threadIdx.x + 256 * i, k = k0 + at;
+      int64_t f = -1, t = -1;
+      if (k >= 0 && k < sq.count) sq.move(k, keep[(int64_t)b * a.K + k], f, t);
+      from[buf][at] = f;
+      to[buf][at] = t;
+    }
+  };
+  find(begin, 0);
+  __syncthreads();
+  int buf = 0;
+  for (int k0 = begin; k0 < sq.count; k0 += BT) {
+    const bool more = k0 + BT < sq.count;
+    const int next = buf == 2 ? 0 : buf + 1;
+    if (slice == 0) {
+      constexpr int CPER = BT * 8 / 256;  // 8-code pieces of a lane, at most (cube_m 64)
+      const int lc = lm - 3;
+      f16x8 cv[CPER];
+#pragma unroll
+      for (int i = 0; i < CPER; ++i) {
+        const int e = threadIdx.x + 256 * i, k = e >> lc;
+        if (k < BT && to[buf][k] >= 0)
+          cv[i] = *reinterpret_cast<const f16x8*>(codes + (from[buf][k] << lm) + 8 * (e & ((1 << lc) - 1)));
+      }
+      if (more) find(k0 + BT, next);
+      wait_vmcnt<0>();
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < CPER; ++i) {
+        const int e = threadIdx.x + 256 * i, k = e >> lc;
+        if (k < BT && to[buf][k] >= 0)
+          *reinterpret_cast<f16x8*>(codes + (to[buf][k] << lm) + 8 * (e & ((1 << lc) - 1))) = cv[i];
+      }
+    } else {
+      // lane: column threadIdx % 8 of the slice, groups threadIdx / 8 and 32 on
+      f16x8 v[2];
+      const int c = threadIdx.x & 7;
+      auto at = [&](int64_t row) { return values + (row & ~(int64_t)7) * DV + 8 * c + (row & 7); };
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int k = 8 * ((threadIdx.x >> 3) + 32 * i) + j;
+          if (to[buf][k] >= 0) v[i][j] = *at(from[buf][k]);
+        }
+      if (more) find(k0 + BT, next);
+      wait_vmcnt<0>();
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int k = 8 * ((threadIdx.x >> 3) + 32 * i);
+        bool all = true;  // a group lies in one page
+#pragma unroll
+        for (int j = 0; j < 8; ++j) all = all && to[buf][k + j] >= 0;
+        if (all) {
+          *reinterpret_cast<f16x8*>(at(to[buf][k])) = v[i];
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (to[buf][k + j] >= 0) *at(to[buf][k + j]) = v[i][j];
+        }
+      }
+    }
+    // the barrier above lies between this batch's reads and its writes, and
+    // behind the next batch's places; that batch reads nothing written here
+    buf = next;
+  }
+}
+
 hipError_t launch_cache_compact(const CacheDims& d, f16* codes, f16* values, const int* table, const int* lens,
                                 const int* keep, const int* keep_lens, int K, hipStream_t s) {
-  const int lh = log2_of(cache_compact_heads(d.layers * (int64_t)d.B, d.H, d.DV)), groups = (d.H + (1 << lh) - 1) >> lh;
-  const dim3 grid((unsigned)((int64_t)d.layers * d.B * groups)), block(256);
-  const int lp = log2_of(d.P), lm = log2_of(d.M);
-#define MORPHO_CACHE_COMPACT(DV)                                                                               \
-  MORPHO_KLAUNCH((cache_compact_kernel<DV>), grid, block, 0, s, codes, values, table, lens, keep, keep_lens,   \
-                 d.B, d.H, lm, d.pages, d.W, lp, K, lh)
+  const CompactArgs a{d.B, d.H, log2_of(d.M), d.pages, d.W, log2_of(d.P), K};
+  const int64_t sequences = (int64_t)d.layers * d.B;
+  const int heads = cache_compact_heads(sequences, d.H, d.DV, K);
+  const dim3 block(256);
+#define MORPHO_CACHE_COMPACT(DV)                                                                                   \
+  do {                                                                                                             \
+    if (heads)                                                                                                     \
+      MORPHO_KLAUNCH((cache_compact_kernel<DV>), dim3((unsigned)(sequences * ((d.H + heads - 1) / heads))), block, \
+                     0, s, a, codes, values, table, lens, keep, keep_lens, log2_of(heads));                       \
+    else                                                                                                           \
+      MORPHO_KLAUNCH((cache_compact_long_kernel<DV>), dim3((unsigned)(sequences * d.H * (DV / 8 + 1))), block, 0,  \
+                     s, a, codes, values, table, lens, keep, keep_lens);                                          \
+  } while (0)
   if (d.DV == 32)
     MORPHO_CACHE_COMPACT(32);
   else if (d.DV == 64)
