@@ -17,6 +17,14 @@ LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libmorphott
 _lib = None
 
 
+class Cache(ctypes.Structure):
+    """``morpho_cache``: a pool of pages."""
+
+    _fields_ = [("codes", ctypes.c_void_p), ("values", ctypes.c_void_p), ("layers", ctypes.c_int64),
+                ("pages", ctypes.c_int64), ("H", ctypes.c_int64), ("cube_m", ctypes.c_int64),
+                ("head_dim_v", ctypes.c_int64), ("page_size", ctypes.c_int64)]
+
+
 def lib() -> ctypes.CDLL:
     global _lib
     if _lib is None:
@@ -51,6 +59,18 @@ def lib() -> ctypes.CDLL:
         L.morpho_soft_backward.restype = ctypes.c_int
         L.morpho_soft_backward.argtypes = ([vp] * 8 + [vp] * 6 + [i64] * 5
                                            + [ctypes.c_float, ctypes.c_int, ctypes.c_int, vp, vp, sz, vp])
+        pool = ctypes.POINTER(Cache)
+        L.morpho_cache_append.restype = ctypes.c_int
+        L.morpho_cache_append.argtypes = [vp, vp, pool, vp, vp, vp, vp, i64, i64, i64, ctypes.c_int, vp]
+        L.morpho_cache_attention_workspace_size.restype = sz
+        L.morpho_cache_attention_workspace_size.argtypes = [pool] + [i64] * 4
+        L.morpho_cache_attention.restype = ctypes.c_int
+        L.morpho_cache_attention.argtypes = ([vp] * 3 + [pool] + [vp] * 6 + [i64] * 4
+                                             + [ctypes.c_float, ctypes.c_int, vp, sz, vp])
+        L.morpho_cache_copy_pages.restype = ctypes.c_int
+        L.morpho_cache_copy_pages.argtypes = [pool, vp, vp, i64, vp]
+        L.morpho_cache_compact.restype = ctypes.c_int
+        L.morpho_cache_compact.argtypes = [pool] + [vp] * 4 + [i64] * 3 + [vp]
         L.morpho_timing_enable.restype = ctypes.c_int
         L.morpho_timing_enable.argtypes = [ctypes.c_int]
         L.morpho_timing_only.restype = ctypes.c_int
@@ -81,6 +101,10 @@ def soft_forward_workspace_size(B: int, N: int, D: int, H: int, cube_m: int) -> 
 
 def soft_backward_workspace_size(B: int, N: int, D: int, H: int, cube_m: int, have_forward_workspace: bool) -> int:
     return int(lib().morpho_soft_backward_workspace_size(B, N, D, H, cube_m, int(have_forward_workspace)))
+
+
+def cache_attention_workspace_size(cache: Cache, B: int, n: int, seq_pages: int, max_len: int) -> int:
+    return int(lib().morpho_cache_attention_workspace_size(ctypes.byref(cache), B, n, seq_pages, max_len))
 
 
 def timing_enable(enable: bool) -> None:

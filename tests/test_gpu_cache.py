@@ -561,6 +561,62 @@ def test_a_captured_step_follows_the_lengths():
             assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
+def test_c_abi_direct_matches_the_ops():
+    """The C entry points with a workspace of the caller's, against the torch ops."""
+    import ctypes
+
+    from morphottention_amd import capi
+    L = capi.lib()
+    p = Problem(2, 2, 2, 16, 64, [900, 1500], seed=12)
+    d = p.device()
+    pool = capi.Cache(d["codes"].data_ptr(), d["values"].data_ptr(), 1, d["codes"].shape[0], 2, 16, 64, 64)
+    ref = ctypes.byref(pool)
+    W, stream = d["table"].shape[1], torch.cuda.current_stream().cuda_stream
+    want = p.attend(d, max_len=1502)
+    out, lse = torch.empty_like(want[0]), torch.empty_like(want[1])
+    size = capi.cache_attention_workspace_size(pool, 2, 2, W, 1502)
+    assert size > 0
+    ws = torch.empty(size, dtype=torch.uint8, device=DEV)
+    assert L.morpho_cache_attention(d["phi"].data_ptr(), d["gq"].data_ptr(), d["gk"].data_ptr(), ref,
+                                    d["table"].data_ptr(), d["lens"].data_ptr(), None, None, out.data_ptr(),
+                                    lse.data_ptr(), 2, 2, W, 1502, p.scale, 1, ws.data_ptr(), size, stream) == 0
+    assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+    x, w = torch.randn((2, 2, 128), device=DEV).half(), torch.randn((160, 128), device=DEV).half() / 11
+    phi = torch.empty((2, 2, 2, 16), dtype=torch.float16, device=DEV)
+    mine = d["codes"].clone(), d["values"].clone()
+    assert L.morpho_cache_append(x.data_ptr(), w.data_ptr(), ref, d["table"].data_ptr(), d["lens"].data_ptr(), None,
+                                 phi.data_ptr(), 2, 2, W, 0, stream) == 0
+    assert torch.equal(phi, ma.morpho_cache_append(x, w, mine[0], mine[1], d["table"], d["lens"]))
+    assert torch.equal(mine[0].view(torch.int16), d["codes"].view(torch.int16))
+    assert torch.equal(mine[1].view(torch.int16), d["values"].view(torch.int16))
+
+
+def test_refused_tensors():
+    """Wrong types, shapes, layouts and places raise before anything runs."""
+    p = Problem(2, 2, 2, 16, 64, [9, 15], seed=13)
+    d = p.device()
+    call = lambda **kw: p.attend(d | kw)  # noqa: E731
+    for kw, text in (({"phi": d["phi"].float()}, "float16"), ({"codes": d["codes"].cpu()}, "CUDA"),
+                     ({"phi": d["phi"].transpose(0, 1)}, "contiguous"), ({"table": d["table"].long()}, "int32"),
+                     ({"lens": d["lens"][:1]}, "lens must be"), ({"table": d["table"][:1]}, "table must be"),
+                     ({"gq": d["gq"][:1]}, "gate_q must be"), ({"phi": d["phi"][:, :, :1].contiguous()}, "phi must be"),
+                     ({"values": d["values"][:1]}, "values must be"), ({"new_lens": d["lens"].float()}, "int32"),
+                     ({"codes": d["codes"][None]}, "codes must be")):
+        with pytest.raises((RuntimeError, NotImplementedError), match=text if text != "CUDA" else None):
+            call(**kw)
+    with pytest.raises(RuntimeError, match="tree must be"):
+        p.attend(d, tree=torch.zeros((2, 2), dtype=torch.int32, device=DEV))
+    big = Problem(1, 65, 1, 16, 32, [3], seed=14)
+    with pytest.raises(RuntimeError, match="64 drafted"):
+        big.attend(big.device(), tree=torch.zeros((1, 65), dtype=torch.int64, device=DEV))
+    with pytest.raises(RuntimeError, match="X must be"):
+        ma.morpho_cache_append(torch.zeros((2, 2, 64), device=DEV).half(), torch.zeros((160, 128), device=DEV).half(),
+                               d["codes"], d["values"], d["table"], d["lens"])
+    with pytest.raises(RuntimeError, match="weights must be"):
+        ma.morpho_cache_append(torch.zeros((2, 2, 128), device=DEV).half(), torch.zeros((128, 160), device=DEV).half(),
+                               d["codes"], d["values"], d["table"], d["lens"])
+
+
 def test_another_stream():
     p = Problem(2, 3, 2, 16, 64, [900, 1500], seed=11)
     d = p.device()
