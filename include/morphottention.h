@@ -248,7 +248,10 @@ size_t morpho_cache_attention_workspace_size(const morpho_cache* cache, int64_t 
  * where bit k of tree[b][i] is set. A row that sees nothing, and a padding
  * row, gets out 0 and lse -FLT_MAX. max_len: at least the longest lens[b] +
  * new_lens[b]; it sets the launch shape only (a longer sequence is still
- * computed in full). cache->layers must be 1. */
+ * computed in full). cache->layers must be 1.
+ * Numeric range: scale * log2(e) * gate_q[h][c] * gate_k[h][c] * (2 phi - 1) of
+ * a query must stay below 65,504 for every code, or the row is NaN. A value
+ * that is not finite reaches the rows that see its key, and no other. */
 int morpho_cache_attention(const void* phi, const void* gate_q, const void* gate_k, const morpho_cache* cache,
                            const int32_t* table, const int32_t* lens, const int32_t* new_lens, const int64_t* tree,
                            void* out, float* lse, int64_t B, int64_t n, int64_t seq_pages, int64_t max_len,

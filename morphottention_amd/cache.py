@@ -124,7 +124,8 @@ def morpho_cache_attention(phi: torch.Tensor, gate_q: torch.Tensor, gate_k: torc
         work is split, not what is computed; the table's whole length if not given.
     :returns: ``out`` ``[B, n, D]`` and the base-2 log-sum-exp of the row scores
         ``[B * H, n]`` (float32). A row that sees nothing, and a padding row,
-        has 0 and ``-FLT_MAX``.
+        has 0 and ``-FLT_MAX``. ``scale * gate_q * gate_k`` has to stay below
+        22,700 (codes within [0, 1]), as in the whole-sequence forward.
     """
     if max_len is not None and max_len <= 0:
         raise ValueError(f"max_len must be positive (got {max_len})")
@@ -177,6 +178,7 @@ class MorphoCache:
     :param num_heads, cube_m, head_dim: of the layers' ``MorphoAttention``.
     :param num_layers: layers that share the account of pages.
     :param page_size: tokens a page: 32, 64, 128 or 256.
+    :param device: where the pages are; the kernels need a ROCm device.
 
     A step appends tokens to some sequences and is then committed::
 
