@@ -149,7 +149,7 @@ int soft_bwd_slots(const Dims& d);    // workgroup slots of both backward kernel
 // kernels_cache.hip: the paged cache of key codes and values (CacheDims).
 struct CacheAttnBuffers {
   float* o;    // [B, H, n, nsplit, DV] unnormalised sums of a piece's weighted values
-  float4* st;  // [B, H, n, nsplit] {reference, sum of weights, the output's divisor, row constant}
+  float4* st;  // [B, H, n, nsplit] {reference, sum of weights, row constant, 0}
 };
 hipError_t launch_cache_append(const CacheDims& d, const _Float16* X, const _Float16* W, _Float16* codes,
                                _Float16* values, const int* table, const int* lens, const int* new_lens,

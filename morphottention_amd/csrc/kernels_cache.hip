@@ -112,8 +112,10 @@ struct CacheSource {
 // keeps what is 2^-36 of the largest.
 // LO: the weights enter the value product as hi / lo pairs, and the output is
 // exact to fp32 rounding too (where reading the keys is the bound, the second
-// product is free). Without, they are rounded to fp16 once, and the normaliser
-// sums the rounded ones (a product with ones: no VALU work).
+// product is free). Without, they are rounded to fp16 once: each moves its
+// value's share by up to 2^-11, the divisor sums them unrounded. (Summing the
+// rounded ones, by a product with ones, costs a seventh of the MFMAs; what it
+// would take off, their mean error, is 2^-12 over the root of the keys.)
 template <int M, int DV, int QT, bool LO>
 struct CacheRows {
   static constexpr int KC = CacheTile<M, DV>::KC, NT = CacheTile<M, DV>::NT;
@@ -122,7 +124,6 @@ struct CacheRows {
   f32x4 off[QT];  // minus the reference, in every register
   float thr[QT];  // exponent from which the reference moves: 15, -inf before the first score
   float sum[QT];  // of this lane's weights
-  f32x4 l16[QT];  // !LO: sum of all rounded weights, in every register
   f32x4 O[QT][NT];
 
   // Rows first .. first + 16 QT - 1, those from n on repeating the last; rc: the rows' constants.
@@ -159,7 +160,6 @@ struct CacheRows {
       off[t] = f32x4{};
       thr[t] = kNegInf;
       sum[t] = 0.f;
-      l16[t] = f32x4{};
 #pragma unroll
       for (int c = 0; c < NT; ++c) O[t][c] = f32x4{};
     }
@@ -220,7 +220,6 @@ struct CacheRows {
           s[n][t][1] -= up;
         }
         sum[t] *= f;
-        l16[t] *= f;
 #pragma unroll
         for (int c = 0; c < NT; ++c) O[t][c] *= f;
       }
@@ -234,8 +233,8 @@ struct CacheRows {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           p[j] = fast_exp2(s[n][t][j >> 2][j & 3]);
-          sum[t] += p[j];
           if constexpr (LO) {
+            sum[t] += p[j];  // one after another: few registers (few rows are bound by loads in flight)
             f16 ph, pl;
             split_exact(p[j], ph, pl);
             hi[j] = ph;
@@ -244,10 +243,7 @@ struct CacheRows {
             hi[j] = (f16)p[j];
           }
         }
-        if constexpr (!LO) {
-          const f16 one = (f16)1.f;
-          l16[t] = mfma16x16(f16x8{one, one, one, one, one, one, one, one}, hi, l16[t]);
-        }
+        if constexpr (!LO) sum[t] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
 #pragma unroll
         for (int c = 0; c < NT; ++c) {
           O[t][c] = mfma16x16(T[n].v[c], hi, O[t][c]);
@@ -262,13 +258,11 @@ struct CacheRows {
     add<false>(T, [](int) { return 0u; }, [](int, const float(&)[8], unsigned) {});
   }
 
-  // After the last tile: the reference, the sum of the weights for the
-  // log-sum-exp and the one that the output is divided by.
-  __device__ __forceinline__ void finish(int t, float& ref, float& l, float& div) {
+  // After the last tile: the reference and the sum of the weights.
+  __device__ __forceinline__ void finish(int t, float& ref, float& l) const {
     ref = thr[t] > 0.f ? -off[t][0] : -1e30f;  // nothing seen: below every other
-    l = sum[t] + __shfl_xor(sum[t], 16);  // the lane groups hold their own keys of the same 16 queries
+    l = sum[t] + __shfl_xor(sum[t], 16);       // the lane groups hold their own keys of the same 16 queries
     l += __shfl_xor(l, 32);
-    div = LO ? l : l16[t][0];
   }
 };
 
@@ -356,18 +350,18 @@ struct CacheOut {
   float* part_o;
   float4* part_st;
   int n, H, b, h, nb, nsplit, sp;
-  // m, l: reference and sum of the weights; div: what the output is divided by; r: the row constant
-  __device__ __forceinline__ void operator()(int i, int c, f32x4 o, float m, float l, float div, float r) const {
+  // m, l: reference and sum of the weights; r: the row constant
+  __device__ __forceinline__ void operator()(int i, int c, f32x4 o, float m, float l, float r) const {
     if (i >= n) return;
     const int64_t at = ((int64_t)b * H + h) * n + i;
     if (nsplit > 1) {
       if (i >= nb) return;  // the joining kernel writes padding rows
       *reinterpret_cast<f32x4*>(part_o + (at * nsplit + sp) * DV + c) = o;
-      if (c == 0) part_st[at * nsplit + sp] = float4{m, l, div, r};
+      if (c == 0) part_st[at * nsplit + sp] = float4{m, l, r, 0.f};
       return;
     }
     const bool some = i < nb && l != 0.f;  // padding rows and rows that see nothing get 0
-    const float inv = some ? 1.f / div : 0.f;
+    const float inv = some ? 1.f / l : 0.f;
     f16x4 y;
 #pragma unroll
     for (int k = 0; k < 4; ++k) y[k] = some ? (f16)(o[k] * inv) : (f16)0.f;
@@ -472,8 +466,8 @@ __global__ __launch_bounds__(256) void cache_attn_few_kernel(
 
   __shared__ __align__(16) float so[4][16][DV + 4];
   __shared__ float sm[4][16], sl[4][16], sr[16];
-  float ref, l, div;
-  R.finish(0, ref, l, div);
+  float ref, l;
+  R.finish(0, ref, l);
 #pragma unroll
   for (int c = 0; c < NT; ++c) *reinterpret_cast<f32x4*>(&so[w][c16][16 * c + 4 * g]) = R.O[0][c];
   if (g == 0) {
@@ -497,7 +491,7 @@ __global__ __launch_bounds__(256) void cache_attn_few_kernel(
       l += f * sl[k][q];
       o += f * *reinterpret_cast<const f32x4*>(&so[k][q][c]);
     }
-    put(q, c, o, m, l, l, sr[q]);
+    put(q, c, o, m, l, sr[q]);
   }
 }
 
@@ -506,7 +500,7 @@ __global__ __launch_bounds__(256) void cache_attn_few_kernel(
 // order in which the lanes read them as operands (a wave fetches every fourth
 // operand; 1 KiB each, conflict-free both ways).
 template <int M, int DV, int QT>
-__global__ __launch_bounds__(256, 2) void cache_attn_rows_kernel(
+__global__ __launch_bounds__(256, M <= 32 && DV <= 64 ? 3 : 2) void cache_attn_rows_kernel(
     CacheAttnArgs a, const f16* __restrict__ phi, const f16* __restrict__ gate_q, const f16* __restrict__ gate_k,
     const f16* __restrict__ codes, const f16* __restrict__ values, const int* __restrict__ table,
     const int* __restrict__ lens, const int* __restrict__ new_lens, const int64_t* __restrict__ tree,
@@ -671,10 +665,10 @@ __global__ __launch_bounds__(256, 2) void cache_attn_rows_kernel(
   const CacheOut<DV> put{out, lse, part_o, part_st, a.n, a.H, b, h, sq.nb, a.nsplit, blk.sp};
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
-    float ref, l, div;
-    R.finish(t, ref, l, div);
+    float ref, l;
+    R.finish(t, ref, l);
 #pragma unroll
-    for (int c = 0; c < NT; ++c) put(qw + 16 * t + c16, 16 * c + 4 * g, R.O[t][c], ref, l, div, rc[t]);
+    for (int c = 0; c < NT; ++c) put(qw + 16 * t + c16, 16 * c + 4 * g, R.O[t][c], ref, l, rc[t]);
   }
 }
 
@@ -695,41 +689,39 @@ __global__ __launch_bounds__(256) void cache_join_kernel(CacheAttnArgs a, int64_
   const SeqLen sq = seq_len(lens, new_lens, b, a.n, a.W << a.lp);
   const int pieces =
       at < rows && i < sq.nb ? min(a.nsplit, (sq.total + a.split_keys - 1) / a.split_keys) : 0;
-  float m = -1e30f, l = 0.f, div = 0.f, r = 0.f;
+  float m = -1e30f, l = 0.f, r = 0.f;
   f32x4 o = {};
   for (int s = k; s < pieces; s += NG) {
     const float4 st = part_st[at * a.nsplit + s];
     const f32x4 x = *reinterpret_cast<const f32x4*>(part_o + (at * a.nsplit + s) * DV + c);
     const float nm = fmaxf(m, st.x), f = fast_exp2(m - nm), fs = fast_exp2(st.x - nm);
     l = l * f + st.y * fs;
-    div = div * f + st.z * fs;
     o = o * f + x * fs;
-    r = st.w;  // the same in every piece
+    r = st.z;  // the same in every piece
     m = nm;
   }
   if constexpr (NG > 1) {
     __shared__ __align__(16) float so[ROWS][NG][DV];
-    __shared__ float4 ss[ROWS][NG];
+    __shared__ float2 ss[ROWS][NG];
     *reinterpret_cast<f32x4*>(&so[rl][k][c]) = o;
-    if (c == 0) ss[rl][k] = float4{m, l, div, 0.f};
+    if (c == 0) ss[rl][k] = float2{m, l};
     __syncthreads();
     if (k != 0) return;
 #pragma unroll
     for (int e = 1; e < NG; ++e) m = fmaxf(m, ss[rl][e].x);
-    l = div = 0.f;
+    l = 0.f;
     o = f32x4{};
 #pragma unroll
     for (int e = 0; e < NG; ++e) {
-      const float4 st = ss[rl][e];
+      const float2 st = ss[rl][e];
       const float f = fast_exp2(st.x - m);
       l += f * st.y;
-      div += f * st.z;
       o += f * *reinterpret_cast<const f32x4*>(&so[rl][e][c]);
     }
   }
   if (at >= rows) return;
   const CacheOut<DV> put{out, lse, nullptr, nullptr, a.n, a.H, b, h, sq.nb, 1, 0};
-  put(i, c, o, m, l, div, r);
+  put(i, c, o, m, l, r);
 }
 
 namespace {

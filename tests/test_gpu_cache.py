@@ -8,10 +8,9 @@ Tolerances (fp16 rounds by at most 2^-11 of a value):
   most (2^-22 + m 2^-23) S in base 2, taken with both signs by the weights and
   their sum; the exponential and the split of a weight add 2^-20. Summing k
   weights one after another adds k 2^-24 at most, the lanes' partial sums have
-  k / 16 terms each. Beyond 64 new tokens the weights are rounded to fp16 and
-  the divisor sums the rounded ones: sum p (1 + e) v / sum p (1 + e), |e| <=
-  2^-11, is off by at most 2^-11 sum p |v - out| / sum p <= 2^-10 max |v| (to
-  first order; 2^-9.9 with the rest).
+  k / 16 terms each. Beyond 64 new tokens the weights of the values are rounded
+  to fp16, those of the divisor are not: sum p (1 + e) v / sum p, |e| <= 2^-11,
+  is off by at most 2^-11 max |v|.
 * log-sum-exp: the score's error, the row constant's of the same size, and 2^-20
   (1 + |lse|).
 * append: a sum of D products in fp32, D 2^-24 sum |x w| at most, the sigmoid's
@@ -122,7 +121,7 @@ class Problem:
                     lse[b, h, i] = top + torch.log2(w.sum()) - r[i]
                     rel = 2 * e * math.log(2) + 2.0 ** -20 + len(at) / 16 * 2.0 ** -24
                     if n > 64:
-                        rel += 2.0 ** -9.9
+                        rel += 2.0 ** -11
                     tol_out[b, i, h] = out[b, i, h].abs() * 2.0 ** -11 + rel * v[at].abs().max() + 2.0 ** -25
                     tol_lse[b, h, i] = 2 * e + 2.0 ** -20 * (1 + lse[b, h, i].abs()) + len(at) / 16 * 2.0 ** -24
         return (out.reshape(B, n, H * dv), lse.reshape(B * H, n), tol_out.reshape(B, n, H * dv),
