@@ -230,6 +230,9 @@ struct CacheRows {
       for (int t = 0; t < QT; ++t) {
         f16x8 hi, lo;
         float p[8];
+        // the exponentials go before another wave's products (B4 n1000 over
+        // 4096 keys 90.2 -> 87.9 us; the products first 89.2)
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           p[j] = fast_exp2(s[n][t][j >> 2][j & 3]);
@@ -243,6 +246,7 @@ struct CacheRows {
             hi[j] = (f16)p[j];
           }
         }
+        __builtin_amdgcn_s_setprio(0);
         if constexpr (!LO) sum[t] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
 #pragma unroll
         for (int c = 0; c < NT; ++c) {
@@ -1002,24 +1006,24 @@ __global__ __launch_bounds__(kGemmThreads) void cache_append_tile_kernel(
   const int m0 = BM * tr, n0 = BN * tc;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const AppendRows rows{a.shift ? lens : nullptr, a.NR, a.n};
+  // the tile's rows: token (-1: none) and place in the pool (-1: not stored),
+  // looked up before the main loop, which hides the chain of loads
+  int my_token = -1;
+  int64_t my_place = -1;
+  if (threadIdx.x < BM && m0 + (int)threadIdx.x < a.TR) {
+    const int r = m0 + threadIdx.x, b = r / a.NR, i = r - b * a.NR - rows.shift(b);
+    if (i >= 0 && i < a.n) {
+      my_token = b * a.n + i;
+      my_place = token_row(a, table, lens, new_lens, b, i);
+    }
+  }
   f32x4 acc[G::FI][G::FJ];
   G::run(X, a.D, Wt, a.D, a.TR, a.C, m0, n0, 0, a.D, lds, acc, rows);
-  // the tile's rows: token (-1: none) and place in the pool (-1: not stored)
   auto token = reinterpret_cast<int*>(lds);
   auto place = reinterpret_cast<int64_t*>(lds + BM * 4);
   if (threadIdx.x < BM) {
-    const int r = m0 + threadIdx.x;
-    int t = -1;
-    int64_t p = -1;
-    if (r < a.TR) {
-      const int b = r / a.NR, i = r - b * a.NR - rows.shift(b);
-      if (i >= 0 && i < a.n) {
-        t = b * a.n + i;
-        p = token_row(a, table, lens, new_lens, b, i);
-      }
-    }
-    token[threadIdx.x] = t;
-    place[threadIdx.x] = p;
+    token[threadIdx.x] = my_token;
+    place[threadIdx.x] = my_place;
   }
   __syncthreads();
   const int wm = w / G::WN, wn = w % G::WN, c16 = lane & 15, g = lane >> 4;
