@@ -831,15 +831,16 @@ __device__ __forceinline__ f16* value_place(const CacheAppendArgs& a, f16* value
 }
 
 // Few tokens: a workgroup of 8 waves per 16 CT output columns and 16 TT
-// tokens. Each wave contracts an eighth of D, 32 wide steps that it brings to
+// tokens. Each wave contracts an eighth of D, 64 wide steps that it brings to
 // LDS for itself (no barriers), and the partial tiles are added in LDS, the
 // upper four waves' first.
 // The operands go through LDS because a lane of the MFMA holds 16 bytes of the
 // row lane % 16: loaded so from row-major memory, neighbouring lanes are rows
-// apart, and the address unit takes them one at a time. Here four neighbours
-// fetch 64 bytes of a row (chunk p of row r holds k chunk p ^ (r / 4 % 4), so
-// that the reads of 8 rows of one chunk hit all banks). T 192, D 2048, C 4096:
-// 19.4 us loaded directly.
+// apart, and the address unit takes them one at a time. Here eight neighbours
+// fetch a 128-byte line of a row (place p of row r holds k chunk p ^ (r / 2 %
+// 8), so that the reads of 16 rows of one chunk hit all banks). T 192, D 2048,
+// C 4096: 19.4 us loaded directly, 13.1 by half lines (the L1 loses the other
+// half before its turn).
 template <int CT, int TT>
 __global__ __launch_bounds__(512) void cache_append_rows_kernel(CacheAppendArgs a, const f16* __restrict__ X,
                                                                const f16* __restrict__ Wt, f16* __restrict__ codes,
@@ -848,8 +849,9 @@ __global__ __launch_bounds__(512) void cache_append_rows_kernel(CacheAppendArgs 
                                                                const int* __restrict__ lens,
                                                                const int* __restrict__ new_lens,
                                                                f16* __restrict__ phi) {
-  constexpr int NF = CT + TT, NS = CT == 4 ? 2 : 3;  // operands of a step, 1 KiB each; steps in LDS
-  constexpr int kStage = NF * 1024, kSum = 4 * 16 * TT * (16 * CT + 4) * 4;
+  // operands of a step, 2 KiB each, and steps in LDS: as many as fit
+  constexpr int NF = CT + TT, NS = NF <= 3 ? 3 : NF == 4 ? 2 : 1;
+  constexpr int kStage = NF * 2048, kSum = 4 * 16 * TT * (16 * CT + 4) * 4;
   __shared__ __align__(1024) char smem[8 * NS * kStage > kSum ? 8 * NS * kStage : kSum];
   auto part = reinterpret_cast<float(*)[16 * TT][16 * CT + 4]>(smem);  // [wave][token][column]
   __shared__ int64_t slot[16 * TT];
@@ -861,54 +863,72 @@ __global__ __launch_bounds__(512) void cache_append_rows_kernel(CacheAppendArgs 
   for (int c = 0; c < CT; ++c)
 #pragma unroll
     for (int t = 0; t < TT; ++t) acc[c][t] = f32x4{};
-  const int s0 = a.D / 32 * w / 8, ns = a.D / 32 * (w + 1) / 8 - s0;  // this wave's steps
-  // a lane's byte offsets from the step's first k of row 0 of the tile; rows
-  // past the end repeat the last
-  unsigned off[NF];
-  {
-    const int r = lane >> 2, chunk = (lane & 3) ^ ((lane >> 4) & 3);
+  const int steps = (a.D + 63) / 64, s0 = steps * w / 8, ns = steps * (w + 1) / 8 - s0;  // this wave's steps
+  // a lane's byte offsets from the step's first k of row 0 of the tile, 8 rows
+  // at a time; rows past the end repeat the last
+  unsigned off[NF][2];
 #pragma unroll
-    for (int c = 0; c < CT; ++c) off[c] = (unsigned)(min(16 * c + r, a.C - 1 - col0) * a.D + 8 * chunk) * 2u;
+  for (int i = 0; i < 2; ++i) {
+    const int r = 8 * i + (lane >> 3), chunk = (lane & 7) ^ ((r >> 1) & 7);
 #pragma unroll
-    for (int t = 0; t < TT; ++t) off[CT + t] = (unsigned)(min(16 * t + r, a.T - 1 - t0) * a.D + 8 * chunk) * 2u;
+    for (int c = 0; c < CT; ++c) off[c][i] = (unsigned)(min(16 * c + r, a.C - 1 - col0) * a.D + 8 * chunk) * 2u;
+#pragma unroll
+    for (int t = 0; t < TT; ++t) off[CT + t][i] = (unsigned)(min(16 * t + r, a.T - 1 - t0) * a.D + 8 * chunk) * 2u;
   }
-  const char* wp = reinterpret_cast<const char*>(Wt + (int64_t)col0 * a.D + 32 * s0);
-  const char* xp = reinterpret_cast<const char*>(X + (int64_t)t0 * a.D + 32 * s0);
+  // D is a multiple of 32: of a last step of 32 the upper chunks repeat the lower ones, for nothing
+  const bool odd = (a.D & 63) != 0;
+  const unsigned upper[2] = {((lane & 7) ^ ((lane >> 4) & 7)) >= 4 ? 64u : 0u,
+                             ((lane & 7) ^ (((lane >> 4) + 4) & 7)) >= 4 ? 64u : 0u};
+  const char* wp = reinterpret_cast<const char*>(Wt + (int64_t)col0 * a.D + 64 * s0);
+  const char* xp = reinterpret_cast<const char*>(X + (int64_t)t0 * a.D + 64 * s0);
   const unsigned mine = (unsigned)(w * NS * kStage);
   const unsigned base = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)smem + mine;
-  unsigned fill = 0, read = 0;  // the next step's place, that of the step at hand
-  auto issue = [&]() {
+  unsigned at = 0;  // place of the step at hand, which the step NS behind it takes
+  auto issue = [&](int i, unsigned to) {
+    const bool half = odd && s0 + i == steps - 1;
 #pragma unroll
-    for (int f = 0; f < NF; ++f) lds_dma16_so(f < CT ? wp : xp, off[f], base + fill + 1024u * (unsigned)f);
-    wp += 64;
-    xp += 64;
-    fill = fill == (NS - 1) * kStage ? 0 : fill + kStage;
+    for (int f = 0; f < NF; ++f)
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        lds_dma16_so(f < CT ? wp : xp, off[f][k] - (half ? upper[k] : 0u), base + to + 2048u * f + 1024u * k);
+    wp += 128;
+    xp += 128;
   };
 #pragma unroll
-  for (int i = 0; i < NS - 1; ++i)
-    if (i < ns) issue();
+  for (int i = 0; i < NS; ++i)
+    if (i < ns) issue(i, (unsigned)(i * kStage));
   if (threadIdx.x < 16 * TT) {
     const int t = min(t0 + (int)threadIdx.x, a.T - 1), b = t / a.n;
     slot[threadIdx.x] = token_row(a, table, lens, new_lens, b, t - b * a.n);
   }
-  const char* from = smem + mine + 16 * (4 * c16 + (g ^ ((c16 >> 2) & 3)));
   for (int i = 0; i < ns; ++i) {
-    // the step has landed, those behind it may not have; the reads of the one
-    // before, whose place the next issue takes, are done
-    if (i + NS - 2 < ns && NS > 2)
-      wait_vmcnt_lgkm0<(NS - 2) * NF>();
+    // the step has landed, those behind it may not have
+    if (NS > 1 && i + NS <= ns)
+      wait_vmcnt<(NS - 1) * 2 * NF>();
     else
-      wait_vmcnt_lgkm0<0>();
+      wait_vmcnt<0>();
     asm volatile("" ::: "memory");
-    if (i + NS - 1 < ns) issue();
-    f16x8 fr[NF];
+    f16x8 fr[2][NF];
 #pragma unroll
-    for (int f = 0; f < NF; ++f) fr[f] = *reinterpret_cast<const f16x8*>(from + read + 1024 * f);
-    read = read == (NS - 1) * kStage ? 0 : read + kStage;
+    for (int k = 0; k < 2; ++k)
 #pragma unroll
-    for (int c = 0; c < CT; ++c)
+      for (int f = 0; f < NF; ++f)
+        fr[k][f] = *reinterpret_cast<const f16x8*>(smem + mine + at + 2048 * f + 128 * c16 +
+                                                   16 * ((4 * k + g) ^ ((c16 >> 1) & 7)));
+    // read, so that the next step may take its place
+    __builtin_amdgcn_s_waitcnt(15 | (7 << 4) | (0 << 8) | (3 << 14));  // lgkmcnt(0)
+    asm volatile("" ::: "memory");
+    if (i + NS < ns) issue(i + NS, at);
+    at = at == (NS - 1) * kStage ? 0 : at + kStage;
+    const bool half = odd && s0 + i == steps - 1;
 #pragma unroll
-      for (int t = 0; t < TT; ++t) acc[c][t] = mfma16x16(fr[c], fr[CT + t], acc[c][t]);
+    for (int k = 0; k < 2; ++k) {
+      if (k == 1 && half) break;  // uniform
+#pragma unroll
+      for (int c = 0; c < CT; ++c)
+#pragma unroll
+        for (int t = 0; t < TT; ++t) acc[c][t] = mfma16x16(fr[k][c], fr[k][CT + t], acc[c][t]);
+    }
   }
   __syncthreads();  // the sums take the steps' place
   auto place = [&](int c, int t) { return reinterpret_cast<f32x4*>(&part[w & 3][16 * t + c16][16 * c + 4 * g]); };
