@@ -340,11 +340,12 @@ inline CacheAttnPlan cache_attn_plan(int B, int H, int n, int64_t max_len) {
 
 // Shape of an append's projection of T tokens to C columns: 16 x tokens rows
 // and 16 x columns columns a workgroup that divides the contraction among its
-// waves, or (tokens = 0) tiles of 128 x 128. us by shape (tokens x
-// columns), D 2048 C 4096: T 16 1x1 4.5, 2x1 4.8; T 64 2x2 8.3, 4x2 10.3, 4x1
-// 10.1; T 128 4x2 11.6, 4x4 13.0; T 256 4x2 20.2, 4x4 15.4; D 1024 C 1280: T
-// 128 2x2 4.4, 4x2 5.5; T 256 4x2 5.8, 2x2 7.3, 4x4 7.3; T 512 4x4 8.4, 4x2
-// 10.7: the widest tile that still gives about a workgroup to every second CU.
+// waves, or (tokens = 0) tiles of 128 x 128. us by shape (tokens x columns), D
+// 2048 C 4096: T 16 1x1 5.2, 2x1 5.6; T 64 2x2 6.5, 4x2 8.2, 1x1 8.7; T 128 4x2
+// 8.2, 2x2 10.6, 4x4 10.2; T 256 4x4 11.0, 4x2 14.4; T 512 4x4 19.1, tiles 28.5;
+// T 1024 35.7, 29.2; D 1024 C 1280: T 192 2x2 4.2, 4x2 5.0; T 384 4x2 5.5, 4x4
+// 7.3; T 768 4x4 8.0, tiles 15.8; T 2048 19.2, 15.8: the smallest shape that
+// still is one round of the 256 CUs, then two rounds of the largest, then tiles.
 struct CacheAppendShape {
   int tokens, columns;
 };

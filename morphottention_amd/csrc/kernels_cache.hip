@@ -849,8 +849,10 @@ __global__ __launch_bounds__(512) void cache_append_rows_kernel(CacheAppendArgs 
                                                                const int* __restrict__ lens,
                                                                const int* __restrict__ new_lens,
                                                                f16* __restrict__ phi) {
-  // operands of a step, 2 KiB each, and steps in LDS: as many as fit
-  constexpr int NF = CT + TT, NS = NF <= 3 ? 3 : NF == 4 ? 2 : 1;
+  // operands of a step, 2 KiB each, and steps in LDS: two where three fit (one
+  // more was up to 8 % slower; the waves cover each other's waits), one of the
+  // smallest, where the first wait counts most
+  constexpr int NF = CT + TT, NS = NF == 3 || NF == 4 ? 2 : 1;
   constexpr int kStage = NF * 2048, kSum = 4 * 16 * TT * (16 * CT + 4) * 4;
   __shared__ __align__(1024) char smem[8 * NS * kStage > kSum ? 8 * NS * kStage : kSum];
   auto part = reinterpret_cast<float(*)[16 * TT][16 * CT + 4]>(smem);  // [wave][token][column]
