@@ -169,6 +169,7 @@ class CacheStep:
     lens: torch.Tensor
     new_lens: torch.Tensor | None
     max_len: int
+    stamps: list[int]
 
 
 class MorphoCache:
@@ -190,7 +191,8 @@ class MorphoCache:
 
     Until then the sequences keep their old lengths, so a step that is dropped
     leaves them as they were. After a tree of drafts :meth:`accept` takes the
-    accepted tokens instead.
+    accepted tokens instead. A step is good for one commit, and only as long as
+    its sequences have not changed otherwise.
     """
 
     def __init__(self, num_pages: int, num_heads: int, cube_m: int, head_dim: int, *, num_layers: int = 1,
@@ -213,6 +215,7 @@ class MorphoCache:
         self._uses = [0] * num_pages
         self._pages: dict[int, list[int]] = {}
         self._lens: dict[int, int] = {}
+        self._stamp: dict[int, int] = {}  # changes with the tokens of a sequence
         self._next = 0
 
     # ---- account
@@ -251,13 +254,13 @@ class MorphoCache:
     def new(self) -> int:
         """A new, empty sequence."""
         seq, self._next = self._next, self._next + 1
-        self._pages[seq], self._lens[seq] = [], 0
+        self._pages[seq], self._lens[seq], self._stamp[seq] = [], 0, 0
         return seq
 
     def free(self, seq: int) -> None:
         """Give a sequence up; its pages that no fork shares are free again."""
         self._drop(self._pages.pop(self._known(seq)))
-        del self._lens[seq]
+        del self._lens[seq], self._stamp[seq]
 
     def _ints(self, rows) -> torch.Tensor:
         return torch.tensor(rows, dtype=torch.int32, device=self.codes.device)
@@ -290,6 +293,7 @@ class MorphoCache:
         self._drop(self._pages[seq][keep:])
         del self._pages[seq][keep:]
         self._lens[seq] = length
+        self._stamp[seq] += 1
 
     def _own(self, wanted: list[tuple[int, int, int]]) -> None:
         """For each (seq, first, end): the pages that hold positions first .. end - 1
@@ -335,17 +339,24 @@ class MorphoCache:
         rows = [(self._pages[s] + [-1] * width)[:width] for s in seqs]
         n = max(counts)
         return CacheStep(seqs, counts, n, self._ints(rows), self._ints([self._lens[s] for s in seqs]),
-                         self._ints(counts) if min(counts) < n else None, max(ends))
+                         self._ints(counts) if min(counts) < n else None, max(ends), [self._stamp[s] for s in seqs])
+
+    def _still(self, step: CacheStep) -> None:
+        if any(self._stamp[self._known(s)] != stamp for s, stamp in zip(step.seqs, step.stamps)):
+            raise RuntimeError("the step's sequences have changed since it was made")
 
     def commit(self, step: CacheStep) -> None:
         """The step's tokens belong to their sequences."""
+        self._still(step)
         for s, c in zip(step.seqs, step.counts):
-            self._lens[self._known(s)] += c
+            self._lens[s] += c
+            self._stamp[s] += 1
 
     def accept(self, step: CacheStep, kept: list[list[int]]) -> None:
         """After a step of drafts: of each sequence the drafts ``kept[b]`` (ascending
         places among its drafts, e.g. the accepted path) are its next tokens,
         the others are dropped."""
+        self._still(step)
         if len(kept) != len(step.seqs):
             raise ValueError("kept must have a list for each sequence of the step")
         for k, c in zip(kept, step.counts):
@@ -357,7 +368,7 @@ class MorphoCache:
                                  self._ints([list(k) + [0] * (most - len(k)) for k in kept]),
                                  keep_lens=self._ints([len(k) for k in kept]))
         for s, k in zip(step.seqs, kept):
-            self._lens[self._known(s)] += len(k)
+            self._lens[s] += len(k)
             self.truncate(s, self._lens[s])
 
     def evict(self, seq: int, kept: list[int]) -> None:

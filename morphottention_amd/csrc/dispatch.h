@@ -330,6 +330,13 @@ inline CacheAttnPlan cache_attn_plan(int B, int H, int n, int64_t max_len) {
     keys = (max_len * wgs + 511) / 512;
     if (keys < 512) keys = 512;
   }
+  // partial rows (DV + 4 floats each) and workgroups stay below 2^20
+  const int64_t most = ((int64_t)1 << 20) / ((int64_t)B * H * n);
+  if (most <= 1) {
+    keys = max_len;
+  } else if (keys < (max_len + most - 1) / most) {
+    keys = (max_len + most - 1) / most;
+  }
   if (max_len <= keys + keys / 2) keys = max_len;  // half a piece is not worth the join
   keys = (keys + 127) / 128 * 128;
   p.nsplit = (int)((max_len + keys - 1) / keys);

@@ -271,6 +271,21 @@ def test_account(plain, seed):
     assert c.free_pages == 40
 
 
+def test_a_stale_step_is_refused(plain):
+    """A step whose sequences have changed commits nothing, of any of them."""
+    c = ma.MorphoCache(8, 1, 16, 32)
+    a, b = c.new(), c.new()
+    c.commit(c.step([a, b], 70))
+    for change in (lambda: c.commit(first), lambda: c.truncate(b, 65), lambda: c.evict(b, [0, 1]), lambda: c.free(b)):
+        first, step = c.step([a], 1), c.step([a, b], 3)
+        change()
+        before = c.length(a), c.free_pages
+        for again in (lambda: c.commit(step), lambda: c.accept(step, [[0], [1]])):
+            with pytest.raises((RuntimeError, KeyError)):
+                again()
+        assert (c.length(a), c.free_pages) == before
+
+
 def test_account_refusals(plain):
     c = ma.MorphoCache(2, 1, 16, 32)
     s = c.new()
@@ -341,6 +356,7 @@ def test_attention_rules(rules):
         assert qblocks * (64 * qt if qt else 16) >= n > (qblocks - 1) * (64 * qt if qt else 16)
         assert keys % 128 == 0 and nsplit >= 1 and nsplit * keys >= L > (nsplit - 1) * keys
         assert nsplit * keys < 2 ** 31
+        assert nsplit == 1 or B * H * n * nsplit <= 2 ** 20  # partial rows
         if qt < 2:
             assert nsplit <= 64
         else:
