@@ -132,9 +132,9 @@ struct CacheRows {
     const int c16 = lane & 15, g = lane >> 4;
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
+      float r = 0.f;
       const int row = min(first + 16 * t + c16, a.n - 1);
       const f16* pr = phi + (((int64_t)b * a.n + row) * a.H + h) * M;
-      float r = 0.f;
 #pragma unroll
       for (int c = 0; c < KC; ++c) {
         const int c0 = M == 16 ? 8 * (g & 1) : 32 * c + 8 * g;
@@ -370,7 +370,12 @@ struct CacheOut {
 #pragma unroll
     for (int k = 0; k < 4; ++k) y[k] = some ? (f16)(o[k] * inv) : (f16)0.f;
     *reinterpret_cast<f16x4*>(out + (((int64_t)b * n + i) * H + h) * DV + c) = y;
-    if (c == 0) lse[at] = some ? m + __log2f(l) - r : -kFltMax;
+    if (c == 0) {
+      // a difference of larger numbers: the logarithm of the mantissa alone, in
+      // [-1, 0), is good to 2^-24, and the rest is added in 64 bits
+      const double lg = (double)fast_log2(__builtin_amdgcn_frexp_mantf(l)) + (double)__builtin_amdgcn_frexp_expf(l);
+      lse[at] = some ? (float)((double)m + lg - (double)r) : -kFltMax;
+    }
   }
 };
 
@@ -436,8 +441,10 @@ __global__ __launch_bounds__(256) void cache_attn_few_kernel(
   if (within(tile + 4)) pb = src.page_of(tile + 4);
 
   CacheRows<M, DV, 1, true> R;
+  __shared__ float sr[16];  // the row constants, which the main loop need not hold
   float rc[1];
   R.start(a, phi, gate_q, gate_k, b, h, 0, lane, rc);
+  if (threadIdx.x < 16) sr[c16] = rc[0];
   const uint64_t bits[1] = {tree ? (uint64_t)tree[(int64_t)b * a.n + min(c16, a.n - 1)] : 0};
 
   // adds cur, with the next tile's loads in flight
@@ -469,7 +476,7 @@ __global__ __launch_bounds__(256) void cache_attn_few_kernel(
   }
 
   __shared__ __align__(16) float so[4][16][DV + 4];
-  __shared__ float sm[4][16], sl[4][16], sr[16];
+  __shared__ float sm[4][16], sl[4][16];
   float ref, l;
   R.finish(0, ref, l);
 #pragma unroll
@@ -477,7 +484,6 @@ __global__ __launch_bounds__(256) void cache_attn_few_kernel(
   if (g == 0) {
     sm[w][c16] = ref;
     sl[w][c16] = l;
-    if (w == 0) sr[c16] = rc[0];
   }
   __syncthreads();
   const CacheOut<DV> put{out, lse, part_o, part_st, a.n, a.H, b, h, sq.nb, a.nsplit, blk.sp};
@@ -602,8 +608,12 @@ __global__ __launch_bounds__(256, M <= 32 && DV <= 64 ? 3 : 2) void cache_attn_r
   if (stages > 1) issue(pg[1]);
 
   CacheRows<M, DV, QT, LO> R;
+  __shared__ float sr[4][16 * QT];  // each wave's row constants
   float rc[QT];
   R.start(a, phi, gate_q, gate_k, b, h, qw, lane, rc);
+#pragma unroll
+  for (int t = 0; t < QT; ++t)
+    if (g == 0) sr[w][16 * t + c16] = rc[t];
   uint64_t bits[QT];
 #pragma unroll
   for (int t = 0; t < QT; ++t)
@@ -671,8 +681,9 @@ __global__ __launch_bounds__(256, M <= 32 && DV <= 64 ? 3 : 2) void cache_attn_r
   for (int t = 0; t < QT; ++t) {
     float ref, l;
     R.finish(t, ref, l);
+    const float r = sr[w][16 * t + c16];
 #pragma unroll
-    for (int c = 0; c < NT; ++c) put(qw + 16 * t + c16, 16 * c + 4 * g, R.O[t][c], ref, l, rc[t]);
+    for (int c = 0; c < NT; ++c) put(qw + 16 * t + c16, 16 * c + 4 * g, R.O[t][c], ref, l, r);
   }
 }
 
@@ -693,15 +704,16 @@ __global__ __launch_bounds__(256) void cache_join_kernel(CacheAttnArgs a, int64_
   const SeqLen sq = seq_len(lens, new_lens, b, a.n, a.W << a.lp);
   const int pieces =
       at < rows && i < sq.nb ? min(a.nsplit, (sq.total + a.split_keys - 1) / a.split_keys) : 0;
-  float m = -1e30f, l = 0.f, r = 0.f;
+  float m = -1e30f, l = 0.f;
+  float r = 0.f;
   f32x4 o = {};
   for (int s = k; s < pieces; s += NG) {
     const float4 st = part_st[at * a.nsplit + s];
+    r = st.z;  // the same in every piece
     const f32x4 x = *reinterpret_cast<const f32x4*>(part_o + (at * a.nsplit + s) * DV + c);
     const float nm = fmaxf(m, st.x), f = fast_exp2(m - nm), fs = fast_exp2(st.x - nm);
     l = l * f + st.y * fs;
     o = o * f + x * fs;
-    r = st.z;  // the same in every piece
     m = nm;
   }
   if constexpr (NG > 1) {
