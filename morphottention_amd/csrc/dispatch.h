@@ -376,13 +376,13 @@ inline int cache_append_rows(int B, int n, int C) {
 }
 
 // Heads of a compaction's workgroup, a power of two: as many as leave four
-// tokens a batch (4096 values) and 512 workgroups. 0: the columns of a head are
-// divided among workgroups, for many tokens of a sequence or few sequences. us
-// with a workgroup a head, divided (dv64 m16 unless said): 48 heads of 1196
-// tokens (dv32 m64) 66, 19; 16 of 16000 1668, 211; 512 of 1000 166, 144; 2048 of
-// 1000 556, 571; 32 of 100 9.5, 5.9; 512 of 100 15, 34; 8192 of 100 248, 611.
+// tokens a batch (4096 values) and 512 workgroups. 0: more than 64 tokens of a
+// sequence may move, and the columns of a head are divided among workgroups. us
+// with a workgroup a head, divided (dv64 m16 unless said): 192 heads of 81 tokens
+// (dv128 m32) 21, 11; 32 of 100 9.5, 6.6; 512 of 100 15, 11; 8192 of 100 249,
+// 141; 48 of 1196 (dv32 m64) 66, 16; 2048 of 1000 556, 359; 16 of 16000 1668, 213.
 inline int cache_compact_heads(int64_t sequences, int H, int DV, int K) {
-  if (K > 256 || (K > 64 && sequences * H <= 128)) return 0;
+  if (K > 64) return 0;
   int hg = 1;
   while (2 * hg * DV <= 1024 && hg < H && sequences * ((H + 2 * hg - 1) / (2 * hg)) >= 512) hg *= 2;
   return hg;

@@ -1303,76 +1303,76 @@ __global__ __launch_bounds__(256) void cache_compact_kernel(CompactArgs a, f16* 
   }
 }
 
-// Many tokens a sequence: one workgroup a (layer, sequence, head, 8 value
-// columns) and one a (layer, sequence, head) for the codes, 512 tokens a
-// batch, from a whole group of 8 places on. A lane gathers the 8 values of a
-// group and column and stores them as one; the next batch's places are found
-// while this one's values come.
-template <int DV>
+// Many tokens a sequence: one workgroup a (layer, sequence, head, CW value
+// columns or 2 CW codes), 4096 / CW tokens a batch, from a whole group of 8
+// places on. A lane gathers the 8 values of a group and column and stores them
+// as one; the next batch's places are found while this one's values come.
+template <int DV, int CW>
 __global__ __launch_bounds__(256) void cache_compact_long_kernel(CompactArgs a, f16* codes, f16* values,
                                                                 const int* __restrict__ table,
                                                                 const int* __restrict__ lens,
                                                                 const int* __restrict__ keep,
                                                                 const int* __restrict__ keep_lens) {
-  constexpr int BT = 512, SL = DV / 8 + 1;
+  constexpr int BT = kCompactValues / CW, CP = CW / 4;  // tokens of a batch; 8-code pieces of a slice
   // three batches' places: one is written while a slower wave still reads the one before last
   __shared__ int64_t from[3][BT], to[3][BT];
-  const int H = a.H, lm = a.lm, lp = a.lp;
+  const int H = a.H, lm = a.lm, lp = a.lp, code_slices = max((1 << lm) / (8 * CP), 1);
   int id = blockIdx.x;
-  const int slice = id % SL;  // 0: codes
-  id /= SL;
+  const int slice = id % (code_slices + DV / CW);
+  id /= code_slices + DV / CW;
   const int h = id % H;
   id /= H;
   const int b = id % a.B, layer = id / a.B;
   const CompactSeq sq(a, table, lens, keep_lens, b);
-  codes += (((int64_t)layer * a.pages * H) << (lm + lp)) + ((int64_t)h << (lm + lp));
-  values += (((int64_t)layer * a.pages * H * DV) << lp) + (((int64_t)h * DV) << lp) + 64 * (slice - 1);
   const int begin = -(int)(sq.base & 7);  // kept token of the first place of a group, mostly not one
   auto find = [&](int k0, int buf) {
-#pragma unroll
-    for (int i = 0; i < BT / 256; ++i) {
-      const int at = threadIdx.x + 256 * i, k = k0 + at;
+    for (int at = threadIdx.x; at < BT; at += 256) {
+      const int k = k0 + at;
       int64_t f = -1, t = -1;
       if (k >= 0 && k < sq.count) sq.move(k, keep[(int64_t)b * a.K + k], f, t);
       from[buf][at] = f;
       to[buf][at] = t;
     }
   };
+  if (sq.count == 0) return;
   find(begin, 0);
   __syncthreads();
   int buf = 0;
   for (int k0 = begin; k0 < sq.count; k0 += BT) {
     const bool more = k0 + BT < sq.count;
     const int next = buf == 2 ? 0 : buf + 1;
-    if (slice == 0) {
-      constexpr int CPER = BT * 8 / 256;  // 8-code pieces of a lane, at most (cube_m 64)
-      const int lc = lm - 3;
-      f16x8 cv[CPER];
+    if (slice < code_slices) {
+      f16* const pool = codes + (((int64_t)layer * a.pages * H) << (lm + lp)) + ((int64_t)h << (lm + lp)) +
+                        8 * CP * slice;
+      const int lc = min(lm - 3, __builtin_ctz(CP));  // log2 of the slice's pieces
+      f16x8 cv[4];
 #pragma unroll
-      for (int i = 0; i < CPER; ++i) {
+      for (int i = 0; i < 4; ++i) {
         const int e = threadIdx.x + 256 * i, k = e >> lc;
         if (k < BT && to[buf][k] >= 0)
-          cv[i] = *reinterpret_cast<const f16x8*>(codes + (from[buf][k] << lm) + 8 * (e & ((1 << lc) - 1)));
+          cv[i] = *reinterpret_cast<const f16x8*>(pool + (from[buf][k] << lm) + 8 * (e & ((1 << lc) - 1)));
       }
       if (more) find(k0 + BT, next);
       wait_vmcnt<0>();
       __syncthreads();
 #pragma unroll
-      for (int i = 0; i < CPER; ++i) {
+      for (int i = 0; i < 4; ++i) {
         const int e = threadIdx.x + 256 * i, k = e >> lc;
         if (k < BT && to[buf][k] >= 0)
-          *reinterpret_cast<f16x8*>(codes + (to[buf][k] << lm) + 8 * (e & ((1 << lc) - 1))) = cv[i];
+          *reinterpret_cast<f16x8*>(pool + (to[buf][k] << lm) + 8 * (e & ((1 << lc) - 1))) = cv[i];
       }
     } else {
-      // lane: column threadIdx % 8 of the slice, groups threadIdx / 8 and 32 on
+      f16* const pool = values + (((int64_t)layer * a.pages * H * DV) << lp) + (((int64_t)h * DV) << lp) +
+                        8 * CW * (slice - code_slices);
+      // lane: column threadIdx % CW of the slice, two groups
       f16x8 v[2];
-      const int c = threadIdx.x & 7;
-      auto at = [&](int64_t row) { return values + (row & ~(int64_t)7) * DV + 8 * c + (row & 7); };
+      const int c = threadIdx.x % CW, g0 = threadIdx.x / CW;
+      auto at = [&](int64_t row) { return pool + (row & ~(int64_t)7) * DV + 8 * c + (row & 7); };
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const int k = 8 * ((threadIdx.x >> 3) + 32 * i) + j;
+          const int k = 8 * (g0 + 256 / CW * i) + j;
           if (to[buf][k] >= 0) v[i][j] = *at(from[buf][k]);
         }
       if (more) find(k0 + BT, next);
@@ -1380,7 +1380,7 @@ __global__ __launch_bounds__(256) void cache_compact_long_kernel(CompactArgs a, 
       __syncthreads();
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int k = 8 * ((threadIdx.x >> 3) + 32 * i);
+        const int k = 8 * (g0 + 256 / CW * i);
         bool all = true;  // a group lies in one page
 #pragma unroll
         for (int j = 0; j < 8; ++j) all = all && to[buf][k + j] >= 0;
@@ -1399,6 +1399,14 @@ __global__ __launch_bounds__(256) void cache_compact_long_kernel(CompactArgs a, 
   }
 }
 
+template <int DV, int CW>
+void launch_cache_compact_long(const CompactArgs& a, int64_t sequences, f16* codes, f16* values, const int* table,
+                               const int* lens, const int* keep, const int* keep_lens, hipStream_t s) {
+  const int code_slices = (1 << a.lm) / (2 * CW) > 1 ? (1 << a.lm) / (2 * CW) : 1;
+  MORPHO_KLAUNCH((cache_compact_long_kernel<DV, CW>), dim3((unsigned)(sequences * a.H * (code_slices + DV / CW))),
+                 dim3(256), 0, s, a, codes, values, table, lens, keep, keep_lens);
+}
+
 hipError_t launch_cache_compact(const CacheDims& d, f16* codes, f16* values, const int* table, const int* lens,
                                 const int* keep, const int* keep_lens, int K, hipStream_t s) {
   const CompactArgs a{d.B, d.H, log2_of(d.M), d.pages, d.W, log2_of(d.P), K};
@@ -1410,9 +1418,12 @@ hipError_t launch_cache_compact(const CacheDims& d, f16* codes, f16* values, con
     if (heads)                                                                                                     \
       MORPHO_KLAUNCH((cache_compact_kernel<DV>), dim3((unsigned)(sequences * ((d.H + heads - 1) / heads))), block, \
                      0, s, a, codes, values, table, lens, keep, keep_lens, log2_of(heads));                       \
+    else if (K <= 128)                                                                                             \
+      launch_cache_compact_long<DV, 32>(a, sequences, codes, values, table, lens, keep, keep_lens, s);            \
+    else if (K <= 256)                                                                                             \
+      launch_cache_compact_long<DV, 16>(a, sequences, codes, values, table, lens, keep, keep_lens, s);            \
     else                                                                                                           \
-      MORPHO_KLAUNCH((cache_compact_long_kernel<DV>), dim3((unsigned)(sequences * d.H * (DV / 8 + 1))), block, 0,  \
-                     s, a, codes, values, table, lens, keep, keep_lens);                                          \
+      launch_cache_compact_long<DV, 8>(a, sequences, codes, values, table, lens, keep, keep_lens, s);             \
   } while (0)
   if (d.DV == 32)
     MORPHO_CACHE_COMPACT(32);

@@ -384,4 +384,4 @@ def test_append_rules(rules):
 def test_compact_rules(rules):
     assert [r[0] for r in rules([(2, 384, 16, 64, 9), (2, 1, 16, 64, 9), (2, 24, 2, 32, 1196), (2, 512, 16, 64, 100),
                                  (2, 4, 8, 64, 100), (2, 10000, 3, 128, 64), (2, 10000, 32, 32, 5)])] \
-        == [8, 1, 0, 16, 0, 4, 32]
+        == [8, 1, 0, 0, 0, 4, 32]
