@@ -231,18 +231,21 @@ def test_padding_codes_may_hold_anything(n):
     _check(p.attend(p.device()), p.reference())
 
 
-def test_pages_that_the_pool_does_not_have():
+@pytest.mark.parametrize("n", [3, 20, 70])
+@pytest.mark.parametrize("P", [32, 64])
+def test_pages_that_the_pool_does_not_have(n, P):
     """Their keys are left out, wherever they lie."""
-    p = Problem(2, 3, 2, 32, 64, [300, 500], P=64, seed=5)
-    gone = {0: [0, 3], 1: [2]}
+    p = Problem(2, n, 2, 32, 64, [300, 500], P=P, seed=5)
+    gone = {0: [0, 3, 300 // P], 1: [2, 5]}
     for b, rows in gone.items():
         for i, k in enumerate(rows):
-            p.table[b, k] = -1 if i == 0 else p.codes.shape[0] + 7
+            p.table[b, k] = (-1, p.codes.shape[0] + 7, 2 ** 31 - 1)[i]
 
     def drop(b):
         T = p.lens[b] + p.news[b]
-        return [t for t in range(T) if t // 64 in gone[b]]
+        return [t for t in range(T) if t // P in gone[b]]
     _check(p.attend(p.device()), p.reference(drop=drop))
+    _check(p.attend(p.device(), causal=False), p.reference("full", drop=drop))
 
 
 def test_lengths_past_the_table_and_negative():
@@ -558,6 +561,58 @@ def test_a_captured_step_follows_the_lengths():
             got = out.clone(), lse.clone()
             want = go()
             assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_a_pool_beyond_32_bits():
+    """Pages more than 2^32 bytes into a pool: the same results as near its start."""
+    H, m, dv, P, far = 16, 16, 64, 64, 34000  # 128 KiB of values a page
+    p = Problem(2, 3, H, m, dv, [100, 190], seed=15)
+    d = p.device()
+    pages = p.codes.shape[0]
+    big = {k: torch.empty((far + pages, *d[k].shape[1:]), dtype=torch.float16, device=DEV) for k in ("codes", "values")}
+    x = torch.randn((2, 3, H * dv), device=DEV).half()
+    w = (torch.randn((H * m + H * dv, H * dv), device=DEV) / 32).half()
+    keep = torch.tensor([[1, 5, 60, 99], [0, 2, 3, 150]], dtype=torch.int32, device=DEV)
+    zero = torch.zeros(2, dtype=torch.int32, device=DEV)
+    for k in big:
+        big[k][far:] = d[k]
+    outs = []
+    for pool, off in ((d, 0), (big, far)):
+        table = d["table"] + off
+        phi = ma.morpho_cache_append(x, w, pool["codes"], pool["values"], table, d["lens"])
+        out, lse = ma.morpho_cache_attention(phi, d["gq"], d["gk"], pool["codes"], pool["values"], table, d["lens"],
+                                             scale=p.scale)
+        ma.morpho_cache_compact(pool["codes"], pool["values"], table, zero, keep)
+        ma.morpho_cache_copy_pages(pool["codes"], pool["values"], table[0, :2].contiguous(), table[1, :2].contiguous())
+        outs.append([phi, out, lse, pool["codes"][off:].clone(), pool["values"][off:].clone()])
+    assert big["values"].numel() * 2 > 2 ** 32
+    for a, b in zip(*outs):
+        assert torch.equal(a.view(torch.int16) if a.dtype == torch.float16 else a,
+                           b.view(torch.int16) if b.dtype == torch.float16 else b)
+
+
+def test_two_graphs_in_turn():
+    """Two captured calls with partial results, replayed in turn: each has its own."""
+    ps = [Problem(2, n, 2, 16, 64, [3000, 2000 + n], seed=n) for n in (1, 30)]
+    ds = [p.device() for p in ps]
+    want = [[t.clone() for t in p.attend(d)] for p, d in zip(ps, ds)]
+    torch.cuda.synchronize()
+    graphs, got = [], []
+    for p, d in zip(ps, ds):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            got.append(p.attend(d))
+        graphs.append(g)
+    for _ in range(3):
+        for out, lse in got:
+            out.zero_()
+            lse.zero_()
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
+        ps[0].attend(ds[0])  # the program's own work in between
 
 
 def test_c_abi_direct_matches_the_ops():
