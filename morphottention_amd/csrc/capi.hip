@@ -625,7 +625,7 @@ bool misaligned_ints(const void* a, const void* b = nullptr, const void* c = nul
 }
 CacheAttnPlan cache_plan(const CacheDims& d, int64_t max_len) {
   const int64_t cap = (int64_t)d.W * d.P;
-  return cache_attn_plan(d.B, d.H, d.n, max_len < cap ? max_len : cap);
+  return cache_attn_plan(d.B, d.H, d.n, max_len < cap ? max_len : cap, d.M, d.DV);
 }
 size_t cache_part_o_bytes(const CacheDims& d, const CacheAttnPlan& p) {
   return align_up((size_t)d.B * d.H * d.n * p.nsplit * d.DV * 4);

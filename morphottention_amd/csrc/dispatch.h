@@ -304,30 +304,42 @@ struct CacheDims {
 
 // Launch shape of the attention over the cache. qt = 0: up to 16 new tokens,
 // which the four waves of a workgroup share while they divide the keys. qt >
-// 0: 64 qt of them a workgroup (row block), 16 qt for each wave. The keys of a
-// sequence are cut into pieces of split_keys, one workgroup each; with more
-// than one piece a second kernel joins the partial results.
+// 0: 64 qt of them a workgroup (row block), 16 qt for each wave. pairs: the
+// weights enter the value product as hi / lo pairs. The keys of a sequence are
+// cut into pieces of split_keys, one workgroup each; with more than one piece a
+// second kernel joins the partial results.
 struct CacheAttnPlan {
   int qt, qblocks, nsplit, split_keys;
+  bool pairs;
 };
-inline CacheAttnPlan cache_attn_plan(int B, int H, int n, int64_t max_len) {
+inline CacheAttnPlan cache_attn_plan(int B, int H, int n, int64_t max_len, int M, int DV) {
   CacheAttnPlan p;
-  p.qt = n <= 16 ? 0 : n <= 64 ? 1 : 2;
+  p.pairs = n <= 64;  // bound by reading the keys; beyond, pairs take a third longer (B4 n1000 80 -> 108 us)
+  // More than 64 rows: with 64 a workgroup, four of them fit on a CU where the
+  // codes and values of a head are few, and they even out sequences and row
+  // blocks of different lengths; 128 read the keys half as often. us, H16 dv64,
+  // 64 and 128 rows: B4 n1000 over 4096 m16 80, 84; B8 n500 over 1000 to 3000
+  // 54, 59; B16 n65 30, 34; B1 n3000 over none m32 35, 48; B4 n2048 over none
+  // (1024 workgroups of 128) 48, 49, n4096 (2048) 159, 141; m64 B8 n256 H32 132,
+  // 93; dv128 m32 B4 n1000 99, 81.
+  p.qt = n <= 16 ? 0 : n <= 64 ? 1 : M > 32 || DV > 64 || (int64_t)B * H * ((n + 127) / 128) > 1024 ? 2 : 1;
   p.qblocks = p.qt ? (n + 64 * p.qt - 1) / (64 * p.qt) : 1;
   const int64_t wgs = (int64_t)B * H * p.qblocks;
   // Short pieces balance sequences of different lengths and fill the chip with
   // few of them; each costs a partial result. B64 n1 H16, 1 to 8191 tokens, us
   // with the join: one piece 58, of 2048 48, 1024 44, 512 42, 256 56; B1 n1 H16
   // m32, 131071 tokens: of 512 84, 2048 79, 4096 75; trees of 48, B16 H32 m64,
-  // 300 to 4000 tokens: of 2048 70, 512 54, 256 76. From 128 rows a workgroup on, the partial results
-  // cost more than they gain once every CU has two workgroups (B4 n1000 H16
-  // m16 over 4096: of 1024 174, one piece 162).
+  // 300 to 4000 tokens: of 2048 70, 512 54, 256 76. With more rows the partial
+  // results cost more than they gain once every CU has as many workgroups as it
+  // holds: four of 64 rows, two of 128 (64 rows, up to 512, 1024, 2048 workgroups:
+  // B16 n128 35, 32, 35; B1 n1000 over 8000 61, 52, 57; B8 n500 over 1000 to
+  // 3000 55, 55, 68; 128 rows, up to 512, 1024: m64 B8 n256 H32 97, 131).
   int64_t keys;
-  if (p.qt < 2) {
+  if (p.pairs) {
     keys = (max_len + 63) / 64;
     if (keys < (wgs < 1024 ? 512 : 1024)) keys = wgs < 1024 ? 512 : 1024;
   } else {
-    keys = (max_len * wgs + 511) / 512;
+    keys = (max_len * wgs + 1024 / p.qt - 1) / (1024 / p.qt);
     if (keys < 512) keys = 512;
   }
   // partial rows (DV + 4 floats each) and workgroups stay below 2^20

@@ -125,6 +125,7 @@ struct CacheRows {
   float thr[QT];  // exponent from which the reference moves: 15, -inf before the first score
   float sum[QT];  // of this lane's weights
   f32x4 O[QT][NT];
+  bool ready = false;  // every row has a reference
 
   // Rows first .. first + 16 QT - 1, those from n on repeating the last; rc: the rows' constants.
   __device__ __forceinline__ void start(const CacheAttnArgs& a, const f16* phi, const f16* gate_q, const f16* gate_k,
@@ -165,6 +166,20 @@ struct CacheRows {
     }
   }
 
+  // Exponents of the weights: row t of this lane, its 4 keys of block i.
+  __device__ __forceinline__ f32x4 score(const CacheTile<M, DV>& T, int t, int i) const {
+    f32x4 s = mfma16x16(T.k[i][0], u[t][0], off[t]);
+    if constexpr (M != 16) {
+      s = mfma16x16(T.k[i][0], u[t][KC], s);
+#pragma unroll
+      for (int c = 1; c < KC; ++c) {
+        s = mfma16x16(T.k[i][c], u[t][c], s);
+        s = mfma16x16(T.k[i][c], u[t][KC + c], s);
+      }
+    }
+    return s;
+  }
+
   // Adds NK tiles. seen(t): bit j: row t of this lane sees key j of its 8; read
   // only if MASKED. again(t, p, seen): called with the weights if MASKED.
   template <bool MASKED, int NK, class Seen, class Again>
@@ -179,15 +194,7 @@ struct CacheRows {
       for (int t = 0; t < QT; ++t)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          s[n][t][i] = mfma16x16(T[n].k[i][0], u[t][0], off[t]);
-          if (M != 16) {
-            s[n][t][i] = mfma16x16(T[n].k[i][0], u[t][KC], s[n][t][i]);
-#pragma unroll
-            for (int c = 1; c < KC; ++c) {
-              s[n][t][i] = mfma16x16(T[n].k[i][c], u[t][c], s[n][t][i]);
-              s[n][t][i] = mfma16x16(T[n].k[i][c], u[t][KC + c], s[n][t][i]);
-            }
-          }
+          s[n][t][i] = score(T[n], t, i);
         }
     unsigned vis[QT];
 #pragma unroll
@@ -256,10 +263,80 @@ struct CacheRows {
         if constexpr (MASKED) again(t, p, vis[t]);
       }
   }
-  // Adds tiles that every row sees all of.
+  // Adds tiles that every row sees all of. Single weights tell by their sum
+  // whether the reference has to move: while 8 sum to at most 65504, each is an
+  // fp16 number. So no maximum is taken, and the exponentials need not wait for
+  // one (B4 n4096 over none 147 -> 140 us, B4 n1000 dv128 82.7 -> 80.8, over
+  // 4096 keys dv64 81.2 -> 80.4). Pairs are bound by other things.
   template <int NK>
   __device__ __forceinline__ void add_clear(const CacheTile<M, DV> (&T)[NK]) {
-    add<false>(T, [](int) { return 0u; }, [](int, const float(&)[8], unsigned) {});
+    if constexpr (LO) {
+      add<false>(T, [](int) { return 0u; }, [](int, const float(&)[8], unsigned) {});
+      return;
+    }
+    f32x4 s[NK][QT][2];
+#pragma unroll
+    for (int n = 0; n < NK; ++n)
+#pragma unroll
+      for (int t = 0; t < QT; ++t)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) s[n][t][i] = score(T[n], t, i);
+    // moves row t's reference by the scores from tile n on: to 10 below the
+    // top, or 8 like it would already sum to half of what moves it again
+    auto settle = [&](int n, int t) {
+      float m = kNegInf;
+#pragma unroll
+      for (int k = 0; k < NK; ++k)
+        if (k >= n)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) m = fmaxf(m, s[k][t][j >> 2][j & 3]);
+      m = fmaxf(m, __shfl_xor(m, 16));
+      m = fmaxf(m, __shfl_xor(m, 32));
+      const bool first = thr[t] == kNegInf;
+      const float up = first ? m - 10.f : fmaxf(m - 10.f, 0.f);
+      const float f = first ? 1.f : fast_exp2(-up);
+      off[t] -= up;
+      thr[t] = 15.f;
+#pragma unroll
+      for (int k = 0; k < NK; ++k)
+        if (k >= n) {
+          s[k][t][0] -= up;
+          s[k][t][1] -= up;
+        }
+      sum[t] *= f;
+#pragma unroll
+      for (int c = 0; c < NT; ++c) O[t][c] *= f;
+    };
+    if (!ready) {
+#pragma unroll
+      for (int t = 0; t < QT; ++t) settle(0, t);
+      ready = true;
+    }
+#pragma unroll
+    for (int n = 0; n < NK; ++n)
+#pragma unroll
+      for (int t = 0; t < QT; ++t) {
+        f16x8 w;
+        auto weigh = [&]() {
+          float p[8];
+          __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            p[j] = fast_exp2(s[n][t][j >> 2][j & 3]);
+            w[j] = (f16)p[j];
+          }
+          __builtin_amdgcn_s_setprio(0);
+          return ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+        };
+        float part = weigh();
+        if (__any(part > 65504.f)) {
+          settle(n, t);
+          part = weigh();
+        }
+        sum[t] += part;
+#pragma unroll
+        for (int c = 0; c < NT; ++c) O[t][c] = mfma16x16(T[n].v[c], w, O[t][c]);
+      }
   }
 
   // After the last tile: the reference and the sum of the weights.
@@ -412,6 +489,10 @@ struct CacheBlock {
 
 // Up to 16 rows: the four waves of a workgroup share them and take every
 // fourth tile of the piece's keys, straight into registers, one tile ahead.
+// Bound by reading the keys: B64 n1 H16 m16 dv64, 1 to 8191 tokens (158 MB) 34.9
+// us, 4.5 TB/s; B1 n1 H16 m32 dv64, 131071 tokens (403 MB) 70 us, 5.7 TB/s. Short
+// sequences by the chain lengths, page, key: B1 n1, 99 tokens 4.4 us, of which
+// an empty launch is 2.5.
 template <int M, int DV>
 __global__ __launch_bounds__(256) void cache_attn_few_kernel(
     CacheAttnArgs a, const f16* __restrict__ phi, const f16* __restrict__ gate_q, const f16* __restrict__ gate_k,
@@ -516,13 +597,17 @@ __global__ __launch_bounds__(256) void cache_attn_few_kernel(
 // the keys pass through LDS, 64 a stage and three stages, filled by DMA in the
 // order in which the lanes read them as operands (a wave fetches every fourth
 // operand; 1 KiB each, conflict-free both ways).
-template <int M, int DV, int QT>
-__global__ __launch_bounds__(256, M <= 32 && DV <= 64 ? 3 : 2) void cache_attn_rows_kernel(
+// Drafts are bound by reading the keys (B16 n48 H32 m64 dv64, 300 to 4000
+// tokens, 198 MB: 43 us, 4.6 TB/s); pieces of prompts by the exponentials,
+// conversions and sums beside the matrix products of the few waves of a SIMD, and
+// by workgroups of different lengths (B4 n1000 behind 3000 to 4096 tokens H16
+// m16 dv64: 80 us, 0.5 PFLOP/s; at n4096 over none 140 us).
+template <int M, int DV, int QT, bool LO>
+__global__ __launch_bounds__(256, M > 32 || DV > 64 ? 2 : LO || QT > 1 ? 3 : 4) void cache_attn_rows_kernel(
     CacheAttnArgs a, const f16* __restrict__ phi, const f16* __restrict__ gate_q, const f16* __restrict__ gate_k,
     const f16* __restrict__ codes, const f16* __restrict__ values, const int* __restrict__ table,
     const int* __restrict__ lens, const int* __restrict__ new_lens, const int64_t* __restrict__ tree,
     f16* __restrict__ out, float* __restrict__ lse, float* __restrict__ part_o, float4* __restrict__ part_st) {
-  constexpr bool LO = QT == 1;
   constexpr int NT = DV / 16, NF = CacheTile<M, DV>::kFrags, PER = NF / 2;  // DMA pieces of a wave and stage
   static_assert(NF % 2 == 0, "a stage's operands divide evenly among four waves");
   __shared__ __align__(1024) char lds[3][2 * NF * 1024];
@@ -695,7 +780,8 @@ __global__ __launch_bounds__(256, M <= 32 && DV <= 64 ? 3 : 2) void cache_attn_r
 }
 
 // Joins the pieces of the rows: DV / 4 lanes hold a row's columns, NG such
-// groups take its pieces in turn, and the groups are added in order.
+// groups take its pieces in turn, and the groups are added in order. Bound by
+// its launch: B64 n1 H16 of up to 9 pieces 4.4 us where an empty one takes 4.0.
 template <int DV, int NG>
 __global__ __launch_bounds__(256) void cache_join_kernel(CacheAttnArgs a, int64_t rows, const int* __restrict__ lens,
                                                         const int* __restrict__ new_lens,
@@ -774,10 +860,12 @@ hipError_t launch_cache_attn_t(const CacheDims& d, const CacheAttnPlan& p, const
                  tree, out, lse, part.o, part.st)
   if (p.qt == 0)
     MORPHO_CACHE_ATTN(cache_attn_few_kernel<M, DV>);
-  else if (p.qt == 1)
-    MORPHO_CACHE_ATTN(cache_attn_rows_kernel<M, DV, 1>);
-  else
-    MORPHO_CACHE_ATTN(cache_attn_rows_kernel<M, DV, 2>);
+  else if (p.pairs)
+    MORPHO_CACHE_ATTN(cache_attn_rows_kernel<M, DV, 1, true>);
+  else if (p.qt == 2)
+    MORPHO_CACHE_ATTN(cache_attn_rows_kernel<M, DV, 2, false>);
+  else if constexpr (M <= 32 && DV <= 64)
+    MORPHO_CACHE_ATTN(cache_attn_rows_kernel<M, DV, 1, false>);
 #undef MORPHO_CACHE_ATTN
   return hipGetLastError();
 }
@@ -859,7 +947,7 @@ __device__ __forceinline__ f16* value_place(const CacheAppendArgs& a, f16* value
 // fetch a 128-byte line of a row (place p of row r holds k chunk p ^ (r / 2 %
 // 8), so that the reads of 16 rows of one chunk hit all banks). T 192, D 2048,
 // C 4096: 19.4 us loaded directly, 13.1 by half lines (the L1 loses the other
-// half before its turn).
+// half before its turn), 10.8 so.
 template <int CT, int TT>
 __global__ __launch_bounds__(512) void cache_append_rows_kernel(CacheAppendArgs a, const f16* __restrict__ X,
                                                                const f16* __restrict__ Wt, f16* __restrict__ codes,
@@ -1163,7 +1251,9 @@ hipError_t launch_cache_append(const CacheDims& d, const f16* X, const f16* W, f
 }
 
 // ---------------------------------------------------------------- page copies
-// One launch for all layers: 16 KiB of a page's codes or values a workgroup.
+// One launch for all layers: 16 KiB of a page's codes or values a workgroup,
+// four loads of a lane in flight. Bound by memory: 550 MB read and written (2
+// layers, 700 pages) in 111 us, 5.0 TB/s, a large copy's rate.
 constexpr int kCopyBytes = 16384;
 __global__ __launch_bounds__(256) void cache_copy_kernel(char* __restrict__ codes, char* __restrict__ values,
                                                         const int* __restrict__ src, const int* __restrict__ dst,

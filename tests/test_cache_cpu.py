@@ -312,11 +312,11 @@ PROGRAM = r'''
 #include "dispatch.h"
 using namespace morpho;
 int main() {
-  long long what, a, b, c, d;
-  while (scanf("%lld %lld %lld %lld %lld", &what, &a, &b, &c, &d) == 5) {
+  long long what, a, b, c, d, m, dv;
+  while (scanf("%lld %lld %lld %lld %lld %lld %lld", &what, &a, &b, &c, &d, &m, &dv) == 7) {
     if (what == 0) {
-      const CacheAttnPlan p = cache_attn_plan((int)a, (int)b, (int)c, d);
-      printf("%d %d %d %d\n", p.qt, p.qblocks, p.nsplit, p.split_keys);
+      const CacheAttnPlan p = cache_attn_plan((int)a, (int)b, (int)c, d, (int)m, (int)dv);
+      printf("%d %d %d %d\n", p.pairs ? p.qt : p.qt + 10, p.qblocks, p.nsplit, p.split_keys);
     } else if (what == 1) {
       const CacheAppendShape p = cache_append_shape((int)a, (int)b);
       printf("%d %d %d 0\n", p.tokens, p.columns, cache_append_rows((int)c, (int)d, (int)b));
@@ -338,7 +338,7 @@ def rules(tmp_path_factory):
                     str(d / "rules.cpp"), "-o", str(d / "rules")], check=True)
 
     def evaluate(rows):
-        text = "".join(" ".join(map(str, r)) + "\n" for r in rows)
+        text = "".join(" ".join(map(str, (*r, 16, 64)[:7])) + "\n" for r in rows)
         out = subprocess.run([str(d / "rules")], input=text, capture_output=True, text=True, check=True).stdout
         return [tuple(map(int, line.split())) for line in out.splitlines()]
 
@@ -351,16 +351,20 @@ def test_attention_rules(rules):
     rng = random.Random(1)
     cases = [(rng.choice([1, 2, 7, 64, 500]), rng.choice([1, 3, 16, 32]), rng.choice([1, 16, 17, 64, 65, 1000, 5000]),
               rng.choice([1, 127, 512, 513, 768, 769, 5000, 131072, 2 ** 30])) for _ in range(400)]
-    for (B, H, n, L), (qt, qblocks, nsplit, keys) in zip(cases, rules([(0, *c) for c in cases])):
-        assert qt == (0 if n <= 16 else 1 if n <= 64 else 2)
+    cases = [(*c, m, dv) for c in cases for m, dv in ((16, 32), (32, 64), (64, 64), (16, 128))]
+    for (B, H, n, L, m, dv), (qt, qblocks, nsplit, keys) in zip(cases, rules([(0, *c) for c in cases])):
+        pairs, qt = qt < 10, qt % 10
+        assert pairs == (n <= 64)
+        many = m == 64 or dv == 128 or B * H * -(-n // 128) > 1024
+        assert qt == (0 if n <= 16 else 2 if n > 64 and many else 1)
         assert qblocks * (64 * qt if qt else 16) >= n > (qblocks - 1) * (64 * qt if qt else 16)
         assert keys % 128 == 0 and nsplit >= 1 and nsplit * keys >= L > (nsplit - 1) * keys
         assert nsplit * keys < 2 ** 31
         assert nsplit == 1 or B * H * n * nsplit <= 2 ** 20  # partial rows
-        if qt < 2:
+        if pairs:
             assert nsplit <= 64
         else:
-            assert nsplit == 1 or nsplit * B * H * qblocks <= 512 + B * H * qblocks
+            assert nsplit == 1 or nsplit * B * H * qblocks <= 1024 // qt + B * H * qblocks
     # measured points: direct at short lengths, pieces for long ones and ragged batches
     assert [r[2] for r in rules([(0, 1, 8, 1, 100), (0, 64, 16, 1, 1000), (0, 64, 16, 1, 8192), (0, 1, 16, 1, 131071),
                                  (0, 16, 32, 48, 4048), (0, 4, 16, 1000, 5096)])] == [1, 1, 8, 64, 8, 1]

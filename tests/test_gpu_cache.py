@@ -265,6 +265,43 @@ def test_score_ranges(gate):
     _check(p.attend(p.device()), p.reference())
 
 
+@pytest.mark.parametrize("n,m,dv", [(8, 16, 64), (40, 32, 32), (70, 16, 64), (70, 32, 32), (70, 64, 64), (130, 16, 128)])
+@pytest.mark.parametrize("top", [20.0, 400.0])
+@pytest.mark.parametrize("order", ["rising", "falling", "peaks"])
+def test_references_that_move(n, m, dv, top, order):
+    """Scores up to 1.44 top: every tile passes the ones before it, none does, or a few keys do."""
+    p = Problem(2, n, 2, m, dv, [450, 130], seed=m + n, scale=top / m)
+    g = torch.Generator().manual_seed(n)
+    p.gq, p.gk = torch.ones_like(p.gq), torch.ones_like(p.gk)
+    p.phi = (1 - 0.1 * torch.rand(p.phi.shape, generator=g)).half()  # positive factors of the codes
+    for b in range(2):
+        T = p.k[b].shape[0]
+        at = torch.linspace(0, 1, T)[:, None, None]
+        if order == "falling":
+            at = 1 - at
+        if order == "peaks":
+            at = (torch.rand((T, 1, 1), generator=g) < 0.02).float()
+        p.k[b] = (at * (1 - 0.05 * torch.rand((T, 2, m), generator=g))).half()
+        p.store(b)
+    _check(p.attend(p.device()), p.reference())
+    _check(p.attend(p.device(), causal=False), p.reference("full"))
+
+
+@pytest.mark.parametrize("m,dv", [(16, 32), (16, 64), (32, 32), (32, 64)])
+def test_many_sequences_of_many_rows(m, dv):
+    """Three sequences 90 times over, so many row blocks that they are larger ones."""
+    p = Problem(3, 130, 2, m, dv, [0, 65, 150], news=[130, 97, 128], seed=m + dv)
+    d = p.device()
+    for k in ("phi", "table", "lens", "new_lens"):
+        d[k] = d[k].repeat(90, *[1] * (d[k].dim() - 1))
+    out, lse = p.attend(d)
+    want = p.reference()
+    for i in (0, 1, 44, 89):
+        _check((out[3 * i : 3 * i + 3], lse[6 * i : 6 * i + 6]), want)
+    same = out.view(90, 3, 130, -1), lse.view(90, 6, 130)
+    assert all(torch.equal(x, x[:1].expand_as(x)) for x in same)
+
+
 def test_attention_repeats_bit_for_bit():
     p = Problem(2, 3, 2, 16, 64, [4000, 2500], seed=8)
     d = p.device()
