@@ -217,7 +217,11 @@ int morpho_soft_backward(const void* grad_out, const void* X, const void* W_phi,
  * device memory and are read by the kernels, so a captured graph follows
  * them. The kernels check them: a page outside the pool, or a position past
  * the table's seq_pages * page_size, is neither read nor written (its key is
- * left out), negative lengths count as 0. seq_pages * page_size <= 2^30. */
+ * left out), negative lengths count as 0.
+ *
+ * Sizes: H * cube_m and H * head_dim_v <= 65536, layers <= 65535, seq_pages *
+ * page_size <= 2^30, B * n <= 2^22, B * n * H <= 2^23 and B * H * layers *
+ * head_dim_v <= 2^25. */
 typedef struct morpho_cache {
   void* codes;
   void* values;
