@@ -150,9 +150,10 @@ def morpho_cache_compact(codes: torch.Tensor, values: torch.Tensor, table: torch
     """Move token ``lens[b] + keep[b, k]`` to position ``lens[b] + k``, in place and
     in every layer: the accepted path of a tree to the front of its drafts
     (``lens``: the tokens before them), or what is left after tokens were
-    evicted (``lens``: 0).
+    evicted (``lens``: 0). No other sequence of the call may have a page that
+    tokens move to.
 
-    :param keep: int32 ``[B, kept]``; has to ascend along each row.
+    :param keep: int32 ``[B, kept]``; has to ascend along each row, none twice.
     :param keep_lens: int32 ``[B]``, how many of them count.
     """
     ops.cache_compact(codes, values, table, lens, keep, keep_lens)
