@@ -270,8 +270,10 @@ int morpho_cache_copy_pages(const morpho_cache* cache, const int32_t* src, const
 /* Moves token lens[b] + keep[b][k] of sequence b to position lens[b] + k, k <
  * keep_lens[b] (NULL: keep_cols), in place and in every layer. keep [B,
  * keep_cols] int32 has to ascend along a row, no entry twice (then every token
- * is moved before its place is taken); a negative entry moves nothing. No other
- * sequence of the call may have a page that tokens move to. */
+ * is moved before its place is taken). An entry below its own place, keep[b][k]
+ * < k, moves nothing: a negative one, and where negative ones stand before it
+ * one that would move its token forward. No other sequence of the call may have
+ * a page that tokens move to. */
 int morpho_cache_compact(const morpho_cache* cache, const int32_t* table, const int32_t* lens, const int32_t* keep,
                          const int32_t* keep_lens, int64_t B, int64_t keep_cols, int64_t seq_pages,
                          morpho_stream_t stream);

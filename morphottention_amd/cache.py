@@ -153,7 +153,9 @@ def morpho_cache_compact(codes: torch.Tensor, values: torch.Tensor, table: torch
     evicted (``lens``: 0). No other sequence of the call may have a page that
     tokens move to.
 
-    :param keep: int32 ``[B, kept]``; has to ascend along each row, none twice.
+    :param keep: int32 ``[B, kept]``; has to ascend along each row, none twice. An
+        entry below its own place (``keep[b, k] < k``, negative ones among them)
+        moves nothing.
     :param keep_lens: int32 ``[B]``, how many of them count.
     """
     ops.cache_compact(codes, values, table, lens, keep, keep_lens)

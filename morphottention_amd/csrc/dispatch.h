@@ -387,6 +387,14 @@ inline int cache_append_rows(int B, int n, int C) {
   return rounds(n) > 6 || rounds(shifted) == rounds(n) ? shifted : n;
 }
 
+// Where the k-th entry of a compaction's row takes its token from, counted from
+// the row's base; -1: it moves nothing. Ascending entries without a negative
+// one are never below their own place. One that is lower would move its token
+// forward, to a place from which a later batch of the same workgroup may still
+// have to read: it is left out, so that whatever the rows hold, an entry's
+// source lies behind the places of all entries before it.
+constexpr int cache_compact_source(int entry, int k) { return entry < k ? -1 : entry; }
+
 // Heads of a compaction's workgroup, a power of two: as many as leave four
 // tokens a batch (4096 values) and 512 workgroups. 0: more than 64 tokens of a
 // sequence may move, and the columns of a head are divided among workgroups. us

@@ -1296,10 +1296,10 @@ hipError_t launch_cache_copy(const CacheDims& d, f16* codes, f16* values, const 
 }
 
 // ---------------------------------------------------------------- compaction
-// keep ascends, so a token never moves back over one that has yet to move (its
-// place is at most its source): a workgroup that moves its share of a
-// sequence's tokens in order, each batch read whole before it is written, needs
-// no other memory. A value's line holds 8 tokens of 8 columns, so a lone token
+// A token's place is at most its source (cache_compact_source leaves out what
+// would move forward), so every source lies behind the places of the entries
+// before it: a workgroup that moves its share of a sequence's tokens in order,
+// each batch read whole before it is written, needs no other memory. A value's line holds 8 tokens of 8 columns, so a lone token
 // touches 8 times its bytes; that bounds a tree's accepted path.
 struct CompactArgs {
   int B, H, lm, pages, W, lp, K;
@@ -1319,8 +1319,9 @@ struct CompactSeq {
     const int page = table[pos >> lp];
     return (unsigned)page < (unsigned)pages ? (((int64_t)page * H) << lp) + (pos & ((1 << lp) - 1)) : -1;
   }
-  // where the k-th kept token, rel behind base, comes from; -1: it stays or is not there
-  __device__ __forceinline__ void move(int k, int rel, int64_t& from, int64_t& to) const {
+  // where the k-th kept token, entry k of the row, comes from; -1: it stays or is not there
+  __device__ __forceinline__ void move(int k, int entry, int64_t& from, int64_t& to) const {
+    const int rel = cache_compact_source(entry, k);
     from = rel < 0 ? -1 : place(base + rel);
     to = place(base + k);
     if (from < 0 || from == to) to = -1;
@@ -1491,7 +1492,8 @@ __global__ __launch_bounds__(256) void cache_compact_long_kernel(CompactArgs a, 
       }
     }
     // the barrier above lies between this batch's reads and its writes, and
-    // behind the next batch's places; that batch reads nothing written here
+    // behind the next batch's places; that batch reads nothing written here, for
+    // its sources lie behind all of this one's places
     buf = next;
   }
 }

@@ -1,0 +1,76 @@
+"""What the paged cache promises for calls that its documentation allows but that are
+easy to get wrong, without a GPU."""
+
+from __future__ import annotations
+
+import os
+import random
+import shutil
+import subprocess
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+# ---------------------------------------------------------------- compaction in place
+COMPACT = r'''
+#include <cstdio>
+#include <vector>
+#include "dispatch.h"
+// A row's tokens 0 .. n - 1 moved as a workgroup moves them: batches in order,
+// each read whole before it is written.
+int main() {
+  int n, batch, count;
+  while (scanf("%d %d %d", &n, &batch, &count) == 3) {
+    std::vector<int> keep(count), token(n), got(count);
+    for (int& k : keep) scanf("%d", &k);
+    for (int i = 0; i < n; ++i) token[i] = i;
+    for (int k0 = 0; k0 < count; k0 += batch) {
+      const int k1 = k0 + batch < count ? k0 + batch : count;
+      for (int k = k0; k < k1; ++k) {
+        const int from = morpho::cache_compact_source(keep[k], k);
+        got[k] = from >= 0 && from < n ? token[from] : -1;
+      }
+      for (int k = k0; k < k1; ++k)
+        if (got[k] >= 0 && k < n) token[k] = got[k];
+    }
+    for (int i = 0; i < n; ++i) printf("%d ", token[i]);
+    printf("\n");
+  }
+}
+'''
+
+
+@pytest.fixture(scope="module")
+def compact(tmp_path_factory):
+    if shutil.which("g++") is None:
+        pytest.skip("g++ not available")
+    d = tmp_path_factory.mktemp("cache_compact")
+    (d / "compact.cpp").write_text(COMPACT)
+    subprocess.run(["g++", "-std=c++17", "-O1", f"-I{ROOT}/morphottention_amd/csrc", str(d / "compact.cpp"), "-o",
+                    str(d / "compact")], check=True)
+
+    def move(rows):
+        text = "".join(f"{n} {batch} {len(keep)} {' '.join(map(str, keep))}\n" for n, batch, keep in rows)
+        out = subprocess.run([str(d / "compact")], input=text, capture_output=True, text=True, check=True).stdout
+        return [list(map(int, line.split())) for line in out.splitlines()]
+
+    return move
+
+
+def test_compaction_in_batches_is_the_move_at_once(compact):
+    """Every entry takes its token from where it was before the call, in batches of
+    any length and whatever the row holds; one below its place moves nothing."""
+    rng = random.Random(3)
+    rows = [(60, 16, [-1, *range(40)]), (60, 16, [-2, -1, *range(3, 40)]), (20, 4, [5, 5, 4, 1, 19, 20, 7])]
+    for _ in range(300):
+        n = rng.randint(1, 60)
+        keep = [rng.randint(-3, n + 3) for _ in range(rng.randint(1, n))]
+        rows += [(n, batch, k) for batch in (1, 4, 16) for k in (keep, sorted(keep))]
+    for (n, batch, keep), got in zip(rows, compact(rows)):
+        want = list(range(n))
+        for k, entry in enumerate(keep):
+            if k <= entry < n:
+                want[k] = entry
+        assert got == want, (n, batch, keep)
