@@ -9,6 +9,11 @@ import shutil
 import subprocess
 
 import pytest
+import torch
+
+import morphottention_amd as ma
+from morphottention_amd import autograd
+from morphottention_amd import cache as cache_module
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
@@ -74,3 +79,43 @@ def test_compaction_in_batches_is_the_move_at_once(compact):
             if k <= entry < n:
                 want[k] = entry
         assert got == want, (n, batch, keep)
+
+
+# ---------------------------------------------------------------- steps
+@pytest.fixture
+def recorded(monkeypatch):
+    """The kernels' calls, recorded instead of made."""
+    calls = []
+    for module, name in ((autograd, "morpho_cache_append"), (autograd, "morpho_cache_attention"),
+                         (cache_module, "morpho_cache_copy_pages"), (cache_module, "morpho_cache_compact")):
+        def record(*args, _name=name, **kw):
+            calls.append(_name)
+            return torch.zeros(1), torch.zeros(1)
+        monkeypatch.setattr(module, name, record)
+    return calls
+
+
+def _layer(**kw):
+    return ma.MorphoAttention(64, 2, 16, causal=True, **kw)
+
+
+def test_forward_cached_refuses_a_step_that_is_not_good_any_more(recorded):
+    """After the step's sequence was freed, shortened or committed its pages may be
+    another sequence's: nothing is stored."""
+    layer = _layer()
+    weights = layer.pack_cache_weights()
+    x = torch.zeros((1, 3, 64), dtype=torch.float16)
+    for change in ("free", "truncate", "evict", "commit", "accept"):
+        c = ma.MorphoCache(8, 2, 16, 32, page_size=32)
+        a = c.new()
+        c.commit(c.step([a], 40))
+        step = c.step([a], 3)
+        with torch.no_grad():
+            layer.forward_cached(x, weights, c, step)
+        assert recorded == ["morpho_cache_append", "morpho_cache_attention"]
+        {"free": lambda: c.free(a), "truncate": lambda: c.truncate(a, 40), "evict": lambda: c.evict(a, [0, 1]),
+         "commit": lambda: c.commit(step), "accept": lambda: c.accept(step, [[0, 1]])}[change]()
+        recorded.clear()
+        with torch.no_grad(), pytest.raises(KeyError if change == "free" else RuntimeError):
+            layer.forward_cached(x, weights, c, step)
+        assert not recorded, change
