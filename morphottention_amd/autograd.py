@@ -198,6 +198,8 @@ class MorphoAttention(nn.Module):
         :param step: from ``cache.step``; the caller commits it after the last layer.
             A step that was committed, or whose sequences have changed since it was
             made, raises before anything is stored.
+            ``x`` has to have a row of ``step.n`` tokens for each of its sequences
+            (more are padding where the sequences' counts differ).
         :param layer: this layer's index in the cache.
         :param tree: int64 ``[B, n]``, the drafts that each drafted token sees
             (see :func:`morphottention_amd.morpho_cache_attention`).
@@ -208,7 +210,7 @@ class MorphoAttention(nn.Module):
             raise ValueError("mask_diag with a tree: leave a draft's own bit out instead")
         if torch.is_grad_enabled() and x.requires_grad:
             raise RuntimeError("the cache serves inference and has no gradients: call it under torch.no_grad()")
-        cache._still(step)
+        cache._check(step, x)
         codes, values = cache.codes[layer], cache.values[layer]
         with torch.no_grad():
             phi = morpho_cache_append(x.contiguous(), weights, codes, values, step.table, step.lens,

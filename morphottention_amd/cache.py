@@ -348,6 +348,15 @@ class MorphoCache:
         if any(self._stamp[self._known(s)] != stamp for s, stamp in zip(step.seqs, step.stamps)):
             raise RuntimeError("the step's sequences have changed since it was made")
 
+    def _check(self, step: CacheStep, x: torch.Tensor) -> None:
+        """Raise if ``x`` are not the step's new tokens, ``[sequences, step.n, ...]``, or
+        if the step is not good any more: its pages may be another sequence's. Where
+        the counts differ the kernels know them, and ``x`` may be padded further."""
+        self._still(step)
+        B, n = len(step.seqs), step.n
+        if x.dim() < 2 or x.shape[0] != B or x.shape[1] < n or (x.shape[1] > n and step.new_lens is None):
+            raise ValueError(f"x must have {B} rows of {n} tokens, as the step has (got {tuple(x.shape)})")
+
     def commit(self, step: CacheStep) -> None:
         """The step's tokens belong to their sequences."""
         self._still(step)

@@ -119,3 +119,30 @@ def test_forward_cached_refuses_a_step_that_is_not_good_any_more(recorded):
         with torch.no_grad(), pytest.raises(KeyError if change == "free" else RuntimeError):
             layer.forward_cached(x, weights, c, step)
         assert not recorded, change
+
+
+@pytest.mark.parametrize("shape", [(2, 7, 64), (1, 8, 64), (3, 8, 64), (3, 9, 64), (2, 0, 64), (16, 64), (128,)])
+@pytest.mark.parametrize("counts", [8, [8, 3]])
+def test_forward_cached_refuses_tokens_that_are_not_the_steps(recorded, shape, counts):
+    """Fewer tokens would leave committed places unwritten, more would be stored
+    without being the step's."""
+    layer = _layer()
+    c = ma.MorphoCache(8, 2, 16, 32, page_size=32)
+    step = c.step([c.new(), c.new()], counts)
+    with torch.no_grad(), pytest.raises(ValueError, match="2 rows of 8 tokens"):
+        layer.forward_cached(torch.zeros(shape, dtype=torch.float16), layer.pack_cache_weights(), c, step)
+    assert not recorded
+
+
+def test_forward_cached_takes_wider_padding_only_where_counts_tell(recorded):
+    """A step of equal counts has no list of them on the device: a ninth token would
+    be stored. Where the counts differ it is padding."""
+    layer = _layer()
+    weights, x = layer.pack_cache_weights(), torch.zeros((2, 9, 64), dtype=torch.float16)
+    c = ma.MorphoCache(8, 2, 16, 32, page_size=32)
+    with torch.no_grad():
+        with pytest.raises(ValueError, match="2 rows of 8 tokens"):
+            layer.forward_cached(x, weights, c, c.step([c.new(), c.new()], 8))
+        assert not recorded
+        layer.forward_cached(x, weights, c, c.step([c.new(), c.new()], [8, 3]))
+        assert recorded
