@@ -24,7 +24,8 @@ from torch import nn
 
 from . import capi
 from ._ops import add_op_namespace_prefix, ops
-from .cache import CacheStep, MorphoCache, morpho_cache_append, morpho_cache_attention, pack_cache_weights
+from .cache import (CacheStep, MorphoCache, morpho_cache_append, morpho_cache_attention, pack_cache_weights,
+                    refuse_grad)
 
 
 @torch.library.register_fake(add_op_namespace_prefix("forward"))
@@ -192,7 +193,8 @@ class MorphoAttention(nn.Module):
     def forward_cached(self, x: torch.Tensor, weights: torch.Tensor, cache: MorphoCache, step: CacheStep, *,
                        layer: int = 0, tree: torch.Tensor | None = None) -> torch.Tensor:
         """New tokens ``x`` ``[B, n, D]`` of the step's sequences: stored in ``cache``,
-        and their attention over the sequences so far. Inference only.
+        and their attention over the sequences so far. Inference only: raises where
+        ``x``, ``weights`` or a parameter of the layer would need a gradient.
 
         :param weights: :meth:`pack_cache_weights`, made once.
         :param step: from ``cache.step``; the caller commits it after the last layer.
@@ -208,8 +210,7 @@ class MorphoAttention(nn.Module):
             raise ValueError("forward_cached needs a causal layer: later tokens must not change earlier ones")
         if tree is not None and self.mask_diag:
             raise ValueError("mask_diag with a tree: leave a draft's own bit out instead")
-        if torch.is_grad_enabled() and x.requires_grad:
-            raise RuntimeError("the cache serves inference and has no gradients: call it under torch.no_grad()")
+        refuse_grad(x, weights, self.W_phi, self.gate_q, self.gate_k, self.W_V)
         cache._check(step, x)
         codes, values = cache.codes[layer], cache.values[layer]
         with torch.no_grad():

@@ -66,7 +66,8 @@ _PROJECTION_BITS = {"sigmoid": 0, "hardtanh01": 4, "identity": 8}
 _MASK_DIAG = 2
 
 
-def _no_grad(*tensors) -> None:
+def refuse_grad(*tensors) -> None:
+    """Raise if a gradient of one of the tensors would be needed."""
     if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
         raise RuntimeError("the cache serves inference and has no gradients: call it under torch.no_grad()")
 
@@ -99,7 +100,7 @@ def morpho_cache_append(x: torch.Tensor, weights: torch.Tensor, codes: torch.Ten
     """
     if projection not in _PROJECTION_BITS:
         raise ValueError(f"projection must be one of {sorted(_PROJECTION_BITS)} (got {projection!r})")
-    _no_grad(x, weights)
+    refuse_grad(x, weights)
     return ops.cache_append(x, weights, codes, values, table, lens, new_lens, _PROJECTION_BITS[projection])
 
 
@@ -131,7 +132,7 @@ def morpho_cache_attention(phi: torch.Tensor, gate_q: torch.Tensor, gate_k: torc
         raise ValueError(f"max_len must be positive (got {max_len})")
     if tree is not None and mask_diag:
         raise ValueError("mask_diag with a tree: leave a draft's own bit out instead")
-    _no_grad(phi, gate_q, gate_k)
+    refuse_grad(phi, gate_q, gate_k)
     out, lse = ops.cache_attention(phi, gate_q, gate_k, codes, values, table, lens, new_lens, tree, scale, causal,
                                    _MASK_DIAG if mask_diag else 0, max_len or 0)
     return out, lse

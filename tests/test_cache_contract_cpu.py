@@ -146,3 +146,24 @@ def test_forward_cached_takes_wider_padding_only_where_counts_tell(recorded):
         assert not recorded
         layer.forward_cached(x, weights, c, c.step([c.new(), c.new()], [8, 3]))
         assert recorded
+
+
+def test_forward_cached_raises_where_a_gradient_would_be_needed(recorded):
+    """Of the input, the packed weights or any parameter: none is dropped silently."""
+    layer = _layer()
+    weights, x = layer.pack_cache_weights(), torch.zeros((1, 3, 64), dtype=torch.float16)
+    c = ma.MorphoCache(8, 2, 16, 32, page_size=32)
+    step = c.step([c.new()], 3)
+    for p in layer.parameters():
+        p.requires_grad_(False)
+    for t in (x, weights, *layer.parameters()):
+        t.requires_grad_(True)
+        with pytest.raises(RuntimeError, match="no gradients"):
+            layer.forward_cached(x, weights, c, step)
+        assert not recorded
+        with torch.no_grad():
+            layer.forward_cached(x, weights, c, step)
+        t.requires_grad_(False)
+        recorded.clear()
+    layer.forward_cached(x, weights, c, step)  # a frozen layer needs none
+    assert recorded
