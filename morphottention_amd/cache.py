@@ -34,6 +34,7 @@ would need a gradient raises.
 from __future__ import annotations
 
 from dataclasses import dataclass
+from itertools import count
 
 import torch
 
@@ -162,6 +163,11 @@ def morpho_cache_compact(codes: torch.Tensor, values: torch.Tensor, table: torch
     ops.cache_compact(codes, values, table, lens, keep, keep_lens)
 
 
+# What the tokens of a sequence are changes its stamp. No two are alike, of one
+# cache or of several: a step is good for the sequences that it was made for.
+_stamps = count()
+
+
 @dataclass
 class CacheStep:
     """New tokens of some sequences: what one forward pass of all layers needs."""
@@ -219,7 +225,7 @@ class MorphoCache:
         self._uses = [0] * num_pages
         self._pages: dict[int, list[int]] = {}
         self._lens: dict[int, int] = {}
-        self._stamp: dict[int, int] = {}  # changes with the tokens of a sequence
+        self._stamp: dict[int, int] = {}
         self._next = 0
 
     # ---- account
@@ -258,7 +264,7 @@ class MorphoCache:
     def new(self) -> int:
         """A new, empty sequence."""
         seq, self._next = self._next, self._next + 1
-        self._pages[seq], self._lens[seq], self._stamp[seq] = [], 0, 0
+        self._pages[seq], self._lens[seq], self._stamp[seq] = [], 0, next(_stamps)
         return seq
 
     def free(self, seq: int) -> None:
@@ -297,7 +303,7 @@ class MorphoCache:
         self._drop(self._pages[seq][keep:])
         del self._pages[seq][keep:]
         self._lens[seq] = length
-        self._stamp[seq] += 1
+        self._stamp[seq] = next(_stamps)
 
     def _own(self, wanted: list[tuple[int, int, int]]) -> None:
         """For each (seq, first, end): the pages that hold positions first .. end - 1
@@ -347,7 +353,7 @@ class MorphoCache:
 
     def _still(self, step: CacheStep) -> None:
         if any(self._stamp[self._known(s)] != stamp for s, stamp in zip(step.seqs, step.stamps)):
-            raise RuntimeError("the step's sequences have changed since it was made")
+            raise RuntimeError("the step's sequences have changed since it was made, or are another cache's")
 
     def _check(self, step: CacheStep, x: torch.Tensor) -> None:
         """Raise if ``x`` are not the step's new tokens, ``[sequences, step.n, ...]``, or
@@ -363,7 +369,7 @@ class MorphoCache:
         self._still(step)
         for s, c in zip(step.seqs, step.counts):
             self._lens[s] += c
-            self._stamp[s] += 1
+            self._stamp[s] = next(_stamps)
 
     def accept(self, step: CacheStep, kept: list[list[int]]) -> None:
         """After a step of drafts: of each sequence the drafts ``kept[b]`` (ascending

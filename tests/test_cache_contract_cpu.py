@@ -167,3 +167,22 @@ def test_forward_cached_raises_where_a_gradient_would_be_needed(recorded):
         recorded.clear()
     layer.forward_cached(x, weights, c, step)  # a frozen layer needs none
     assert recorded
+
+
+def test_a_step_of_another_cache_is_refused(recorded):
+    """Caches number their sequences alike (a draft model's and its target's): a step
+    of one names pages that mean nothing in the other."""
+    layer = _layer()
+    weights, x = layer.pack_cache_weights(), torch.zeros((1, 3, 64), dtype=torch.float16)
+    one, two = (ma.MorphoCache(8, 2, 16, 32, page_size=32) for _ in range(2))
+    a, b = one.new(), two.new()
+    assert a == b
+    step = one.step([a], 3)
+    with torch.no_grad():
+        for call in (lambda: layer.forward_cached(x, weights, two, step), lambda: two.commit(step),
+                     lambda: two.accept(step, [[1]])):
+            with pytest.raises(RuntimeError, match="another cache"):
+                call()
+    assert not recorded and two.length(b) == 0 and two.pages(b) == ()
+    one.commit(step)
+    assert one.length(a) == 3
