@@ -310,6 +310,7 @@ class MorphoCache:
         exist and belong to the sequence alone. Nothing changes when the pool
         has too few pages left."""
         P = self.page_size
+        wanted = [(seq, first, end) for seq, first, end in wanted if first < end]
         shared, grow = [], []
         spare: dict[int, int] = {}
         for seq, first, end in wanted:

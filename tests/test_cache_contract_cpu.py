@@ -186,3 +186,20 @@ def test_a_step_of_another_cache_is_refused(recorded):
     assert not recorded and two.length(b) == 0 and two.pages(b) == ()
     one.commit(step)
     assert one.length(a) == 3
+
+
+def test_a_sequence_without_new_tokens_keeps_its_pages(recorded):
+    """A count of 0 writes nothing, so a shared page that is not full is not copied,
+    and a full pool is no obstacle."""
+    c = ma.MorphoCache(3, 2, 16, 32, page_size=32)
+    a = c.new()
+    c.commit(c.step([a], 64))
+    b = c.fork(a)
+    c.truncate(b, 40)
+    before = c.pages(b)
+    assert before == c.pages(a)
+    c.commit(c.step([a, b], [3, 0]))  # the last page is a's third
+    assert c.pages(b) == before and c.free_pages == 0 and not recorded
+    c.free(a)
+    c.commit(c.step([b], 1))
+    assert c.pages(b) == before and not recorded  # nobody else has it any more
