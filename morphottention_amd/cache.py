@@ -33,8 +33,8 @@ would need a gradient raises.
 
 from __future__ import annotations
 
-from dataclasses import dataclass
-from itertools import count
+import itertools
+from dataclasses import dataclass, field
 
 import torch
 
@@ -163,9 +163,24 @@ def morpho_cache_compact(codes: torch.Tensor, values: torch.Tensor, table: torch
     ops.cache_compact(codes, values, table, lens, keep, keep_lens)
 
 
-# What the tokens of a sequence are changes its stamp. No two are alike, of one
-# cache or of several: a step is good for the sequences that it was made for.
-_stamps = count()
+# What changes the tokens of a sequence gives it a new stamp. They rise and are
+# never given twice, by one cache or several: a step is good only for the
+# sequences that it was made for.
+_stamps = itertools.count()
+
+
+class _Claim:
+    """A step's claim on the pages of its new tokens. It ends with the step (and its
+    copies): when the cache takes the step back, or when nobody has it any more."""
+
+    def __init__(self, claims: dict[int, dict[int, int]], mine: dict[int, int]) -> None:
+        self.claims, self.key, self.dropped = claims, next(_stamps), False
+        claims[self.key] = mine
+
+    def end(self) -> None:
+        self.claims.pop(self.key, None)
+
+    __del__ = end
 
 
 @dataclass
@@ -180,6 +195,7 @@ class CacheStep:
     new_lens: torch.Tensor | None
     max_len: int
     stamps: list[int]
+    claim: _Claim | None = field(default=None, repr=False, compare=False)
 
 
 class MorphoCache:
@@ -200,9 +216,12 @@ class MorphoCache:
         cache.commit(step)
 
     Until then the sequences keep their old lengths, so a step that is dropped
-    leaves them as they were. After a tree of drafts :meth:`accept` takes the
-    accepted tokens instead. A step is good for one commit, and only as long as
-    its sequences have not changed otherwise.
+    leaves their tokens as they were. Its pages are free again after :meth:`drop`,
+    or once nobody has the step any more (an exception, say). After a tree of
+    drafts :meth:`accept` takes the accepted tokens instead. A step is good for
+    one commit, and only as long as its sequences have not changed otherwise.
+    Steps of one sequence that are made before either is committed write to the
+    same places.
     """
 
     def __init__(self, num_pages: int, num_heads: int, cube_m: int, head_dim: int, *, num_layers: int = 1,
@@ -226,12 +245,16 @@ class MorphoCache:
         self._pages: dict[int, list[int]] = {}
         self._lens: dict[int, int] = {}
         self._stamp: dict[int, int] = {}
+        # of each step that is neither committed nor dropped: its stamp, and {seq: end of the new tokens}
+        self._claims: dict[int, dict[int, int]] = {}
+        self._grown: set[int] = set()  # sequences that may have pages past their tokens
         self._next = 0
 
     # ---- account
     @property
     def free_pages(self) -> int:
-        """Pages that no sequence has."""
+        """Pages that no sequence has, and no step claims for one."""
+        self._shrink()
         return len(self._free)
 
     def length(self, seq: int) -> int:
@@ -239,7 +262,7 @@ class MorphoCache:
         return self._lens[self._known(seq)]
 
     def pages(self, seq: int) -> tuple[int, ...]:
-        """The pages of a sequence, in order."""
+        """The pages of a sequence, in order (with those of a step that is not committed yet)."""
         return tuple(self._pages[self._known(seq)])
 
     def _known(self, seq: int) -> int:
@@ -261,6 +284,24 @@ class MorphoCache:
             if self._uses[p] == 0:
                 self._free.append(p)
 
+    def _cut(self, seq: int, length: int) -> bool:
+        """Give up the pages of a sequence past ``length`` tokens."""
+        keep = -(-length // self.page_size)
+        gone = self._pages[seq][keep:]
+        self._drop(gone)
+        del self._pages[seq][keep:]
+        return bool(gone)
+
+    def _shrink(self) -> None:
+        """Give up the pages past the tokens of sequences that no step claims any more."""
+        claims = self._claims.copy().items()  # of which any may end while this runs
+        for seq in list(self._grown):
+            ends = [claim[seq] for stamp, claim in claims if seq in claim and stamp > self._stamp[seq]]
+            if not ends:
+                self._grown.discard(seq)
+            if self._cut(seq, max([self._lens[seq], *ends])) and not ends:
+                self._stamp[seq] = next(_stamps)  # nor is a step good that was taken apart
+
     def new(self) -> int:
         """A new, empty sequence."""
         seq, self._next = self._next, self._next + 1
@@ -271,6 +312,7 @@ class MorphoCache:
         """Give a sequence up; its pages that no fork shares are free again."""
         self._drop(self._pages.pop(self._known(seq)))
         del self._lens[seq], self._stamp[seq]
+        self._grown.discard(seq)
 
     def _ints(self, rows) -> torch.Tensor:
         return torch.tensor(rows, dtype=torch.int32, device=self.codes.device)
@@ -285,6 +327,8 @@ class MorphoCache:
         that is not full is copied, since both will append to theirs."""
         length = self._lens[self._known(seq)]
         full, rest = divmod(length, self.page_size)
+        if rest and not self._free:
+            self._shrink()
         own = self._take(1) if rest else []
         if rest:
             self._copy([(self._pages[seq][full], own[0])])
@@ -299,18 +343,15 @@ class MorphoCache:
         """Forget the tokens of a sequence from position ``length`` on."""
         if not 0 <= length <= self._lens[self._known(seq)]:
             raise ValueError(f"length must be 0 .. {self._lens[seq]} (got {length})")
-        keep = -(-length // self.page_size)
-        self._drop(self._pages[seq][keep:])
-        del self._pages[seq][keep:]
+        self._cut(seq, length)
+        self._grown.discard(seq)
         self._lens[seq] = length
         self._stamp[seq] = next(_stamps)
 
-    def _own(self, wanted: list[tuple[int, int, int]]) -> None:
-        """For each (seq, first, end): the pages that hold positions first .. end - 1
-        exist and belong to the sequence alone. Nothing changes when the pool
-        has too few pages left."""
+    def _missing(self, wanted: list[tuple[int, int, int]]) -> tuple[list[tuple[int, int]], list[int]]:
+        """For each (seq, first, end): which of the pages that hold positions first ..
+        end - 1 are shared (seq, index), and how many there are none of."""
         P = self.page_size
-        wanted = [(seq, first, end) for seq, first, end in wanted if first < end]
         shared, grow = [], []
         spare: dict[int, int] = {}
         for seq, first, end in wanted:
@@ -323,7 +364,21 @@ class MorphoCache:
                     shared.append((seq, k))
                     spare[p] = left - 1
             grow.append(max(0, -(-end // P) - len(have)))
-        fresh = self._take(len(shared) + sum(grow))
+        return shared, grow
+
+    def _own(self, wanted: list[tuple[int, int, int]]) -> None:
+        """For each (seq, first, end): the pages that hold positions first .. end - 1
+        exist and belong to the sequence alone. No sequence's tokens or pages for
+        them change when the pool has too few pages left."""
+        shared, grow = self._missing(wanted)
+        need = len(shared) + sum(grow)
+        if need > len(self._free):
+            self._shrink()
+            shared, grow = self._missing(wanted)  # it may have taken pages of these sequences
+            need = len(shared) + sum(grow)
+        if not need:
+            return
+        fresh = self._take(need)
         pairs = []
         for seq, k in shared:
             page = fresh.pop()
@@ -345,14 +400,28 @@ class MorphoCache:
         if len(counts) != len(seqs) or min(counts) < 0 or max(counts) == 0:
             raise ValueError("counts must be one number, or one for each sequence, not negative and not all 0")
         ends = [self._lens[self._known(s)] + c for s, c in zip(seqs, counts)]
-        self._own([(s, self._lens[s], e) for s, e in zip(seqs, ends)])
+        self._own([(s, self._lens[s], e) for s, c, e in zip(seqs, counts, ends) if c])
+        self._grown.update(seqs)
+        claim = _Claim(self._claims, dict(zip(seqs, ends)))
         width = max(-(-e // self.page_size) for e in ends)
         rows = [(self._pages[s] + [-1] * width)[:width] for s in seqs]
         n = max(counts)
         return CacheStep(seqs, counts, n, self._ints(rows), self._ints([self._lens[s] for s in seqs]),
-                         self._ints(counts) if min(counts) < n else None, max(ends), [self._stamp[s] for s in seqs])
+                         self._ints(counts) if min(counts) < n else None, max(ends), [self._stamp[s] for s in seqs], claim)
+
+    def drop(self, step: CacheStep) -> None:
+        """Give a step up that is not committed: its pages past the tokens of its
+        sequences are free again. (A page that it copied on write stays the
+        sequence's own.)"""
+        if step.claim is None or step.claim.claims is not self._claims:
+            raise RuntimeError("the step is another cache's")
+        step.claim.dropped = True
+        step.claim.end()
+        self._shrink()
 
     def _still(self, step: CacheStep) -> None:
+        if step.claim is not None and step.claim.dropped:
+            raise RuntimeError("the step was dropped")
         if any(self._stamp[self._known(s)] != stamp for s, stamp in zip(step.seqs, step.stamps)):
             raise RuntimeError("the step's sequences have changed since it was made, or are another cache's")
 
@@ -368,9 +437,15 @@ class MorphoCache:
     def commit(self, step: CacheStep) -> None:
         """The step's tokens belong to their sequences."""
         self._still(step)
+        stamp = next(_stamps)
         for s, c in zip(step.seqs, step.counts):
-            self._lens[s] += c
-            self._stamp[s] = next(_stamps)
+            self._lens[s] = length = self._lens[s] + c
+            self._stamp[s] = stamp
+            if (len(self._pages[s]) - 1) * self.page_size >= length:
+                self._cut(s, length)  # what other steps claimed: none is good any more
+        self._grown.difference_update(step.seqs)
+        if step.claim is not None:
+            step.claim.end()
 
     def accept(self, step: CacheStep, kept: list[list[int]]) -> None:
         """After a step of drafts: of each sequence the drafts ``kept[b]`` (ascending
@@ -390,6 +465,8 @@ class MorphoCache:
         for s, k in zip(step.seqs, kept):
             self._lens[s] += len(k)
             self.truncate(s, self._lens[s])
+        if step.claim is not None:
+            step.claim.end()
 
     def evict(self, seq: int, kept: list[int]) -> None:
         """Keep only the tokens at positions ``kept`` (ascending) of a sequence; they

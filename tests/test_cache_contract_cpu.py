@@ -3,6 +3,8 @@ easy to get wrong, without a GPU."""
 
 from __future__ import annotations
 
+import copy
+import dataclasses
 import os
 import random
 import shutil
@@ -203,3 +205,122 @@ def test_a_sequence_without_new_tokens_keeps_its_pages(recorded):
     c.free(a)
     c.commit(c.step([b], 1))
     assert c.pages(b) == before and not recorded  # nobody else has it any more
+
+
+def test_a_dropped_step_gives_its_pages_back(recorded):
+    """By drop(), or when nobody has it any more: the pool is as it was, and another
+    sequence can have the pages."""
+    c = ma.MorphoCache(8, 2, 16, 32, page_size=32)
+    a, b = c.new(), c.new()
+    c.commit(c.step([a], 40))
+    assert c.free_pages == 6
+    c.step([a], 7 * 32 - 40)
+    assert c.free_pages == 6 and c.length(a) == 40
+    step = c.step([a], 7 * 32 - 40)
+    assert c.free_pages == 1
+    c.drop(step)
+    assert c.free_pages == 6
+    with torch.no_grad():
+        for call in (lambda: c.commit(step), lambda: c.accept(step, [[0]]),
+                     lambda: _layer().forward_cached(torch.zeros((1, step.n, 64)), None, c, step)):
+            with pytest.raises(RuntimeError):
+                call()
+    c.drop(step)  # again: nothing left to do
+    try:
+        step = c.step([a], 100)
+        raise KeyError("between step and commit")
+    except KeyError:
+        del step
+    c.commit(c.step([b], 6 * 32))  # all that a's tokens leave
+    assert c.free_pages == 0 and c.length(a) == 40 and not recorded
+
+
+def test_a_step_that_is_there_keeps_its_pages(recorded):
+    """A full pool takes nothing from a step that can still be committed, from its
+    copies, or from another step of the same sequence."""
+    c = ma.MorphoCache(8, 2, 16, 32, page_size=32)
+    a, b = c.new(), c.new()
+    step = c.step([a], 5 * 32)
+    with pytest.raises(RuntimeError, match="cache is full"):
+        c.step([b], 4 * 32)
+    step = dataclasses.replace(step, table=step.table.clone())
+    with pytest.raises(RuntimeError, match="cache is full"):
+        c.step([b], 4 * 32)
+    step = copy.copy(step)
+    shorter, longer = c.step([a], 70), c.step([a], 7 * 32)
+    assert c.free_pages == 1
+    c.drop(longer)
+    assert c.free_pages == 3
+    c.drop(shorter)
+    assert c.free_pages == 3
+    c.commit(step)
+    assert c.length(a) == 5 * 32 and len(c.pages(a)) == 5
+    with pytest.raises(RuntimeError, match="another cache"):
+        ma.MorphoCache(8, 2, 16, 32).drop(step)
+    c.drop(step)  # it is committed: no harm
+    assert c.length(a) == 5 * 32 and c.free_pages == 3
+    other = c.step([a], 1)
+    long = c.step([a], 64)
+    c.commit(other)  # the long one is not good any more, and claims nothing
+    assert c.free_pages == 2 and long is not None
+
+
+@pytest.mark.parametrize("seed", range(8))
+def test_account_with_steps_in_flight(recorded, seed):
+    """Several steps at once, committed, accepted or dropped in any order: no page has
+    two owners or is lost, a step's pages are its own until it ends, and those
+    that nobody claims can be had."""
+    rng = random.Random(seed)
+    c = ma.MorphoCache(24, 2, 16, 32, page_size=32)
+    steps, seqs = [], [c.new() for _ in range(4)]
+    for _ in range(300):
+        act = rng.choice(["step", "step", "step", "commit", "accept", "drop", "lose", "truncate", "fork", "free", "evict"])
+        s = rng.choice(seqs)
+        try:
+            if act == "step":
+                mine = rng.sample(seqs, rng.randint(1, 3))
+                counts = [rng.choice([0, 1, 33, 100]) for _ in mine]
+                if max(counts):
+                    steps.append(c.step(mine, counts))
+            elif act in ("commit", "accept") and steps:
+                step = steps.pop(rng.randrange(len(steps)))
+                c.commit(step) if act == "commit" else c.accept(step, [list(range(0, k, 2)) for k in step.counts])
+            elif act == "drop" and steps:
+                c.drop(steps.pop(rng.randrange(len(steps))))
+            elif act == "lose" and steps:
+                del steps[rng.randrange(len(steps))]
+            elif act == "truncate":
+                c.truncate(s, rng.randint(0, c.length(s)))
+            elif act == "evict":
+                c.evict(s, list(range(0, c.length(s), 2)))
+            elif act == "fork" and len(seqs) < 7:
+                seqs.append(c.fork(s))
+            elif act == "free" and len(seqs) > 3:
+                c.free(s)
+                seqs.remove(s)
+        except (RuntimeError, KeyError) as e:
+            assert any(t in str(e) for t in ("cache is full", "have changed", "no sequence"))
+        uses = [0] * c.num_pages
+        for s in seqs:
+            for p in c.pages(s):
+                uses[p] += 1
+            assert len(c.pages(s)) * 32 >= c.length(s)
+        assert uses == c._uses and sorted(c._free) == [p for p in range(c.num_pages) if not uses[p]]
+        good = []
+        for step in steps:
+            try:
+                c._still(step)
+            except (RuntimeError, KeyError):
+                continue
+            good.append(step)
+            for b, (s, k) in enumerate(zip(step.seqs, step.counts)):
+                for t in range(c.length(s), c.length(s) + k):
+                    page = int(step.table[b, t // 32])
+                    assert c.pages(s)[t // 32] == page and uses[page] == 1
+    steps.clear()
+    good.clear()
+    del step
+    assert c.free_pages == 24 - len({p for s in seqs for p in c.pages(s)[: -(-c.length(s) // 32)]})
+    for s in seqs:
+        c.free(s)
+    assert c.free_pages == 24 and not c._claims and not c._grown
