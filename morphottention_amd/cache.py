@@ -317,10 +317,15 @@ class MorphoCache:
     def _ints(self, rows) -> torch.Tensor:
         return torch.tensor(rows, dtype=torch.int32, device=self.codes.device)
 
-    def _copy(self, pairs: list[tuple[int, int]]) -> None:
-        if pairs:
-            morpho_cache_copy_pages(self.codes, self.values, self._ints([a for a, _ in pairs]),
-                                    self._ints([b for _, b in pairs]))
+    def _copies(self, pages: list[int], fresh: list[int]) -> None:
+        """Copy pages to taken ones, before the account says so: where that raises
+        (while a graph is captured, say), all of ``fresh`` are free again."""
+        try:
+            if pages:
+                morpho_cache_copy_pages(self.codes, self.values, self._ints(pages), self._ints(fresh[: len(pages)]))
+        except BaseException:
+            self._drop(fresh)
+            raise
 
     def fork(self, seq: int) -> int:
         """A new sequence with the same tokens. Full pages are shared; a page
@@ -330,8 +335,7 @@ class MorphoCache:
         if rest and not self._free:
             self._shrink()
         own = self._take(1) if rest else []
-        if rest:
-            self._copy([(self._pages[seq][full], own[0])])
+        self._copies(self._pages[seq][full : full + len(own)], own)
         shared = self._pages[seq][:full]
         for p in shared:
             self._uses[p] += 1
@@ -379,15 +383,13 @@ class MorphoCache:
         if not need:
             return
         fresh = self._take(need)
-        pairs = []
+        self._copies([self._pages[seq][k] for seq, k in shared], fresh)
+        pages = iter(fresh)
         for seq, k in shared:
-            page = fresh.pop()
-            pairs.append((self._pages[seq][k], page))
             self._uses[self._pages[seq][k]] -= 1
-            self._pages[seq][k] = page
+            self._pages[seq][k] = next(pages)
         for (seq, _, _), count in zip(wanted, grow):
-            self._pages[seq] += [fresh.pop() for _ in range(count)]
-        self._copy(pairs)
+            self._pages[seq] += itertools.islice(pages, count)
 
     # ---- steps
     def step(self, seqs: list[int], counts: int | list[int]) -> CacheStep:

@@ -324,3 +324,23 @@ def test_account_with_steps_in_flight(recorded, seed):
     for s in seqs:
         c.free(s)
     assert c.free_pages == 24 and not c._claims and not c._grown
+
+
+def test_a_copy_that_fails_changes_no_account(monkeypatch):
+    """Where the pages cannot be copied (the copy raises, as host tensors in a graph
+    capture do), no sequence gets a page without its tokens, and none is lost."""
+    c = ma.MorphoCache(8, 2, 16, 32, page_size=32)
+    a = c.new()
+    c.commit(c.step([a], 64))
+    b = c.fork(a)
+    c.truncate(b, 40)
+    before = c.pages(a), c.pages(b), c.free_pages, list(c._uses)
+
+    def fail(*args):
+        raise RuntimeError("no copy")
+    monkeypatch.setattr(cache_module, "morpho_cache_copy_pages", fail)
+    for call in (lambda: c.fork(b), lambda: c.step([b], 1), lambda: c.step([a, b], [64, 3]), lambda: c.evict(a, [1, 2])):
+        with pytest.raises(RuntimeError, match="no copy"):
+            call()
+        assert (c.pages(a), c.pages(b), c.free_pages, c._uses) == before
+        assert sorted(c._free) == [p for p in range(8) if not c._uses[p]]
