@@ -255,7 +255,9 @@ size_t morpho_cache_attention_workspace_size(const morpho_cache* cache, int64_t 
  * computed in full). cache->layers must be 1.
  * Numeric range: scale * log2(e) * gate_q[h][c] * gate_k[h][c] * (2 phi - 1) of
  * a query must stay below 65,504 for every code, or the row is NaN. A value
- * that is not finite reaches the rows that see its key, and no other. */
+ * that is not finite reaches the rows that see its key, and no other: their
+ * column is the sum of such values (infinite, or NaN where both infinities or a
+ * NaN are among them), however small the weight. */
 int morpho_cache_attention(const void* phi, const void* gate_q, const void* gate_k, const morpho_cache* cache,
                            const int32_t* table, const int32_t* lens, const int32_t* new_lens, const int64_t* tree,
                            void* out, float* lse, int64_t B, int64_t n, int64_t seq_pages, int64_t max_len,

@@ -713,7 +713,10 @@ MORPHO_EXPORT int morpho_cache_attention(const void* phi, const void* gate_q, co
                                   static_cast<const _Float16*>(gate_k), static_cast<const _Float16*>(cache->codes),
                                   static_cast<const _Float16*>(cache->values), table, lens, new_lens, tree, o, lse,
                                   part, scale, mode & MORPHO_MODE_CAUSAL, mode & MORPHO_MODE_MASK_DIAG, s));
-  if (need) MORPHO_LAUNCH("cache_join", launch_cache_attn_join(d, plan, lens, new_lens, part, o, lse, s));
+  if (need)
+    MORPHO_LAUNCH("cache_join",
+                  launch_cache_attn_join(d, plan, static_cast<const _Float16*>(cache->values), table, lens, new_lens,
+                                         tree, part, o, lse, mode & MORPHO_MODE_CAUSAL, mode & MORPHO_MODE_MASK_DIAG, s));
   return MORPHO_OK;
 }
 

@@ -159,8 +159,10 @@ hipError_t launch_cache_attn(const CacheDims& d, const CacheAttnPlan& plan, cons
                              const _Float16* values, const int* table, const int* lens, const int* new_lens,
                              const int64_t* tree, _Float16* out, float* lse, const CacheAttnBuffers& part, float scale,
                              int causal, int mask_diag, hipStream_t s);
-hipError_t launch_cache_attn_join(const CacheDims& d, const CacheAttnPlan& plan, const int* lens, const int* new_lens,
-                                  const CacheAttnBuffers& part, _Float16* out, float* lse, hipStream_t s);
+hipError_t launch_cache_attn_join(const CacheDims& d, const CacheAttnPlan& plan, const _Float16* values,
+                                  const int* table, const int* lens, const int* new_lens, const int64_t* tree,
+                                  const CacheAttnBuffers& part, _Float16* out, float* lse, int causal, int mask_diag,
+                                  hipStream_t s);
 hipError_t launch_cache_copy(const CacheDims& d, _Float16* codes, _Float16* values, const int* src, const int* dst,
                              int count, hipStream_t s);
 hipError_t launch_cache_compact(const CacheDims& d, _Float16* codes, _Float16* values, const int* table,

@@ -431,30 +431,75 @@ struct CacheOut {
   float* part_o;
   float4* part_st;
   int n, H, b, h, nb, nsplit, sp;
-  // m, l: reference and sum of the weights; r: the row constant
-  __device__ __forceinline__ void operator()(int i, int c, f32x4 o, float m, float l, float r) const {
-    if (i >= n) return;
+  __device__ __forceinline__ f16* row(int i, int c) const { return out + (((int64_t)b * n + i) * H + h) * DV + c; }
+  // m, l: reference and sum of the weights; r: the row constant. Not 0: the
+  // result has columns that are not finite (settle_columns).
+  __device__ __forceinline__ unsigned operator()(int i, int c, f32x4 o, float m, float l, float r) const {
+    if (i >= n) return 0;
     const int64_t at = ((int64_t)b * H + h) * n + i;
     if (nsplit > 1) {
-      if (i >= nb) return;  // the joining kernel writes padding rows
+      if (i >= nb) return 0;  // the joining kernel writes padding rows
       *reinterpret_cast<f32x4*>(part_o + (at * nsplit + sp) * DV + c) = o;
       if (c == 0) part_st[at * nsplit + sp] = float4{m, l, r, 0.f};
-      return;
+      return 0;
     }
     const bool some = i < nb && l != 0.f;  // padding rows and rows that see nothing get 0
     const float inv = some ? 1.f / l : 0.f;
     f16x4 y;
 #pragma unroll
     for (int k = 0; k < 4; ++k) y[k] = some ? (f16)(o[k] * inv) : (f16)0.f;
-    *reinterpret_cast<f16x4*>(out + (((int64_t)b * n + i) * H + h) * DV + c) = y;
+    *reinterpret_cast<f16x4*>(row(i, c)) = y;
     if (c == 0) {
       // a difference of larger numbers: the logarithm of the mantissa alone, in
       // [-1, 0), is good to 2^-24, and the rest is added in 64 bits
       const double lg = (double)fast_log2(__builtin_amdgcn_frexp_mantf(l)) + (double)__builtin_amdgcn_frexp_expf(l);
       lse[at] = some ? (float)((double)m + lg - (double)r) : -kFltMax;
     }
+    // an exponent of all ones carries into bit 15 of its half
+    const uint64_t bits = __builtin_bit_cast(uint64_t, y);
+    return ((((unsigned)bits & 0x7c007c00u) + 0x04000400u) | (((unsigned)(bits >> 32) & 0x7c007c00u) + 0x04000400u)) &
+           0x80008000u;
   }
 };
+
+// Columns c .. c + 3 of a finished row, those of them that are not finite. The
+// weight of every key that a row sees is positive, so a value that is not finite
+// decides its column whatever the weight: infinite, or NaN where both infinities
+// or a NaN are among them. The value product does not keep to that (0 times an
+// infinity where a weight rounds to nothing, infinities of both signs where it is
+// a pair of halves), so such a column becomes the sum of the values that are not
+// finite. The keys are read once more, which nothing but
+// such a row pays for (the kernels' times: the same with and without, +-1 %).
+// v, stride: the head's values in page 0, and a page's; pages: the sequence's, of
+// `count` in the pool; i: the row; bits: its drafts; l: the sum of its weights
+// (scores that are not numbers leave nothing to settle); out: column c of it.
+template <int DV>
+__device__ __forceinline__ void settle_columns(const f16* v, int64_t stride, const int* pages, int count, int lp,
+                                               const CacheMask& mask, int i, uint64_t bits, float l, f16* out,
+                                               int c) {
+  if (!__builtin_isfinite(l)) return;
+  f16x4* at = reinterpret_cast<f16x4*>(out);
+  f16x4 y = *at;
+  if (!(not_finite(y[0]) || not_finite(y[1]) || not_finite(y[2]) || not_finite(y[3]))) return;
+  f32x4 sum = {};
+#pragma unroll 1
+  for (int key = 0; key < mask.total; key += 8) {
+    const int page = pages[key >> lp];
+    const unsigned seen = mask(i, bits, key);
+    if ((unsigned)page >= (unsigned)count || seen == 0) continue;
+    const f16* from = v + page * stride + ((key & ((1 << lp) - 1)) * DV + 8 * c);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const f16x8 x = *reinterpret_cast<const f16x8*>(from + 8 * k);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sum[k] += (seen >> j) & 1 && not_finite(x[j]) ? (float)x[j] : 0.f;
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (not_finite(y[k]) && sum[k] != 0.f) y[k] = (f16)sum[k];
+  *at = y;
+}
 
 // What a workgroup works on: heads fastest (a page's heads are neighbours in
 // memory, and with a multiple of 8 heads all row blocks of a head share an
@@ -589,7 +634,10 @@ __global__ __launch_bounds__(256) void cache_attn_few_kernel(
       l += f * sl[k][q];
       o += f * *reinterpret_cast<const f32x4*>(&so[k][q][c]);
     }
-    put(q, c, o, m, l, sr[q]);
+    if (put(q, c, o, m, l, sr[q]))
+      settle_columns<DV>(values + (((int64_t)h * DV) << a.lp), ((int64_t)a.H * DV) << a.lp, table + (int64_t)b * a.W,
+                         a.pages, a.lp, mask, q, tree ? (uint64_t)tree[(int64_t)b * a.n + q] : 0, l,
+                         put.row(q, c), c);
   }
 }
 
@@ -769,13 +817,25 @@ __global__ __launch_bounds__(256, M > 32 || DV > 64 ? 2 : LO || QT > 1 ? 3 : 4) 
     close();
   }
   const CacheOut<DV> put{out, lse, part_o, part_st, a.n, a.H, b, h, sq.nb, a.nsplit, blk.sp};
+  unsigned odd[QT];
+  float weights[QT];
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
-    float ref, l;
-    R.finish(t, ref, l);
+    float ref;
+    R.finish(t, ref, weights[t]);
     const float r = sr[w][16 * t + c16];
+    odd[t] = 0;
 #pragma unroll
-    for (int c = 0; c < NT; ++c) put(qw + 16 * t + c16, 16 * c + 4 * g, R.O[t][c], ref, l, r);
+    for (int c = 0; c < NT; ++c) odd[t] |= put(qw + 16 * t + c16, 16 * c + 4 * g, R.O[t][c], ref, weights[t], r);
+  }
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    if (!odd[t]) continue;
+    const int i = qw + 16 * t + c16;
+#pragma unroll 1
+    for (int c = 4 * g; c < DV; c += 16)
+      settle_columns<DV>(reinterpret_cast<const f16*>(vh), vpage / 2, src.row, src.pages, src.lp, mask, i, bits[t],
+                         weights[t], put.row(i, c), c);
   }
 }
 
@@ -783,8 +843,10 @@ __global__ __launch_bounds__(256, M > 32 || DV > 64 ? 2 : LO || QT > 1 ? 3 : 4) 
 // groups take its pieces in turn, and the groups are added in order. Bound by
 // its launch: B64 n1 H16 of up to 9 pieces 4.4 us where an empty one takes 4.0.
 template <int DV, int NG>
-__global__ __launch_bounds__(256) void cache_join_kernel(CacheAttnArgs a, int64_t rows, const int* __restrict__ lens,
+__global__ __launch_bounds__(256) void cache_join_kernel(CacheAttnArgs a, int64_t rows, const f16* __restrict__ values,
+                                                        const int* __restrict__ table, const int* __restrict__ lens,
                                                         const int* __restrict__ new_lens,
+                                                        const int64_t* __restrict__ tree,
                                                         const float* __restrict__ part_o,
                                                         const float4* __restrict__ part_st, f16* __restrict__ out,
                                                         float* __restrict__ lse) {
@@ -830,12 +892,15 @@ __global__ __launch_bounds__(256) void cache_join_kernel(CacheAttnArgs a, int64_
   }
   if (at >= rows) return;
   const CacheOut<DV> put{out, lse, nullptr, nullptr, a.n, a.H, b, h, sq.nb, 1, 0};
-  put(i, c, o, m, l, r);
+  const CacheMask mask{sq.ctx, sq.nb, sq.total, a.causal, a.mask_diag, tree != nullptr};
+  if (put(i, c, o, m, l, r))
+    settle_columns<DV>(values + (((int64_t)h * DV) << a.lp), ((int64_t)a.H * DV) << a.lp, table + (int64_t)b * a.W,
+                       a.pages, a.lp, mask, i, tree ? (uint64_t)tree[(int64_t)b * a.n + i] : 0, l, put.row(i, c), c);
 }
 
 namespace {
 int log2_of(int p) { return __builtin_ctz((unsigned)p); }
-CacheAttnArgs attn_args(const CacheDims& d, const CacheAttnPlan& p) {
+CacheAttnArgs attn_args(const CacheDims& d, const CacheAttnPlan& p, int causal, int mask_diag) {
   CacheAttnArgs a{};
   a.B = d.B;
   a.n = d.n;
@@ -846,6 +911,8 @@ CacheAttnArgs attn_args(const CacheDims& d, const CacheAttnPlan& p) {
   a.qblocks = p.qblocks;
   a.nsplit = p.nsplit;
   a.split_keys = p.split_keys;
+  a.causal = causal;
+  a.mask_diag = mask_diag;
   return a;
 }
 
@@ -875,22 +942,22 @@ hipError_t launch_cache_attn(const CacheDims& d, const CacheAttnPlan& plan, cons
                              const f16* gate_k, const f16* codes, const f16* values, const int* table,
                              const int* lens, const int* new_lens, const int64_t* tree, f16* out, float* lse,
                              const CacheAttnBuffers& part, float scale, int causal, int mask_diag, hipStream_t s) {
-  CacheAttnArgs a = attn_args(d, plan);
+  CacheAttnArgs a = attn_args(d, plan, causal, mask_diag);
   a.sl2e = scale * kLog2e;
-  a.causal = causal;
-  a.mask_diag = mask_diag;
   MORPHO_MDV_DISPATCH(launch_cache_attn_t, d, plan, a, phi, gate_q, gate_k, codes, values, table, lens, new_lens, tree,
                       out, lse, part, s);
 }
 
-hipError_t launch_cache_attn_join(const CacheDims& d, const CacheAttnPlan& plan, const int* lens, const int* new_lens,
-                                  const CacheAttnBuffers& part, f16* out, float* lse, hipStream_t s) {
-  const CacheAttnArgs a = attn_args(d, plan);
+hipError_t launch_cache_attn_join(const CacheDims& d, const CacheAttnPlan& plan, const f16* values, const int* table,
+                                  const int* lens, const int* new_lens, const int64_t* tree,
+                                  const CacheAttnBuffers& part, f16* out, float* lse, int causal, int mask_diag,
+                                  hipStream_t s) {
+  const CacheAttnArgs a = attn_args(d, plan, causal, mask_diag);
   const int64_t rows = (int64_t)d.B * d.H * d.n;
   // few pieces: one group a row, its loads all independent; many: groups that share them
 #define MORPHO_CACHE_JOIN(DV, NG)                                                                            \
   MORPHO_KLAUNCH((cache_join_kernel<DV, NG>), dim3((unsigned)((rows * (DV / 4) * NG + 255) / 256)), dim3(256), 0, s, \
-                 a, rows, lens, new_lens, part.o, part.st, out, lse)
+                 a, rows, values, table, lens, new_lens, tree, part.o, part.st, out, lse)
   const bool many = plan.nsplit > 8;
   if (d.DV == 32 && many)
     MORPHO_CACHE_JOIN(32, 32);

@@ -3,6 +3,8 @@ easy to get wrong, on the GPU."""
 
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
@@ -47,3 +49,79 @@ def test_entries_below_their_place_move_nothing(dv, lead, kept):
         codes[:, pt, :, to % P] = new[0]
         values[:, pt, :, to % P // 8, :, to % 8] = new[1]
     assert torch.equal(dc.cpu(), codes) and torch.equal(dval.cpu(), values)
+
+
+# ---------------------------------------------------------------- values that are not finite
+
+def _attention_case(B, n, H, m, dv, lens, P, seed, gate=1.0):
+    g = torch.Generator().manual_seed(seed)
+    per = -(-(max(lens) + n) // P)
+    pages = B * per + 1
+    table = torch.randperm(pages, generator=g)[: B * per].view(B, per)
+    codes = torch.rand((pages, H, P, m), generator=g).half()
+    values = torch.randn((pages, H, P // 8, dv, 8), generator=g).half()
+    phi = torch.rand((B, n, H, m), generator=g).half()
+    gq, gk = (torch.full((H, m), gate).half(), torch.ones((H, m)).half())
+    return codes, values, table, phi, gq, gk
+
+
+def _seen(n, L, mask, mask_diag, tree):
+    """[n, L + n]: which of the positions a new token sees."""
+    seen = torch.ones((n, L + n), dtype=torch.bool)
+    if tree is not None:
+        seen[:, L:] = (tree[:, None] >> torch.arange(n)) & 1 == 1
+    elif mask == "causal":
+        seen = torch.tril(seen, L)
+    if mask_diag:
+        seen[torch.arange(n), L + torch.arange(n)] = False
+    return seen
+
+
+@pytest.mark.parametrize("n,H,m,dv,L,P", [(1, 2, 16, 64, 700, 64), (1, 2, 32, 128, 5000, 64), (5, 1, 64, 32, 333, 32),
+                                          (20, 2, 16, 64, 500, 64), (50, 1, 64, 64, 3000, 128), (70, 2, 16, 64, 300, 64),
+                                          (70, 1, 64, 128, 700, 256), (150, 1, 32, 32, 2500, 32), (130, 2, 16, 128, 40, 64)])
+@pytest.mark.parametrize("mask,mask_diag", [("causal", False), ("causal", True), ("full", True), ("tree", False)])
+@pytest.mark.parametrize("gate", [1.0, 300.0])
+def test_values_that_are_not_finite_decide_their_column(n, H, m, dv, L, P, mask, mask_diag, gate):
+    """Weights are positive, so an infinite value makes its column infinite in every
+    row that sees it, however small its weight is (gate 300: most vanish) and
+    wherever in a tile, piece or page it lies; both infinities, or a NaN, make it
+    NaN. Every other place is, bit for bit, what it is with 0 in those places."""
+    if mask == "tree" and n > 64:
+        pytest.skip("a tree holds at most 64 drafts")
+    lens = [L, L // 3 + 1]
+    codes, values, table, phi, gq, gk = _attention_case(2, n, H, m, dv, lens, P, n + L, gate)
+    g = torch.Generator().manual_seed(n)
+    tree = None
+    if mask == "tree":
+        bits = [[1 << k | (1 << k // 2 if k else 0) for k in range(n)] for _ in range(2)]
+        tree = torch.tensor([[x - 2 ** 64 if x >> 63 else x for x in row] for row in bits], dtype=torch.int64)
+    # per sequence and head: (position, column, value); column 1 gets both infinities, 2 a NaN
+    strange = [[[(int(torch.randint(0, lens[b] + n, (1,), generator=g)), c, v)
+                 for c, v in ((0, "inf"), (1, "inf"), (1, "-inf"), (2, "nan"), (2, "inf"), (5, "-inf"), (dv - 1, "inf"),
+                              (dv // 2, "-inf"), (dv // 2, "-inf"))] +
+                [(0, 7, "inf"), (lens[b] + n - 1, 8, "-inf"), (31, 9, "inf"), (32, 10, "-inf"), (lens[b], 11, "inf")]
+                for _ in range(H)] for b in range(2)]
+    clean, sums = values.clone(), torch.zeros((2, n, H, dv))
+    for b in range(2):
+        seen = _seen(n, lens[b], mask, mask_diag, None if tree is None else tree[b])
+        for h in range(H):
+            for t, c, v in strange[b][h]:
+                page, s = int(table[b, t // P]), t % P
+                values[page, h, s // 8, c, s % 8] = float(v)
+                clean[page, h, s // 8, c, s % 8] = 0
+            # one value a place: the last that was written
+            for (t, c), v in {(t, c): v for t, c, v in strange[b][h]}.items():
+                sums[b, seen[:, t], h, c] += float(v)
+    args = [t.to(DEV) for t in (phi, gq, gk, codes)]
+    rest = dict(scale=m ** -0.5, causal=mask != "full", mask_diag=mask_diag,
+                tree=None if tree is None else tree.to(DEV))
+    got, want = (ma.morpho_cache_attention(*args, v.to(DEV), table.int().to(DEV), _ints(lens), **rest)
+                 for v in (values, clean))
+    out, ref = (t[0].cpu().view(2, n, H, dv) for t in (got, want))
+    assert torch.equal(got[1], want[1])  # the sums of weights know nothing of values
+    assert ref.isfinite().all()
+    expect = torch.where(sums == 0, ref, sums.half())
+    same = (out == expect) | (out.isnan() & expect.isnan())
+    assert same.all(), (~same).nonzero()[:8].tolist()
+    assert (sums == math.inf).any() and (sums == -math.inf).any() and sums.isnan().any() and (sums == 0).any()
