@@ -468,7 +468,8 @@ struct CacheOut {
 // or a NaN are among them. The value product does not keep to that (0 times an
 // infinity where a weight rounds to nothing, infinities of both signs where it is
 // a pair of halves), so such a column becomes the sum of the values that are not
-// finite. The keys are read once more, which nothing but
+// finite. Where all are finite, single weights were rounded up and the largest
+// value with them past the range. The keys are read once more, which nothing but
 // such a row pays for (the kernels' times: the same with and without, +-1 %).
 // v, stride: the head's values in page 0, and a page's; pages: the sequence's, of
 // `count` in the pool; i: the row; bits: its drafts; l: the sum of its weights
@@ -497,7 +498,7 @@ __device__ __forceinline__ void settle_columns(const f16* v, int64_t stride, con
   }
 #pragma unroll
   for (int k = 0; k < 4; ++k)
-    if (not_finite(y[k]) && sum[k] != 0.f) y[k] = (f16)sum[k];
+    if (not_finite(y[k])) y[k] = sum[k] != 0.f ? (f16)sum[k] : (f16)__builtin_copysignf(65504.f, (float)y[k]);
   *at = y;
 }
 

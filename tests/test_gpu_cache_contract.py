@@ -125,3 +125,23 @@ def test_values_that_are_not_finite_decide_their_column(n, H, m, dv, L, P, mask,
     same = (out == expect) | (out.isnan() & expect.isnan())
     assert same.all(), (~same).nonzero()[:8].tolist()
     assert (sums == math.inf).any() and (sums == -math.inf).any() and sums.isnan().any() and (sums == 0).any()
+
+
+@pytest.mark.parametrize("n", [1, 40, 70, 200])
+@pytest.mark.parametrize("alike", [False, True])
+def test_the_largest_value_stays_finite(n, alike):
+    """The mean of values that are all the largest number is that number: weights
+    rounded to 16 bits must not lift it past the range. With keys that are all
+    alike but one, the weights of a row are rounded alike, up in many rows."""
+    codes, values, table, phi, gq, gk = _attention_case(1, n, 2, 16, 64, [600], 64, n)
+    if alike:
+        codes[:] = codes[0, 0, 0]
+        codes[table[0, 0], :, 0] = torch.rand(16, generator=torch.Generator().manual_seed(2)).half()
+    values[..., ::2, :], values[..., 1::2, :] = 65504.0, -65504.0
+    out, _ = ma.morpho_cache_attention(*(t.to(DEV) for t in (phi, gq, gk, codes, values)), table.int().to(DEV),
+                                       _ints([600]), scale=0.25)
+    # the output's rounding is none here; a weight's, beyond 64 tokens, at most 2^-11, and the sums' are below 2^-16
+    sign = torch.ones(64, dtype=torch.float64)
+    sign[1::2] = -1
+    off = (out.double().cpu().view(n, 2, 64) * sign - 65504).abs().max().item()
+    assert off <= 65504 * (2.0 ** -11 + 2.0 ** -16 if n > 64 else 2.0 ** -16) + 16, off
