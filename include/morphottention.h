@@ -253,6 +253,8 @@ size_t morpho_cache_attention_workspace_size(const morpho_cache* cache, int64_t 
  * row, gets out 0 and lse -FLT_MAX. max_len: at least the longest lens[b] +
  * new_lens[b]; it sets the launch shape only (a longer sequence is still
  * computed in full). cache->layers must be 1.
+ * Precision: exact to fp32 rounding for n <= 64; beyond, every softmax weight
+ * is rounded to float16 once before it meets its value.
  * Numeric range: scale * log2(e) * gate_q[h][c] * gate_k[h][c] * (2 phi - 1) of
  * a query must stay below 65,504 for every code, or the row is NaN. A value
  * that is not finite reaches the rows that see its key, and no other: their

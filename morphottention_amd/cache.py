@@ -127,7 +127,10 @@ def morpho_cache_attention(phi: torch.Tensor, gate_q: torch.Tensor, gate_k: torc
     :returns: ``out`` ``[B, n, D]`` and the base-2 log-sum-exp of the row scores
         ``[B * H, n]`` (float32). A row that sees nothing, and a padding row,
         has 0 and ``-FLT_MAX``. ``scale * gate_q * gate_k`` has to stay below
-        22,700 (codes within [0, 1]), as in the whole-sequence forward.
+        22,700 (codes within [0, 1]), as in the whole-sequence forward. Up to 64
+        new tokens the result is exact to fp32 rounding; beyond, where the weights
+        are the bound, each is rounded to float16 once (2^-11 of its value), as in
+        the whole-sequence forward: ``n`` of at most 64 a call avoids that.
     """
     if max_len is not None and max_len <= 0:
         raise ValueError(f"max_len must be positive (got {max_len})")
