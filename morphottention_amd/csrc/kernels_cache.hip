@@ -470,7 +470,7 @@ struct CacheOut {
 // a pair of halves), so such a column becomes the sum of the values that are not
 // finite. Where all are finite, single weights were rounded up and the largest
 // value with them past the range. The keys are read once more, which nothing but
-// such a row pays for (the kernels' times: the same with and without, +-1 %).
+// such a row pays for (15 shapes with and without: -1.7 to 1.9 %, mean -0.1).
 // v, stride: the head's values in page 0, and a page's; pages: the sequence's, of
 // `count` in the pool; i: the row; bits: its drafts; l: the sum of its weights
 // (scores that are not numbers leave nothing to settle); out: column c of it.
