@@ -265,6 +265,36 @@ int morpho_cache_attention(const void* phi, const void* gate_q, const void* gate
                            void* out, float* lse, int64_t B, int64_t n, int64_t seq_pages, int64_t max_len,
                            float scale, int mode, void* workspace, size_t workspace_bytes, morpho_stream_t stream);
 
+/* The same where sequences have their first pages in common (forks of one
+ * prompt): the new tokens of all of a group's sequences attend to the common
+ * keys together, which are read once, and then each to its own. Group g are the
+ * sequences members[starts[g]] .. members[starts[g + 1] - 1], which have the
+ * same first pages[g] entries in their table rows, whole pages of tokens before
+ * the new ones; group[b] is the group of sequence b, or -1. Every sequence of a
+ * group stands in members once. A group's common keys are left to a sequence
+ * whose lens[b] does not reach their end. All four are int32 device memory that
+ * the host does not read. max_prefix, max_rest: at least the most common tokens
+ * of a group, and the most tokens (with the new ones) of a sequence behind them;
+ * they set the launch shape only. n <= 64. Results as morpho_cache_attention's to
+ * fp32 rounding. */
+typedef struct morpho_shared_prefix {
+  const int32_t* members; /* [members_count] */
+  const int32_t* starts;  /* [groups + 1] */
+  const int32_t* group;   /* [B] */
+  const int32_t* pages;   /* [groups] */
+  int64_t members_count, groups, max_prefix, max_rest;
+} morpho_shared_prefix;
+
+size_t morpho_cache_shared_attention_workspace_size(const morpho_cache* cache, int64_t B, int64_t n, int64_t seq_pages,
+                                                    int64_t members, int64_t groups, int64_t max_prefix,
+                                                    int64_t max_rest);
+
+int morpho_cache_shared_attention(const void* phi, const void* gate_q, const void* gate_k, const morpho_cache* cache,
+                                  const int32_t* table, const int32_t* lens, const int32_t* new_lens,
+                                  const int64_t* tree, const morpho_shared_prefix* shared, void* out, float* lse,
+                                  int64_t B, int64_t n, int64_t seq_pages, float scale, int mode, void* workspace,
+                                  size_t workspace_bytes, morpho_stream_t stream);
+
 /* Copies page src[k] to page dst[k], k < count, in every layer (int32 device
  * memory). A pair with a page outside the pool is left out. No page may be
  * written by two pairs, or written by one and read by another. */
@@ -281,6 +311,68 @@ int morpho_cache_copy_pages(const morpho_cache* cache, const int32_t* src, const
 int morpho_cache_compact(const morpho_cache* cache, const int32_t* table, const int32_t* lens, const int32_t* keep,
                          const int32_t* keep_lens, int64_t B, int64_t keep_cols, int64_t seq_pages,
                          morpho_stream_t stream);
+
+/* Page tables and slot maps of a step of new tokens, on the device. Sequence b
+ * has lens[b] tokens, new_lens[b] new ones (NULL: n each; at most n) and its
+ * first held[b] table entries are its pages. It needs ceil((lens + new) /
+ * page_size) pages: what it has beyond that goes back to the free pages, a stack
+ * free_pages[0 .. free_count[0] - 1] with room for free_room, and its entries
+ * become -1; what it lacks is taken from the top of the stack, after all that goes
+ * back, in the order of the sequences: from the first one on for which the rest
+ * does not suffice, none that lacks pages gets any. Taken pages given back in the
+ * same order lie as before. table, held, free_pages and free_count are updated.
+ * granted [B] int32: the new tokens, or 0 where the sequence got no pages or its
+ * table row is too short (then nothing of it changes). slots [B, n] int64: the
+ * place of each new token, page * page_size + its place in the page; -1 for
+ * padding. Pages that go back must be the sequence's alone. The workspace may be
+ * NULL where its size is 0. Sizes: B * n <= 2^22, seq_pages * page_size <= 2^30. */
+size_t morpho_cache_plan_workspace_size(int64_t B, int64_t n);
+int morpho_cache_plan(int32_t* table, int32_t* held, const int32_t* lens, const int32_t* new_lens, int32_t* free_pages,
+                      int32_t* free_count, int64_t free_room, int32_t* granted, int64_t* slots, int64_t B, int64_t n,
+                      int64_t seq_pages, int64_t page_size, void* workspace, size_t workspace_bytes,
+                      morpho_stream_t stream);
+
+/* ------------------------------------------------ verification of drafts
+ * Which drafted tokens the target keeps, and the next token, so that what comes
+ * out has the target's distribution. No reference counterpart.
+ *
+ * tokens [B, n] int64, n <= 64: token 0 of a sequence is decided, the others
+ * are drafts. tree [B, n] int64 as in morpho_cache_attention (or NULL: a chain):
+ * token i was drafted behind the one of the highest bit below i of tree[b][i]
+ * (none: it is never reached). new_lens [B] int32 (or NULL: n each): the tokens of
+ * each sequence; 0: padding. logits [B, n, vocab]: row i the target's behind token
+ * i. draft_logits [B, n - 1, vocab] (or NULL, or data NULL): row i those that the
+ * drafts behind token i were drawn from, independently of each other; NULL:
+ * drafts were not drawn. Both at `temperature`, of one type, with strides in
+ * elements and the vocabulary contiguous. uniform [B, n] float32 in [0, 1):
+ * number i decides on draft i, number 0 draws the next token.
+ *
+ * With p and q the softmax of the rows behind the token at hand over temperature
+ * (q 1 at the draft where drafts were not drawn), r = p and Z = 1: the drafts
+ * behind it are asked in ascending order, draft t is kept if uniform q(t) Z < r(t)
+ * and is then the token at hand; else r becomes max(r / Z - q, 0) (r without t) and
+ * Z its sum. When none is left, the next token is the first whose running sum of r
+ * passes uniform Z. temperature 0: a draft is kept if it is the target's best
+ * token, which is the next one at the end; of equal ones the lowest. NaN and -inf
+ * logits have no chance, an infinite one shares with its like alone; a row without
+ * any gives token -1. Sums are in 64 bits.
+ *
+ * keep [B, n] int32: the places of the kept tokens, 0 first, ascending, then -1
+ * (what morpho_cache_compact takes); keep_lens [B] int32 how many; token [B]
+ * int64: the next token, -1 for padding. vocab <= 4,000,000; temperature 0, or 1e-4
+ * to 1e4. */
+enum { MORPHO_FLOAT16 = 0, MORPHO_BFLOAT16 = 1, MORPHO_FLOAT32 = 2 };
+typedef struct morpho_logits {
+  const void* data;
+  int64_t batch_stride, row_stride;
+} morpho_logits;
+
+size_t morpho_verify_workspace_size(int64_t B, int64_t n, int64_t vocab, int type, int have_draft, int have_tree,
+                                    double temperature);
+int morpho_verify_drafts(const morpho_logits* logits, const morpho_logits* draft_logits, int type,
+                         const int64_t* tokens, const float* uniform, const int64_t* tree, const int32_t* new_lens,
+                         int32_t* keep, int32_t* keep_lens, int64_t* token, int64_t B, int64_t n, int64_t vocab,
+                         double temperature, void* workspace, size_t workspace_bytes, morpho_stream_t stream);
 
 /* Per-kernel timing for measurement harnesses. No reference counterpart.
  * When enabled (process-wide), every kernel the library launches, from any

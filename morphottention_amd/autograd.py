@@ -197,7 +197,8 @@ class MorphoAttention(nn.Module):
         ``x``, ``weights`` or a parameter of the layer would need a gradient.
 
         :param weights: :meth:`pack_cache_weights`, made once.
-        :param step: from ``cache.step``; the caller commits it after the last layer.
+        :param step: from ``cache.step``; the caller commits it after the last layer
+            (or from the ``step`` of a loop, which takes it).
             A step that was committed, or whose sequences have changed since it was
             made, raises before anything is stored.
             ``x`` has to have a row of ``step.n`` tokens for each of its sequences
@@ -218,7 +219,7 @@ class MorphoAttention(nn.Module):
                                       new_lens=step.new_lens, projection=self.projection)
             out, _ = morpho_cache_attention(phi, self.gate_q, self.gate_k, codes, values, step.table, step.lens,
                                             new_lens=step.new_lens, tree=tree, scale=self.scale,
-                                            mask_diag=self.mask_diag, max_len=step.max_len)
+                                            mask_diag=self.mask_diag, max_len=step.max_len, shared=step.shared)
         return out
 
 

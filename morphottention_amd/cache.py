@@ -21,11 +21,14 @@ before the new ones) in device memory, and may be captured in a graph:
 * :func:`morpho_cache_attention` lets them attend: one token a sequence, pieces
   of a prompt, or a tree of drafted tokens;
 * :func:`morpho_cache_copy_pages` and :func:`morpho_cache_compact` copy pages and
-  move kept tokens together, in all layers at once.
+  move kept tokens together, in all layers at once;
+* :func:`morpho_cache_plan` gives the sequences pages for their new tokens, and
+  takes back what they do not need, on the device.
 
 :class:`MorphoCache` owns the tensors and keeps account of the pages (sharing
-between forks, copies on write, rollback). ``MorphoAttention.forward_cached``
-runs a layer on it.
+between forks, copies on write, rollback); a :class:`MorphoLoop` keeps that of some
+sequences on the device, for steps that the host does not see.
+``MorphoAttention.forward_cached`` runs a layer on either.
 
 The cache serves inference: none of this is differentiable, and a call that
 would need a gradient raises.
@@ -61,6 +64,19 @@ def _cache_copy_pages_fake(codes, values, src, dst):
 @torch.library.register_fake(add_op_namespace_prefix("cache_compact"))
 def _cache_compact_fake(codes, values, table, lens, keep, keep_lens=None):
     return None
+
+
+@torch.library.register_fake(add_op_namespace_prefix("cache_shared_attention"))
+def _cache_shared_attention_fake(phi, gate_q, gate_k, codes, values, table, lens, new_lens, tree, members, starts, group,
+                                 pages, max_prefix, max_rest, scale, causal, variant=0):
+    B, n, H, _m = phi.shape
+    return [phi.new_empty((B, n, H * values.shape[3])), phi.new_empty((B * H, n), dtype=torch.float32)]
+
+
+@torch.library.register_fake(add_op_namespace_prefix("cache_plan"))
+def _cache_plan_fake(table, held, lens, free_pages, free_count, n, new_lens, page_size):
+    B = table.shape[0]
+    return [table.new_empty((B,)), table.new_empty((B, n), dtype=torch.int64)]
 
 
 _PROJECTION_BITS = {"sigmoid": 0, "hardtanh01": 4, "identity": 8}
@@ -105,11 +121,61 @@ def morpho_cache_append(x: torch.Tensor, weights: torch.Tensor, codes: torch.Ten
     return ops.cache_append(x, weights, codes, values, table, lens, new_lens, _PROJECTION_BITS[projection])
 
 
+# most new tokens of a sequence for which a shared prefix is read once: up to here
+# the keys are the bound, beyond the matrix work, which sharing does not lessen
+_MOST_SHARED = 64
+
+
+@dataclass
+class SharedPrefix:
+    """Which sequences of a batch have their first pages in common.
+
+    :param members: int32, the sequences (rows of the batch) that share, group by group.
+    :param starts: int32 ``[groups + 1]``, where each group begins in ``members``.
+    :param group: int32 ``[B]``, the group of each sequence, -1 for none.
+    :param pages: int32 ``[groups]``, how many pages of its table row each group's
+        sequences have in common: whole pages of tokens before the new ones.
+    :param max_prefix: at least the most common tokens of a group.
+    :param max_rest: at least the most tokens, new ones among them, of a sequence
+        behind its common ones. Both set how the work is split, not what is
+        computed; the table's whole length if not given.
+
+    The tensors are read on the device. :meth:`of` makes them from lists.
+    """
+
+    members: torch.Tensor
+    starts: torch.Tensor
+    group: torch.Tensor
+    pages: torch.Tensor
+    max_prefix: int | None = None
+    max_rest: int | None = None
+
+    @classmethod
+    def of(cls, groups: list[list[int]], pages: list[int], batch: int, *, device=None, max_prefix: int | None = None,
+           max_rest: int | None = None) -> SharedPrefix:
+        """From each group's sequences and their common pages."""
+        members = [b for g in groups for b in g]
+        if not groups or len(groups) != len(pages) or not all(groups):
+            raise ValueError("groups and pages must have one or more entries, as many each, and no group none")
+        if len(set(members)) != len(members) or min(members) < 0 or max(members) >= batch:
+            raise ValueError(f"a sequence must be one of 0 .. {batch - 1}, in one group at most")
+        if min(pages) < 0:
+            raise ValueError("pages must not be negative")
+        where = [-1] * batch
+        for k, g in enumerate(groups):
+            for b in g:
+                where[b] = k
+        starts = list(itertools.accumulate((len(g) for g in groups), initial=0))
+        ints = lambda v: torch.tensor(v, dtype=torch.int32, device=device)  # noqa: E731
+        return cls(ints(members), ints(starts), ints(where), ints(pages), max_prefix, max_rest)
+
+
 def morpho_cache_attention(phi: torch.Tensor, gate_q: torch.Tensor, gate_k: torch.Tensor, codes: torch.Tensor,
                            values: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, *,
                            new_lens: torch.Tensor | None = None, tree: torch.Tensor | None = None, scale: float = 1.0,
                            causal: bool = True, mask_diag: bool = False,
-                           max_len: int | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+                           max_len: int | None = None,
+                           shared: SharedPrefix | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """Attention of new tokens, appended before, over their sequences.
 
     :param phi: their codes ``[B, n, H, cube_m]``, from :func:`morpho_cache_append`.
@@ -124,6 +190,10 @@ def morpho_cache_attention(phi: torch.Tensor, gate_q: torch.Tensor, gate_k: torc
     :param mask_diag: drop each token's own key.
     :param max_len: at least the longest ``lens[b] + new_lens[b]``. Sets how the
         work is split, not what is computed; the table's whole length if not given.
+    :param shared: which sequences have their first pages in common (forks of a
+        prompt). The common keys are then read once for all of them, which
+        changes the result by fp32 rounding only. Beyond 64 new tokens, where
+        reading is not the bound, it makes no difference.
     :returns: ``out`` ``[B, n, D]`` and the base-2 log-sum-exp of the row scores
         ``[B * H, n]`` (float32). A row that sees nothing, and a padding row,
         has 0 and ``-FLT_MAX``. ``scale * gate_q * gate_k`` has to stay below
@@ -137,6 +207,15 @@ def morpho_cache_attention(phi: torch.Tensor, gate_q: torch.Tensor, gate_k: torc
     if tree is not None and mask_diag:
         raise ValueError("mask_diag with a tree: leave a draft's own bit out instead")
     refuse_grad(phi, gate_q, gate_k)
+    if shared is not None:
+        if min(shared.max_prefix or 1, shared.max_rest or 1) <= 0:
+            raise ValueError("max_prefix and max_rest must be positive")
+        if phi.shape[1] <= _MOST_SHARED:
+            out, lse = ops.cache_shared_attention(phi, gate_q, gate_k, codes, values, table, lens, new_lens, tree,
+                                                  shared.members, shared.starts, shared.group, shared.pages,
+                                                  shared.max_prefix or 0, shared.max_rest or 0, scale, causal,
+                                                  _MASK_DIAG if mask_diag else 0)
+            return out, lse
     out, lse = ops.cache_attention(phi, gate_q, gate_k, codes, values, table, lens, new_lens, tree, scale, causal,
                                    _MASK_DIAG if mask_diag else 0, max_len or 0)
     return out, lse
@@ -164,6 +243,68 @@ def morpho_cache_compact(codes: torch.Tensor, values: torch.Tensor, table: torch
     :param keep_lens: int32 ``[B]``, how many of them count.
     """
     ops.cache_compact(codes, values, table, lens, keep, keep_lens)
+
+
+def morpho_cache_plan(table: torch.Tensor, held: torch.Tensor, lens: torch.Tensor, free_pages: torch.Tensor,
+                      free_count: torch.Tensor, n: int, *, new_lens: torch.Tensor | None = None,
+                      page_size: int = 64) -> tuple[torch.Tensor, torch.Tensor]:
+    """Pages for a step's new tokens, and back what the sequences do not need.
+
+    A sequence needs ``ceil((lens[b] + new_lens[b]) / page_size)`` pages. What it
+    holds beyond that goes back to the free ones first; what it lacks is then taken
+    from them in the order of the sequences. From the first one on for which they
+    do not suffice, none that lacks pages gets any (no later one overtakes it).
+
+    :param table: int32 ``[B, seq_pages]``, updated: taken pages are entered, the
+        entries of those that go back become -1.
+    :param held: int32 ``[B]``, how many pages of its row each sequence has, updated.
+    :param lens: int32 ``[B]``, tokens of each sequence before the new ones.
+    :param free_pages: int32, a stack of free pages, updated, with room for all that
+        may come back.
+    :param free_count: int32 ``[1]``, how many there are, updated.
+    :param n: new tokens of each sequence, at most.
+    :param new_lens: int32 ``[B]``, new tokens of each where not all have ``n``. 0
+        for all gives back what lies behind ``lens``: pages that go back must be
+        the sequence's alone.
+    :returns: ``granted`` int32 ``[B]``, the new tokens, or 0 where a sequence got no
+        pages or its row of the table is too short (nothing of it changes then),
+        and ``slots`` int64 ``[B, n]``, the place of each new token in the pool's
+        tokens, ``page * page_size`` + its place in the page, -1 for padding.
+    """
+    granted, slots = ops.cache_plan(table, held, lens, free_pages, free_count, n, new_lens, page_size)
+    return granted, slots
+
+
+def _same(a: list[int], b: list[int], most: int) -> int:
+    """How many first entries two sequences' pages have in common, ``most`` at most.
+    What is shared is always shared from the first page on."""
+    lo, hi = 0, min(len(a), len(b), most)
+    while lo < hi:
+        mid = (lo + hi + 1) // 2
+        lo, hi = (mid, hi) if a[mid - 1] == b[mid - 1] else (lo, mid - 1)
+    return lo
+
+
+def _groups(rows: list[list[int]], full: list[int]) -> list[tuple[list[int], int]]:
+    """Groups of rows with common first pages, and how many: those that spare the
+    most pages (a group of k with c common ones spares (k - 1) c), of which a row
+    is in one. full: the pages of each that may be shared."""
+    def best(mine: list[int], depth: int) -> tuple[int, list[tuple[list[int], int]]]:
+        by_page: dict[int, list[int]] = {}
+        for b in mine:
+            if full[b] > depth:
+                by_page.setdefault(rows[b][depth], []).append(b)
+        spared, found = 0, []
+        for k in by_page.values():
+            if len(k) < 2:
+                continue
+            common = min(_same(rows[k[0]], rows[b], full[b]) for b in k)
+            deeper, inner = best(k, common)
+            here = (len(k) - 1) * common
+            spared += max(here, deeper)
+            found += inner if deeper > here else [(k, common)]
+        return spared, found
+    return best(list(range(len(rows))), 0)[1]
 
 
 # What changes the tokens of a sequence gives it a new stamp. They rise and are
@@ -199,6 +340,8 @@ class CacheStep:
     max_len: int
     stamps: list[int]
     claim: _Claim | None = field(default=None, repr=False, compare=False)
+    shared: SharedPrefix | None = None
+    loop: MorphoLoop | None = field(default=None, repr=False, compare=False)
 
 
 class MorphoCache:
@@ -251,6 +394,7 @@ class MorphoCache:
         # of each step that is neither committed nor dropped: its stamp, and {seq: end of the new tokens}
         self._claims: dict[int, dict[int, int]] = {}
         self._grown: set[int] = set()  # sequences that may have pages past their tokens
+        self._away: set[int] = set()  # sequences whose account a loop keeps
         self._next = 0
 
     # ---- account
@@ -271,6 +415,8 @@ class MorphoCache:
     def _known(self, seq: int) -> int:
         if seq not in self._pages:
             raise KeyError(f"no sequence {seq}")
+        if seq in self._away:
+            raise RuntimeError(f"sequence {seq} is in a loop, which has to be closed first")
         return seq
 
     def _take(self, count: int) -> list[int]:
@@ -395,9 +541,29 @@ class MorphoCache:
             self._pages[seq] += itertools.islice(pages, count)
 
     # ---- steps
-    def step(self, seqs: list[int], counts: int | list[int]) -> CacheStep:
+    def _shared(self, seqs: list[int], ends: list[int]) -> SharedPrefix | None:
+        """What the sequences have in common of the pages that their tokens fill; ends:
+        where their new tokens end."""
+        full = [self._lens[s] // self.page_size for s in seqs]
+        groups = _groups([self._pages[s] for s in seqs], full)
+        if not groups:
+            return None
+        common = [0] * len(seqs)
+        for k, count in groups:
+            for b in k:
+                common[b] = count
+        return SharedPrefix.of([k for k, _ in groups], [count for _, count in groups], len(seqs),
+                               device=self.codes.device, max_prefix=max(common) * self.page_size,
+                               max_rest=max(1, *(e - c * self.page_size for e, c in zip(ends, common))))
+
+    def step(self, seqs: list[int], counts: int | list[int], *, shared: bool = False) -> CacheStep:
         """Pages for new tokens of some sequences: ``counts`` tokens of each, or a
-        list with as many for each."""
+        list with as many for each.
+
+        :param shared: read what forks have in common once for all of them (worth it
+            from a few sequences with a few hundred common tokens on; see
+            :class:`SharedPrefix`).
+        """
         seqs = list(seqs)
         if not seqs or len(set(seqs)) != len(seqs):
             raise ValueError("a step takes one or more different sequences")
@@ -412,12 +578,26 @@ class MorphoCache:
         rows = [(self._pages[s] + [-1] * width)[:width] for s in seqs]
         n = max(counts)
         return CacheStep(seqs, counts, n, self._ints(rows), self._ints([self._lens[s] for s in seqs]),
-                         self._ints(counts) if min(counts) < n else None, max(ends), [self._stamp[s] for s in seqs], claim)
+                         self._ints(counts) if min(counts) < n else None, max(ends), [self._stamp[s] for s in seqs], claim,
+                         self._shared(seqs, ends) if shared else None)
+
+    def loop(self, seqs: list[int], n: int, room: int, *, pages: int | None = None, shared: bool = False) -> MorphoLoop:
+        """Steps of up to ``n`` new tokens of some sequences, whose account the device
+        keeps until the loop is closed.
+
+        :param room: the tokens that a sequence may have at most, new ones among them.
+        :param pages: free pages that the loop takes along; as many as the sequences
+            need for ``room`` tokens if not given, or what there is.
+        :param shared: as in :meth:`step`, for what they have in common now.
+        """
+        return MorphoLoop(self, seqs, n, room, pages, shared)
 
     def drop(self, step: CacheStep) -> None:
         """Give a step up that is not committed: its pages past the tokens of its
         sequences are free again. (A page that it copied on write stays the
         sequence's own.)"""
+        if step.loop is not None:
+            raise RuntimeError("a loop's step: the loop takes its tokens, or the next one's in their place")
         if step.claim is None or step.claim.claims is not self._claims:
             raise RuntimeError("the step is another cache's")
         step.claim.dropped = True
@@ -425,6 +605,8 @@ class MorphoCache:
         self._shrink()
 
     def _still(self, step: CacheStep) -> None:
+        if step.loop is not None:
+            raise RuntimeError("a loop's step: the loop takes its tokens")
         if step.claim is not None and step.claim.dropped:
             raise RuntimeError("the step was dropped")
         if any(self._stamp[self._known(s)] != stamp for s, stamp in zip(step.seqs, step.stamps)):
@@ -434,7 +616,10 @@ class MorphoCache:
         """Raise if ``x`` are not the step's new tokens, ``[sequences, step.n, ...]``, or
         if the step is not good any more: its pages may be another sequence's. Where
         the counts differ the kernels know them, and ``x`` may be padded further."""
-        self._still(step)
+        if step.loop is not None:
+            step.loop._still(self, step)
+        else:
+            self._still(step)
         B, n = len(step.seqs), step.n
         if x.dim() < 2 or x.shape[0] != B or x.shape[1] < n or (x.shape[1] > n and step.new_lens is None):
             raise ValueError(f"x must have {B} rows of {n} tokens, as the step has (got {tuple(x.shape)})")
@@ -452,11 +637,15 @@ class MorphoCache:
         if step.claim is not None:
             step.claim.end()
 
-    def accept(self, step: CacheStep, kept: list[list[int]]) -> None:
+    def accept(self, step: CacheStep, kept: list[list[int]] | tuple[torch.Tensor, torch.Tensor]) -> None:
         """After a step of drafts: of each sequence the drafts ``kept[b]`` (ascending
         places among its drafts, e.g. the accepted path) are its next tokens,
-        the others are dropped."""
+        the others are dropped. ``kept`` may also be the pair ``keep``, ``keep_lens``
+        of :func:`morphottention_amd.morpho_verify_drafts`, which is then read from
+        the device."""
         self._still(step)
+        if isinstance(kept, tuple) and len(kept) == 2 and all(isinstance(t, torch.Tensor) for t in kept):
+            kept = [row[:k] for row, k in zip(kept[0].tolist(), kept[1].tolist())]
         if len(kept) != len(step.seqs):
             raise ValueError("kept must have a list for each sequence of the step")
         for k, c in zip(kept, step.counts):
@@ -485,3 +674,120 @@ class MorphoCache:
             morpho_cache_compact(self.codes, self.values, self._ints([self._pages[seq]]), self._ints([still]),
                                  self._ints([[k - still for k in kept[still:]]]))
         self.truncate(seq, len(kept))
+
+
+class MorphoLoop:
+    """Steps of some sequences of a cache, with the account of their pages on the
+    device, so that the host need not know how many tokens a step kept and the steps
+    may be captured in a graph and replayed::
+
+        with cache.loop(seqs, n, room) as loop:
+            step = loop.step()                         # pages for n new tokens of each
+            for i, layer in enumerate(layers):
+                x = layer.forward_cached(x, weights[i], cache, step, layer=i, tree=tree)
+            keep, keep_lens, token = morpho_verify_drafts(logits_of(x), tokens, uniform, tree=tree,
+                                                          new_lens=step.new_lens)
+            loop.accept(step, keep, keep_lens)         # their lengths, on the device
+
+    ``step.new_lens`` are the tokens that got places: 0 for a sequence for which the
+    loop's pages did not suffice, or that has no room left. Until :meth:`close` (which
+    the ``with`` block calls) the cache refuses calls on the sequences; then their
+    lengths are read and the pages that are left go back to the cache.
+
+    ``table``, ``held``, ``lens``, ``free_pages`` and ``free_count`` are the account, as
+    :func:`morpho_cache_plan` takes it.
+    """
+
+    def __init__(self, cache: MorphoCache, seqs: list[int], n: int, room: int, pages: int | None = None,
+                 shared: bool = False) -> None:
+        seqs = list(seqs)
+        if not seqs or len(set(seqs)) != len(seqs):
+            raise ValueError("a loop takes one or more different sequences")
+        lens = [cache._lens[cache._known(s)] for s in seqs]
+        if n <= 0 or room < max(lens) + n:
+            raise ValueError(f"n must be positive, and room at least the longest sequence and n ({max(lens)} + {n})")
+        if pages is not None and pages < 0:
+            raise ValueError("pages must not be negative")
+        P = cache.page_size
+        # a page that is not full belongs to its sequence alone from here on
+        cache._own([(s, l, l + 1) for s, l in zip(seqs, lens) if l % P])
+        for s, l in zip(seqs, lens):
+            cache._cut(s, l)
+        cache._grown.difference_update(seqs)
+        width = -(-room // P)
+        rows = [cache._pages[s] for s in seqs]
+        need = sum(width - len(r) for r in rows)
+        cache._shrink()
+        self._free = cache._take(min(need, len(cache._free)) if pages is None else pages)
+        try:
+            self.cache, self.seqs, self.n, self.room = cache, seqs, n, room
+            self.shared = cache._shared(seqs, [room] * len(seqs)) if shared else None
+            self.table = cache._ints([r + [-1] * (width - len(r)) for r in rows])
+            self.held = cache._ints([len(r) for r in rows])
+            self.lens = cache._ints(lens)
+            # room for every page that may come back
+            self.free_pages = cache._ints(self._free + [-1] * (sum(len(r) for r in rows) + 1))
+            self.free_count = cache._ints([len(self._free)])
+        except BaseException:
+            cache._drop(self._free)
+            raise
+        for s in seqs:
+            cache._stamp[s] = next(_stamps)  # steps that were made before are not good any more
+        cache._away.update(seqs)
+        self._last: CacheStep | None = None
+        self._open = True
+
+    def __enter__(self) -> MorphoLoop:
+        return self
+
+    def __exit__(self, *exc) -> None:
+        self.close()
+
+    def _still(self, cache: MorphoCache, step: CacheStep) -> None:
+        if not self._open or cache is not self.cache:
+            raise RuntimeError("the step's loop is closed, or another cache's")
+        if step is not self._last:
+            raise RuntimeError("the loop has made another step since")
+
+    def step(self, new_lens: torch.Tensor | None = None) -> CacheStep:
+        """Places for ``n`` new tokens of each sequence, or ``new_lens`` (int32 ``[B]``).
+        A step whose tokens are not accepted before the next one leaves none."""
+        if not self._open:
+            raise RuntimeError("the loop is closed")
+        granted, slots = morpho_cache_plan(self.table, self.held, self.lens, self.free_pages, self.free_count, self.n,
+                                           new_lens=new_lens, page_size=self.cache.page_size)
+        self.slots = slots
+        self._last = CacheStep(self.seqs, [self.n] * len(self.seqs), self.n, self.table, self.lens, granted, self.room,
+                               [], None, self.shared, self)
+        return self._last
+
+    def accept(self, step: CacheStep, keep: torch.Tensor | None = None, keep_lens: torch.Tensor | None = None) -> None:
+        """The step's tokens belong to their sequences: all that got places, or those at
+        places ``keep`` (int32 ``[B, n]``, ascending, ``keep_lens`` of each), which move
+        together, as :func:`morphottention_amd.morpho_verify_drafts` gives them."""
+        self._still(self.cache, step)
+        if (keep is None) != (keep_lens is None):
+            raise ValueError("keep and keep_lens go together")
+        if keep is not None:
+            keep_lens = torch.minimum(keep_lens, step.new_lens)
+            morpho_cache_compact(self.cache.codes, self.cache.values, self.table, self.lens, keep, keep_lens=keep_lens)
+        self.lens.add_(step.new_lens if keep is None else keep_lens)
+
+    def close(self) -> None:
+        """Give the account back to the cache (reads it from the device)."""
+        if not self._open:
+            return
+        cache, P = self.cache, self.cache.page_size
+        lens, held, rows = self.lens.tolist(), self.held.tolist(), self.table.tolist()
+        left = self.free_pages.tolist()[: int(self.free_count)]
+        self._open = False
+        cache._away.difference_update(self.seqs)
+        for s, length, have, row in zip(self.seqs, lens, held, rows):
+            mine = row[:have]
+            for p in mine[len(cache._pages[s]):]:
+                cache._uses[p] = 1
+            cache._pages[s] = mine
+            cache._lens[s] = length
+            cache._stamp[s] = next(_stamps)
+            cache._cut(s, length)
+        cache._drop(left)

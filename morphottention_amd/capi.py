@@ -25,6 +25,20 @@ class Cache(ctypes.Structure):
                 ("head_dim_v", ctypes.c_int64), ("page_size", ctypes.c_int64)]
 
 
+class SharedPrefix(ctypes.Structure):
+    """``morpho_shared_prefix``: which sequences have which pages in common."""
+
+    _fields_ = [("members", ctypes.c_void_p), ("starts", ctypes.c_void_p), ("group", ctypes.c_void_p),
+                ("pages", ctypes.c_void_p), ("members_count", ctypes.c_int64), ("groups", ctypes.c_int64),
+                ("max_prefix", ctypes.c_int64), ("max_rest", ctypes.c_int64)]
+
+
+class Logits(ctypes.Structure):
+    """``morpho_logits``: rows of logits and their strides in elements."""
+
+    _fields_ = [("data", ctypes.c_void_p), ("batch_stride", ctypes.c_int64), ("row_stride", ctypes.c_int64)]
+
+
 def lib() -> ctypes.CDLL:
     global _lib
     if _lib is None:
@@ -71,6 +85,21 @@ def lib() -> ctypes.CDLL:
         L.morpho_cache_copy_pages.argtypes = [pool, vp, vp, i64, vp]
         L.morpho_cache_compact.restype = ctypes.c_int
         L.morpho_cache_compact.argtypes = [pool] + [vp] * 4 + [i64] * 3 + [vp]
+        L.morpho_cache_shared_attention_workspace_size.restype = sz
+        L.morpho_cache_shared_attention_workspace_size.argtypes = [pool] + [i64] * 7
+        L.morpho_cache_shared_attention.restype = ctypes.c_int
+        L.morpho_cache_shared_attention.argtypes = ([vp] * 3 + [pool] + [vp] * 4 + [ctypes.POINTER(SharedPrefix), vp, vp]
+                                                    + [i64] * 3 + [ctypes.c_float, ctypes.c_int, vp, sz, vp])
+        L.morpho_cache_plan_workspace_size.restype = sz
+        L.morpho_cache_plan_workspace_size.argtypes = [i64, i64]
+        L.morpho_cache_plan.restype = ctypes.c_int
+        L.morpho_cache_plan.argtypes = [vp] * 6 + [i64, vp, vp] + [i64] * 4 + [vp, sz, vp]
+        rows = ctypes.POINTER(Logits)
+        L.morpho_verify_workspace_size.restype = sz
+        L.morpho_verify_workspace_size.argtypes = [i64] * 3 + [ctypes.c_int] * 3 + [ctypes.c_double]
+        L.morpho_verify_drafts.restype = ctypes.c_int
+        L.morpho_verify_drafts.argtypes = ([rows, rows, ctypes.c_int] + [vp] * 7 + [i64] * 3
+                                           + [ctypes.c_double, vp, sz, vp])
         L.morpho_timing_enable.restype = ctypes.c_int
         L.morpho_timing_enable.argtypes = [ctypes.c_int]
         L.morpho_timing_only.restype = ctypes.c_int

@@ -720,6 +720,96 @@ MORPHO_EXPORT int morpho_cache_attention(const void* phi, const void* gate_q, co
   return MORPHO_OK;
 }
 
+namespace {
+int make_shared_plan(const morpho_cache* cache, int64_t B, int64_t n, int64_t seq_pages, int64_t members,
+                     int64_t groups, int64_t max_prefix, int64_t max_rest, CacheDims& d, CacheSharedPlan& p) {
+  const int st = make_cache_dims(cache, false, B, n, seq_pages, d);
+  if (st != MORPHO_OK) return st;
+  if (members <= 0 || members > B || groups <= 0 || groups > members)
+    return fail(MORPHO_ERR_INVALID_ARGUMENT, "members must be 1 to B, groups 1 to members (got %lld and %lld)",
+                (long long)members, (long long)groups);
+  if (max_prefix <= 0 || max_rest <= 0)
+    return fail(MORPHO_ERR_INVALID_ARGUMENT, "max_prefix and max_rest must be positive");
+  if (n > 64) return fail(MORPHO_ERR_UNSUPPORTED, "shared prefixes take at most 64 new tokens (got %lld)", (long long)n);
+  const int64_t cap = (int64_t)d.W * d.P;
+  p = cache_shared_plan(d.B, d.H, d.n, (int)members, (int)groups, max_prefix < cap ? max_prefix : cap,
+                        max_rest < cap ? max_rest : cap, d.M, d.DV);
+  if ((int64_t)d.B * d.H * p.rest.qblocks * p.rest.nsplit > (1 << 23) || (int64_t)d.H * p.rblocks * p.np > (1 << 23))
+    return fail(MORPHO_ERR_INVALID_ARGUMENT, "problem too large: B*H*pieces must be at most 2^23");
+  return MORPHO_OK;
+}
+size_t shared_part_o_bytes(const CacheDims& d, const CacheSharedPlan& p) {
+  return align_up((size_t)d.B * d.H * d.n * (p.np + p.rest.nsplit) * d.DV * 4);
+}
+size_t shared_bytes(const CacheDims& d, const CacheSharedPlan& p) {
+  return shared_part_o_bytes(d, p) + align_up((size_t)d.B * d.H * d.n * (p.np + p.rest.nsplit) * 16);
+}
+}  // namespace
+
+MORPHO_EXPORT size_t morpho_cache_shared_attention_workspace_size(const morpho_cache* cache, int64_t B, int64_t n,
+                                                                  int64_t seq_pages, int64_t members, int64_t groups,
+                                                                  int64_t max_prefix, int64_t max_rest) {
+  CacheDims d;
+  CacheSharedPlan p;
+  std::string keep = g_last_error;
+  const int st = make_shared_plan(cache, B, n, seq_pages, members, groups, max_prefix, max_rest, d, p);
+  g_last_error = keep;
+  return st == MORPHO_OK ? shared_bytes(d, p) : 0;
+}
+
+MORPHO_EXPORT int morpho_cache_shared_attention(const void* phi, const void* gate_q, const void* gate_k,
+                                                const morpho_cache* cache, const int32_t* table, const int32_t* lens,
+                                                const int32_t* new_lens, const int64_t* tree,
+                                                const morpho_shared_prefix* shared, void* out, float* lse, int64_t B,
+                                                int64_t n, int64_t seq_pages, float scale, int mode, void* workspace,
+                                                size_t workspace_bytes, morpho_stream_t stream) {
+  g_last_error.clear();
+  if (!shared) return fail(MORPHO_ERR_INVALID_ARGUMENT, "Null shared pointer");
+  CacheDims d;
+  CacheSharedPlan plan;
+  int st = make_shared_plan(cache, B, n, seq_pages, shared->members_count, shared->groups, shared->max_prefix,
+                            shared->max_rest, d, plan);
+  if (st != MORPHO_OK) return st;
+  if (!__builtin_isfinite(scale)) return fail(MORPHO_ERR_INVALID_ARGUMENT, "scale must be a finite number");
+  if ((mode & ~(MORPHO_MODE_CAUSAL | MORPHO_MODE_MASK_DIAG)) != 0)
+    return fail(MORPHO_ERR_INVALID_ARGUMENT, "invalid mode bits 0x%x (causal | mask_diag)", mode);
+  if (tree && (mode & MORPHO_MODE_MASK_DIAG))
+    return fail(MORPHO_ERR_INVALID_ARGUMENT, "MORPHO_MODE_MASK_DIAG with a tree: leave a draft's own bit out instead");
+  if (!phi || !gate_q || !gate_k || !table || !lens || !out || !lse || !shared->members || !shared->starts ||
+      !shared->group || !shared->pages)
+    return fail(MORPHO_ERR_INVALID_ARGUMENT, "Null pointer");
+  if ((st = check_pool(cache)) != MORPHO_OK) return st;
+  if (misaligned(phi) || misaligned(out) || misaligned(lse))
+    return fail(MORPHO_ERR_INVALID_ARGUMENT, "tensor pointers must be 16-byte aligned");
+  if (misaligned_ints(table, lens, new_lens) ||
+      misaligned_ints(shared->members, shared->starts, shared->group, shared->pages) ||
+      (reinterpret_cast<uintptr_t>(tree) & 7) != 0)
+    return fail(MORPHO_ERR_INVALID_ARGUMENT, "int32 pointers must be 4-byte aligned, tree 8-byte");
+  const size_t need = shared_bytes(d, plan);
+  if (!workspace || workspace_bytes < need)
+    return fail(MORPHO_ERR_WORKSPACE, "shared cache attention workspace needs %zu bytes (got %zu)", need,
+                workspace_bytes);
+  if ((reinterpret_cast<uintptr_t>(workspace) & 255) != 0)
+    return fail(MORPHO_ERR_WORKSPACE, "workspace must be 256-byte aligned");
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  const CacheAttnBuffers part{static_cast<float*>(workspace),
+                              reinterpret_cast<float4*>(static_cast<char*>(workspace) + shared_part_o_bytes(d, plan))};
+  const CacheSharedCall call{shared->members, shared->starts,           shared->group,
+                             shared->pages,   (int)shared->members_count, (int)shared->groups};
+  auto* o = static_cast<_Float16*>(out);
+  const int causal = mode & MORPHO_MODE_CAUSAL, diag = mode & MORPHO_MODE_MASK_DIAG;
+  MORPHO_LAUNCH("cache_shared",
+                launch_cache_shared(d, plan, call, static_cast<const _Float16*>(phi),
+                                    static_cast<const _Float16*>(gate_q), static_cast<const _Float16*>(gate_k),
+                                    static_cast<const _Float16*>(cache->codes),
+                                    static_cast<const _Float16*>(cache->values), table, lens, new_lens, tree, o, lse,
+                                    part, scale, causal, diag, s));
+  MORPHO_LAUNCH("cache_shared_join",
+                launch_cache_shared_join(d, plan, call, static_cast<const _Float16*>(cache->values), table, lens,
+                                         new_lens, tree, part, o, lse, causal, diag, s));
+  return MORPHO_OK;
+}
+
 MORPHO_EXPORT int morpho_cache_copy_pages(const morpho_cache* cache, const int32_t* src, const int32_t* dst,
                                           int64_t count, morpho_stream_t stream) {
   g_last_error.clear();
@@ -754,6 +844,150 @@ MORPHO_EXPORT int morpho_cache_compact(const morpho_cache* cache, const int32_t*
   MORPHO_LAUNCH("cache_compact", launch_cache_compact(d, static_cast<_Float16*>(cache->codes),
                                                       static_cast<_Float16*>(cache->values), table, lens, keep,
                                                       keep_lens, (int)keep_cols, s));
+  return MORPHO_OK;
+}
+
+namespace {
+int check_plan_sizes(int64_t B, int64_t n, int64_t seq_pages, int64_t page_size) {
+  if (B <= 0 || n <= 0 || seq_pages <= 0) return fail(MORPHO_ERR_INVALID_ARGUMENT, "Invalid dimensions");
+  if (page_size != 32 && page_size != 64 && page_size != 128 && page_size != 256)
+    return fail(MORPHO_ERR_UNSUPPORTED, "page_size must be 32, 64, 128 or 256 (got %lld)", (long long)page_size);
+  if (seq_pages > kMaxCacheTokens / page_size)
+    return fail(MORPHO_ERR_INVALID_ARGUMENT, "cache too large: seq_pages * page_size must be at most 2^30");
+  if (B > (1 << 22) || n > (1 << 22) || B * n > (1 << 22))
+    return fail(MORPHO_ERR_INVALID_ARGUMENT, "problem too large: needs B*n <= 2^22");
+  return MORPHO_OK;
+}
+}  // namespace
+
+MORPHO_EXPORT size_t morpho_cache_plan_workspace_size(int64_t B, int64_t n) {
+  if (B <= 0 || n <= 0 || B > (1 << 22) || n > (1 << 22) || B * n > (1 << 22) || cache_plan_fused(B, n)) return 0;
+  return align_up(16 + (size_t)B * 16);
+}
+
+MORPHO_EXPORT int morpho_cache_plan(int32_t* table, int32_t* held, const int32_t* lens, const int32_t* new_lens,
+                                    int32_t* free_pages, int32_t* free_count, int64_t free_room, int32_t* granted,
+                                    int64_t* slots, int64_t B, int64_t n, int64_t seq_pages, int64_t page_size,
+                                    void* workspace, size_t workspace_bytes, morpho_stream_t stream) {
+  g_last_error.clear();
+  int st = check_plan_sizes(B, n, seq_pages, page_size);
+  if (st != MORPHO_OK) return st;
+  if (free_room < 0 || free_room > INT_MAX) return fail(MORPHO_ERR_INVALID_ARGUMENT, "Invalid dimensions");
+  if (!table || !held || !lens || !free_count || !granted || !slots || (!free_pages && free_room > 0))
+    return fail(MORPHO_ERR_INVALID_ARGUMENT, "Null pointer");
+  if (misaligned_ints(table, held, lens, new_lens) || misaligned_ints(free_pages, free_count, granted) ||
+      (reinterpret_cast<uintptr_t>(slots) & 7) != 0)
+    return fail(MORPHO_ERR_INVALID_ARGUMENT, "int32 pointers must be 4-byte aligned, slots 8-byte");
+  const size_t need = morpho_cache_plan_workspace_size(B, n);
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(MORPHO_ERR_WORKSPACE, "cache plan workspace needs %zu bytes (got %zu)", need, workspace_bytes);
+  if (need && (reinterpret_cast<uintptr_t>(workspace) & 255) != 0)
+    return fail(MORPHO_ERR_WORKSPACE, "workspace must be 256-byte aligned");
+  CachePlanArgs a{};
+  a.table = table;
+  a.held = held;
+  a.lens = lens;
+  a.new_lens = new_lens;
+  a.free_pages = free_pages;
+  a.free_count = free_count;
+  a.granted = granted;
+  a.slots = slots;
+  a.room = free_room;
+  a.B = (int)B;
+  a.n = (int)n;
+  a.W = (int)seq_pages;
+  a.lp = __builtin_ctz((unsigned)page_size);
+  a.workspace = need ? workspace : nullptr;
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  MORPHO_LAUNCH("cache_plan", launch_cache_plan(a, s));
+  return MORPHO_OK;
+}
+
+// ---------------------------------------------------------------- verification of drafted tokens
+namespace {
+int make_verify_plan(int64_t B, int64_t n, int64_t vocab, int type, bool draft, bool tree, double temperature,
+                     VerifyPlan& p) {
+  if (B <= 0 || n <= 0 || vocab <= 0) return fail(MORPHO_ERR_INVALID_ARGUMENT, "Invalid dimensions");
+  if (type != MORPHO_FLOAT16 && type != MORPHO_BFLOAT16 && type != MORPHO_FLOAT32)
+    return fail(MORPHO_ERR_UNSUPPORTED, "logits must be float16, bfloat16 or float32 (got type %d)", type);
+  if (n > 64) return fail(MORPHO_ERR_UNSUPPORTED, "a step holds at most 64 drafted tokens (got %lld)", (long long)n);
+  if (vocab > kVerifyMaxVocab)
+    return fail(MORPHO_ERR_INVALID_ARGUMENT, "problem too large: needs vocab <= %d", kVerifyMaxVocab);
+  if (!(temperature == 0.0 || (temperature >= 1e-4 && temperature <= 1e4)))
+    return fail(MORPHO_ERR_INVALID_ARGUMENT, "temperature must be 0, or 1e-4 to 1e4 (got %g)", temperature);
+  if (B > (1 << 22)) return fail(MORPHO_ERR_INVALID_ARGUMENT, "problem too large: needs B*(2n-1)*chunks <= 2^23");
+  const bool best = temperature == 0.0;
+  const int64_t rows = B * (draft && !best ? 2 * n - 1 : n);
+  p = verify_plan(rows, (int)vocab, type == MORPHO_FLOAT32 ? 4 : 2, tree, draft && !best, best);
+  if (rows * p.chunks > (1 << 23))
+    return fail(MORPHO_ERR_INVALID_ARGUMENT, "problem too large: needs B*(2n-1)*chunks <= 2^23");
+  return MORPHO_OK;
+}
+size_t verify_stats_bytes(int64_t B, int64_t n, const VerifyPlan& p) {
+  return align_up((size_t)B * (2 * n - 1) * p.chunks * sizeof(VerifyStat));
+}
+size_t verify_bytes(int64_t B, int64_t n, const VerifyPlan& p) {
+  return verify_stats_bytes(B, n, p) + align_up((size_t)p.rounds * B * p.chunks * 8);
+}
+bool bad_rows(const morpho_logits& r, int type) {
+  return (reinterpret_cast<uintptr_t>(r.data) & (type == MORPHO_FLOAT32 ? 3 : 1)) != 0;
+}
+}  // namespace
+
+MORPHO_EXPORT size_t morpho_verify_workspace_size(int64_t B, int64_t n, int64_t vocab, int type, int have_draft,
+                                                  int have_tree, double temperature) {
+  VerifyPlan p;
+  std::string keep = g_last_error;
+  const int st = make_verify_plan(B, n, vocab, type, have_draft != 0, have_tree != 0, temperature, p);
+  g_last_error = keep;
+  return st == MORPHO_OK ? verify_bytes(B, n, p) : 0;
+}
+
+MORPHO_EXPORT int morpho_verify_drafts(const morpho_logits* logits, const morpho_logits* draft_logits, int type,
+                                       const int64_t* tokens, const float* uniform, const int64_t* tree,
+                                       const int32_t* new_lens, int32_t* keep, int32_t* keep_lens, int64_t* token,
+                                       int64_t B, int64_t n, int64_t vocab, double temperature, void* workspace,
+                                       size_t workspace_bytes, morpho_stream_t stream) {
+  g_last_error.clear();
+  VerifyPlan plan;
+  const bool draft = draft_logits && draft_logits->data && n > 1;
+  int st = make_verify_plan(B, n, vocab, type, draft, tree != nullptr, temperature, plan);
+  if (st != MORPHO_OK) return st;
+  if (!logits || !logits->data || !tokens || !uniform || !keep || !keep_lens || !token)
+    return fail(MORPHO_ERR_INVALID_ARGUMENT, "Null pointer");
+  if (bad_rows(*logits, type) || (draft && bad_rows(*draft_logits, type)))
+    return fail(MORPHO_ERR_INVALID_ARGUMENT, "logits must be aligned to their type");
+  if (misaligned_ints(uniform, new_lens, keep, keep_lens) ||
+      ((reinterpret_cast<uintptr_t>(tokens) | reinterpret_cast<uintptr_t>(tree) | reinterpret_cast<uintptr_t>(token)) &
+       7) != 0)
+    return fail(MORPHO_ERR_INVALID_ARGUMENT, "32-bit pointers must be 4-byte aligned, 64-bit ones 8-byte");
+  const size_t need = verify_bytes(B, n, plan);
+  if (!workspace || workspace_bytes < need)
+    return fail(MORPHO_ERR_WORKSPACE, "verification workspace needs %zu bytes (got %zu)", need, workspace_bytes);
+  if ((reinterpret_cast<uintptr_t>(workspace) & 255) != 0)
+    return fail(MORPHO_ERR_WORKSPACE, "workspace must be 256-byte aligned");
+  VerifyArgs a{};
+  a.p = VerifyRows{logits->data, logits->batch_stride, logits->row_stride};
+  a.best = temperature == 0.0;
+  if (draft && !a.best) a.q = VerifyRows{draft_logits->data, draft_logits->batch_stride, draft_logits->row_stride};
+  a.tokens = tokens;
+  a.uniform = uniform;
+  a.tree = tree;
+  a.new_lens = new_lens;
+  a.keep = keep;
+  a.keep_lens = keep_lens;
+  a.token = token;
+  a.stats = static_cast<VerifyStat*>(workspace);
+  a.masses = reinterpret_cast<double*>(static_cast<char*>(workspace) + verify_stats_bytes(B, n, plan));
+  a.c = a.best ? 0.0 : 32.0 * 1.44269504088896340736 / temperature;
+  a.B = (int)B;
+  a.n = (int)n;
+  a.V = (int)vocab;
+  a.chunk = plan.chunk;
+  a.chunks = plan.chunks;
+  a.rounds = plan.rounds;
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  MORPHO_LAUNCH("verify", launch_verify(a, plan, type, s));
   return MORPHO_OK;
 }
 

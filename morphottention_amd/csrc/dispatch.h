@@ -408,4 +408,53 @@ inline int cache_compact_heads(int64_t sequences, int H, int DV, int K) {
   return hg;
 }
 
+// Launch shape of the attention where sequences have their first pages in
+// common: np pieces of split_keys common keys for row blocks of 16 qt rows (of
+// one group), and the sequences' own keys as without (rest).
+struct CacheSharedPlan {
+  int qt, rblocks, np, split_keys;
+  CacheAttnPlan rest;
+};
+// members: sequences that are in a group; max_prefix, max_rest: at least the
+// longest common part and the longest rest with its new tokens.
+inline CacheSharedPlan cache_shared_plan(int B, int H, int n, int members, int groups, int64_t max_prefix,
+                                         int64_t max_rest, int M, int DV) {
+  CacheSharedPlan p;
+  p.rest = cache_attn_plan(B, H, n, max_rest, M, DV);
+  p.qt = 1;
+  // every group's last block may be part of one
+  const int64_t rows = (int64_t)members * n;
+  p.rblocks = (int)(rows / (16 * p.qt) + groups);
+  int64_t keys = 512;
+  // partial rows (DV + 4 floats each) and workgroups stay below 2^20 or so
+  const int64_t most = ((int64_t)1 << 20) / ((int64_t)B * H * n) > 1 ? ((int64_t)1 << 20) / ((int64_t)B * H * n) : 1;
+  if (keys < (max_prefix + most - 1) / most) keys = (max_prefix + most - 1) / most;
+  keys = (keys + 127) / 128 * 128;
+  p.np = (int)((max_prefix + keys - 1) / keys);
+  p.split_keys = (int)keys;
+  return p;
+}
+
+// ---------------------------------------------------------------- verification of drafted tokens
+// A row of logits in chunks of `pieces` times 256 times 16 bytes, a workgroup
+// each; rounds: of masses that are summed by the whole chip.
+struct VerifyPlan {
+  int pieces, chunk, chunks, rounds;
+};
+constexpr int kVerifyMaxVocab = 4000000, kVerifyMaxChunks = 1024;
+inline VerifyPlan verify_plan(int64_t rows, int vocab, int element_bytes, bool tree, bool draft, bool best) {
+  VerifyPlan p;
+  const int per = 16 / element_bytes;
+  auto chunks = [&](int pieces) { return (vocab + per - 1 + 256 * per * pieces - 1) / (256 * per * pieces); };
+  p.pieces = rows * chunks(4) < 1024 && chunks(1) <= 256 ? 1 : 4;
+  p.chunk = 256 * per * p.pieces;
+  p.chunks = chunks(p.pieces);
+  p.rounds = best || p.chunks == 1 ? 0 : draft && tree ? 2 : 1;
+  return p;
+}
+
+// ---------------------------------------------------------------- page tables from lengths
+// Whether one workgroup does all of it, the slots too.
+inline bool cache_plan_fused(int64_t B, int64_t n) { return B <= 1024 && B * n <= 8192; }
+
 }  // namespace morpho

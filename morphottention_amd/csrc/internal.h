@@ -168,6 +168,62 @@ hipError_t launch_cache_copy(const CacheDims& d, _Float16* codes, _Float16* valu
 hipError_t launch_cache_compact(const CacheDims& d, _Float16* codes, _Float16* values, const int* table,
                                 const int* lens, const int* keep, const int* keep_lens, int K, hipStream_t s);
 
+// kernels_cache_shared.hip: attention where sequences have their first pages in common.
+struct CacheSharedCall {
+  const int* members;  // [members_count] sequences, group by group
+  const int* starts;   // [groups + 1] a group's first place in members
+  const int* group;    // [B] a sequence's group
+  const int* pages;    // [groups] pages in common
+  int members_count, groups;
+};
+// The common keys' pieces and every sequence's own: [B, H, n, np + rest.nsplit] parts.
+hipError_t launch_cache_shared(const CacheDims& d, const CacheSharedPlan& plan, const CacheSharedCall& call,
+                               const _Float16* phi, const _Float16* gate_q, const _Float16* gate_k,
+                               const _Float16* codes, const _Float16* values, const int* table, const int* lens,
+                               const int* new_lens, const int64_t* tree, _Float16* out, float* lse,
+                               const CacheAttnBuffers& part, float scale, int causal, int mask_diag, hipStream_t s);
+hipError_t launch_cache_shared_join(const CacheDims& d, const CacheSharedPlan& plan, const CacheSharedCall& call,
+                                    const _Float16* values, const int* table, const int* lens, const int* new_lens,
+                                    const int64_t* tree, const CacheAttnBuffers& part, _Float16* out, float* lse,
+                                    int causal, int mask_diag, hipStream_t s);
+
+// kernels_cache_plan.hip: page tables and slot maps from lengths.
+struct CachePlanArgs {
+  int *table, *held;
+  const int *lens, *new_lens;
+  int *free_pages, *free_count, *granted;
+  int64_t* slots;
+  int64_t room;     // places of free_pages
+  int B, n, W, lp;  // sequences, new tokens of each, pages a sequence, log2 of the page size
+  void* workspace;  // of the second kernel (null: there is none)
+};
+hipError_t launch_cache_plan(const CachePlanArgs& a, hipStream_t s);
+
+// kernels_verify.hip: verification of drafted tokens.
+struct VerifyRows {
+  const void* data;
+  int64_t batch_stride, row_stride;  // in elements
+};
+struct VerifyStat {
+  double sum;  // of the weights below top
+  float top;
+  int best;  // place of top (temperature 0 only)
+};
+struct VerifyArgs {
+  VerifyRows p, q;  // the target's logits [B, n, V], the drafter's [B, n - 1, V] (or null)
+  const int64_t* tokens;
+  const float* uniform;
+  const int64_t* tree;
+  const int* new_lens;
+  int *keep, *keep_lens;
+  int64_t* token;
+  VerifyStat* stats;  // [B n + B (n - 1), chunks]
+  double* masses;     // [rounds, B, chunks]
+  double c;           // 32 log2(e) / temperature
+  int B, n, V, chunk, chunks, rounds, best;
+};
+hipError_t launch_verify(const VerifyArgs& a, const VerifyPlan& p, int type, hipStream_t s);
+
 // Timing hooks (capi.hip). When timing is enabled, timing_begin opens a
 // record (a name and two events) for the launcher call that follows, and the
 // kernel launches inside it take the record's events through

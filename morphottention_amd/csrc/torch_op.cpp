@@ -13,6 +13,7 @@
 #include <torch/library.h>
 
 #include <optional>
+#include <utility>
 #include <vector>
 
 #include "../../include/morphottention.h"
@@ -316,12 +317,15 @@ at::Tensor op_cache_append(const at::Tensor& X, const at::Tensor& weights, const
   return phi;
 }
 
-std::vector<at::Tensor> op_cache_attention(const at::Tensor& phi, const at::Tensor& gate_q, const at::Tensor& gate_k,
-                                           const at::Tensor& codes, const at::Tensor& values, const at::Tensor& table,
-                                           const at::Tensor& lens, const std::optional<at::Tensor>& new_lens,
-                                           const std::optional<at::Tensor>& tree, double scale, bool causal,
-                                           int64_t variant, int64_t max_len) {
-  const int mode = mode_of(causal, variant);
+struct AttentionCall {
+  morpho_cache cache;
+  CacheCall call;
+  int64_t B, n;
+};
+AttentionCall check_attention_call(const at::Tensor& phi, const at::Tensor& gate_q, const at::Tensor& gate_k,
+                                   const at::Tensor& codes, const at::Tensor& values, const at::Tensor& table,
+                                   const at::Tensor& lens, const std::optional<at::Tensor>& new_lens,
+                                   const std::optional<at::Tensor>& tree) {
   const morpho_cache c = check_pool(codes, values, false);
   check(phi, "phi");
   check(gate_q, "gate_q");
@@ -339,6 +343,19 @@ std::vector<at::Tensor> op_cache_attention(const at::Tensor& phi, const at::Tens
                     tree->size(0) == B && tree->size(1) == n && tree->device() == codes.device(),
                 "tree must be a contiguous int64 [B, n] CUDA tensor on the device of codes");
   }
+  return {c, k, B, n};
+}
+
+std::vector<at::Tensor> op_cache_attention(const at::Tensor& phi, const at::Tensor& gate_q, const at::Tensor& gate_k,
+                                           const at::Tensor& codes, const at::Tensor& values, const at::Tensor& table,
+                                           const at::Tensor& lens, const std::optional<at::Tensor>& new_lens,
+                                           const std::optional<at::Tensor>& tree, double scale, bool causal,
+                                           int64_t variant, int64_t max_len) {
+  const int mode = mode_of(causal, variant);
+  const AttentionCall call = check_attention_call(phi, gate_q, gate_k, codes, values, table, lens, new_lens, tree);
+  const morpho_cache& c = call.cache;
+  const CacheCall& k = call.call;
+  const int64_t B = call.B, n = call.n;
   TORCH_CHECK(max_len >= 0, "max_len must not be negative (0: the table's length), got ", max_len);
   if (max_len == 0) max_len = k.seq_pages * c.page_size;
   const c10::hip::HIPGuardMasqueradingAsCUDA guard(codes.device());
@@ -385,6 +402,133 @@ void op_cache_compact(const at::Tensor& codes, const at::Tensor& values, const a
            "cache_compact");
 }
 
+// ---- a decoding loop on the device (no reference op)
+std::vector<at::Tensor> op_cache_shared_attention(const at::Tensor& phi, const at::Tensor& gate_q,
+                                                  const at::Tensor& gate_k, const at::Tensor& codes,
+                                                  const at::Tensor& values, const at::Tensor& table,
+                                                  const at::Tensor& lens, const std::optional<at::Tensor>& new_lens,
+                                                  const std::optional<at::Tensor>& tree, const at::Tensor& members,
+                                                  const at::Tensor& starts, const at::Tensor& group,
+                                                  const at::Tensor& pages, int64_t max_prefix, int64_t max_rest,
+                                                  double scale, bool causal, int64_t variant) {
+  const int mode = mode_of(causal, variant);
+  const AttentionCall k = check_attention_call(phi, gate_q, gate_k, codes, values, table, lens, new_lens, tree);
+  for (const auto& [t, name] : {std::pair<const at::Tensor&, const char*>(members, "members"),
+                                {starts, "starts"}, {group, "group"}, {pages, "pages"}}) {
+    check_ints(t, name, codes);
+    TORCH_CHECK(t.dim() == 1, name, " must have one dimension");
+  }
+  TORCH_CHECK(group.size(0) == k.B, "group must be [B]");
+  TORCH_CHECK(pages.size(0) > 0 && starts.size(0) == pages.size(0) + 1, "starts must be [groups + 1], pages [groups]");
+  const int64_t cap = k.call.seq_pages * k.cache.page_size;
+  TORCH_CHECK(max_prefix >= 0 && max_rest >= 0, "max_prefix and max_rest must not be negative (0: the table's length)");
+  const morpho_shared_prefix shared{members.data_ptr<int32_t>(), starts.data_ptr<int32_t>(),
+                                    group.data_ptr<int32_t>(),   pages.data_ptr<int32_t>(),
+                                    members.size(0),             pages.size(0),
+                                    max_prefix ? max_prefix : cap, max_rest ? max_rest : cap};
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(codes.device());
+  auto out = at::empty({k.B, k.n, k.cache.H * k.cache.head_dim_v}, phi.options());
+  auto lse = at::empty({k.B * k.cache.H, k.n}, phi.options().dtype(at::kFloat));
+  const size_t ws_bytes = morpho_cache_shared_attention_workspace_size(
+      &k.cache, k.B, k.n, k.call.seq_pages, shared.members_count, shared.groups, shared.max_prefix, shared.max_rest);
+  at::Tensor ws;
+  if (ws_bytes) ws = at::empty({(int64_t)ws_bytes}, phi.options().dtype(at::kByte));
+  raise_on(morpho_cache_shared_attention(phi.data_ptr(), gate_q.data_ptr(), gate_k.data_ptr(), &k.cache, k.call.table,
+                                         k.call.lens, k.call.new_lens, tree ? tree->data_ptr<int64_t>() : nullptr,
+                                         &shared, out.data_ptr(), lse.data_ptr<float>(), k.B, k.n, k.call.seq_pages,
+                                         (float)scale, mode, ws_bytes ? ws.data_ptr() : nullptr, ws_bytes,
+                                         current_stream(codes)),
+           "cache_shared_attention");
+  return {out, lse};
+}
+
+std::vector<at::Tensor> op_cache_plan(const at::Tensor& table, const at::Tensor& held, const at::Tensor& lens,
+                                      const at::Tensor& free_pages, const at::Tensor& free_count, int64_t n,
+                                      const std::optional<at::Tensor>& new_lens, int64_t page_size) {
+  check_ints(table, "table", table);
+  check_ints(held, "held", table);
+  check_ints(lens, "lens", table);
+  check_ints(free_pages, "free_pages", table);
+  check_ints(free_count, "free_count", table);
+  TORCH_CHECK(table.dim() == 2, "table must be [B, seq_pages]");
+  const int64_t B = table.size(0);
+  TORCH_CHECK(held.dim() == 1 && held.size(0) == B, "held must be [B]");
+  TORCH_CHECK(lens.dim() == 1 && lens.size(0) == B, "lens must be [B]");
+  TORCH_CHECK(free_pages.dim() == 1, "free_pages must have one dimension");
+  TORCH_CHECK(free_count.numel() == 1, "free_count must be one number");
+  if (new_lens) {
+    check_ints(*new_lens, "new_lens", table);
+    TORCH_CHECK(new_lens->dim() == 1 && new_lens->size(0) == B, "new_lens must be [B]");
+  }
+  TORCH_CHECK(n > 0 && n <= (1 << 22), "n must be 1 to 2^22, got ", n);
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(table.device());
+  auto granted = at::empty({B}, table.options());
+  auto slots = at::empty({B, n}, table.options().dtype(at::kLong));
+  const size_t ws_bytes = morpho_cache_plan_workspace_size(B, n);
+  at::Tensor ws;
+  if (ws_bytes) ws = at::empty({(int64_t)ws_bytes}, table.options().dtype(at::kByte));
+  raise_on(morpho_cache_plan(table.data_ptr<int32_t>(), held.data_ptr<int32_t>(), lens.data_ptr<int32_t>(),
+                             new_lens ? new_lens->data_ptr<int32_t>() : nullptr, free_pages.data_ptr<int32_t>(),
+                             free_count.data_ptr<int32_t>(), free_pages.size(0), granted.data_ptr<int32_t>(),
+                             slots.data_ptr<int64_t>(), B, n, table.size(1), page_size,
+                             ws_bytes ? ws.data_ptr() : nullptr, ws_bytes, current_stream(table)),
+           "cache_plan");
+  return {granted, slots};
+}
+
+// The rows of a tensor of logits: any strides but the last one's.
+morpho_logits check_logits(const at::Tensor& t, const char* name, const at::Tensor& logits, int64_t B, int64_t rows,
+                           int64_t vocab) {
+  TORCH_CHECK(t.is_cuda() && t.device() == logits.device(), name, " must be a CUDA tensor on the device of logits");
+  TORCH_CHECK(t.scalar_type() == logits.scalar_type(), name, " must have the type of logits");
+  TORCH_CHECK(t.dim() == 3 && t.size(0) == B && t.size(1) == rows && t.size(2) == vocab, name, " must be [", B, ", ",
+              rows, ", ", vocab, "]");
+  TORCH_CHECK(vocab == 1 || t.stride(2) == 1, name, " must be contiguous along the vocabulary");
+  return {t.data_ptr(), t.stride(0), t.stride(1)};
+}
+
+std::vector<at::Tensor> op_verify_drafts(const at::Tensor& logits, const at::Tensor& tokens, const at::Tensor& uniform,
+                                         const std::optional<at::Tensor>& tree,
+                                         const std::optional<at::Tensor>& new_lens,
+                                         const std::optional<at::Tensor>& draft_logits, double temperature) {
+  TORCH_CHECK(logits.is_cuda(), "logits must be a CUDA tensor");
+  const auto st = logits.scalar_type();
+  TORCH_CHECK(st == at::kHalf || st == at::kBFloat16 || st == at::kFloat,
+              "logits must be float16, bfloat16 or float32");
+  TORCH_CHECK(logits.dim() == 3, "logits must be [B, n, vocab]");
+  const int64_t B = logits.size(0), n = logits.size(1), V = logits.size(2);
+  const morpho_logits p = check_logits(logits, "logits", logits, B, n, V);
+  morpho_logits q{nullptr, 0, 0};
+  if (draft_logits && n > 1) q = check_logits(*draft_logits, "draft_logits", logits, B, n - 1, V);
+  auto flat = [&](const at::Tensor& t, at::ScalarType type, const char* name, const char* type_name) {
+    TORCH_CHECK(t.is_cuda() && t.device() == logits.device(), name, " must be a CUDA tensor on the device of logits");
+    TORCH_CHECK(t.scalar_type() == type && t.is_contiguous() && t.dim() == 2 && t.size(0) == B && t.size(1) == n, name,
+                " must be a contiguous ", type_name, " [B, n] tensor");
+  };
+  flat(tokens, at::kLong, "tokens", "int64");
+  flat(uniform, at::kFloat, "uniform", "float32");
+  if (tree) flat(*tree, at::kLong, "tree", "int64");
+  if (new_lens) {
+    check_ints(*new_lens, "new_lens", logits);
+    TORCH_CHECK(new_lens->dim() == 1 && new_lens->size(0) == B, "new_lens must be [B]");
+  }
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(logits.device());
+  const int type = st == at::kHalf ? MORPHO_FLOAT16 : st == at::kBFloat16 ? MORPHO_BFLOAT16 : MORPHO_FLOAT32;
+  auto keep = at::empty({B, n}, logits.options().dtype(at::kInt));
+  auto keep_lens = at::empty({B}, logits.options().dtype(at::kInt));
+  auto token = at::empty({B}, logits.options().dtype(at::kLong));
+  const size_t ws_bytes = morpho_verify_workspace_size(B, n, V, type, q.data != nullptr, tree.has_value(), temperature);
+  at::Tensor ws;
+  if (ws_bytes) ws = at::empty({(int64_t)ws_bytes}, logits.options().dtype(at::kByte));
+  raise_on(morpho_verify_drafts(&p, &q, type, tokens.data_ptr<int64_t>(), uniform.data_ptr<float>(),
+                                tree ? tree->data_ptr<int64_t>() : nullptr,
+                                new_lens ? new_lens->data_ptr<int32_t>() : nullptr, keep.data_ptr<int32_t>(),
+                                keep_lens.data_ptr<int32_t>(), token.data_ptr<int64_t>(), B, n, V, temperature,
+                                ws_bytes ? ws.data_ptr() : nullptr, ws_bytes, current_stream(logits)),
+           "verify_drafts");
+  return {keep, keep_lens, token};
+}
+
 }  // namespace
 
 TORCH_LIBRARY(morphottention, m) {
@@ -410,6 +554,13 @@ TORCH_LIBRARY(morphottention, m) {
   m.def("cache_copy_pages(Tensor(a!) codes, Tensor(b!) values, Tensor src, Tensor dst) -> ()");
   m.def("cache_compact(Tensor(a!) codes, Tensor(b!) values, Tensor table, Tensor lens, Tensor keep, "
         "Tensor? keep_lens=None) -> ()");
+  m.def("cache_shared_attention(Tensor phi, Tensor gate_q, Tensor gate_k, Tensor codes, Tensor values, Tensor table, "
+        "Tensor lens, Tensor? new_lens, Tensor? tree, Tensor members, Tensor starts, Tensor group, Tensor pages, "
+        "int max_prefix, int max_rest, float scale, bool causal, int variant=0) -> Tensor[]");
+  m.def("cache_plan(Tensor(a!) table, Tensor(b!) held, Tensor lens, Tensor(c!) free_pages, Tensor(d!) free_count, "
+        "int n, Tensor? new_lens, int page_size) -> Tensor[]");
+  m.def("verify_drafts(Tensor logits, Tensor tokens, Tensor uniform, Tensor? tree, Tensor? new_lens, "
+        "Tensor? draft_logits, float temperature) -> Tensor[]");
 }
 
 TORCH_LIBRARY_IMPL(morphottention, CUDA, m) {
@@ -423,4 +574,7 @@ TORCH_LIBRARY_IMPL(morphottention, CUDA, m) {
   m.impl("cache_attention", &op_cache_attention);
   m.impl("cache_copy_pages", &op_cache_copy_pages);
   m.impl("cache_compact", &op_cache_compact);
+  m.impl("cache_shared_attention", &op_cache_shared_attention);
+  m.impl("cache_plan", &op_cache_plan);
+  m.impl("verify_drafts", &op_verify_drafts);
 }
