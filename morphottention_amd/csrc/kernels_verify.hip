@@ -41,16 +41,16 @@ __constant__ double kExp2Table[32] = {
     0x1.b7f76f2fb5e47p+0, 0x1.c199bdd85529cp+0, 0x1.cb720dcef9069p+0, 0x1.d5818dcfba487p+0, 0x1.dfc97337b9b5fp+0,
     0x1.ea4afa2a490dap+0, 0x1.f50765b6e4540p+0};
 
-// The weight exp((x - top) / temperature) of a logit, as 2^(v / 32) with v = x c -
-// top c <= 0, c = 32 log2(e) / temperature: v = 32 e + i + r, |r| <= 1/2, and 2^(r /
-// 32) is a polynomial of degree 5 through its Chebyshev nodes (2^-52.6 off at
+// The weight exp((x - top) / temperature) of a logit, as 2^(v / 32) with v = (x -
+// top) c <= 0, c = 32 log2(e) / temperature (the difference first: logits may be as
+// large as their type allows): v = 32 e + i + r, |r| <= 1/2, and 2^(r / 32) is a polynomial of degree 5 through its Chebyshev nodes (2^-52.6 off at
 // most). The table's 32 numbers are one in each pair of LDS banks, so lanes that
 // read any of them never wait for each other. NaN and -inf weigh nothing.
 struct Weigh {
   const double* table;  // LDS
-  double c, topc;       // of a finite top
+  double c, top;        // a finite top
   __device__ __forceinline__ double operator()(float x) const {
-    const double v = fmax(fma((double)x, c, -topc), -40000.0);
+    const double v = fmax(((double)x - top) * c, -40000.0);
     const double t = v + 0x1.8p52;
     const int n = (int)__builtin_bit_cast(int64_t, t);
     const double r = v - (t - 0x1.8p52);
@@ -67,7 +67,7 @@ struct Weigh {
 __device__ __forceinline__ double weight_below(const double* table, double c, float x, float top) {
   if (top == __builtin_inff()) return x == top ? 1.0 : 0.0;
   if (top == kNegInf) return 0.0;
-  return Weigh{table, c, (double)top * c}(x);
+  return Weigh{table, c, (double)top}(x);
 }
 
 struct Bf16 {
@@ -188,7 +188,7 @@ __global__ __launch_bounds__(256) void verify_stats_kernel(VerifyArgs a) {
 #pragma unroll
       for (int e = 0; e < E; ++e) sum += x[u][e] == top ? 1.0 : 0.0;
   } else if (top > kNegInf) {
-    const Weigh weigh{table, a.c, (double)top * a.c};
+    const Weigh weigh{table, a.c, (double)top};
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -392,7 +392,7 @@ struct Walk {
     Rest r;
     r.p = row_of<T>(a.p, b, node);
     r.ptop = s.top[0][node];
-    r.wp = Weigh{s.table, a.c, (double)r.ptop * a.c};
+    r.wp = Weigh{s.table, a.c, (double)r.ptop};
     r.ap = s.sum[0][node] > 0.0 ? pa / s.sum[0][node] : 0.0;
     r.q = nullptr;
     r.aq = 0.0;
@@ -402,7 +402,7 @@ struct Walk {
       if (qc > 0.0) {
         r.q = row_of<T>(a.q, b, node);
         r.qtop = s.top[1][node];
-        r.wq = Weigh{s.table, a.c, (double)r.qtop * a.c};
+        r.wq = Weigh{s.table, a.c, (double)r.qtop};
         r.aq = s.sum[1][node] > 0.0 ? qc / s.sum[1][node] : 0.0;
       }
     } else {
