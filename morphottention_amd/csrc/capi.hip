@@ -927,7 +927,7 @@ size_t verify_stats_bytes(int64_t B, int64_t n, const VerifyPlan& p) {
   return align_up((size_t)B * (2 * n - 1) * p.chunks * sizeof(VerifyStat));
 }
 size_t verify_bytes(int64_t B, int64_t n, const VerifyPlan& p) {
-  return verify_stats_bytes(B, n, p) + align_up((size_t)p.rounds * B * p.chunks * 8);
+  return verify_stats_bytes(B, n, p) + align_up((size_t)p.rounds * B * (n - 1) * p.chunks * 8);
 }
 bool bad_rows(const morpho_logits& r, int type) {
   return (reinterpret_cast<uintptr_t>(r.data) & (type == MORPHO_FLOAT32 ? 3 : 1)) != 0;

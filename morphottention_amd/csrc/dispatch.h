@@ -437,7 +437,7 @@ inline CacheSharedPlan cache_shared_plan(int B, int H, int n, int members, int g
 
 // ---------------------------------------------------------------- verification of drafted tokens
 // A row of logits in chunks of `pieces` times 256 times 16 bytes, a workgroup
-// each; rounds: of masses that are summed by the whole chip.
+// each; rounds: rejections behind a token whose remainder the whole chip sums.
 struct VerifyPlan {
   int pieces, chunk, chunks, rounds;
 };
@@ -449,7 +449,7 @@ inline VerifyPlan verify_plan(int64_t rows, int vocab, int element_bytes, bool t
   p.pieces = rows * chunks(4) < 1024 && chunks(1) <= 256 ? 1 : 4;
   p.chunk = 256 * per * p.pieces;
   p.chunks = chunks(p.pieces);
-  p.rounds = best || p.chunks == 1 ? 0 : draft && tree ? 2 : 1;
+  p.rounds = best || !draft || p.chunks == 1 ? 0 : tree ? 3 : 1;
   return p;
 }
 

@@ -218,10 +218,11 @@ struct VerifyArgs {
   int *keep, *keep_lens;
   int64_t* token;
   VerifyStat* stats;  // [B n + B (n - 1), chunks]
-  double* masses;     // [rounds, B, chunks]
+  double* masses;     // [rounds, B, n - 1, chunks]
   double c;           // 32 log2(e) / temperature
   int B, n, V, chunk, chunks, rounds, best;
 };
+constexpr int kVerifyThreads = 1024;
 hipError_t launch_verify(const VerifyArgs& a, const VerifyPlan& p, int type, hipStream_t s);
 
 // Timing hooks (capi.hip). When timing is enabled, timing_begin opens a
