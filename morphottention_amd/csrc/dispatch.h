@@ -436,18 +436,17 @@ inline CacheSharedPlan cache_shared_plan(int B, int H, int n, int members, int g
 }
 
 // ---------------------------------------------------------------- verification of drafted tokens
-// A row of logits in chunks of `pieces` times 256 times 16 bytes, a workgroup
-// each; rounds: rejections behind a token whose remainder the whole chip sums.
+// A row of logits in chunks of `pieces` times 64 times 16 bytes, a wave each; rounds: rejections behind a token whose remainder the whole chip sums.
 struct VerifyPlan {
   int pieces, chunk, chunks, rounds;
 };
-constexpr int kVerifyMaxVocab = 4000000, kVerifyMaxChunks = 1024;
+constexpr int kVerifyMaxVocab = 4000000, kVerifyMaxChunks = 4096;
 inline VerifyPlan verify_plan(int64_t rows, int vocab, int element_bytes, bool tree, bool draft, bool best) {
   VerifyPlan p;
   const int per = 16 / element_bytes;
-  auto chunks = [&](int pieces) { return (vocab + per - 1 + 256 * per * pieces - 1) / (256 * per * pieces); };
-  p.pieces = rows * chunks(4) < 1024 && chunks(1) <= 256 ? 1 : 4;
-  p.chunk = 256 * per * p.pieces;
+  auto chunks = [&](int pieces) { return (vocab + per - 1 + 64 * per * pieces - 1) / (64 * per * pieces); };
+  p.pieces = rows * chunks(4) < 4096 && chunks(1) <= 256 ? 1 : 4;
+  p.chunk = 64 * per * p.pieces;
   p.chunks = chunks(p.pieces);
   p.rounds = best || !draft || p.chunks == 1 ? 0 : tree ? 3 : 1;
   return p;

@@ -12,7 +12,7 @@
 //
 // The results are whole numbers that depend on which side of a border a sum of
 // up to millions of terms falls, so weights and sums are in 64 bits: the order of
-// the terms then moves a border by 2^-50 or so, and the same inputs give the same
+// the terms then moves a border by 2^-48 or so, and the same inputs give the same
 // tokens as any other 64-bit evaluation. (In 32 bits one of a thousand sampled
 // tokens is another one.)
 //
@@ -22,6 +22,9 @@
 //    the first, second, ... rejection behind a token, by the whole chip.
 // 3. verify_kernel: the decisions and the next token, one workgroup a sequence; a
 //    remainder that step 2 did not come to is summed here.
+// A chunk is what one wave takes at a time, 64 U pieces of 16 bytes. Small, since
+// the last step draws from one on a single CU (chunks of four times the size: 9 us of
+// 18 there).
 #include <limits.h>
 
 #include "common.h"
@@ -31,61 +34,68 @@ namespace morpho {
 
 namespace {
 
-// 2^(i / 32)
-__constant__ double kExp2Table[32] = {
-    0x1.0000000000000p+0, 0x1.059b0d3158574p+0, 0x1.0b5586cf9890fp+0, 0x1.11301d0125b51p+0, 0x1.172b83c7d517bp+0,
-    0x1.1d4873168b9aap+0, 0x1.2387a6e756238p+0, 0x1.29e9df51fdee1p+0, 0x1.306fe0a31b715p+0, 0x1.371a7373aa9cbp+0,
-    0x1.3dea64c123422p+0, 0x1.44e086061892dp+0, 0x1.4bfdad5362a27p+0, 0x1.5342b569d4f82p+0, 0x1.5ab07dd485429p+0,
-    0x1.6247eb03a5585p+0, 0x1.6a09e667f3bcdp+0, 0x1.71f75e8ec5f74p+0, 0x1.7a11473eb0187p+0, 0x1.82589994cce13p+0,
-    0x1.8ace5422aa0dbp+0, 0x1.93737b0cdc5e5p+0, 0x1.9c49182a3f090p+0, 0x1.a5503b23e255dp+0, 0x1.ae89f995ad3adp+0,
-    0x1.b7f76f2fb5e47p+0, 0x1.c199bdd85529cp+0, 0x1.cb720dcef9069p+0, 0x1.d5818dcfba487p+0, 0x1.dfc97337b9b5fp+0,
-    0x1.ea4afa2a490dap+0, 0x1.f50765b6e4540p+0};
+// The bits of 2^(i / 64) less i 2^46, so that adding n 2^46 with n = 64 e + i gives
+// those of 2^(n / 64).
+__constant__ uint64_t kExp2Table[64] = {
+    0x3ff0000000000000, 0x3fefec9a3e778061, 0x3fefd9b0d3158574, 0x3fefc74518759bc8, 0x3fefb5586cf9890f, 0x3fefa3ec32d3d1a2,
+    0x3fef9301d0125b51, 0x3fef829aaea92de0, 0x3fef72b83c7d517b, 0x3fef635beb6fcb75, 0x3fef54873168b9aa, 0x3fef463b88628cd6,
+    0x3fef387a6e756238, 0x3fef2b4565e27cdd, 0x3fef1e9df51fdee1, 0x3fef1285a6e4030b, 0x3fef06fe0a31b715, 0x3feefc08b26416ff,
+    0x3feef1a7373aa9cb, 0x3feee7db34e59ff7, 0x3feedea64c123422, 0x3feed60a21f72e2a, 0x3feece086061892d, 0x3feec6a2b5c13cd0,
+    0x3feebfdad5362a27, 0x3feeb9b2769d2ca7, 0x3feeb42b569d4f82, 0x3feeaf4736b527da, 0x3feeab07dd485429, 0x3feea76f15ad2148,
+    0x3feea47eb03a5585, 0x3feea23882552225, 0x3feea09e667f3bcd, 0x3fee9fb23c651a2f, 0x3fee9f75e8ec5f74, 0x3fee9feb564267c9,
+    0x3feea11473eb0187, 0x3feea2f336cf4e62, 0x3feea589994cce13, 0x3feea8d99b4492ed, 0x3feeace5422aa0db, 0x3feeb1ae99157736,
+    0x3feeb737b0cdc5e5, 0x3feebd829fde4e50, 0x3feec49182a3f090, 0x3feecc667b5de565, 0x3feed503b23e255d, 0x3feede6b5579fdbf,
+    0x3feee89f995ad3ad, 0x3feef3a2b84f15fb, 0x3feeff76f2fb5e47, 0x3fef0c1e904bc1d2, 0x3fef199bdd85529c, 0x3fef27f12e57d14b,
+    0x3fef3720dcef9069, 0x3fef472d4a07897c, 0x3fef5818dcfba487, 0x3fef69e603db3285, 0x3fef7c97337b9b5f, 0x3fef902ee78b3ff6,
+    0x3fefa4afa2a490da, 0x3fefba1bee615a27, 0x3fefd0765b6e4540, 0x3fefe7c1819e90d8};
 
-// The weight exp((x - top) / temperature) of a logit, as 2^(v / 32) with v = (x -
-// top) c <= 0, c = 32 log2(e) / temperature (the difference first: logits may be as
-// large as their type allows): v = 32 e + i + r, |r| <= 1/2, and 2^(r / 32) is a polynomial
-// of degree 5 through its Chebyshev nodes (2^-52.6 off at most). The table's 32
-// numbers are one in each pair of LDS banks, so lanes that read any of them never
-// wait for each other. NaN and -inf weigh nothing.
-__device__ __forceinline__ double exp2_rest(double r) {
-  double y = 0x1.5d885e6ef14a6p-35;
-  y = fma(y, r, 0x1.3b2b301f1eb9cp-27);
-  y = fma(y, r, 0x1.c6b08d70380ddp-20);
-  y = fma(y, r, 0x1.ebfbdff7feebap-13);
-  y = fma(y, r, 0x1.62e42fefa39efp-6);
-  return fma(y, r, 1.0);
+// 2^(v / 64), v >= -64000: with v = n + r, |r| <= 1/2, 2^(n / 64) from the table and
+// 2^(r / 64) by a polynomial of degree 4 through its Chebyshev nodes (2^-48.5 off at
+// most; of a table of 32, one number in each pair of LDS banks, and degree 5 the sums
+// take 6 % longer).
+__device__ __forceinline__ double exp2_64(const uint64_t* table, double v) {
+  const double t = v + 0x1.8p52;
+  const int n = (int)__builtin_bit_cast(int64_t, t);
+  const double r = v - (t - 0x1.8p52);
+  double y = 0x1.3b2ad0385b409p-31;
+  y = fma(y, r, 0x1.c6b0c40d8c4e9p-23);
+  y = fma(y, r, 0x1.ebfbdff82ac52p-15);
+  y = fma(y, r, 0x1.62e42fefa0352p-7);
+  y = fma(y, r, 1.0);
+  typedef int i32x2 __attribute__((ext_vector_type(2)));
+  i32x2 z = __builtin_bit_cast(i32x2, table[n & 63]);  // LDS
+  int hi = z[1];
+  asm("v_lshl_add_u32 %0, %1, 14, %0" : "+v"(hi) : "v"(n));  // (the compiler adds 64 bits, in five instructions)
+  z[1] = hi;
+  return y * __builtin_bit_cast(double, z);
 }
+// The weight exp((x - top) / temperature) of a logit, 2^(v / 64) with v = (x - top) c
+// <= 0, c = 64 log2(e) / temperature. The difference comes first: logits may be as
+// large as their type allows. An infinite top is 1e39 here, and so is an infinite x,
+// which then weighs 1 where any other weighs nothing. What weighs less than 2^-1000,
+// NaN and -inf too, weighs that; below 2^-900 is taken for nothing everywhere.
+constexpr double kNothing = 0x1p-900;
 struct Weigh {
-  const double* table;  // LDS
-  double c, top;        // a finite top
+  const uint64_t* table;
+  double c, top;
+  __device__ __forceinline__ Weigh(const uint64_t* table, double c, float top)
+      : table(table), c(c), top(fmin(fmax((double)top, -1e39), 1e39)) {}
   __device__ __forceinline__ double operator()(float x) const {
-    const double v = fmax(((double)x - top) * c, -40000.0);
-    const double t = v + 0x1.8p52;
-    const int n = (int)__builtin_bit_cast(int64_t, t);
-    return __builtin_amdgcn_ldexp(exp2_rest(v - (t - 0x1.8p52)) * table[n & 31], n >> 5);
+    return exp2_64(table, fmax((fmin((double)x, 1e39) - top) * c, -64000.0));
   }
 };
-// For sums: fewer instructions. The product comes before the difference, which
-// costs every weight the same factor, 1 + 2^-53 top c / 46: for |top c| below 2^16 or
-// so. What weighs less than 2^-1000, NaN and -inf too, weighs that.
+// For long sums: two instructions less. The product comes before the difference, which
+// costs every weight the same factor, 1 + 2^-53 top c / 92: for |top c| below 2^17.
 struct WeighFast {
-  const double* table;
+  const uint64_t* table;
   double c, topc;
   __device__ __forceinline__ double operator()(float x) const {
-    const double v = fmax(fma((double)x, c, -topc), -32000.0);
-    const double t = v + 0x1.8p52;
-    const int n = (int)__builtin_bit_cast(int64_t, t);
-    typedef int i32x2 __attribute__((ext_vector_type(2)));
-    i32x2 y = __builtin_bit_cast(i32x2, table[n & 31]);
-    y[1] += (n & ~31) << 15;
-    return exp2_rest(v - (t - 0x1.8p52)) * __builtin_bit_cast(double, y);
+    return exp2_64(table, fmax(fma((double)x, c, -topc), -64000.0));
   }
 };
-// Any top: of an infinite one its own kind weigh 1, and nothing where all are -inf.
-__device__ __forceinline__ double weight_below(const double* table, double c, float x, float top) {
-  if (top == __builtin_inff()) return x == top ? 1.0 : 0.0;
-  if (top == kNegInf) return 0.0;
-  return Weigh{table, c, (double)top}(x);
+__device__ __forceinline__ double weight_below(const uint64_t* table, double c, float x, float top) {
+  const double w = Weigh(table, c, top)(x);
+  return w > kNothing && top > kNegInf ? w : 0.0;
 }
 
 struct Bf16 {
@@ -95,9 +105,50 @@ __device__ __forceinline__ float value_of(f16 x) { return (float)x; }
 __device__ __forceinline__ float value_of(Bf16 x) { return __builtin_bit_cast(float, (unsigned)x.bits << 16); }
 __device__ __forceinline__ float value_of(float x) { return x; }
 
+// The value of the lane that step K of a reduction pairs this one with (K of 6: lanes
+// 1, 2, 4, 8, 16 and 32 away or their mirror images, which by then hold the same).
+template <int K>
+__device__ __forceinline__ int paired(int x) {
+  if constexpr (K < 4) {
+    constexpr int kDpp[4] = {0xb1, 0x4e, 0x141, 0x140};  // quad_perm 1 0 3 2, 2 3 0 1, row_half_mirror, row_mirror
+    return __builtin_amdgcn_mov_dpp(x, kDpp[K], 0xf, 0xf, false);
+  } else {
+    return __shfl_xor(x, K == 4 ? 16 : 32);
+  }
+}
+template <int K>
+__device__ __forceinline__ double paired(double x) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, x);
+  const unsigned lo = (unsigned)paired<K>((int)(unsigned)b), hi = (unsigned)paired<K>((int)(unsigned)(b >> 32));
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+template <int K>
+__device__ __forceinline__ float paired(float x) {
+  return __builtin_bit_cast(float, paired<K>(__builtin_bit_cast(int, x)));
+}
 __device__ __forceinline__ double wave_sum(double x) {
+  x += paired<0>(x);
+  x += paired<1>(x);
+  x += paired<2>(x);
+  x += paired<3>(x);
+  x += paired<4>(x);
+  return x + paired<5>(x);
+}
+__device__ __forceinline__ float wave_max(float x) {
+  x = fmaxf(x, paired<0>(x));
+  x = fmaxf(x, paired<1>(x));
+  x = fmaxf(x, paired<2>(x));
+  x = fmaxf(x, paired<3>(x));
+  x = fmaxf(x, paired<4>(x));
+  return fmaxf(x, paired<5>(x));
+}
+// Sum over the lanes up to this one.
+__device__ __forceinline__ double wave_upto(double x, int lane) {
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o);
+  for (int o = 1; o < 64; o <<= 1) {
+    const double y = __shfl_up(x, o);
+    x += lane >= o ? y : 0.0;
+  }
   return x;
 }
 
@@ -180,102 +231,77 @@ __device__ __forceinline__ const VerifyStat* stats_of(const VerifyArgs& a, bool 
 
 }  // namespace
 
-// One chunk of a row a workgroup: 256 U pieces of 16 bytes. Bound by the weights'
-// instructions (18 of 64 bits and 5 of 32 an element) where the chip is full.
+// A chunk of a row a wave. Bound by the weights' instructions (11 of 64 bits and 6 of
+// 32 an element) where the chip is full.
 template <class T, int U, bool BEST>
-__global__ __launch_bounds__(256, 8) void verify_stats_kernel(VerifyArgs a) {
+__global__ __launch_bounds__(256, 8) void verify_stats_kernel(VerifyArgs a, int rows) {
   constexpr int E = 16 / sizeof(T);
-  __shared__ double table[32], sums[4];
-  __shared__ float tops[4];
-  __shared__ int places[4];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int row = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
+  __shared__ uint64_t table[64];
+  const int lane = threadIdx.x & 63;
+  if constexpr (!BEST) {
+    if (threadIdx.x < 64) table[threadIdx.x] = kExp2Table[threadIdx.x];
+    __syncthreads();
+  }
+  const int id = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+  const int row = id / a.chunks, chunk = id - row * a.chunks;
+  if (row >= rows) return;
   const bool draft = row >= a.B * a.n;
-  const int k = draft ? row - a.B * a.n : row, per = draft ? a.n - 1 : a.n, b = k / per, i = k % per;
+  const int k = draft ? row - a.B * a.n : row, per = draft ? a.n - 1 : a.n, b = k / per, i = k - b * per;
   const int nb = tokens_of(a, b);
   if (i >= nb) return;
   // what a token without drafts of its own would have drawn from is not asked for
   if (draft && !__any(lane > i && lane < nb && parent_of(a, b, lane) == i)) return;
-  if (threadIdx.x < 32) table[threadIdx.x] = kExp2Table[threadIdx.x];
   const T* p = row_of<T>(draft ? a.q : a.p, b, i);
-  const int shift = shift_of(p);
+  const int first = (chunk * U * 64 + lane) * E - shift_of(p);
   Piece<T> x[U];
 #pragma unroll
-  for (int u = 0; u < U; ++u) x[u].load(p, ((chunk * U + u) * 256 + (int)threadIdx.x) * E - shift, a.V);
+  for (int u = 0; u < U; ++u) x[u].load(p, first + u * 64 * E, a.V);
   float top = kNegInf;
   int place = INT_MAX;
 #pragma unroll
   for (int u = 0; u < U; ++u)
 #pragma unroll
     for (int e = 0; e < E; ++e) {
+      const float v = x[u][e];
       if constexpr (BEST) {
-        if (x[u][e] > top) {  // in ascending order: the lowest of equal ones
-          top = x[u][e];
-          place = Piece<T>::index(((chunk * U + u) * 256 + (int)threadIdx.x) * E - shift, e, a.V);
-        }
+        const bool more = v > top;  // in ascending order: the lowest of equal ones
+        place = more ? Piece<T>::index(first + u * 64 * E, e, a.V) : place;
+        top = more ? v : top;
       } else {
-        top = fmaxf(top, x[u][e]);
+        top = fmaxf(top, v);
       }
-    }
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const float other = __shfl_xor(top, o);
-    if constexpr (BEST) {
-      const int at = __shfl_xor(place, o);
-      if (other > top || (other == top && at < place)) {
-        top = other;
-        place = at;
-      }
-    } else {
-      top = fmaxf(top, other);
-    }
-  }
-  if (lane == 0) {
-    tops[w] = top;
-    places[w] = place;
-  }
-  __syncthreads();
-  top = tops[0];
-  place = places[0];
-#pragma unroll
-  for (int e = 1; e < 4; ++e)
-    if (tops[e] > top || (BEST && tops[e] == top && places[e] < place)) {
-      top = tops[e];
-      place = places[e];
     }
   VerifyStat& out = a.stats[(int64_t)row * a.chunks + chunk];
   if constexpr (BEST) {
-    if (threadIdx.x == 0) out = VerifyStat{0.0, top, top > kNegInf ? place : -1};
+    const float all = wave_max(top);
+    place = top == all ? place : INT_MAX;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) place = min(place, __shfl_xor(place, o));
+    if (lane == 0) out = VerifyStat{0.0, all, all > kNegInf ? place : -1};
     return;
   }
+  top = wave_max(top);
   double sum = 0.0;
-  if (top == __builtin_inff()) {
+  auto add = [&](const auto& weigh) {
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int u = 0; u < U; ++u) {
+      // one piece after another: registers for eight waves a SIMD, whose loads and
+      // sums overlap
+      asm volatile("" : "+v"(x[u].raw));  // converted again, not kept converted
 #pragma unroll
-      for (int e = 0; e < E; ++e) sum += x[u][e] == top ? 1.0 : 0.0;
-  } else if (top > kNegInf) {
-    auto add = [&](const auto& weigh) {
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        // one piece after another: registers for eight waves a SIMD, whose loads
-        // and sums overlap
-        asm volatile("" : "+v"(x[u].raw));  // converted again, not kept converted
-#pragma unroll
-        for (int e = 0; e < E; ++e) sum += weigh(x[u][e]);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    };
+      for (int e = 0; e < E; ++e) sum += weigh(x[u][e]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  if (top > kNegInf) {
     const double topc = (double)top * a.c;
-    if (fabs(topc) < 65536.0)
+    if (fabs(topc) < 131072.0)
       add(WeighFast{table, a.c, topc});
     else
-      add(Weigh{table, a.c, (double)top});
+      add(Weigh(table, a.c, top));
+    sum = wave_sum(sum);
   }
-  sum = wave_sum(sum);
-  if (lane == 0) sums[w] = sum;
-  __syncthreads();
-  if (threadIdx.x == 0) out = VerifyStat{(sums[0] + sums[1]) + (sums[2] + sums[3]), top, -1};
+  if (lane == 0) out = VerifyStat{sum, top, -1};
 }
 
 namespace {
@@ -287,55 +313,78 @@ struct RowSum {
 };
 // Joins a row's chunks with `per` lanes (a power of two), of which this is number `sub`.
 __device__ __forceinline__ RowSum row_sum(const VerifyStat* st, int chunks, bool real, int sub, int per,
-                                          const double* table, double c) {
+                                          const uint64_t* table, double c) {
   VerifyStat mine{0.0, kNegInf, -1};
   if (real && sub < chunks) mine = st[sub];
   float top = mine.top;
   for (int k = sub + per; real && k < chunks; k += per) top = fmaxf(top, st[k].top);
   for (int o = 1; o < per; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
-  double sum = mine.sum > 0.0 ? mine.sum * weight_below(table, c, mine.top, top) : 0.0;
+  double sum = mine.sum * weight_below(table, c, mine.top, top);
   for (int k = sub + per; real && k < chunks; k += per)
-    sum = fma(st[k].sum, st[k].sum > 0.0 ? weight_below(table, c, st[k].top, top) : 0.0, sum);
+    sum = fma(st[k].sum, weight_below(table, c, st[k].top, top), sum);
   for (int o = 1; o < per; o <<= 1) sum += __shfl_xor(sum, o);
   return {top, sum};
 }
+// The sums of all rows of a sequence, by a workgroup of NT: 2^k lanes a row, as many
+// rows at a time as it has. `parent`: of the lane's draft.
+template <bool DRAFT, int NT>
+__device__ __forceinline__ void row_sums(const VerifyArgs& a, int b, int nb, int parent, const uint64_t* table,
+                                         RowSum (&rows)[2][64]) {
+  int per = 1;
+  while (per < a.chunks && per < 64) per *= 2;
+  const int sub = threadIdx.x & (per - 1);
+  uint64_t inner = 0;  // tokens with drafts
+  if constexpr (DRAFT)
+    for (int i = 0; i < nb; ++i)
+      if (__any(parent == i)) inner |= (uint64_t)1 << i;
+  for (int r0 = 0; r0 < (DRAFT ? 2 * nb : nb); r0 += NT / per) {
+    const int r = r0 + threadIdx.x / per, kind = r >= nb, i = r - kind * nb;
+    const bool real = r < (DRAFT ? 2 * nb : nb) && (!kind || (inner >> i & 1));
+    const RowSum x = row_sum(stats_of(a, kind, b, real ? i : 0), a.chunks, real, sub, per, table, a.c);
+    if (real && sub == 0) rows[kind][i] = x;
+  }
+  __syncthreads();
+}
+// The chance of a logit in its row.
+__device__ __forceinline__ double chance(const uint64_t* table, double c, float x, const RowSum& row) {
+  return row.sum > 0.0 ? weight_below(table, c, x, row.top) / row.sum : 0.0;
+}
 
-// r = max(ap wp - aq wq, 0) of a token's logits, wp and wq their weights below the
-// rows' largest; 0 where it is one of `count` that were turned down.
+// r of logits lp and lq of a token in the target's and the drafter's row.
 template <bool DRAFT>
 struct Rest {
   Weigh p, q;
   double ap, aq;
-  bool pinf, qinf;
-  const int64_t* gone;
-  int count;
   // state (pa, qc) of the decisions: r = max(pa p - qc q, 0)
-  __device__ __forceinline__ Rest(const double* table, double c, const RowSum& ps, const RowSum& qs, double pa,
+  __device__ __forceinline__ Rest(const uint64_t* table, double c, const RowSum& ps, const RowSum& qs, double pa,
                                   double qc)
-      : p{table, c, (double)ps.top}, q{table, c, (double)qs.top}, ap(ps.sum > 0.0 ? pa / ps.sum : 0.0),
-        aq(DRAFT && qc > 0.0 && qs.sum > 0.0 ? qc / qs.sum : 0.0), pinf(ps.top == __builtin_inff()),
-        qinf(DRAFT && qs.top == __builtin_inff()), gone(nullptr), count(0) {}
-  // Of the 16 bytes of elements from `first` on; 0 where there are none.
-  template <class T, int E>
-  __device__ __forceinline__ void of(const Piece<T>& lp, const Piece<T>& lq, int first, int V, double (&r)[E]) const {
+      : p(table, c, ps.top), q(table, c, qs.top), ap(ps.sum > 0.0 ? pa / ps.sum : 0.0),
+        aq(DRAFT && qc > 0.0 && qs.sum > 0.0 ? qc / qs.sum : 0.0) {}
+  __device__ __forceinline__ double operator()(float lp, float lq) const {
+    double r = fma(ap, p(lp), -kNothing);
+    if constexpr (DRAFT) r = fma(-aq, q(lq), r);
+    return fmax(r, 0.0);
+  }
+  // The mass of a chunk, by a wave.
+  template <class T, int U>
+  __device__ __forceinline__ double chunk_mass(const T* prow, const T* qrow, int chunk, int shift, int V,
+                                               int lane) const {
+    constexpr int E = 16 / sizeof(T);
+    const int first = (chunk * U * 64 + lane) * E - shift;
+    Piece<T> x[U], y[U];
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      r[e] = 0.0;
-      if (ap > 0.0) r[e] = ap * (pinf ? (lp[e] == __builtin_inff() ? 1.0 : 0.0) : p(lp[e]));
-      if constexpr (DRAFT) {
-        if (aq > 0.0) r[e] -= aq * (qinf ? (lq[e] == __builtin_inff() ? 1.0 : 0.0) : q(lq[e]));
-        r[e] = fmax(r[e], 0.0);
-      }
+    for (int u = 0; u < U; ++u) {
+      x[u].load(prow, first + u * 64 * E, V);
+      if constexpr (DRAFT) y[u].load(qrow, first + u * 64 * E, V);
     }
-    if constexpr (!DRAFT) {
-      for (int k = 0; k < count; ++k) {
-        const int64_t t = gone[k];
-        if (!__any(t >= first && t < first + E)) continue;
+    double sum = 0.0;
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-          r[e] = t == Piece<T>::index(first, e, V) ? 0.0 : r[e];
-      }
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) sum += (*this)(x[u][e], DRAFT ? y[u][e] : 0.f);
+      __builtin_amdgcn_sched_barrier(0);
     }
+    return wave_sum(sum);
   }
 };
 
@@ -347,7 +396,7 @@ struct Asked {
   double pa = 1.0, qc = 0.0, Z = 1.0;  // r = max(pa p - qc q, 0), and its sum
   int kept = -1, rejections = 0;
   bool fresh = false;  // the masses of the last rejection are those of r
-  // masses_of(k, pa, qc): the sum of r's masses after rejection k; stop(k): end there
+  // sum_of(k, pa, qc): the sum of r's masses after rejection k; stop(k): end there (false)
   template <class Sum, class Stop>
   __device__ __forceinline__ bool run(uint64_t kids, double p, double q, double u, const Sum& sum_of, const Stop& stop) {
     for (; kids; kids &= kids - 1) {
@@ -399,40 +448,18 @@ __device__ __forceinline__ double* masses_of(const VerifyArgs& a, int round, int
 
 }  // namespace
 
-// The sums of all rows of a sequence, by a workgroup of NT: 2^k lanes a row, as many
-// rows at a time as it has. `parent`: of the lane's draft.
-template <bool DRAFT, int NT>
-__device__ __forceinline__ void row_sums(const VerifyArgs& a, int b, int nb, int parent, const double* table,
-                                         RowSum (&rows)[2][64]) {
-  int per = 1;
-  while (per < a.chunks && per < 64) per *= 2;
-  const int sub = threadIdx.x & (per - 1);
-  uint64_t inner = 0;  // tokens with drafts
-  if constexpr (DRAFT)
-    for (int i = 0; i < nb; ++i)
-      if (__any(parent == i)) inner |= (uint64_t)1 << i;
-  for (int r0 = 0; r0 < (DRAFT ? 2 * nb : nb); r0 += NT / per) {
-    const int r = r0 + threadIdx.x / per, kind = r >= nb, i = r - kind * nb;
-    const bool real = r < (DRAFT ? 2 * nb : nb) && (!kind || (inner >> i & 1));
-    const RowSum x = row_sum(stats_of(a, kind, b, real ? i : 0), a.chunks, real, sub, per, table, a.c);
-    if (real && sub == 0) rows[kind][i] = x;
-  }
-  __syncthreads();
-}
-
-// What r has in one chunk after rejection number `round` behind a token, if there
-// are as many and no draft is kept before. In a chain the token is the one at whose
-// draft it ends, known to a workgroup after the sums of all rows; in a tree it is any
-// that has drafts (its place on the path is not asked for): there every wave decides
-// by itself, and most workgroups end after three round trips to memory.
+// What r has in a chunk (one a wave) after rejection number `round` behind a token, if
+// there are as many and no draft is kept before. In a chain the token is the one at
+// whose draft it ends, known to a workgroup after the sums of all rows; in a tree it is
+// any that has drafts (its place on the path is not asked for): there every wave decides
+// by itself, and most end after three round trips to memory.
 template <class T, int U, bool CHAIN>
-__global__ __launch_bounds__(256) void verify_mass_kernel(VerifyArgs a, int round) {
-  constexpr int E = 16 / sizeof(T);
-  __shared__ double table[32], sums[4];
+__global__ __launch_bounds__(256) void verify_mass_kernel(VerifyArgs a, int round, int groups) {
+  __shared__ uint64_t table[64];
   __shared__ RowSum rows[2][64];
-  const int chunk = blockIdx.x % a.chunks, k = blockIdx.x / a.chunks, b = CHAIN ? k : k / (a.n - 1);
-  int node = CHAIN ? 0 : k % (a.n - 1);
-  const int lane = threadIdx.x & 63, nb = tokens_of(a, b);
+  const int lane = threadIdx.x & 63, k = blockIdx.x / groups, b = CHAIN ? k : k / (a.n - 1);
+  const int chunk = 4 * (blockIdx.x - k * groups) + (threadIdx.x >> 6), nb = tokens_of(a, b);
+  int node = CHAIN ? 0 : k - b * (a.n - 1);
   if (nb < 2) return;
   const Draft d(a, b, nb, lane);
   if (!CHAIN && __builtin_popcountll(__ballot(d.parent == node)) <= round) return;
@@ -441,7 +468,7 @@ __global__ __launch_bounds__(256) void verify_mass_kernel(VerifyArgs a, int roun
     lp = value_of(row_of<T>(a.p, b, d.parent)[d.token]);
     lq = value_of(row_of<T>(a.q, b, d.parent)[d.token]);
   }
-  if (threadIdx.x < 32) table[threadIdx.x] = kExp2Table[threadIdx.x];
+  if (threadIdx.x < 64) table[threadIdx.x] = kExp2Table[threadIdx.x];
   __syncthreads();
   RowSum ps, qs;
   if constexpr (CHAIN) {
@@ -452,8 +479,8 @@ __global__ __launch_bounds__(256) void verify_mass_kernel(VerifyArgs a, int roun
     ps = row_sum(stats_of(a, false, b, node), a.chunks, true, lane, 64, table, a.c);
     qs = row_sum(stats_of(a, true, b, node), a.chunks, true, lane, 64, table, a.c);
   }
-  const double p = ps.sum > 0.0 ? weight_below(table, a.c, lp, ps.top) / ps.sum : 0.0;
-  const double q = qs.sum > 0.0 ? weight_below(table, a.c, lq, qs.top) / qs.sum : 0.0;
+  if (chunk >= a.chunks) return;
+  const double p = chance(table, a.c, lp, ps), q = chance(table, a.c, lq, qs);
   double pa = 1.0, qc = 1.0;  // after the first rejection
   if constexpr (CHAIN) {
     const uint64_t ends = __ballot(d.parent >= 0 && !(d.u * q < p));
@@ -470,42 +497,21 @@ __global__ __launch_bounds__(256) void verify_mass_kernel(VerifyArgs a, int roun
     pa = asked.pa;
     qc = asked.qc;
   }
-  const Rest<true> rest(table, a.c, ps, qs, pa, qc);
-  const T *prow = row_of<T>(a.p, b, node), *qrow = row_of<T>(a.q, b, node);
-  const int first = (chunk * U * 256 + (int)threadIdx.x) * E - shift_of(prow);
-  double sum = 0.0;
-  Piece<T> x, y;
-  x.load(prow, first, a.V);
-  y.load(qrow, first, a.V);
-#pragma unroll 1
-  for (int u = 0; u < U; ++u) {
-    const Piece<T> lp0 = x, lq0 = y;
-    if (u + 1 < U) {
-      x.load(prow, first + (u + 1) * 256 * E, a.V);
-      y.load(qrow, first + (u + 1) * 256 * E, a.V);
-    }
-    double r[E];
-    rest.of(lp0, lq0, first + u * 256 * E, a.V, r);
-#pragma unroll
-    for (int e = 0; e < E; ++e) sum += r[e];
-  }
-  sum = wave_sum(sum);
-  if (lane == 0) sums[threadIdx.x >> 6] = sum;
-  __syncthreads();
-  if (threadIdx.x == 0) masses_of(a, round, b, node)[chunk] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+  const T* prow = row_of<T>(a.p, b, node);
+  const double m = Rest<true>(table, a.c, ps, qs, pa, qc)
+                       .template chunk_mass<T, U>(prow, row_of<T>(a.q, b, node), chunk, shift_of(prow), a.V, lane);
+  if (lane == 0) masses_of(a, round, b, node)[chunk] = m;
 }
 
 // The decisions of a sequence from the root on, and its next token.
 template <class T, bool BEST, bool DRAFT, int U>
 __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(VerifyArgs a) {
   constexpr int E = 16 / sizeof(T), NT = kVerifyThreads, NW = NT / 64;
-  __shared__ double table[32], part[NW], masses[kVerifyMaxChunks];
+  __shared__ uint64_t table[64];
+  __shared__ double part[NW], masses[kVerifyMaxChunks];
   __shared__ RowSum rows[2][64];
-  __shared__ int best[64];
-  __shared__ int64_t gone_tokens[64];
-  __shared__ int found, last[NW], chosen;
-  __shared__ double chosen_before;
-  const int b = blockIdx.x, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  __shared__ int best[64], found, last[NW];
+  const int b = blockIdx.x, lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int nb = tokens_of(a, b);
   int32_t* keep = a.keep + (int64_t)b * a.n;
   if (nb == 0) {
@@ -524,10 +530,10 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(VerifyArgs a) {
       lp = value_of(row_of<T>(a.p, b, d.parent)[d.token]);
       if constexpr (DRAFT) lq = value_of(row_of<T>(a.q, b, d.parent)[d.token]);
     }
-    if (threadIdx.x < 32) table[threadIdx.x] = kExp2Table[threadIdx.x];
+    if (threadIdx.x < 64) table[threadIdx.x] = kExp2Table[threadIdx.x];
     __syncthreads();
-  }
-  if constexpr (BEST) {
+    row_sums<DRAFT, NT>(a, b, nb, d.parent, table, rows);
+  } else {
     int per = 1;
     while (per < a.chunks && per < 64) per *= 2;
     const int sub = threadIdx.x & (per - 1);
@@ -536,22 +542,20 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(VerifyArgs a) {
       const VerifyStat* st = stats_of(a, false, b, min(r, nb - 1));
       float top = kNegInf;
       int at = INT_MAX;
-      for (int c = sub; c < a.chunks; c += per)
-        if (st[c].top > top) {
-          top = st[c].top;
-          at = st[c].best;
-        }
+      for (int c = sub; c < a.chunks; c += per) {
+        const VerifyStat x = st[c];
+        at = x.top > top ? x.best : at;
+        top = fmaxf(top, x.top);
+      }
       for (int o = 1; o < per; o <<= 1) {
         const float x = __shfl_xor(top, o);
         const int other = __shfl_xor(at, o);
-        if (x > top || (x == top && other < at)) at = other;
+        at = x > top || (x == top && other < at) ? other : at;
         top = fmaxf(top, x);
       }
       if (r < nb && sub == 0) best[r] = top > kNegInf ? at : -1;
     }
     __syncthreads();
-  } else {
-    row_sums<DRAFT, NT>(a, b, nb, d.parent, table, rows);
   }
 
   int node = 0;
@@ -575,54 +579,9 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(VerifyArgs a) {
     if (threadIdx.x == 0) a.token[b] = best[node];
     return;
   }
-  double p = 0.0, q = 0.0;
-  if (d.known(a)) {
-    const RowSum ps = rows[0][d.parent];
-    p = ps.sum > 0.0 ? weight_below(table, a.c, lp, ps.top) / ps.sum : 0.0;
-    if constexpr (DRAFT) {
-      const RowSum qs = rows[1][d.parent];
-      q = qs.sum > 0.0 ? weight_below(table, a.c, lq, qs.top) / qs.sum : 0.0;
-    }
-  }
-  // sum of one number a lane over the workgroup
-  auto group_sum = [&](double x) {
-    x = wave_sum(x);
-    __syncthreads();
-    if (lane == 0) part[w] = x;
-    __syncthreads();
-    double sum = 0.0;
-#pragma unroll
-    for (int k = 0; k < NW; ++k) sum += part[k];
-    return sum;
-  };
-  // lane's share of a chunk: a run of pieces of 16 bytes, so that lanes are in the
-  // tokens' order
-  constexpr int RUN = (256 * U + NT - 1) / NT;
-  auto chunk_first = [&](int chunk, int shift) { return (chunk * 256 * U + (int)threadIdx.x * RUN) * E - shift; };
-  const bool has_share = (int)threadIdx.x * RUN < 256 * U;
-  auto rest_of = [&](const Rest<DRAFT>& rest, const T* prow, const T* qrow, int first, double (&r)[E]) {
-    Piece<T> x, y;
-    x.load(prow, first, a.V);
-    if (DRAFT && rest.aq > 0.0)
-      y.load(qrow, first, a.V);
-    else
-      y = x;
-    rest.of(x, y, first, a.V, r);
-  };
-  auto chunk_mass = [&](const Rest<DRAFT>& rest, const T* prow, const T* qrow, int chunk, int shift) {
-    double sum = 0.0;
-    if (has_share) {
-#pragma unroll
-      for (int u = 0; u < RUN; ++u) {
-        double r[E];
-        rest_of(rest, prow, qrow, chunk_first(chunk, shift) + u * E, r);
-#pragma unroll
-        for (int e = 0; e < E; ++e) sum += r[e];
-      }
-    }
-    return group_sum(sum);
-  };
-
+  const double u0 = (double)a.uniform[(int64_t)b * a.n];
+  const int mine = max(d.parent, 0);
+  const double p = chance(table, a.c, lp, rows[0][mine]), q = DRAFT ? chance(table, a.c, lq, rows[1][mine]) : 0.0;
   double pa = 1.0, qc = 0.0;
   uint64_t gone = 0;   // drafts that were turned down, where they were not drawn
   bool fresh = false;  // `masses` are r's
@@ -641,10 +600,9 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(VerifyArgs a) {
             } else {
               const T *prow = row_of<T>(a.p, b, node), *qrow = row_of<T>(a.q, b, node);
               const Rest<DRAFT> rest(table, a.c, rows[0][node], rows[1][node], apa, aqc);
-              const int shift = shift_of(prow);
-              for (int c = 0; c < a.chunks; ++c) {
-                const double m = chunk_mass(rest, prow, qrow, c, shift);
-                if (threadIdx.x == 0) masses[c] = m;
+              for (int c = w; c < a.chunks; c += NW) {
+                const double m = rest.template chunk_mass<T, U>(prow, qrow, c, shift_of(prow), a.V, lane);
+                if (lane == 0) masses[c] = m;
               }
             }
             __syncthreads();
@@ -676,126 +634,127 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(VerifyArgs a) {
   }
   write_path();
 
-  // r's masses where the last event was no rejection with any left: the chunks'
-  // own, without what was turned down
+  // The next token: the first whose running sum of r passes u Z; where rounding leaves
+  // none, the last one of the chunk that has a mass.
   const T* prow = row_of<T>(a.p, b, node);
   const T* qrow = DRAFT && qc > 0.0 ? row_of<T>(a.q, b, node) : prow;
   const int shift = shift_of(prow);
-  RowSum ps = rows[0][node], qs{0.f, 0.0};
-  if (DRAFT && qc > 0.0) qs = rows[1][node];
-  Rest<DRAFT> rest(table, a.c, ps, qs, pa, qc);
-  double Z = 0.0;
-  if (!(DRAFT && fresh)) {
-    auto own_masses = [&]() {
-      __syncthreads();
-      const VerifyStat* st = stats_of(a, false, b, node);
-      for (int c = threadIdx.x; c < a.chunks; c += NT)
-        masses[c] = st[c].sum > 0.0 ? rest.ap * (st[c].sum * weight_below(table, a.c, st[c].top, ps.top)) : 0.0;
-      __syncthreads();
-    };
-    own_masses();
-    if constexpr (!DRAFT) {
-      if (gone) {
-        if (threadIdx.x < 64 && (gone >> lane & 1))
-          gone_tokens[__builtin_popcountll(gone & (((uint64_t)1 << lane) - 1))] = d.token;
-        __syncthreads();
-        rest.gone = gone_tokens;
-        rest.count = __builtin_popcountll(gone);
-        for (int k = 0; k < rest.count; ++k) {
-          const int64_t t = gone_tokens[k];
-          if (t < 0 || t >= a.V) continue;
-          const int c = (int)((t + shift) / a.chunk);
-          const double m = chunk_mass(rest, prow, prow, c, shift);
-          if (threadIdx.x == 0) masses[c] = m;
-        }
-        __syncthreads();
-        if (mass_sum(masses, a.chunks, lane) == 0.0) {  // nothing is left
-          rest.count = 0;
-          own_masses();
-        }
+  const RowSum ps = rows[0][node], qs = DRAFT && qc > 0.0 ? rows[1][node] : ps;
+  const Rest<DRAFT> rest(table, a.c, ps, qs, pa, qc);
+  // where the last event was no rejection with any left: the chunks' own masses,
+  // without what was turned down
+  auto own_masses = [&]() {
+    __syncthreads();
+    const VerifyStat* st = stats_of(a, false, b, node);
+    for (int c = threadIdx.x; c < a.chunks; c += NT) {
+      const VerifyStat x = st[c];
+      double m = rest.ap * (x.sum * weight_below(table, a.c, x.top, ps.top));
+      uint64_t seen = 0;
+      for (uint64_t left = gone; left; left &= left - 1) {
+        const int i = __builtin_ctzll(left);
+        const int64_t t = a.tokens[(int64_t)b * a.n + i];
+        if (t < 0 || t >= a.V || (int)((t + shift) / a.chunk) != c) continue;
+        bool again = false;
+        for (uint64_t other = seen; other; other &= other - 1)
+          again |= a.tokens[(int64_t)b * a.n + __builtin_ctzll(other)] == t;
+        if (!again) m -= chance(table, a.c, value_of(prow[t]), ps);
+        seen |= (uint64_t)1 << i;
       }
-    }
-  }
-  Z = mass_sum(masses, a.chunks, lane);
-  if (!(Z > 0.0)) {
-    if (threadIdx.x == 0) a.token[b] = -1;
-    return;
-  }
-  // The first token whose running sum passes u Z: its chunk, then within it. Where
-  // rounding leaves none behind a border, the last one that has a mass.
-  const double want = (double)a.uniform[(int64_t)b * a.n] * Z;
-  // Of the lanes' sums in order: whether this lane's end is the first past `want`,
-  // or it is the last with a mass if none is; before: the sum before the first
-  // lane's, then before this one's.
-  auto is_first_past = [&](double sum, double& before) {
-    double upto = sum;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const double x = __shfl_up(upto, o);
-      if (lane >= o) upto += x;
+      masses[c] = fmax(m, 0.0);
     }
     __syncthreads();
-    if (lane == 63) part[w] = upto;
+  };
+  if (!(DRAFT && fresh)) own_masses();
+  for (;;) {
+    // the chunk, by every wave: a run of them a lane
+    const int run = (a.chunks + 63) / 64, c0 = lane * run, c1 = min(c0 + run, a.chunks);
+    double sum = 0.0;
+    for (int c = c0; c < c1; ++c) sum += masses[c];
+    const double upto = wave_upto(sum, lane), Z = __shfl(upto, 63), want = u0 * Z;
+    const uint64_t some = __ballot(sum > 0.0), past = __ballot(sum > 0.0 && upto > want);
+    if (!some) {
+      if (gone) {  // nothing is left: the token's own distribution in its place
+        gone = 0;
+        own_masses();
+        continue;
+      }
+      if (threadIdx.x == 0) a.token[b] = -1;
+      return;
+    }
+    const int at = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some);
+    int chunk = 0;
+    double before = upto - sum, chunk_before = 0.0;
+    for (int c = c0; c < c1; ++c) {
+      const double m = masses[c];
+      if (m > 0.0) {
+        chunk = c;
+        chunk_before = before;
+        if (before + m > want) break;
+      }
+      before += m;
+    }
+    chunk = __shfl(chunk, at);
+    chunk_before = __shfl(chunk_before, at);
+    // within it: Q tokens a lane
+    constexpr int CHUNK = 64 * U * E, Q = CHUNK > NT ? CHUNK / NT : 1;
+    double r[Q];
+    sum = 0.0;
+    const int x0 = chunk * CHUNK - shift + (int)threadIdx.x * Q;
+#pragma unroll
+    for (int e = 0; e < Q; ++e) {
+      const int x = x0 + e;
+      r[e] = 0.0;
+      if ((int)threadIdx.x * Q + e < CHUNK && x >= 0 && x < a.V)
+        r[e] = rest(value_of(prow[x]), DRAFT ? value_of(qrow[x]) : 0.f);
+    }
+    if constexpr (!DRAFT) {
+      for (uint64_t left = gone; left; left &= left - 1) {
+        const int64_t t = __shfl(d.token, __builtin_ctzll(left));
+#pragma unroll
+        for (int e = 0; e < Q; ++e) r[e] = t == x0 + e ? 0.0 : r[e];
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < Q; ++e) sum += r[e];
+    const double here = wave_upto(sum, lane);
+    if (lane == 63) part[w] = here;
     if (threadIdx.x == 0) found = INT_MAX;
     __syncthreads();
-    for (int k = 0; k < w; ++k) before += part[k];
-    const uint64_t past = __ballot(sum > 0.0 && before + upto > want), some = __ballot(sum > 0.0);
-    before += upto - sum;
+    before = chunk_before;
+#pragma unroll
+    for (int k = 0; k < NW; ++k) before += k < w ? part[k] : 0.0;
+    const uint64_t in_past = __ballot(sum > 0.0 && before + here > want), in_some = __ballot(sum > 0.0);
     if (lane == 0) {
-      last[w] = some ? 64 * w + 63 - __builtin_clzll(some) : -1;
-      if (past) atomicMin(&found, 64 * w + __builtin_ctzll(past));
+      last[w] = in_some ? 64 * w + 63 - __builtin_clzll(in_some) : -1;
+      if (in_past) atomicMin(&found, 64 * w + __builtin_ctzll(in_past));
     }
     __syncthreads();
-    int at = found;
-    if (at == INT_MAX) {
-      at = last[0];
+    int pick_lane = found;
+    if (pick_lane == INT_MAX) {
+      pick_lane = -1;
 #pragma unroll
-      for (int k = 1; k < NW; ++k) at = max(at, last[k]);
+      for (int k = 0; k < NW; ++k) pick_lane = max(pick_lane, last[k]);
     }
-    return at == (int)threadIdx.x;
-  };
-  const int run = (a.chunks + NT - 1) / NT, c0 = threadIdx.x * run, c1 = min(c0 + run, a.chunks);
-  double sum = 0.0, before = 0.0;
-  for (int c = c0; c < c1; ++c) sum += masses[c];
-  if (is_first_past(sum, before)) {
-    int pick = 0;
-    double at = before, pick_at = before;
-    for (int c = c0; c < c1; ++c) {
-      if (masses[c] > 0.0) {
-        pick = c;
-        pick_at = at;
-        if (at + masses[c] > want) break;
+    if (pick_lane < 0) {
+      // rounding had left it a mass, of which there is none
+      if (threadIdx.x == 0) masses[chunk] = 0.0;
+      __syncthreads();
+      continue;
+    }
+    if (pick_lane == (int)threadIdx.x) {
+      before += here - sum;
+      int pick = -1;
+      bool done = false;
+#pragma unroll
+      for (int e = 0; e < Q; ++e) {
+        const bool take = !done && r[e] > 0.0;
+        pick = take ? x0 + e : pick;
+        before += r[e];
+        done = done || (take && before > want);
       }
-      at += masses[c];
+      a.token[b] = pick;
     }
-    chosen = pick;
-    chosen_before = pick_at;
-  }
-  __syncthreads();
-  double r[RUN][E];
-  sum = 0.0;
-#pragma unroll
-  for (int u = 0; u < RUN; ++u) {
-    if (has_share) {
-      rest_of(rest, prow, qrow, chunk_first(chosen, shift) + u * E, r[u]);
-#pragma unroll
-      for (int e = 0; e < E; ++e) sum += r[u][e];
-    }
-  }
-  before = chosen_before;
-  if (is_first_past(sum, before)) {
-    int pick = -1;
-    bool done = false;
-#pragma unroll
-    for (int u = 0; u < RUN; ++u)
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (!done && r[u][e] > 0.0) {
-          pick = Piece<T>::index(chunk_first(chosen, shift) + u * E, e, a.V);
-          before += r[u][e];
-          done = before > want;
-        }
-    a.token[b] = pick;
+    return;
   }
 }
 
@@ -803,28 +762,30 @@ namespace {
 template <class T, int U>
 hipError_t launch_verify_u(const VerifyArgs& a, hipStream_t s) {
   const bool draft = a.q.data != nullptr;
-  const dim3 block(256), rows((unsigned)((int64_t)a.B * (draft ? 2 * a.n - 1 : a.n) * a.chunks));
+  const int64_t rows = (int64_t)a.B * (draft ? 2 * a.n - 1 : a.n);
+  const dim3 block(256), all((unsigned)((rows * a.chunks + 3) / 4));
   if (a.best)
-    MORPHO_KLAUNCH((verify_stats_kernel<T, U, true>), rows, block, 0, s, a);
+    MORPHO_KLAUNCH((verify_stats_kernel<T, U, true>), all, block, 0, s, a, (int)rows);
   else
-    MORPHO_KLAUNCH((verify_stats_kernel<T, U, false>), rows, block, 0, s, a);
+    MORPHO_KLAUNCH((verify_stats_kernel<T, U, false>), all, block, 0, s, a, (int)rows);
   hipError_t e = hipGetLastError();
+  const int groups = (a.chunks + 3) / 4;
   for (int k = 0; k < a.rounds && e == hipSuccess; ++k) {
     if (a.tree)
-      MORPHO_KLAUNCH((verify_mass_kernel<T, U, false>), dim3((unsigned)((int64_t)a.B * (a.n - 1) * a.chunks)), block, 0, s,
-                     a, k);
+      MORPHO_KLAUNCH((verify_mass_kernel<T, U, false>), dim3((unsigned)((int64_t)a.B * (a.n - 1) * groups)), block, 0, s, a,
+                     k, groups);
     else
-      MORPHO_KLAUNCH((verify_mass_kernel<T, U, true>), dim3((unsigned)((int64_t)a.B * a.chunks)), block, 0, s, a, k);
+      MORPHO_KLAUNCH((verify_mass_kernel<T, U, true>), dim3((unsigned)((int64_t)a.B * groups)), block, 0, s, a, k, groups);
     e = hipGetLastError();
   }
   if (e != hipSuccess) return e;
-  const dim3 grid((unsigned)a.B), all(kVerifyThreads);
+  const dim3 grid((unsigned)a.B), threads(kVerifyThreads);
   if (a.best)
-    MORPHO_KLAUNCH((verify_kernel<T, true, false, U>), grid, all, 0, s, a);
+    MORPHO_KLAUNCH((verify_kernel<T, true, false, U>), grid, threads, 0, s, a);
   else if (draft)
-    MORPHO_KLAUNCH((verify_kernel<T, false, true, U>), grid, all, 0, s, a);
+    MORPHO_KLAUNCH((verify_kernel<T, false, true, U>), grid, threads, 0, s, a);
   else
-    MORPHO_KLAUNCH((verify_kernel<T, false, false, U>), grid, all, 0, s, a);
+    MORPHO_KLAUNCH((verify_kernel<T, false, false, U>), grid, threads, 0, s, a);
   return hipGetLastError();
 }
 template <class T>

@@ -227,7 +227,7 @@ int main() {
         for (int kind = 0; kind < 8; ++kind) {
           const VerifyPlan p = verify_plan(rows, vocab, size, kind & 1, kind & 2, kind & 4);
           // a row that starts at the last element of 16 bytes has all its elements in the chunks
-          if ((p.pieces != 1 && p.pieces != 4) || p.chunk != 256 * 16 / size * p.pieces ||
+          if ((p.pieces != 1 && p.pieces != 4) || p.chunk != 64 * 16 / size * p.pieces ||
               (long long)p.chunks * p.chunk < vocab + 16 / size - 1 || p.chunks > kVerifyMaxChunks || p.rounds < 0 ||
               ((kind & 4) && p.rounds))
             printf("rows %lld vocab %d size %d: %d chunks of %d\n", rows, vocab, size, p.chunks, p.chunk);
