@@ -57,6 +57,7 @@ struct CacheAttnArgs {
 // Which sequences have their first pages in common (kernels_cache_shared.hip): those
 // keys are the prefix kernel's, in pieces that come before a row's others.
 struct CacheShared {
+  static constexpr bool kJoint = false;  // whether a launch does the prefixes too, by its first workgroups
   const int* group;  // [B] a sequence's group; none where it is not one of them
   const int* pages;  // [G] the pages that a group's sequences have in common
   int groups, np, split;  // groups; pieces of a prefix, keys of a piece
@@ -70,9 +71,12 @@ struct CacheShared {
     return keys <= ctx ? (int)keys : 0;
   }
   __device__ __forceinline__ int pieces_of(int keys) const { return min(np, (keys + split - 1) / split); }
+  __device__ __forceinline__ constexpr int first_block() const { return 0; }
 };
 // Nothing in common.
 struct CacheApart {
+  static constexpr bool kJoint = false;
+  __device__ __forceinline__ constexpr int first_block() const { return 0; }
   __device__ __forceinline__ constexpr int pieces() const { return 0; }
   __device__ __forceinline__ constexpr int skip(int, int, int) const { return 0; }
   __device__ __forceinline__ constexpr int pieces_of(int) const { return 0; }
@@ -546,10 +550,11 @@ __device__ __forceinline__ void settle_columns(const f16* v, int64_t stride, con
 // 1000 to 3000 62.6 -> 57.6; with many rounds it does not matter).
 struct CacheBlock {
   int b, h, sp, qb;
-  __device__ __forceinline__ explicit CacheBlock(const CacheAttnArgs& a) {
-    int id = blockIdx.x;
+  // first: the launch's first workgroup of these
+  __device__ __forceinline__ CacheBlock(const CacheAttnArgs& a, int first) {
+    int id = blockIdx.x - first;
     if (a.causal && a.qblocks > 1 && (id & 256)) {
-      const int round = id & ~255, whole = min(256, (int)gridDim.x - round) & ~7;
+      const int round = id & ~255, whole = min(256, (int)gridDim.x - first - round) & ~7;
       if (id - round < whole) id = round + (whole - 8 - ((id - round) & ~7)) + (id & 7);
     }
     h = id % a.H;
@@ -581,7 +586,9 @@ __global__ __launch_bounds__(256) void cache_attn_few_kernel(
   constexpr int NT = DV / 16;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c16 = lane & 15, g = lane >> 4;
-  const CacheBlock blk(a);
+  if constexpr (Shared::kJoint)
+    if (shared.template prefix<M, DV>(a, phi, gate_q, gate_k, codes, values, table, lens, new_lens, part_o, part_st)) return;
+  const CacheBlock blk(a, shared.first_block());
   const int b = blk.b, h = blk.h;
   const SeqLen sq = seq_len(lens, new_lens, b, a.n, a.W << a.lp);
   const int kb = shared.skip(b, sq.ctx, a.lp) + blk.sp * a.split_keys, parts = shared.pieces() + a.nsplit;
@@ -695,7 +702,10 @@ __global__ __launch_bounds__(256, M > 32 || DV > 64 ? 2 : LO || QT > 1 ? 3 : 4) 
   __shared__ __align__(1024) char lds[3][2 * NF * 1024];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c16 = lane & 15, g = lane >> 4;
-  const CacheBlock blk(a);
+  if constexpr (Shared::kJoint)
+    if (shared.template prefix<M, DV>(a, phi, gate_q, gate_k, codes, values, table, lens, new_lens, part_o, part_st, lds))
+      return;
+  const CacheBlock blk(a, shared.first_block());
   const int b = blk.b, h = blk.h, q0 = blk.qb * 64 * QT, qw = q0 + 16 * QT * w;
   const SeqLen sq = seq_len(lens, new_lens, b, a.n, a.W << a.lp);
   const int kb = shared.skip(b, sq.ctx, a.lp) + blk.sp * a.split_keys, parts = shared.pieces() + a.nsplit;

@@ -633,6 +633,34 @@ size_t cache_part_o_bytes(const CacheDims& d, const CacheAttnPlan& p) {
 size_t cache_attn_bytes(const CacheDims& d, const CacheAttnPlan& p) {
   return p.nsplit == 1 ? 0 : cache_part_o_bytes(d, p) + align_up((size_t)d.B * d.H * d.n * p.nsplit * 16);
 }
+// The launches of a call whose arguments are good.
+int run_cache_attention(const CacheDims& d, const CacheAttnPlan& plan, const void* phi, const void* gate_q,
+                        const void* gate_k, const morpho_cache* cache, const int32_t* table, const int32_t* lens,
+                        const int32_t* new_lens, const int64_t* tree, void* out, float* lse, float scale, int mode,
+                        void* workspace, size_t workspace_bytes, morpho_stream_t stream) {
+  const size_t need = cache_attn_bytes(d, plan);
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(MORPHO_ERR_WORKSPACE, "cache attention workspace needs %zu bytes (got %zu)", need, workspace_bytes);
+  if (need && (reinterpret_cast<uintptr_t>(workspace) & 255) != 0)
+    return fail(MORPHO_ERR_WORKSPACE, "workspace must be 256-byte aligned");
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  CacheAttnBuffers part{nullptr, nullptr};
+  if (need) {
+    part.o = static_cast<float*>(workspace);
+    part.st = reinterpret_cast<float4*>(static_cast<char*>(workspace) + cache_part_o_bytes(d, plan));
+  }
+  auto* o = static_cast<_Float16*>(out);
+  MORPHO_LAUNCH("cache_attn",
+                launch_cache_attn(d, plan, static_cast<const _Float16*>(phi), static_cast<const _Float16*>(gate_q),
+                                  static_cast<const _Float16*>(gate_k), static_cast<const _Float16*>(cache->codes),
+                                  static_cast<const _Float16*>(cache->values), table, lens, new_lens, tree, o, lse,
+                                  part, scale, mode & MORPHO_MODE_CAUSAL, mode & MORPHO_MODE_MASK_DIAG, s));
+  if (need)
+    MORPHO_LAUNCH("cache_join",
+                  launch_cache_attn_join(d, plan, static_cast<const _Float16*>(cache->values), table, lens, new_lens,
+                                         tree, part, o, lse, mode & MORPHO_MODE_CAUSAL, mode & MORPHO_MODE_MASK_DIAG, s));
+  return MORPHO_OK;
+}
 }  // namespace
 
 MORPHO_EXPORT int morpho_cache_append(const void* X, const void* W, const morpho_cache* cache, const int32_t* table,
@@ -696,28 +724,8 @@ MORPHO_EXPORT int morpho_cache_attention(const void* phi, const void* gate_q, co
   const CacheAttnPlan plan = cache_plan(d, max_len);
   if ((int64_t)d.B * d.H * plan.qblocks * plan.nsplit > (1 << 23))
     return fail(MORPHO_ERR_INVALID_ARGUMENT, "problem too large: B*H*pieces must be at most 2^23");
-  const size_t need = cache_attn_bytes(d, plan);
-  if (need && (!workspace || workspace_bytes < need))
-    return fail(MORPHO_ERR_WORKSPACE, "cache attention workspace needs %zu bytes (got %zu)", need, workspace_bytes);
-  if (need && (reinterpret_cast<uintptr_t>(workspace) & 255) != 0)
-    return fail(MORPHO_ERR_WORKSPACE, "workspace must be 256-byte aligned");
-  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  CacheAttnBuffers part{nullptr, nullptr};
-  if (need) {
-    part.o = static_cast<float*>(workspace);
-    part.st = reinterpret_cast<float4*>(static_cast<char*>(workspace) + cache_part_o_bytes(d, plan));
-  }
-  auto* o = static_cast<_Float16*>(out);
-  MORPHO_LAUNCH("cache_attn",
-                launch_cache_attn(d, plan, static_cast<const _Float16*>(phi), static_cast<const _Float16*>(gate_q),
-                                  static_cast<const _Float16*>(gate_k), static_cast<const _Float16*>(cache->codes),
-                                  static_cast<const _Float16*>(cache->values), table, lens, new_lens, tree, o, lse,
-                                  part, scale, mode & MORPHO_MODE_CAUSAL, mode & MORPHO_MODE_MASK_DIAG, s));
-  if (need)
-    MORPHO_LAUNCH("cache_join",
-                  launch_cache_attn_join(d, plan, static_cast<const _Float16*>(cache->values), table, lens, new_lens,
-                                         tree, part, o, lse, mode & MORPHO_MODE_CAUSAL, mode & MORPHO_MODE_MASK_DIAG, s));
-  return MORPHO_OK;
+  return run_cache_attention(d, plan, phi, gate_q, gate_k, cache, table, lens, new_lens, tree, out, lse, scale, mode,
+                             workspace, workspace_bytes, stream);
 }
 
 namespace {
@@ -734,7 +742,8 @@ int make_shared_plan(const morpho_cache* cache, int64_t B, int64_t n, int64_t se
   const int64_t cap = (int64_t)d.W * d.P;
   p = cache_shared_plan(d.B, d.H, d.n, (int)members, (int)groups, max_prefix < cap ? max_prefix : cap,
                         max_rest < cap ? max_rest : cap, d.M, d.DV);
-  if ((int64_t)d.B * d.H * p.rest.qblocks * p.rest.nsplit > (1 << 23) || (int64_t)d.H * p.rblocks * p.np > (1 << 23))
+  if ((int64_t)d.B * d.H * p.rest.qblocks * p.rest.nsplit > (1 << 23) ||
+      (!p.apart && (int64_t)d.H * p.rblocks * p.np > (1 << 22)))
     return fail(MORPHO_ERR_INVALID_ARGUMENT, "problem too large: B*H*pieces must be at most 2^23");
   return MORPHO_OK;
 }
@@ -742,6 +751,7 @@ size_t shared_part_o_bytes(const CacheDims& d, const CacheSharedPlan& p) {
   return align_up((size_t)d.B * d.H * d.n * (p.np + p.rest.nsplit) * d.DV * 4);
 }
 size_t shared_bytes(const CacheDims& d, const CacheSharedPlan& p) {
+  if (p.apart) return cache_attn_bytes(d, p.rest);
   return shared_part_o_bytes(d, p) + align_up((size_t)d.B * d.H * d.n * (p.np + p.rest.nsplit) * 16);
 }
 }  // namespace
@@ -785,10 +795,12 @@ MORPHO_EXPORT int morpho_cache_shared_attention(const void* phi, const void* gat
       misaligned_ints(shared->members, shared->starts, shared->group, shared->pages) ||
       (reinterpret_cast<uintptr_t>(tree) & 7) != 0)
     return fail(MORPHO_ERR_INVALID_ARGUMENT, "int32 pointers must be 4-byte aligned, tree 8-byte");
+  if (plan.apart)
+    return run_cache_attention(d, plan.rest, phi, gate_q, gate_k, cache, table, lens, new_lens, tree, out, lse, scale, mode,
+                               workspace, workspace_bytes, stream);
   const size_t need = shared_bytes(d, plan);
   if (!workspace || workspace_bytes < need)
-    return fail(MORPHO_ERR_WORKSPACE, "shared cache attention workspace needs %zu bytes (got %zu)", need,
-                workspace_bytes);
+    return fail(MORPHO_ERR_WORKSPACE, "cache attention workspace needs %zu bytes (got %zu)", need, workspace_bytes);
   if ((reinterpret_cast<uintptr_t>(workspace) & 255) != 0)
     return fail(MORPHO_ERR_WORKSPACE, "workspace must be 256-byte aligned");
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
@@ -918,7 +930,7 @@ int make_verify_plan(int64_t B, int64_t n, int64_t vocab, int type, bool draft, 
   if (B > (1 << 22)) return fail(MORPHO_ERR_INVALID_ARGUMENT, "problem too large: needs B*(2n-1)*chunks <= 2^23");
   const bool best = temperature == 0.0;
   const int64_t rows = B * (draft && !best ? 2 * n - 1 : n);
-  p = verify_plan(rows, (int)vocab, type == MORPHO_FLOAT32 ? 4 : 2, tree, draft && !best, best);
+  p = verify_plan(rows, (int)n, (int)vocab, type == MORPHO_FLOAT32 ? 4 : 2, tree, draft && !best, best);
   if (rows * p.chunks > (1 << 23))
     return fail(MORPHO_ERR_INVALID_ARGUMENT, "problem too large: needs B*(2n-1)*chunks <= 2^23");
   return MORPHO_OK;

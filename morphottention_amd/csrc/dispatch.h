@@ -409,9 +409,11 @@ inline int cache_compact_heads(int64_t sequences, int H, int DV, int K) {
 }
 
 // Launch shape of the attention where sequences have their first pages in
-// common: np pieces of split_keys common keys for row blocks of 16 qt rows (of
-// one group), and the sequences' own keys as without (rest).
+// common: np pieces of split_keys common keys for row blocks of one group, 16 qt rows
+// that four waves share, or (qt = 0) 64 through LDS; and the sequences' own keys as
+// without (rest). apart: as without throughout.
 struct CacheSharedPlan {
+  bool apart;
   int qt, rblocks, np, split_keys;
   CacheAttnPlan rest;
 };
@@ -420,18 +422,45 @@ struct CacheSharedPlan {
 inline CacheSharedPlan cache_shared_plan(int B, int H, int n, int members, int groups, int64_t max_prefix,
                                          int64_t max_rest, int M, int DV) {
   CacheSharedPlan p;
-  p.rest = cache_attn_plan(B, H, n, max_rest, M, DV);
-  p.qt = 1;
+  // What sharing spares has to be worth a second kernel: us through the Python
+  // functions apart and shared, with what is spared: B16 n1 1024 common tokens (39 MB)
+  // 10.8, 11.9, 2048 (79) 15.9, 11.9; B64 512 (83) 12.0, 12.5, 1024 (165) 16.1, 13.5; B2
+  // 32768 m32 (101) 35, 22; trees of 48, H32 m64: B8 1024 (59) 23.5, 26, 4096 (235) 63,
+  // 46; B16 n20 1024 (39) 17.4, 16.8; all H16 m16 dv64 unless said.
+  p.apart = (int64_t)(members - groups) * max_prefix * H * (M + DV) * 2 < (int64_t)64 << 20;
+  const int64_t rows = (int64_t)members * n, mean = (rows + groups - 1) / groups;
+  // 32 rows a wave where there are many read the keys half as often from L2, with half
+  // the workgroups: B64 n1 (64 rows) 16 rows 19.5, 32 18.5, n16 45, 37; B32 n1 39, 43; 64
+  // rows a wave (registers for two waves a SIMD, which the rest's workgroups then have
+  // too): B64 n1 24, n4 36 against 28; through LDS n4 40.
+  p.qt = n > 16 ? 0 : mean > 32 ? 2 : 1;
+  const int per = p.qt ? 16 * p.qt : 64;
   // every group's last block may be part of one
-  const int64_t rows = (int64_t)members * n;
-  p.rblocks = (int)(rows / (16 * p.qt) + groups);
-  int64_t keys = 512;
+  p.rblocks = (int)(rows / per + groups);
+  const int64_t blocks = (rows + per - 1) / per > groups ? (rows + per - 1) / per : groups;  // most likely
+  // Pieces: every one costs its rows a partial result, so few long ones: 256 workgroups
+  // from 512 keys on, 512 from 2048 on, up to 4096 (B64 8192 common tokens, 32 rows: of 512
+  // 21.0, 1024 18.5, 2048 22.6; B32 65536 m32: of 1024 46, 2048 42, 4096 39; B64 n8 4096: of
+  // 1024 31, 2048 27, 4096 29; B24 4096 m64: of 256 14.4, 512 13.5, 1024 15.1); through LDS 768
+  // from 384 on (trees of 48, 4096: B16 of 1024 65, 2048 61, 4096 89; B8 of 768 47, 3072 60).
+  const int64_t work = max_prefix * H * blocks;
+  int64_t keys;
+  if (p.qt) {
+    keys = work / 256 > 512 ? work / 256 : 512;
+    if (keys > 2048) keys = work / 512 > 2048 ? work / 512 : 2048;
+    if (keys > 4096) keys = 4096;
+  } else {
+    keys = work / 768 > 384 ? work / 768 : 384;
+  }
+  if (keys > max_prefix) keys = max_prefix;
   // partial rows (DV + 4 floats each) and workgroups stay below 2^20 or so
   const int64_t most = ((int64_t)1 << 20) / ((int64_t)B * H * n) > 1 ? ((int64_t)1 << 20) / ((int64_t)B * H * n) : 1;
   if (keys < (max_prefix + most - 1) / most) keys = (max_prefix + most - 1) / most;
   keys = (keys + 127) / 128 * 128;
   p.np = (int)((max_prefix + keys - 1) / keys);
   p.split_keys = (int)keys;
+  const int64_t longest = max_prefix + max_rest < (int64_t)1 << 30 ? max_prefix + max_rest : (int64_t)1 << 30;
+  p.rest = cache_attn_plan(B, H, n, p.apart ? longest : max_rest, M, DV);
   return p;
 }
 
@@ -441,14 +470,14 @@ struct VerifyPlan {
   int pieces, chunk, chunks, rounds;
 };
 constexpr int kVerifyMaxVocab = 4000000, kVerifyMaxChunks = 4096;
-inline VerifyPlan verify_plan(int64_t rows, int vocab, int element_bytes, bool tree, bool draft, bool best) {
+inline VerifyPlan verify_plan(int64_t rows, int n, int vocab, int element_bytes, bool tree, bool draft, bool best) {
   VerifyPlan p;
   const int per = 16 / element_bytes;
   auto chunks = [&](int pieces) { return (vocab + per - 1 + 64 * per * pieces - 1) / (64 * per * pieces); };
   p.pieces = rows * chunks(4) < 4096 && chunks(1) <= 256 ? 1 : 4;
   p.chunk = 64 * per * p.pieces;
   p.chunks = chunks(p.pieces);
-  p.rounds = best || !draft || p.chunks == 1 ? 0 : tree ? 3 : 1;
+  p.rounds = best || !draft || p.chunks == 1 ? 0 : !tree ? 1 : n <= 6 ? n - 1 : 6;
   return p;
 }
 

@@ -38,6 +38,16 @@ class Shared(Problem):
     def shared(self, **kw):
         return ma.SharedPrefix.of(self.groups, self.common, self.B, device=DEV, **kw)
 
+    def device(self):
+        """With a table so wide that sharing is worth it as far as the host knows (64 MB
+        less to read): otherwise the sequences are computed apart."""
+        d = super().device()
+        spared = max(1, sum(map(len, self.groups)) - len(self.groups)) * self.P * self.H * (self.m + self.dv) * 2
+        wide = torch.full((self.B, -(-(64 << 20) // spared)), -1, dtype=torch.int32, device=DEV)
+        wide[:, : self.table.shape[1]] = d["table"]
+        d["table"] = wide
+        return d
+
 
 def _case(n, H=2, m=16, dv=64, P=64, news=None, seed=0, **kw):
     """Two groups of different prefixes that stand apart in the batch, and one sequence of neither."""
@@ -50,7 +60,7 @@ def _case(n, H=2, m=16, dv=64, P=64, news=None, seed=0, **kw):
 @pytest.mark.parametrize("n", [1, 7, 20, 64])
 def test_shapes(m, dv, n):
     p = _case(n, 3, m, dv, news=[n, max(1, n - 3), 0, n, n, n // 2], seed=m + dv + n)
-    _check(p.attend(p.device(), shared=p.shared(max_prefix=320, max_rest=128 + n)), p.reference())
+    _check(p.attend(p.device(), shared=p.shared(max_rest=128 + n)), p.reference())
 
 
 @pytest.mark.parametrize("P", [32, 64, 128, 256])
@@ -85,11 +95,13 @@ def test_trees(n):
 @pytest.mark.parametrize("B,H,n,L,m,dv", [(3, 1, 1, 4096, 16, 64), (2, 2, 3, 2944, 32, 32), (4, 1, 20, 1536, 64, 128),
                                           (2, 2, 64, 1024, 16, 64), (40, 2, 1, 1088, 32, 64)])
 def test_divided_prefixes(B, H, n, L, m, dv):
-    """Prefixes of many pieces; the hints may be short or long without changing the result."""
+    """Prefixes of many pieces; the hints may be short or long without changing the result
+    (the last two: apart, and as long as the table)."""
     p = Shared(B, n, H, m, dv, [L + 7 * b for b in range(B)], [list(range(B))], [L // 64], seed=L)
     d, want = p.device(), p.reference()
-    for hints in ({}, {"max_prefix": L, "max_rest": 7 * B + n}, {"max_prefix": 64, "max_rest": 1},
-                  {"max_prefix": 40 * L, "max_rest": 40 * L}):
+    wide = d["table"].shape[1] * 64
+    for hints in ({}, {"max_prefix": wide, "max_rest": 7 * B + n}, {"max_prefix": wide - 64, "max_rest": 1},
+                  {"max_prefix": L, "max_rest": 7 * B + n}, {"max_prefix": 2 * wide, "max_rest": 2 * wide}):
         _check(p.attend(d, shared=p.shared(**hints)), want)
 
 
@@ -202,7 +214,7 @@ def test_a_captured_call_follows_groups_and_lengths():
             for k in ("codes", "values"):
                 d[k][: dq[k].shape[0]] = dq[k]
             wide[:] = -1
-            wide[:, : dq["table"].shape[1]] = dq["table"]
+            wide[:, : q.table.shape[1]] = dq["table"][:, : q.table.shape[1]]
             d["table"].copy_(wide)
             for k in ("phi", "gq", "gk", "lens"):
                 d[k].copy_(dq[k])

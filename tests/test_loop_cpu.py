@@ -91,6 +91,9 @@ def _verify(p=P, q=None, type=0, tokens=P, uniform=P, tree=None, new_lens=None, 
                                            ws, ws_bytes, None)
 
 
+LONG = {"max_prefix": 1 << 20, "seq_pages": 1 << 15}  # enough in common to be worth it
+
+
 @pytest.mark.parametrize("call,kw,status,text", [
     (_shared, {"none": True}, INVALID, b"Null"), (_shared, {"pool": _pool(cube_m=24)}, UNSUPPORTED, b"cube_m"),
     (_shared, {"pool": _pool(layers=2)}, INVALID, b"one layer"), (_shared, {"pool": _pool(codes=P + 4)}, INVALID, b"16-byte"),
@@ -104,8 +107,8 @@ def _verify(p=P, q=None, type=0, tokens=P, uniform=P, tree=None, new_lens=None, 
     (_shared, {"phi": None}, INVALID, b"Null"), (_shared, {"lse": None}, INVALID, b"Null"),
     (_shared, {"group": P + 2}, INVALID, b"4-byte"), (_shared, {"starts": P + 1}, INVALID, b"4-byte"),
     (_shared, {"tree": P + 4}, INVALID, b"8-byte"), (_shared, {"out": P + 8}, INVALID, b"16-byte"),
-    (_shared, {"ws": None}, WORKSPACE, b"needs"), (_shared, {"ws_bytes": 64}, WORKSPACE, b"needs"),
-    (_shared, {"ws": P + 16}, WORKSPACE, b"256-byte"), (_shared, {"B": 0}, INVALID, b"Invalid dimensions"),
+    (_shared, LONG | {"ws": None}, WORKSPACE, b"needs"), (_shared, LONG | {"ws_bytes": 64}, WORKSPACE, b"needs"),
+    (_shared, LONG | {"ws": P + 16}, WORKSPACE, b"256-byte"), (_shared, {"B": 0}, INVALID, b"Invalid dimensions"),
     (_shared, {"B": 2 ** 40, "n": 2 ** 40}, INVALID, b"too large"),
     (_plan, {"table": None}, INVALID, b"Null"), (_plan, {"held": None}, INVALID, b"Null"),
     (_plan, {"lens": None}, INVALID, b"Null"), (_plan, {"free": None}, INVALID, b"Null"),
@@ -148,10 +151,12 @@ def test_workspace_sizes():
     assert size(2, 4, 100, 0, 1, 0, -1.0) == 0 and size(2, 4, 100, 5, 1, 0, 1.0) == 0
     size = lib.morpho_cache_shared_attention_workspace_size
     pool = _pool()
-    assert size(ctypes.byref(pool), 2, 1, 4, 2, 1, 64, 64) >= 2 * 2 * 2 * (64 * 4 + 16)
-    assert size(ctypes.byref(pool), 2, 65, 4, 2, 1, 64, 64) == 0
+    assert size(ctypes.byref(pool), 2, 1, 4, 2, 1, 64, 64) == 0  # not worth it: one kernel without pieces
+    assert size(ctypes.byref(pool), 2, 1, 1 << 15, 2, 1, 1 << 20, 64) >= 2 * 2 * 2 * (64 * 4 + 16)
+    assert size(ctypes.byref(pool), 2, 65, 1 << 15, 2, 1, 1 << 20, 64) == 0
     # no longer than the table
-    assert size(ctypes.byref(pool), 2, 1, 4, 2, 1, 1 << 40, 1 << 40) == size(ctypes.byref(pool), 2, 1, 4, 2, 1, 256, 256)
+    assert size(ctypes.byref(pool), 2, 1, 1 << 15, 2, 1, 1 << 40, 1 << 40) == \
+        size(ctypes.byref(pool), 2, 1, 1 << 15, 2, 1, 1 << 21, 1 << 21)
 
 
 def test_python_refusals():
@@ -215,9 +220,10 @@ int main() {
               if (B * n > (1 << 22) || B * n * H > (1 << 23)) continue;
               const CacheSharedPlan p = cache_shared_plan(B, H, n, B, G, len, len, 16, dv);
               const long long rows = B * H * n, parts = p.np + p.rest.nsplit;
+              if (p.apart && p.rest.split_keys < 1) printf("apart");
               if (p.np < 1 || p.split_keys % 128 || (long long)p.np * p.split_keys < len ||
-                  (long long)p.rblocks * 16 * p.qt < B * n + (16 * p.qt - 1) * (G > 1 ? 1 : 0) ||
-                  (p.np > 1 && rows * p.np > (1 << 20) + rows) || (rows > (1 << 20) && parts > 4))
+                  (long long)p.rblocks * (p.qt ? 16 * p.qt : 64) < B * n + ((p.qt ? 16 * p.qt : 64) - 1) * (G > 1 ? 1 : 0) ||
+                  (p.np > 1 && rows * p.np > (1 << 20) + rows) || (!p.apart && rows > (1 << 20) && parts > 4))
                 printf("B%lld H%lld n%lld G%lld len%lld: np %d of %d, rblocks %d of 16 x %d\n", B, H, n, G, len, p.np,
                        p.split_keys, p.rblocks, p.qt);
             }
@@ -225,7 +231,7 @@ int main() {
     for (int vocab : {1, 7, 255, 2048, 32000, 50001, 128000, 1000003, kVerifyMaxVocab})
       for (int size : {2, 4})
         for (int kind = 0; kind < 8; ++kind) {
-          const VerifyPlan p = verify_plan(rows, vocab, size, kind & 1, kind & 2, kind & 4);
+          const VerifyPlan p = verify_plan(rows, 7, vocab, size, kind & 1, kind & 2, kind & 4);
           // a row that starts at the last element of 16 bytes has all its elements in the chunks
           if ((p.pieces != 1 && p.pieces != 4) || p.chunk != 64 * 16 / size * p.pieces ||
               (long long)p.chunks * p.chunk < vocab + 16 / size - 1 || p.chunks > kVerifyMaxChunks || p.rounds < 0 ||
