@@ -129,6 +129,22 @@ struct CacheSource {
   }
 };
 
+// split_exact of two weights, to places j and j + 1: three instructions (a
+// conversion takes two numbers, and the remainder is a mixed multiply-add) where one
+// after another they are eight. The remainders are exact, so the halves are the same.
+__device__ __forceinline__ void split_two(float x, float y, int j, f16x8& hi, f16x8& lo) {
+  asm("" : "+v"(x), "+v"(y));
+  int both = __builtin_bit_cast(int, f16x2{(f16)x, (f16)y});
+  asm("" : "+v"(both));  // or each is converted once more by itself
+  const f16x2 h = __builtin_bit_cast(f16x2, both);
+  float minus = -1.f;
+  asm("" : "+s"(minus));  // or the multiply-add becomes a conversion and a difference
+  hi[j] = h[0];
+  hi[j + 1] = h[1];
+  lo[j] = (f16)__builtin_fmaf((float)h[0], minus, x);
+  lo[j + 1] = (f16)__builtin_fmaf((float)h[1], minus, y);
+}
+
 // 16 QT query rows of one (sequence, head) in a wave: the queries, and what
 // they have summed. S^T = K u^T and O^T += V^T P^T on v_mfma_f32_16x16x32_f16:
 // a lane holds 8 keys of the query lane % 16 in both products, so weights
@@ -282,10 +298,7 @@ struct CacheRows {
           p[j] = fast_exp2(s[n][t][j >> 2][j & 3]);
           if constexpr (LO) {
             sum[t] += p[j];  // one after another: few registers (few rows are bound by loads in flight)
-            f16 ph, pl;
-            split_exact(p[j], ph, pl);
-            hi[j] = ph;
-            lo[j] = pl;
+            if (j & 1) split_two(p[j - 1], p[j], j - 1, hi, lo);
           } else {
             hi[j] = (f16)p[j];
           }

@@ -45,31 +45,12 @@ struct PlanNote {
 };
 constexpr int kPlanHeader = 16;  // bytes before the notes: the pages to take from
 
-// Sums over the lanes before and with this one, of 1024; total: all.
-__device__ __forceinline__ int64_t scan1024(int64_t x, int64_t* sums, int64_t& total) {
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int64_t y = __shfl_up(x, o);
-    if (lane >= o) x += y;
-  }
-  __syncthreads();
-  if (lane == 63) sums[w] = x;
-  __syncthreads();
-  int64_t before = 0;
-  total = 0;
-  for (int k = 0; k < 16; ++k) {
-    if (k < w) before += sums[k];
-    total += sums[k];
-  }
-  return before + x;
-}
-
-// Which of 1024 runs, whose ends are `upto`, item j lies in.
+// Which of N runs, whose ends are `upto`, item j lies in.
+template <int N>
 __device__ __forceinline__ int run_of(const int64_t* upto, int64_t j) {
   int lo = 0;
 #pragma unroll
-  for (int step = 512; step; step >>= 1)
+  for (int step = N / 2; step; step >>= 1)
     if (upto[lo + step - 1] <= j) lo += step;
   return lo;
 }
@@ -80,35 +61,82 @@ __device__ __forceinline__ int64_t slot_of(const CachePlanArgs& a, int64_t pos, 
 
 }  // namespace
 
-// One workgroup, 1024 sequences at a time. FUSED: there are no more, and it
-// writes table and slots too.
-template <bool FUSED>
-__global__ __launch_bounds__(1024) void cache_plan_kernel(CachePlanArgs a) {
-  __shared__ int64_t sums[16], upto[1024], from[1024];
-  __shared__ int first[1024], held[1024], tokens[1024];
-  const int t = threadIdx.x;
+// One workgroup, N sequences at a time. FUSED: there are no more, and it writes table
+// and slots too.
+//
+// Who gets pages: the sums `lacks` ascend, so those that get none are the ones behind a
+// point, and the taken pages are those of the runs before it.
+template <int N, bool FUSED>
+__global__ __launch_bounds__(N) void cache_plan_kernel(CachePlanArgs a) {
+  constexpr int NW = N / 64;
+  __shared__ int64_t back_sums[NW], lack_sums[NW], back_upto[N], lack_upto[N];
+  __shared__ unsigned long long taken_here;
+  __shared__ int first[N], held[N], tokens[N];
+  const int t = threadIdx.x, lane = t & 63, w = t >> 6;
   const int64_t room = a.room, count = min(max((int64_t)a.free_count[0], (int64_t)0), room);
-  int64_t back = 0, total;
-  for (int b0 = 0; b0 < a.B; b0 += 1024) {
-    scan1024(b0 + t < a.B ? plan_seq(a, b0 + t).back : 0, sums, total);
-    back += total;
-  }
-  const int64_t top = min(count + back, room);
-  int64_t back_before = 0, lack_before = 0, taken = 0;
-  for (int b0 = 0; b0 < a.B; b0 += 1024) {
-    const int b = b0 + t;
-    PlanSeq q{};
-    if (b < a.B) q = plan_seq(a, b);
-    const int64_t backs = scan1024(q.back, sums, total), back_here = total;
-    const int64_t lacks = lack_before + scan1024(q.lack, sums, total), lack_here = total;
-    const bool ok = b < a.B && q.fits && (q.lack == 0 || lacks <= top);
-    upto[t] = backs;
-    first[t] = (int)q.want;
+  // sums of a tile's pages over the sequences before and with this one, and all
+  auto scan = [&](int64_t& back, int64_t& lack, int64_t& backs, int64_t& lacks) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int64_t x = __shfl_up(back, o), y = __shfl_up(lack, o);
+      back += lane >= o ? x : 0;
+      lack += lane >= o ? y : 0;
+    }
     __syncthreads();
-    for (int64_t j = t; j < back_here; j += 1024) {
-      const int k = run_of(upto, j);
-      const int64_t at = count + back - 1 - (back_before + j);
-      int* entry = a.table + (int64_t)(b0 + k) * a.W + first[k] + (j - (k ? upto[k - 1] : 0));
+    if (lane == 63) {
+      back_sums[w] = back;
+      lack_sums[w] = lack;
+    }
+    __syncthreads();
+    backs = lacks = 0;
+#pragma unroll 4
+    for (int k = 0; k < NW; ++k) {
+      if (k == w) {
+        back += backs;
+        lack += lacks;
+      }
+      backs += back_sums[k];
+      lacks += lack_sums[k];
+    }
+  };
+  PlanSeq q{};
+  if (t < a.B) q = plan_seq(a, t);
+  int64_t back = q.back, lack = q.lack, back_here, lack_here;
+  scan(back, lack, back_here, lack_here);
+  int64_t all_back = back_here;
+  if (!FUSED)
+    for (int b0 = N; b0 < a.B; b0 += N) {
+      int64_t x = b0 + t < a.B ? plan_seq(a, b0 + t).back : 0, y = 0, xs, ys;
+      scan(x, y, xs, ys);
+      all_back += xs;
+    }
+  const int64_t end = count + all_back, top = min(end, room);
+  int64_t back_before = 0, lack_before = 0, taken = 0;
+  for (int b0 = 0; b0 < (FUSED ? 1 : a.B); b0 += N) {
+    const int b = b0 + t;
+    if (b0) {
+      q = PlanSeq{};
+      if (b < a.B) q = plan_seq(a, b);
+      back = q.back;
+      lack = q.lack;
+      scan(back, lack, back_here, lack_here);
+    }
+    const int64_t lacks = lack_before + lack;
+    const bool ok = b < a.B && q.fits && (q.lack == 0 || lacks <= top);
+    back_upto[t] = back;
+    first[t] = (int)q.want;
+    if (FUSED) {
+      lack_upto[t] = lack;
+      held[t] = q.held;
+      tokens[t] = ok ? q.nb : 0;
+    }
+    if (t == 0) taken_here = 0;
+    __syncthreads();
+    if (ok && q.lack > 0) atomicMax(&taken_here, (unsigned long long)lacks);
+    for (int64_t j = t; j < back_here; j += N) {
+      const int k = run_of<N>(back_upto, j);
+      const int64_t at = end - 1 - (back_before + j);
+      int* entry = a.table + (int64_t)(b0 + k) * a.W + first[k] + (j - (k ? back_upto[k - 1] : 0));
       const int page = *entry;
       *entry = -1;
       if (at < room) a.free_pages[at] = page;
@@ -120,21 +148,8 @@ __global__ __launch_bounds__(1024) void cache_plan_kernel(CachePlanArgs a) {
         reinterpret_cast<PlanNote*>(static_cast<char*>(a.workspace) + kPlanHeader)[b] =
             PlanNote{lacks - q.lack, q.held, ok ? q.nb : -1};
     }
-    int64_t got;
-    const int64_t gets = scan1024(ok ? q.lack : 0, sums, got);  // (its barriers: `upto` is read)
-    taken += got;
-    if (FUSED) {
-      upto[t] = gets;
-      held[t] = q.held;
-      tokens[t] = ok ? q.nb : 0;
-      from[t] = lacks - q.lack;
-      __syncthreads();
-      for (int64_t j = t; j < got; j += 1024) {
-        const int k = run_of(upto, j);
-        const int64_t i = j - (k ? upto[k - 1] : 0);
-        a.table[(int64_t)k * a.W + held[k] + i] = a.free_pages[top - 1 - (from[k] + i)];
-      }
-    }
+    __syncthreads();
+    taken = max(taken, (int64_t)taken_here);
     back_before += back_here;
     lack_before += lack_here;
   }
@@ -143,11 +158,20 @@ __global__ __launch_bounds__(1024) void cache_plan_kernel(CachePlanArgs a) {
     if (!FUSED) *static_cast<int64_t*>(a.workspace) = top;
   }
   if (FUSED) {
-    __syncthreads();
-    for (int e = t; e < a.B * a.n; e += 1024) {
+    for (int64_t j = t; j < taken; j += N) {
+      const int k = run_of<N>(lack_upto, j);
+      a.table[(int64_t)k * a.W + held[k] + (j - (k ? lack_upto[k - 1] : 0))] = a.free_pages[top - 1 - j];
+    }
+    // a place on a page that was taken is looked up where that came from
+    for (int e = t; e < a.B * a.n; e += N) {
       const int b = e / a.n, i = e - b * a.n;
-      const int64_t pos = (int64_t)max(a.lens[b], 0) + i;
-      a.slots[e] = i < tokens[b] ? slot_of(a, pos, a.table[(int64_t)b * a.W + (pos >> a.lp)]) : -1;
+      int64_t slot = -1;
+      if (i < tokens[b]) {
+        const int64_t pos = (int64_t)max(a.lens[b], 0) + i, k = pos >> a.lp;
+        slot = slot_of(a, pos, k < held[b] ? a.table[(int64_t)b * a.W + k]
+                                           : a.free_pages[top - 1 - ((b ? lack_upto[b - 1] : 0) + k - held[b])]);
+      }
+      a.slots[e] = slot;
     }
   }
 }
@@ -172,11 +196,15 @@ __global__ __launch_bounds__(256) void cache_slots_kernel(CachePlanArgs a, int b
 }
 
 hipError_t launch_cache_plan(const CachePlanArgs& a, hipStream_t s) {
+  // few sequences: fewer waves to wait for at every barrier
   if (!a.workspace) {
-    MORPHO_KLAUNCH((cache_plan_kernel<true>), dim3(1), dim3(1024), 0, s, a);
+    if (a.B <= 256)
+      MORPHO_KLAUNCH((cache_plan_kernel<256, true>), dim3(1), dim3(256), 0, s, a);
+    else
+      MORPHO_KLAUNCH((cache_plan_kernel<1024, true>), dim3(1), dim3(1024), 0, s, a);
     return hipGetLastError();
   }
-  MORPHO_KLAUNCH((cache_plan_kernel<false>), dim3(1), dim3(1024), 0, s, a);
+  MORPHO_KLAUNCH((cache_plan_kernel<1024, false>), dim3(1), dim3(1024), 0, s, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   const int blocks = (a.n + 1023) / 1024;
