@@ -441,8 +441,11 @@ inline CacheSharedPlan cache_shared_plan(int B, int H, int n, int members, int g
   // Pieces: every one costs its rows a partial result, so few long ones: 256 workgroups
   // from 512 keys on, 512 from 2048 on, up to 4096 (B64 8192 common tokens, 32 rows: of 512
   // 21.0, 1024 18.5, 2048 22.6; B32 65536 m32: of 1024 46, 2048 42, 4096 39; B64 n8 4096: of
-  // 1024 31, 2048 27, 4096 29; B24 4096 m64: of 256 14.4, 512 13.5, 1024 15.1); through LDS 768
-  // from 384 on (trees of 48, 4096: B16 of 1024 65, 2048 61, 4096 89; B8 of 768 47, 3072 60).
+  // 1024 31, 2048 27, 4096 29; B24 4096 m64: of 256 14.4, 512 13.5, 1024 15.1); through LDS
+  // 512 from 1024 on, 1536 from 2048 on (4096 common tokens: trees of 48 of H32 m64 B16 of
+  // 512 101, 1024 63, 2048 57, 4096 76; B8 of 1024 47, 1536 43, 2048 48; B64 n20 m32 of 1024 59,
+  // 2048 54, 4096 72; B16 n64 of 1024 43, 1536 41, 2048 42). 128 rows a workgroup instead of 64:
+  // B16 n64 48, trees 65.
   const int64_t work = max_prefix * H * blocks;
   int64_t keys;
   if (p.qt) {
@@ -450,7 +453,8 @@ inline CacheSharedPlan cache_shared_plan(int B, int H, int n, int members, int g
     if (keys > 2048) keys = work / 512 > 2048 ? work / 512 : 2048;
     if (keys > 4096) keys = 4096;
   } else {
-    keys = work / 768 > 384 ? work / 768 : 384;
+    keys = work / 512 > 1024 ? work / 512 : 1024;
+    if (keys > 2048) keys = work / 1536 > 2048 ? work / 1536 : 2048;
   }
   if (keys > max_prefix) keys = max_prefix;
   // partial rows (DV + 4 floats each) and workgroups stay below 2^20 or so
