@@ -991,7 +991,7 @@ MORPHO_EXPORT int morpho_verify_drafts(const morpho_logits* logits, const morpho
   a.token = token;
   a.stats = static_cast<VerifyStat*>(workspace);
   a.masses = reinterpret_cast<double*>(static_cast<char*>(workspace) + verify_stats_bytes(B, n, plan));
-  a.c = a.best ? 0.0 : 64.0 * 1.44269504088896340736 / temperature;
+  a.c = a.best ? 0.0 : 256.0 * 1.44269504088896340736 / temperature;
   a.B = (int)B;
   a.n = (int)n;
   a.V = (int)vocab;

@@ -219,7 +219,7 @@ struct VerifyArgs {
   int64_t* token;
   VerifyStat* stats;  // [B n + B (n - 1), chunks]
   double* masses;     // [rounds, B, n - 1, chunks]
-  double c;           // 64 log2(e) / temperature
+  double c;           // 256 log2(e) / temperature
   int B, n, V, chunk, chunks, rounds, best;
 };
 constexpr int kVerifyThreads = 1024;
