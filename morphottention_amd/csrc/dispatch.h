@@ -473,7 +473,7 @@ inline CacheSharedPlan cache_shared_plan(int B, int H, int n, int members, int g
 struct VerifyPlan {
   int pieces, chunk, chunks, rounds;
 };
-constexpr int kVerifyMaxVocab = 4000000, kVerifyMaxChunks = 4096;
+constexpr int kVerifyMaxVocab = 4000000, kVerifyMaxChunks = 4096, kVerifyMaxRounds = 6;
 inline VerifyPlan verify_plan(int64_t rows, int n, int vocab, int element_bytes, bool tree, bool draft, bool best) {
   VerifyPlan p;
   const int per = 16 / element_bytes;
@@ -481,7 +481,7 @@ inline VerifyPlan verify_plan(int64_t rows, int n, int vocab, int element_bytes,
   p.pieces = rows * chunks(4) < 4096 && chunks(1) <= 256 ? 1 : 4;
   p.chunk = 64 * per * p.pieces;
   p.chunks = chunks(p.pieces);
-  p.rounds = best || !draft || p.chunks == 1 ? 0 : !tree ? 1 : n <= 6 ? n - 1 : 6;
+  p.rounds = best || !draft || p.chunks == 1 ? 0 : !tree ? 1 : n - 1 < kVerifyMaxRounds ? n - 1 : kVerifyMaxRounds;
   return p;
 }
 

@@ -149,51 +149,78 @@ __device__ __forceinline__ float value_of(f16 x) { return (float)x; }
 __device__ __forceinline__ float value_of(Bf16 x) { return __builtin_bit_cast(float, (unsigned)x.bits << 16); }
 __device__ __forceinline__ float value_of(float x) { return x; }
 
-// The value of the lane that step K of a reduction pairs this one with (K of 6: lanes
-// 1, 2, 4, 8, 16 and 32 away or their mirror images, which by then hold the same).
+// The values that step K of a reduction joins (K of 6: with those of lanes 1, 2, 4, 8,
+// 16 and 32 away or their mirror images, which by then hold the same). Lanes' numbers
+// go over registers here: through LDS a step of 64 bits takes some 150 cycles, and
+// the last kernel is made of such steps.
 template <int K>
-__device__ __forceinline__ int paired(int x) {
+__device__ __forceinline__ void joined(unsigned x, unsigned& a, unsigned& b) {
   if constexpr (K < 4) {
     constexpr int kDpp[4] = {0xb1, 0x4e, 0x141, 0x140};  // quad_perm 1 0 3 2, 2 3 0 1, row_half_mirror, row_mirror
-    return __builtin_amdgcn_mov_dpp(x, kDpp[K], 0xf, 0xf, false);
+    a = x;
+    b = (unsigned)__builtin_amdgcn_mov_dpp((int)x, kDpp[K], 0xf, 0xf, false);
   } else {
-    return __shfl_xor(x, K == 4 ? 16 : 32);
+    const auto r = K == 4 ? __builtin_amdgcn_permlane16_swap(x, x, false, false)
+                          : __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    a = r[0];
+    b = r[1];
   }
 }
-template <int K>
-__device__ __forceinline__ double paired(double x) {
-  const uint64_t b = __builtin_bit_cast(uint64_t, x);
-  const unsigned lo = (unsigned)paired<K>((int)(unsigned)b), hi = (unsigned)paired<K>((int)(unsigned)(b >> 32));
+template <int K, class F>
+__device__ __forceinline__ double join(double x, const F& f) {
+  const uint64_t v = __builtin_bit_cast(uint64_t, x);
+  unsigned al, bl, ah, bh;
+  joined<K>((unsigned)v, al, bl);
+  joined<K>((unsigned)(v >> 32), ah, bh);
+  return f(__builtin_bit_cast(double, (uint64_t)ah << 32 | al), __builtin_bit_cast(double, (uint64_t)bh << 32 | bl));
+}
+template <int K, class F>
+__device__ __forceinline__ float join(float x, const F& f) {
+  unsigned a, b;
+  joined<K>(__builtin_bit_cast(unsigned, x), a, b);
+  return f(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
+}
+// Over runs of `per` lanes, a power of two.
+template <class T, class F>
+__device__ __forceinline__ T join_lanes(T x, int per, const F& f) {
+  if (per > 1) x = join<0>(x, f);
+  if (per > 2) x = join<1>(x, f);
+  if (per > 4) x = join<2>(x, f);
+  if (per > 8) x = join<3>(x, f);
+  if (per > 16) x = join<4>(x, f);
+  if (per > 32) x = join<5>(x, f);
+  return x;
+}
+__device__ __forceinline__ double lanes_sum(double x, int per) {
+  return join_lanes(x, per, [](double a, double b) { return a + b; });
+}
+__device__ __forceinline__ float lanes_max(float x, int per) {
+  return join_lanes(x, per, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ __forceinline__ double wave_sum(double x) { return lanes_sum(x, 64); }
+__device__ __forceinline__ float wave_max(float x) { return lanes_max(x, 64); }
+// The value of lane i, the same i in all of them.
+__device__ __forceinline__ int lane_value(int x, int i) { return __builtin_amdgcn_readlane(x, i); }
+__device__ __forceinline__ double lane_value(double x, int i) {
+  const uint64_t v = __builtin_bit_cast(uint64_t, x);
+  const unsigned lo = (unsigned)lane_value((int)(unsigned)v, i), hi = (unsigned)lane_value((int)(unsigned)(v >> 32), i);
   return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
-template <int K>
-__device__ __forceinline__ float paired(float x) {
-  return __builtin_bit_cast(float, paired<K>(__builtin_bit_cast(int, x)));
-}
-__device__ __forceinline__ double wave_sum(double x) {
-  x += paired<0>(x);
-  x += paired<1>(x);
-  x += paired<2>(x);
-  x += paired<3>(x);
-  x += paired<4>(x);
-  return x + paired<5>(x);
-}
-__device__ __forceinline__ float wave_max(float x) {
-  x = fmaxf(x, paired<0>(x));
-  x = fmaxf(x, paired<1>(x));
-  x = fmaxf(x, paired<2>(x));
-  x = fmaxf(x, paired<3>(x));
-  x = fmaxf(x, paired<4>(x));
-  return fmaxf(x, paired<5>(x));
-}
 // Sum over the lanes up to this one.
-__device__ __forceinline__ double wave_upto(double x, int lane) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const double y = __shfl_up(x, o);
-    x += lane >= o ? y : 0.0;
-  }
-  return x;
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double add_moved(double x) {
+  const uint64_t v = __builtin_bit_cast(uint64_t, x);
+  const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)v, CTRL, ROWS, 0xf, false);
+  const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)(v >> 32), CTRL, ROWS, 0xf, false);
+  return x + __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double wave_upto(double x) {
+  x = add_moved<0x111, 0xf>(x);     // row_shr 1, 2, 4, 8
+  x = add_moved<0x112, 0xf>(x);
+  x = add_moved<0x114, 0xf>(x);
+  x = add_moved<0x118, 0xf>(x);
+  x = add_moved<0x142, 0xa>(x);     // row_bcast 15: of rows 0 and 2 to 1 and 3
+  return add_moved<0x143, 0xc>(x);  // row_bcast 31: of row 1 to 2 and 3
 }
 
 // The token that token i was drafted behind: the highest bit below its own, or
@@ -364,28 +391,31 @@ __device__ __forceinline__ RowSum row_sum(const VerifyStat* st, int chunks, bool
   if (real && sub < chunks) mine = st[sub];
   float top = mine.top;
   for (int k = sub + per; real && k < chunks; k += per) top = fmaxf(top, st[k].top);
-  for (int o = 1; o < per; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
+  top = lanes_max(top, per);
   double sum = mine.sum * weight_below(table, c, mine.top, top);
   for (int k = sub + per; real && k < chunks; k += per)
     sum = fma(st[k].sum, weight_below(table, c, st[k].top, top), sum);
-  for (int o = 1; o < per; o <<= 1) sum += __shfl_xor(sum, o);
-  return {top, sum};
+  return {top, lanes_sum(sum, per)};
 }
-// The sums of all rows of a sequence, by a workgroup of NT: 2^k lanes a row, as many
-// rows at a time as it has. `parent`: of the lane's draft.
+// The sums of the rows that a sequence's drafts ask for, by a workgroup of NT: 2^k
+// lanes a row, as many rows at a time as it has. `parent`: of the lane's draft.
 template <bool DRAFT, int NT>
 __device__ __forceinline__ void row_sums(const VerifyArgs& a, int b, int nb, int parent, const uint64_t* table,
                                          RowSum (&rows)[2][64]) {
   int per = 1;
   while (per < a.chunks && per < 64) per *= 2;
-  const int sub = threadIdx.x & (per - 1);
+  const int lane = threadIdx.x & 63, sub = threadIdx.x & (per - 1);
   uint64_t inner = 0;  // tokens with drafts
-  if constexpr (DRAFT)
-    for (int i = 0; i < nb; ++i)
-      if (__any(parent == i)) inner |= (uint64_t)1 << i;
-  for (int r0 = 0; r0 < (DRAFT ? 2 * nb : nb); r0 += NT / per) {
-    const int r = r0 + threadIdx.x / per, kind = r >= nb, i = r - kind * nb;
-    const bool real = r < (DRAFT ? 2 * nb : nb) && (!kind || (inner >> i & 1));
+  for (int i = 0; i < nb; ++i)
+    if (__any(parent == i)) inner |= (uint64_t)1 << i;
+  // lane k holds the k-th of them
+  const uint64_t below = ((uint64_t)1 << lane) - 1;
+  const int count = __builtin_popcountll(inner);
+  const int to = inner >> lane & 1 ? __builtin_popcountll(inner & below) : count + __builtin_popcountll(~inner & below);
+  const int with_drafts = __builtin_amdgcn_ds_permute(4 * to, lane);
+  for (int r0 = 0; r0 < (DRAFT ? 2 * count : count); r0 += NT / per) {
+    const int r = r0 + threadIdx.x / per, kind = r >= count, i = __shfl(with_drafts, r - kind * count);
+    const bool real = r < (DRAFT ? 2 * count : count);
     const RowSum x = row_sum(stats_of(a, kind, b, real ? i : 0), a.chunks, real, sub, per, table, a.c);
     if (real && sub == 0) rows[kind][i] = x;
   }
@@ -396,6 +426,15 @@ __device__ __forceinline__ double chance(const uint64_t* table, double c, float 
   return row.sum > 0.0 ? weight_below(table, c, x, row.top) / row.sum : 0.0;
 }
 
+// Pieces of the target's and the drafter's row at the same place.
+template <class T>
+struct PiecePair {
+  Piece<T> p, q;
+  __device__ __forceinline__ void load(const T* prow, const T* qrow, int first, int V) {
+    p.load(prow, first, V);
+    q.load(qrow, first, V);
+  }
+};
 // r of logits lp and lq of a token in the target's and the drafter's row.
 template <bool DRAFT>
 struct Rest {
@@ -411,24 +450,19 @@ struct Rest {
     if constexpr (DRAFT) r = fma(-aq, q(lq), r);
     return fmax(r, 0.0);
   }
-  // The mass of a chunk, by a wave.
+  // The mass of a chunk, by a wave: a loop, since what a small launch waits for is its
+  // code (unrolled: x us).
   template <class T, int U>
-  __device__ __forceinline__ double chunk_mass(const T* prow, const T* qrow, int chunk, int shift, int V,
-                                               int lane) const {
-    constexpr int E = 16 / sizeof(T);
-    const int first = (chunk * U * 64 + lane) * E - shift;
-    Piece<T> x[U], y[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      x[u].load(prow, first + u * 64 * E, V);
-      if constexpr (DRAFT) y[u].load(qrow, first + u * 64 * E, V);
-    }
+  __device__ __forceinline__ double mass(PiecePair<T> x, const T* prow, const T* qrow, int first, int V) const {
     double sum = 0.0;
+#pragma unroll 1
+    for (int u = 0;;) {
+      PiecePair<T> next;
+      if (++u < U) next.load(prow, qrow, first + u * 64 * Piece<T>::E, V);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-#pragma unroll
-      for (int e = 0; e < E; ++e) sum += (*this)(x[u][e], DRAFT ? y[u][e] : 0.f);
-      __builtin_amdgcn_sched_barrier(0);
+      for (int e = 0; e < Piece<T>::E; ++e) sum += (*this)(x.p[e], x.q[e]);
+      if (u >= U) break;
+      x = next;
     }
     return wave_sum(sum);
   }
@@ -442,12 +476,12 @@ struct Asked {
   double pa = 1.0, qc = 0.0, Z = 1.0;  // r = max(pa p - qc q, 0), and its sum
   int kept = -1, rejections = 0;
   bool fresh = false;  // the masses of the last rejection are those of r
-  // sum_of(k, pa, qc): the sum of r's masses after rejection k; stop(k): end there (false)
+  // sum_of(i, k, pa, qc): the sum of r's masses after rejection k, that of draft i; stop(k): end there (false)
   template <class Sum, class Stop>
   __device__ __forceinline__ bool run(uint64_t kids, double p, double q, double u, const Sum& sum_of, const Stop& stop) {
     for (; kids; kids &= kids - 1) {
       const int i = __builtin_ctzll(kids);
-      const double pi = __shfl(p, i), qi = __shfl(q, i), ui = __shfl(u, i);
+      const double pi = lane_value(p, i), qi = lane_value(q, i), ui = lane_value(u, i);
       if (ui * qi * Z < fma(pa, pi, -(qc * qi))) {
         kept = i;
         return true;
@@ -455,7 +489,7 @@ struct Asked {
       pa /= Z;
       qc = qc / Z + 1.0;
       if (stop(rejections)) return false;
-      Z = sum_of(rejections, pa, qc);
+      Z = sum_of(i, rejections, pa, qc);
       ++rejections;
       fresh = Z > 0.0;
       if (!fresh) {  // nothing is left: the token's own distribution in its place
@@ -473,11 +507,12 @@ struct Draft {
   int64_t token = -1;
   double u = 0.0;
   __device__ __forceinline__ Draft(const VerifyArgs& a, int b, int nb, int lane) {
-    if (lane > 0 && lane < nb) {
+    if (lane > 0 && lane < a.n) {  // nb may still be on its way
       parent = parent_of(a, b, lane);
       token = a.tokens[(int64_t)b * a.n + lane];
       u = (double)a.uniform[(int64_t)b * a.n + lane];
     }
+    if (lane >= nb) parent = -1, token = -1;
   }
   __device__ __forceinline__ bool known(const VerifyArgs& a) const { return parent >= 0 && token >= 0 && token < a.V; }
 };
@@ -506,9 +541,27 @@ __global__ __launch_bounds__(256) void verify_mass_kernel(VerifyArgs a, int roun
   const int lane = threadIdx.x & 63, k = blockIdx.x / groups, b = CHAIN ? k : k / (a.n - 1);
   const int chunk = 4 * (blockIdx.x - k * groups) + (threadIdx.x >> 6), nb = tokens_of(a, b);
   int node = CHAIN ? 0 : k - b * (a.n - 1);
-  if (nb < 2) return;
   const Draft d(a, b, nb, lane);
-  if (!CHAIN && __builtin_popcountll(__ballot(d.parent == node)) <= round) return;
+  if (nb < 2) return;
+  PiecePair<T> x;
+  const T *prow, *qrow;
+  int first;
+  auto load = [&]() {
+    prow = row_of<T>(a.p, b, node);
+    qrow = row_of<T>(a.q, b, node);
+    first = (min(chunk, a.chunks - 1) * U * 64 + lane) * Piece<T>::E - shift_of(prow);
+    x.load(prow, qrow, first, a.V);
+  };
+  double sums = 0.0;  // lane r: of the masses of round r
+  if constexpr (!CHAIN) {
+    if (__builtin_popcountll(__ballot(d.parent == node)) <= round) return;
+    load();  // early: the sums of the rounds before are on their way at the same time
+#pragma unroll 1
+    for (int r = 0; r < round; ++r) {
+      const double sum = mass_sum(masses_of(a, r, b, node), a.chunks, lane);
+      sums = lane == r ? sum : sums;
+    }
+  }
   float lp = kNegInf, lq = kNegInf;
   if ((CHAIN || d.parent == node) && d.known(a)) {
     lp = value_of(row_of<T>(a.p, b, d.parent)[d.token]);
@@ -532,20 +585,18 @@ __global__ __launch_bounds__(256) void verify_mass_kernel(VerifyArgs a, int roun
     const uint64_t ends = __ballot(d.parent >= 0 && !(d.u * q < p));
     if (!ends) return;
     node = __builtin_ctzll(ends) - 1;
+    load();
     ps = rows[0][node];
     qs = rows[1][node];
   } else {
     Asked asked;
-    if (asked.run(__ballot(d.parent == node), p, q, d.u,
-                  [&](int r, double, double) { return mass_sum(masses_of(a, r, b, node), a.chunks, lane); },
+    if (asked.run(__ballot(d.parent == node), p, q, d.u, [&](int, int r, double, double) { return lane_value(sums, r); },
                   [&](int r) { return r == round; }))
       return;
     pa = asked.pa;
     qc = asked.qc;
   }
-  const T* prow = row_of<T>(a.p, b, node);
-  const double m = Rest<true>(table, a.c, ps, qs, pa, qc)
-                       .template chunk_mass<T, U>(prow, row_of<T>(a.q, b, node), chunk, shift_of(prow), a.V, lane);
+  const double m = Rest<true>(table, a.c, ps, qs, pa, qc).template mass<T, U>(x, prow, qrow, first, a.V);
   if (lane == 0) masses_of(a, round, b, node)[chunk] = m;
 }
 
@@ -556,6 +607,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(VerifyArgs a) {
   __shared__ uint64_t table[kTable];
   __shared__ double part[NW], masses[kVerifyMaxChunks];
   __shared__ RowSum rows[2][64];
+  __shared__ double sums[64];
   __shared__ int best[64], found, last[NW];
   const int b = blockIdx.x, lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int nb = tokens_of(a, b);
@@ -578,6 +630,16 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(VerifyArgs a) {
     }
     if (threadIdx.x < kTable) table[threadIdx.x] = kExp2Table[threadIdx.x];
     __syncthreads();
+    // the masses that draft i's rejection leaves: of the token behind which it was
+    // drafted and the number of its siblings before it (nothing, where it was not asked)
+    if constexpr (DRAFT) {
+      for (int i = w; i < nb; i += NW) {
+        const int node = lane_value(d.parent, i), r = __builtin_popcountll(__ballot(d.parent == node && lane < i));
+        if (node < 0 || r >= a.rounds) continue;
+        const double sum = mass_sum(masses_of(a, r, b, node), a.chunks, lane);
+        if (lane == 0) sums[i] = sum;
+      }
+    }
     row_sums<DRAFT, NT>(a, b, nb, d.parent, table, rows);
   } else {
     int per = 1;
@@ -629,8 +691,10 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(VerifyArgs a) {
   const int mine = max(d.parent, 0);
   const double p = chance(table, a.c, lp, rows[0][mine]), q = DRAFT ? chance(table, a.c, lq, rows[1][mine]) : 0.0;
   double pa = 1.0, qc = 0.0;
-  uint64_t gone = 0;   // drafts that were turned down, where they were not drawn
-  bool fresh = false;  // `masses` are r's
+  const int token = d.known(a) ? (int)d.token : -1;
+  uint64_t gone = 0;   // drafts that were turned down, where they were not drawn: each token once
+  bool fresh = false;  // the masses of the last rejection, at `from` or in `masses`, are r's
+  const double* from = nullptr;
   for (;;) {
     const uint64_t kids = __ballot(d.parent == node);
     int next = -1;
@@ -638,18 +702,21 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(VerifyArgs a) {
       Asked asked;
       asked.run(
           kids, p, q, d.u,
-          [&](int r, double apa, double aqc) {
-            __syncthreads();  // the masses of the rejection before are read
+          [&](int i, int r, double apa, double aqc) {
             if (r < a.rounds) {
-              const double* from = masses_of(a, r, b, node);
-              for (int c = threadIdx.x; c < a.chunks; c += NT) masses[c] = from[c];
-            } else {
-              const T *prow = row_of<T>(a.p, b, node), *qrow = row_of<T>(a.q, b, node);
-              const Rest<DRAFT> rest(table, a.c, rows[0][node], rows[1][node], apa, aqc);
-              for (int c = w; c < a.chunks; c += NW) {
-                const double m = rest.template chunk_mass<T, U>(prow, qrow, c, shift_of(prow), a.V, lane);
-                if (lane == 0) masses[c] = m;
-              }
+              from = masses_of(a, r, b, node);
+              return sums[i];
+            }
+            from = nullptr;
+            __syncthreads();  // the masses of the rejection before are read
+            const T *prow = row_of<T>(a.p, b, node), *qrow = row_of<T>(a.q, b, node);
+            const Rest<DRAFT> rest(table, a.c, rows[0][node], rows[1][node], apa, aqc);
+            for (int c = w; c < a.chunks; c += NW) {
+              const int first = (c * U * 64 + lane) * E - shift_of(prow);
+              PiecePair<T> x;
+              x.load(prow, qrow, first, a.V);
+              const double m = rest.template mass<T, U>(x, prow, qrow, first, a.V);
+              if (lane == 0) masses[c] = m;
             }
             __syncthreads();
             return mass_sum(masses, a.chunks, lane);
@@ -664,14 +731,15 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(VerifyArgs a) {
       gone = 0;
       for (uint64_t left = kids; left; left &= left - 1) {
         const int i = __builtin_ctzll(left);
-        const double pi = __shfl(p, i), ui = __shfl(d.u, i);
-        const bool again = (gone & __ballot(d.token == __shfl(d.token, i))) != 0;  // turned down before
+        const double pi = lane_value(p, i), ui = lane_value(d.u, i);
+        const bool again = (gone & __ballot(token == lane_value(token, i))) != 0;  // turned down before
         if (ui * Z < (again ? 0.0 : pi)) {
           next = i;
           break;
         }
+        if (again) continue;
         gone |= (uint64_t)1 << i;
-        if (!again) Z = fmax(Z - pi, 0.0);
+        Z = fmax(Z - pi, 0.0);
       }
     }
     if (next < 0) break;
@@ -685,38 +753,41 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(VerifyArgs a) {
   const T* prow = row_of<T>(a.p, b, node);
   const T* qrow = DRAFT && qc > 0.0 ? row_of<T>(a.q, b, node) : prow;
   const int shift = shift_of(prow);
-  const RowSum ps = rows[0][node], qs = DRAFT && qc > 0.0 ? rows[1][node] : ps;
+  // (the last of a path has no drafts: its sum is not among the rows')
+  const bool inner = __any(d.parent == node);
+  const RowSum ps = inner ? rows[0][node] : row_sum(stats_of(a, false, b, node), a.chunks, true, lane, 64, table, a.c);
+  const RowSum qs = DRAFT && qc > 0.0 ? rows[1][node] : ps;
   const Rest<DRAFT> rest(table, a.c, ps, qs, pa, qc);
   // where the last event was no rejection with any left: the chunks' own masses,
   // without what was turned down
   auto own_masses = [&]() {
     __syncthreads();
     const VerifyStat* st = stats_of(a, false, b, node);
-    for (int c = threadIdx.x; c < a.chunks; c += NT) {
-      const VerifyStat x = st[c];
+    for (int c0 = 0; c0 < a.chunks; c0 += NT) {  // every lane: lanes' values are read within
+      const int c = c0 + threadIdx.x;
+      const VerifyStat x = st[min(c, a.chunks - 1)];
       double m = rest.ap * (x.sum * weight_below(table, a.c, x.top, ps.top));
-      uint64_t seen = 0;
       for (uint64_t left = gone; left; left &= left - 1) {
-        const int i = __builtin_ctzll(left);
-        const int64_t t = a.tokens[(int64_t)b * a.n + i];
-        if (t < 0 || t >= a.V || (int)((t + shift) / a.chunk) != c) continue;
-        bool again = false;
-        for (uint64_t other = seen; other; other &= other - 1)
-          again |= a.tokens[(int64_t)b * a.n + __builtin_ctzll(other)] == t;
-        if (!again) m -= chance(table, a.c, value_of(prow[t]), ps);
-        seen |= (uint64_t)1 << i;
+        const int i = __builtin_ctzll(left), t = lane_value(token, i);
+        const double there = lane_value(p, i);
+        m -= t >= 0 && (t + shift) / a.chunk == c ? there : 0.0;
       }
-      masses[c] = fmax(m, 0.0);
+      if (c < a.chunks) masses[c] = fmax(m, 0.0);
     }
     __syncthreads();
   };
-  if (!(DRAFT && fresh)) own_masses();
+  if (!(DRAFT && fresh)) {
+    own_masses();
+  } else if (from) {
+    for (int c = threadIdx.x; c < a.chunks; c += NT) masses[c] = from[c];
+    __syncthreads();
+  }
   for (;;) {
     // the chunk, by every wave: a run of them a lane
     const int run = (a.chunks + 63) / 64, c0 = lane * run, c1 = min(c0 + run, a.chunks);
     double sum = 0.0;
     for (int c = c0; c < c1; ++c) sum += masses[c];
-    const double upto = wave_upto(sum, lane), Z = __shfl(upto, 63), want = u0 * Z;
+    const double upto = wave_upto(sum), Z = lane_value(upto, 63), want = u0 * Z;
     const uint64_t some = __ballot(sum > 0.0), past = __ballot(sum > 0.0 && upto > want);
     if (!some) {
       if (gone) {  // nothing is left: the token's own distribution in its place
@@ -739,8 +810,8 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(VerifyArgs a) {
       }
       before += m;
     }
-    chunk = __shfl(chunk, at);
-    chunk_before = __shfl(chunk_before, at);
+    chunk = lane_value(chunk, at);
+    chunk_before = lane_value(chunk_before, at);
     // within it: Q tokens a lane
     constexpr int CHUNK = 64 * U * E, Q = CHUNK > NT ? CHUNK / NT : 1;
     double r[Q];
@@ -755,14 +826,14 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(VerifyArgs a) {
     }
     if constexpr (!DRAFT) {
       for (uint64_t left = gone; left; left &= left - 1) {
-        const int64_t t = __shfl(d.token, __builtin_ctzll(left));
+        const int t = lane_value(token, __builtin_ctzll(left));
 #pragma unroll
         for (int e = 0; e < Q; ++e) r[e] = t == x0 + e ? 0.0 : r[e];
       }
     }
 #pragma unroll
     for (int e = 0; e < Q; ++e) sum += r[e];
-    const double here = wave_upto(sum, lane);
+    const double here = wave_upto(sum);
     if (lane == 63) part[w] = here;
     if (threadIdx.x == 0) found = INT_MAX;
     __syncthreads();
