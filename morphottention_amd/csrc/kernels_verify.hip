@@ -117,6 +117,7 @@ struct Weigh {
   __device__ __forceinline__ double operator()(float x) const {
     return exp2_256(table, fmax((fmin((double)x, 1e39) - top) * c, -256000.0));
   }
+  __device__ __forceinline__ double factor() const { return 1.0; }
 };
 // For long sums with |top c| below 2^40: three instructions less. The weights are over
 // 2^(T / 256) with T the whole number next to top c, the sum's factor() puts it over
@@ -125,6 +126,7 @@ struct Weigh {
 struct WeighFast {
   const uint64_t* table;
   double c, K, rest, low;  // low: 2^-1000 of the top
+  __device__ __forceinline__ static bool fits(double c, float top) { return fabs((double)top * c) < 0x1p40; }
   __device__ __forceinline__ WeighFast(const uint64_t* table, double c, float top) : table(table), c(c) {
     const double T = __builtin_rint((double)top * c);
     K = kWhole - T;
@@ -199,6 +201,19 @@ __device__ __forceinline__ float lanes_max(float x, int per) {
 }
 __device__ __forceinline__ double wave_sum(double x) { return lanes_sum(x, 64); }
 __device__ __forceinline__ float wave_max(float x) { return lanes_max(x, 64); }
+__device__ __forceinline__ uint64_t wave_or(uint64_t x) {
+  auto either = [](unsigned v) {
+    unsigned a, b;
+    joined<0>(v, a, b);
+    joined<1>(a | b, a, b);
+    joined<2>(a | b, a, b);
+    joined<3>(a | b, a, b);
+    joined<4>(a | b, a, b);
+    joined<5>(a | b, a, b);
+    return (unsigned)__builtin_amdgcn_readfirstlane((int)(a | b));
+  };
+  return (uint64_t)either((unsigned)(x >> 32)) << 32 | either((unsigned)x);
+}
 // The value of lane i, the same i in all of them.
 __device__ __forceinline__ int lane_value(int x, int i) { return __builtin_amdgcn_readlane(x, i); }
 __device__ __forceinline__ double lane_value(double x, int i) {
@@ -365,7 +380,7 @@ __global__ __launch_bounds__(256, 8) void verify_stats_kernel(VerifyArgs a, int 
     }
   };
   if (top > kNegInf) {
-    if (fabs((double)top * a.c) < 0x1p40) {
+    if (WeighFast::fits(a.c, top)) {
       const WeighFast weigh(table, a.c, top);
       add(weigh);
       sum *= weigh.factor();
@@ -382,32 +397,30 @@ namespace {
 // A row's largest logit and the sum of its weights.
 struct RowSum {
   float top;
-  double sum;
+  double share;  // 1 / sum, nothing where there is none
 };
 // Joins a row's chunks with `per` lanes (a power of two), of which this is number `sub`.
 __device__ __forceinline__ RowSum row_sum(const VerifyStat* st, int chunks, bool real, int sub, int per,
                                           const uint64_t* table, double c) {
-  VerifyStat mine{0.0, kNegInf, -1};
-  if (real && sub < chunks) mine = st[sub];
-  float top = mine.top;
-  for (int k = sub + per; real && k < chunks; k += per) top = fmaxf(top, st[k].top);
+  float top = kNegInf;
+#pragma unroll 1
+  for (int k = sub; real && k < chunks; k += per) top = fmaxf(top, st[k].top);
   top = lanes_max(top, per);
-  double sum = mine.sum * weight_below(table, c, mine.top, top);
-  for (int k = sub + per; real && k < chunks; k += per)
-    sum = fma(st[k].sum, weight_below(table, c, st[k].top, top), sum);
-  return {top, lanes_sum(sum, per)};
+  double sum = 0.0;
+#pragma unroll 1
+  for (int k = sub; real && k < chunks; k += per) sum = fma(st[k].sum, weight_below(table, c, st[k].top, top), sum);
+  sum = lanes_sum(sum, per);
+  return {top, sum > 0.0 ? 1.0 / sum : 0.0};
 }
 // The sums of the rows that a sequence's drafts ask for, by a workgroup of NT: 2^k
 // lanes a row, as many rows at a time as it has. `parent`: of the lane's draft.
 template <bool DRAFT, int NT>
-__device__ __forceinline__ void row_sums(const VerifyArgs& a, int b, int nb, int parent, const uint64_t* table,
+__device__ __forceinline__ void row_sums(const VerifyArgs& a, int b, int parent, const uint64_t* table,
                                          RowSum (&rows)[2][64]) {
   int per = 1;
   while (per < a.chunks && per < 64) per *= 2;
   const int lane = threadIdx.x & 63, sub = threadIdx.x & (per - 1);
-  uint64_t inner = 0;  // tokens with drafts
-  for (int i = 0; i < nb; ++i)
-    if (__any(parent == i)) inner |= (uint64_t)1 << i;
+  const uint64_t inner = wave_or(parent >= 0 ? (uint64_t)1 << parent : 0);  // tokens with drafts
   // lane k holds the k-th of them
   const uint64_t below = ((uint64_t)1 << lane) - 1;
   const int count = __builtin_popcountll(inner);
@@ -423,7 +436,7 @@ __device__ __forceinline__ void row_sums(const VerifyArgs& a, int b, int nb, int
 }
 // The chance of a logit in its row.
 __device__ __forceinline__ double chance(const uint64_t* table, double c, float x, const RowSum& row) {
-  return row.sum > 0.0 ? weight_below(table, c, x, row.top) / row.sum : 0.0;
+  return weight_below(table, c, x, row.top) * row.share;
 }
 
 // Pieces of the target's and the drafter's row at the same place.
@@ -436,15 +449,15 @@ struct PiecePair {
   }
 };
 // r of logits lp and lq of a token in the target's and the drafter's row.
-template <bool DRAFT>
+template <bool DRAFT, class W>
 struct Rest {
-  Weigh p, q;
+  W p, q;
   double ap, aq;
   // state (pa, qc) of the decisions: r = max(pa p - qc q, 0)
   __device__ __forceinline__ Rest(const uint64_t* table, double c, const RowSum& ps, const RowSum& qs, double pa,
                                   double qc)
-      : p(table, c, ps.top), q(table, c, qs.top), ap(ps.sum > 0.0 ? pa / ps.sum : 0.0),
-        aq(DRAFT && qc > 0.0 && qs.sum > 0.0 ? qc / qs.sum : 0.0) {}
+      : p(table, c, ps.top), q(table, c, qs.top), ap(pa * p.factor() * ps.share),
+        aq(DRAFT && qc > 0.0 ? qc * q.factor() * qs.share : 0.0) {}
   __device__ __forceinline__ double operator()(float lp, float lq) const {
     double r = fma(ap, p(lp), -kNothing);
     if constexpr (DRAFT) r = fma(-aq, q(lq), r);
@@ -467,6 +480,15 @@ struct Rest {
     return wave_sum(sum);
   }
 };
+// The mass of a chunk, of which x is the lane's first pieces.
+template <class T, int U>
+__device__ __forceinline__ double chunk_mass(const uint64_t* table, double c, const RowSum& ps, const RowSum& qs, double pa,
+                                             double qc, const PiecePair<T>& x, const T* prow, const T* qrow, int first,
+                                             int V) {
+  if (WeighFast::fits(c, ps.top) && WeighFast::fits(c, qs.top))
+    return Rest<true, WeighFast>(table, c, ps, qs, pa, qc).template mass<T, U>(x, prow, qrow, first, V);
+  return Rest<true, Weigh>(table, c, ps, qs, pa, qc).template mass<T, U>(x, prow, qrow, first, V);
+}
 
 // The decisions behind one token, drafts that were drawn: drafts of `kids` in
 // order. Lane i of the wave holds draft i's p, q and number; all lanes agree, and so
@@ -486,8 +508,9 @@ struct Asked {
         kept = i;
         return true;
       }
-      pa /= Z;
-      qc = qc / Z + 1.0;
+      const double over = 1.0 / Z;
+      pa *= over;
+      qc = fma(qc, over, 1.0);
       if (stop(rejections)) return false;
       Z = sum_of(i, rejections, pa, qc);
       ++rejections;
@@ -520,6 +543,7 @@ struct Draft {
 // A wave's sum of a row of masses: the same wherever it is taken.
 __device__ __forceinline__ double mass_sum(const double* masses, int chunks, int lane) {
   double sum = 0.0;
+#pragma unroll 1
   for (int c = lane; c < chunks; c += 64) sum += masses[c];
   return wave_sum(sum);
 }
@@ -571,7 +595,7 @@ __global__ __launch_bounds__(256) void verify_mass_kernel(VerifyArgs a, int roun
   __syncthreads();
   RowSum ps, qs;
   if constexpr (CHAIN) {
-    row_sums<true, 256>(a, b, nb, d.parent, table, rows);
+    row_sums<true, 256>(a, b, d.parent, table, rows);
     ps = rows[0][max(d.parent, 0)];
     qs = rows[1][max(d.parent, 0)];
   } else {
@@ -596,7 +620,7 @@ __global__ __launch_bounds__(256) void verify_mass_kernel(VerifyArgs a, int roun
     pa = asked.pa;
     qc = asked.qc;
   }
-  const double m = Rest<true>(table, a.c, ps, qs, pa, qc).template mass<T, U>(x, prow, qrow, first, a.V);
+  const double m = chunk_mass<T, U>(table, a.c, ps, qs, pa, qc, x, prow, qrow, first, a.V);
   if (lane == 0) masses_of(a, round, b, node)[chunk] = m;
 }
 
@@ -633,6 +657,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(VerifyArgs a) {
     // the masses that draft i's rejection leaves: of the token behind which it was
     // drafted and the number of its siblings before it (nothing, where it was not asked)
     if constexpr (DRAFT) {
+#pragma unroll 1
       for (int i = w; i < nb; i += NW) {
         const int node = lane_value(d.parent, i), r = __builtin_popcountll(__ballot(d.parent == node && lane < i));
         if (node < 0 || r >= a.rounds) continue;
@@ -640,7 +665,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(VerifyArgs a) {
         if (lane == 0) sums[i] = sum;
       }
     }
-    row_sums<DRAFT, NT>(a, b, nb, d.parent, table, rows);
+    row_sums<DRAFT, NT>(a, b, d.parent, table, rows);
   } else {
     int per = 1;
     while (per < a.chunks && per < 64) per *= 2;
@@ -689,7 +714,12 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(VerifyArgs a) {
   }
   const double u0 = (double)a.uniform[(int64_t)b * a.n];
   const int mine = max(d.parent, 0);
-  const double p = chance(table, a.c, lp, rows[0][mine]), q = DRAFT ? chance(table, a.c, lq, rows[1][mine]) : 0.0;
+  double p = 0.0, q = 0.0;
+#pragma unroll 1
+  for (int kind = DRAFT; kind >= 0; --kind) {
+    q = p;
+    p = chance(table, a.c, kind ? lq : lp, rows[kind][mine]);
+  }
   double pa = 1.0, qc = 0.0;
   const int token = d.known(a) ? (int)d.token : -1;
   uint64_t gone = 0;   // drafts that were turned down, where they were not drawn: each token once
@@ -710,12 +740,12 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(VerifyArgs a) {
             from = nullptr;
             __syncthreads();  // the masses of the rejection before are read
             const T *prow = row_of<T>(a.p, b, node), *qrow = row_of<T>(a.q, b, node);
-            const Rest<DRAFT> rest(table, a.c, rows[0][node], rows[1][node], apa, aqc);
             for (int c = w; c < a.chunks; c += NW) {
               const int first = (c * U * 64 + lane) * E - shift_of(prow);
               PiecePair<T> x;
               x.load(prow, qrow, first, a.V);
-              const double m = rest.template mass<T, U>(x, prow, qrow, first, a.V);
+              const double m =
+                  chunk_mass<T, U>(table, a.c, rows[0][node], rows[1][node], apa, aqc, x, prow, qrow, first, a.V);
               if (lane == 0) masses[c] = m;
             }
             __syncthreads();
@@ -746,31 +776,31 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(VerifyArgs a) {
     node = next;
     taken |= (uint64_t)1 << node;
   }
-  write_path();
 
   // The next token: the first whose running sum of r passes u Z; where rounding leaves
   // none, the last one of the chunk that has a mass.
+  const VerifyStat* st = stats_of(a, false, b, node);
   const T* prow = row_of<T>(a.p, b, node);
   const T* qrow = DRAFT && qc > 0.0 ? row_of<T>(a.q, b, node) : prow;
   const int shift = shift_of(prow);
   // (the last of a path has no drafts: its sum is not among the rows')
   const bool inner = __any(d.parent == node);
-  const RowSum ps = inner ? rows[0][node] : row_sum(stats_of(a, false, b, node), a.chunks, true, lane, 64, table, a.c);
+  const RowSum ps = inner ? rows[0][node] : row_sum(st, a.chunks, true, lane, 64, table, a.c);
   const RowSum qs = DRAFT && qc > 0.0 ? rows[1][node] : ps;
-  const Rest<DRAFT> rest(table, a.c, ps, qs, pa, qc);
+  const Rest<DRAFT, Weigh> rest(table, a.c, ps, qs, pa, qc);
+  const int in_chunk = token >= 0 ? (token + shift) / (64 * U * E) : -1;
   // where the last event was no rejection with any left: the chunks' own masses,
   // without what was turned down
   auto own_masses = [&]() {
     __syncthreads();
-    const VerifyStat* st = stats_of(a, false, b, node);
     for (int c0 = 0; c0 < a.chunks; c0 += NT) {  // every lane: lanes' values are read within
       const int c = c0 + threadIdx.x;
       const VerifyStat x = st[min(c, a.chunks - 1)];
       double m = rest.ap * (x.sum * weight_below(table, a.c, x.top, ps.top));
       for (uint64_t left = gone; left; left &= left - 1) {
-        const int i = __builtin_ctzll(left), t = lane_value(token, i);
+        const int i = __builtin_ctzll(left);
         const double there = lane_value(p, i);
-        m -= t >= 0 && (t + shift) / a.chunk == c ? there : 0.0;
+        m -= lane_value(in_chunk, i) == c ? there : 0.0;
       }
       if (c < a.chunks) masses[c] = fmax(m, 0.0);
     }
@@ -779,6 +809,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(VerifyArgs a) {
   if (!(DRAFT && fresh)) {
     own_masses();
   } else if (from) {
+#pragma unroll 1
     for (int c = threadIdx.x; c < a.chunks; c += NT) masses[c] = from[c];
     __syncthreads();
   }
@@ -796,7 +827,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(VerifyArgs a) {
         continue;
       }
       if (threadIdx.x == 0) a.token[b] = -1;
-      return;
+      break;
     }
     const int at = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some);
     int chunk = 0;
@@ -871,8 +902,9 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(VerifyArgs a) {
       }
       a.token[b] = pick;
     }
-    return;
+    break;
   }
+  write_path();
 }
 
 namespace {
