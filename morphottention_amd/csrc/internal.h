@@ -222,7 +222,7 @@ struct VerifyArgs {
   double c;           // 256 log2(e) / temperature
   int B, n, V, chunk, chunks, rounds, best;
 };
-constexpr int kVerifyThreads = 1024;
+constexpr int kVerifyThreads = 512, kVerifyMassThreads = 512;
 hipError_t launch_verify(const VerifyArgs& a, const VerifyPlan& p, int type, hipStream_t s);
 
 // Timing hooks (capi.hip). When timing is enabled, timing_begin opens a

@@ -556,14 +556,18 @@ __device__ __forceinline__ double* masses_of(const VerifyArgs& a, int round, int
 // What r has in a chunk (one a wave) after rejection number `round` behind a token, if
 // there are as many and no draft is kept before. In a chain the token is the one at
 // whose draft it ends, known to a workgroup after the sums of all rows; in a tree it is
-// any that has drafts (its place on the path is not asked for): there every wave decides
-// by itself, and most end after three round trips to memory.
+// any that has drafts (its place on the path is not asked for); there a wave takes each
+// of the sums that the decisions ask for.
 template <class T, int U, bool CHAIN>
-__global__ __launch_bounds__(256) void verify_mass_kernel(VerifyArgs a, int round, int groups) {
+__global__ __launch_bounds__(kVerifyMassThreads) void verify_mass_kernel(VerifyArgs a, int round, int groups) {
+  constexpr int NT = kVerifyMassThreads, NW = NT / 64;
+  static_assert(NW >= 2 + kVerifyMaxRounds - 1 && NT >= kTable);
   __shared__ uint64_t table[kTable];
   __shared__ RowSum rows[2][64];
-  const int lane = threadIdx.x & 63, k = blockIdx.x / groups, b = CHAIN ? k : k / (a.n - 1);
-  const int chunk = 4 * (blockIdx.x - k * groups) + (threadIdx.x >> 6), nb = tokens_of(a, b);
+  __shared__ double sums[kVerifyMaxRounds - 1];  // of the masses of the rounds before
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int k = blockIdx.x / groups, b = CHAIN ? k : k / (a.n - 1);
+  const int chunk = NW * (blockIdx.x - k * groups) + w, nb = tokens_of(a, b);
   int node = CHAIN ? 0 : k - b * (a.n - 1);
   const Draft d(a, b, nb, lane);
   if (nb < 2) return;
@@ -576,50 +580,45 @@ __global__ __launch_bounds__(256) void verify_mass_kernel(VerifyArgs a, int roun
     first = (min(chunk, a.chunks - 1) * U * 64 + lane) * Piece<T>::E - shift_of(prow);
     x.load(prow, qrow, first, a.V);
   };
-  double sums = 0.0;  // lane r: of the masses of round r
-  if constexpr (!CHAIN) {
-    if (__builtin_popcountll(__ballot(d.parent == node)) <= round) return;
-    load();  // early: the sums of the rounds before are on their way at the same time
-#pragma unroll 1
-    for (int r = 0; r < round; ++r) {
-      const double sum = mass_sum(masses_of(a, r, b, node), a.chunks, lane);
-      sums = lane == r ? sum : sums;
-    }
-  }
+  const uint64_t kids = __ballot(d.parent == node);
+  if (!CHAIN && __builtin_popcountll(kids) <= round) return;
+  if (threadIdx.x < kTable) table[threadIdx.x] = kExp2Table[threadIdx.x];
+  __syncthreads();
   float lp = kNegInf, lq = kNegInf;
   if ((CHAIN || d.parent == node) && d.known(a)) {
     lp = value_of(row_of<T>(a.p, b, d.parent)[d.token]);
     lq = value_of(row_of<T>(a.q, b, d.parent)[d.token]);
   }
-  if (threadIdx.x < kTable) table[threadIdx.x] = kExp2Table[threadIdx.x];
-  __syncthreads();
-  RowSum ps, qs;
   if constexpr (CHAIN) {
-    row_sums<true, 256>(a, b, d.parent, table, rows);
-    ps = rows[0][max(d.parent, 0)];
-    qs = rows[1][max(d.parent, 0)];
+    row_sums<true, NT>(a, b, d.parent, table, rows);
   } else {
-    ps = row_sum(stats_of(a, false, b, node), a.chunks, true, lane, 64, table, a.c);
-    qs = row_sum(stats_of(a, true, b, node), a.chunks, true, lane, 64, table, a.c);
+    load();  // early: decided while it is on its way
+    if (w < 2) {
+      const RowSum x = row_sum(stats_of(a, w, b, node), a.chunks, true, lane, 64, table, a.c);
+      if (lane == 0) rows[w][0] = x;
+    } else if (w < 2 + round) {
+      const double sum = mass_sum(masses_of(a, w - 2, b, node), a.chunks, lane);
+      if (lane == 0) sums[w - 2] = sum;
+    }
+    __syncthreads();
   }
-  if (chunk >= a.chunks) return;
-  const double p = chance(table, a.c, lp, ps), q = chance(table, a.c, lq, qs);
+  const int mine = CHAIN ? max(d.parent, 0) : 0;
+  const double p = chance(table, a.c, lp, rows[0][mine]), q = chance(table, a.c, lq, rows[1][mine]);
   double pa = 1.0, qc = 1.0;  // after the first rejection
   if constexpr (CHAIN) {
     const uint64_t ends = __ballot(d.parent >= 0 && !(d.u * q < p));
     if (!ends) return;
     node = __builtin_ctzll(ends) - 1;
     load();
-    ps = rows[0][node];
-    qs = rows[1][node];
   } else {
     Asked asked;
-    if (asked.run(__ballot(d.parent == node), p, q, d.u, [&](int, int r, double, double) { return lane_value(sums, r); },
-                  [&](int r) { return r == round; }))
+    if (asked.run(kids, p, q, d.u, [&](int, int r, double, double) { return sums[r]; }, [&](int r) { return r == round; }))
       return;
     pa = asked.pa;
     qc = asked.qc;
   }
+  const RowSum ps = rows[0][CHAIN ? node : 0], qs = rows[1][CHAIN ? node : 0];
+  if (chunk >= a.chunks) return;
   const double m = chunk_mass<T, U>(table, a.c, ps, qs, pa, qc, x, prow, qrow, first, a.V);
   if (lane == 0) masses_of(a, round, b, node)[chunk] = m;
 }
@@ -918,13 +917,15 @@ hipError_t launch_verify_u(const VerifyArgs& a, hipStream_t s) {
   else
     MORPHO_KLAUNCH((verify_stats_kernel<T, U, false>), all, block, 0, s, a, (int)rows);
   hipError_t e = hipGetLastError();
-  const int groups = (a.chunks + 3) / 4;
+  const int groups = (a.chunks + kVerifyMassThreads / 64 - 1) / (kVerifyMassThreads / 64);
+  const dim3 mass_block(kVerifyMassThreads);
   for (int k = 0; k < a.rounds && e == hipSuccess; ++k) {
     if (a.tree)
-      MORPHO_KLAUNCH((verify_mass_kernel<T, U, false>), dim3((unsigned)((int64_t)a.B * (a.n - 1) * groups)), block, 0, s, a,
-                     k, groups);
+      MORPHO_KLAUNCH((verify_mass_kernel<T, U, false>), dim3((unsigned)((int64_t)a.B * (a.n - 1) * groups)), mass_block, 0, s,
+                     a, k, groups);
     else
-      MORPHO_KLAUNCH((verify_mass_kernel<T, U, true>), dim3((unsigned)((int64_t)a.B * groups)), block, 0, s, a, k, groups);
+      MORPHO_KLAUNCH((verify_mass_kernel<T, U, true>), dim3((unsigned)((int64_t)a.B * groups)), mass_block, 0, s, a, k,
+                     groups);
     e = hipGetLastError();
   }
   if (e != hipSuccess) return e;
