@@ -115,7 +115,8 @@ struct Weigh {
   __device__ __forceinline__ Weigh(const uint64_t* table, double c, float top)
       : table(table), c(c), top(fmin(fmax((double)top, -1e39), 1e39)) {}
   __device__ __forceinline__ double operator()(float x) const {
-    return exp2_256(table, fmax((fmin((double)x, 1e39) - top) * c, -256000.0));
+    // the lower bound first: it stands for NaN
+    return exp2_256(table, fmax((fmin(fmax((double)x, -1e39), 1e39) - top) * c, -256000.0));
   }
   __device__ __forceinline__ double factor() const { return 1.0; }
 };

@@ -150,6 +150,22 @@ def test_logits_that_are_not_finite():
             assert want[2][4] == -1 and want[2][6] in (0,)
 
 
+@pytest.mark.parametrize("temperature", [0.3, 0.7, 1.1, 8.0])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_nan_has_no_chance(dtype, temperature):
+    for drawn in (True, False):
+        d = Drafts(6, 5, 3000, TYPES[dtype], drawn=drawn, temperature=temperature, seed=4)
+        d.logits[0, :, ::2] = math.nan
+        d.logits[1, 0, d.tokens[1, 1]] = math.nan  # of a draft
+        d.logits[2, :, 100:] = math.nan
+        if drawn:
+            d.draft[3, 0, d.tokens[3, 1]] = math.nan
+            d.draft[4, :, 1::2] = math.nan
+            d.draft[5] = math.nan
+        want = d.check()
+        assert want[0][1][1] == -1 and 0 <= want[2][2] < 100
+
+
 def test_numbers_and_tokens_at_their_ends():
     d = Drafts(6, 3, 500, torch.float16, seed=2)
     d.uniform[0] = 0.0
