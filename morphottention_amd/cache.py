@@ -728,6 +728,7 @@ class MorphoLoop:
             # room for every page that may come back
             self.free_pages = cache._ints(self._free + [-1] * (sum(len(r) for r in rows) + 1))
             self.free_count = cache._ints([len(self._free)])
+            self._none = cache._ints([0] * len(seqs))
         except BaseException:
             cache._drop(self._free)
             raise
@@ -747,7 +748,7 @@ class MorphoLoop:
         if not self._open or cache is not self.cache:
             raise RuntimeError("the step's loop is closed, or another cache's")
         if step is not self._last:
-            raise RuntimeError("the loop has made another step since")
+            raise RuntimeError("the loop has taken the step's tokens, or made another step since")
 
     def step(self, new_lens: torch.Tensor | None = None) -> CacheStep:
         """Places for ``n`` new tokens of each sequence, or ``new_lens`` (int32 ``[B]``).
@@ -764,14 +765,16 @@ class MorphoLoop:
     def accept(self, step: CacheStep, keep: torch.Tensor | None = None, keep_lens: torch.Tensor | None = None) -> None:
         """The step's tokens belong to their sequences: all that got places, or those at
         places ``keep`` (int32 ``[B, n]``, ascending, ``keep_lens`` of each), which move
-        together, as :func:`morphottention_amd.morpho_verify_drafts` gives them."""
+        together, as :func:`morphottention_amd.morpho_verify_drafts` gives them. Once for
+        each step."""
         self._still(self.cache, step)
         if (keep is None) != (keep_lens is None):
             raise ValueError("keep and keep_lens go together")
         if keep is not None:
-            keep_lens = torch.minimum(keep_lens, step.new_lens)
+            keep_lens = torch.clamp(keep_lens, self._none, step.new_lens)  # no sequence becomes shorter
             morpho_cache_compact(self.cache.codes, self.cache.values, self.table, self.lens, keep, keep_lens=keep_lens)
         self.lens.add_(step.new_lens if keep is None else keep_lens)
+        self._last = None
 
     def close(self) -> None:
         """Give the account back to the cache (reads it from the device)."""

@@ -177,6 +177,45 @@ def test_beyond_64_new_tokens_it_is_the_attention_without():
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("n", [1, 20])
+def test_a_pool_beyond_32_bits(n):
+    """Pages more than 2^32 bytes into a pool: the same results as near its start."""
+    far = 34000  # of 128 KiB of values
+    p = Shared(3, n, 16, 16, 64, [300, 256, 270], [[0, 1, 2]], [4], seed=3)
+    d, shared = p.device(), p.shared()
+    want = [t.clone() for t in p.attend(d, shared=shared)]
+    for k in ("codes", "values"):
+        small, d[k] = d[k], torch.empty((far + d[k].shape[0], *d[k].shape[1:]), dtype=torch.float16, device=DEV)
+        d[k][far:] = small
+    assert d["values"].numel() * 2 > 2 ** 32
+    d["table"] = torch.where(d["table"] >= 0, d["table"] + far, -1)
+    for a, b in zip(p.attend(d, shared=shared), want):
+        assert torch.equal(a, b)
+
+
+def test_two_graphs_in_turn():
+    """Two captured calls with partial results, replayed in turn: each has its own."""
+    ps = [_case(n, seed=n) for n in (1, 30)]
+    ds, sharings = [p.device() for p in ps], [p.shared() for p in ps]
+    want = [[t.clone() for t in p.attend(d, shared=s)] for p, d, s in zip(ps, ds, sharings)]
+    torch.cuda.synchronize()
+    graphs, got = [], []
+    for p, d, s in zip(ps, ds, sharings):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            got.append(p.attend(d, shared=s))
+        graphs.append(g)
+    for _ in range(3):
+        for out, lse in got:
+            out.zero_()
+            lse.zero_()
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
 def test_repeats_bit_for_bit_and_on_another_stream():
     p = Shared(8, 3, 4, 32, 64, [1024 + b for b in range(8)], [list(range(8))], [16], seed=6)
     d, shared = p.device(), p.shared()

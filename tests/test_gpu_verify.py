@@ -228,6 +228,43 @@ def test_a_large_vocabulary():
     d.check()
 
 
+def test_strides_beyond_32_bits():
+    d = Drafts(3, 3, 700, torch.float16, seed=9)
+    want = d.check()
+    far = 2 ** 30 + 3
+    logits = torch.empty(2 * far + 3 * 700, dtype=torch.float16, device=DEV).as_strided((3, 3, 700), (far, 700, 1))
+    draft = torch.empty(far + 3 * 700, dtype=torch.float16, device=DEV).as_strided((3, 2, 700), (700, far, 1))
+    logits.copy_(d.logits)
+    draft.copy_(d.draft)
+    got = ma.morpho_verify_drafts(logits, d.tokens.to(DEV), d.uniform.to(DEV), draft_logits=draft)
+    assert tuple(t.tolist() for t in got) == want
+
+
+def test_two_graphs_in_turn():
+    """Two captured calls, replayed in turn: each has its own chunks and masses."""
+    ds = [Drafts(4, 6, 5000, torch.bfloat16, seed=1), Drafts(4, 20, 5000, torch.float32, tree=True, seed=2)]
+    want = [d.want() for d in ds]
+    inputs = [[t if t is None else t.to(DEV) for t in (d.logits, d.tokens, d.uniform, d.tree, d.draft)] for d in ds]
+    call = lambda x: ma.morpho_verify_drafts(*x[:3], tree=x[3], draft_logits=x[4])  # noqa: E731
+    for x in inputs:
+        call(x)
+    torch.cuda.synchronize()
+    graphs, got = [], []
+    for x in inputs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            got.append(call(x))
+        graphs.append(g)
+    for _ in range(3):
+        for out in got:
+            for t in out:
+                t.zero_()
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        assert [tuple(t.tolist() for t in out) for out in got] == want
+
+
 def test_a_captured_call_follows_its_inputs():
     for kw in ({"tree": True}, {"drawn": False}, {"temperature": 0.0}):
         ds = [Drafts(4, 6, 9000, torch.float16, ragged=True, seed=s, **kw) for s in range(3)]

@@ -414,7 +414,16 @@ def test_loop_refusals(plain):
     for call in (c.commit, c.drop, lambda s: c.accept(s, [[0]])):
         with pytest.raises(RuntimeError, match="loop"):
             call(second)
-    loop.accept(second)
+    # counts that cannot be: no sequence becomes shorter, none gets more than it was granted
+    for k in (-7, 0):
+        loop.accept(loop.step(), torch.zeros((1, 2), dtype=torch.int32), torch.tensor([k], dtype=torch.int32))
+        assert loop.lens.tolist() == [0]
+    second = loop.step()
+    loop.accept(second, torch.tensor([[0, 1]], dtype=torch.int32), torch.tensor([9], dtype=torch.int32))
+    for call in (lambda: loop.accept(second), lambda: c._check(second, x)):
+        with pytest.raises(RuntimeError, match="taken the step's tokens"):
+            call()
+    assert loop.lens.tolist() == [2]
     loop.close()
     loop.close()
     assert c.length(a) == 2 and c.free_pages == 19
