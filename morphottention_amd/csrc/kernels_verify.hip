@@ -323,26 +323,30 @@ __device__ __forceinline__ const VerifyStat* stats_of(const VerifyArgs& a, bool 
 template <class T, int U, bool BEST>
 __global__ __launch_bounds__(256, 8) void verify_stats_kernel(VerifyArgs a, int rows) {
   constexpr int E = 16 / sizeof(T);
+  static_assert(kTable == 256);
   __shared__ uint64_t table[kTable];
   const int lane = threadIdx.x & 63;
-  if constexpr (!BEST) {
-    if (threadIdx.x < kTable) table[threadIdx.x] = kExp2Table[threadIdx.x];
-    __syncthreads();
-  }
+  uint64_t entry = 0;
+  if constexpr (!BEST) entry = kExp2Table[threadIdx.x];  // on its way early
   const int id = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
-  const int row = id / a.chunks, chunk = id - row * a.chunks;
-  if (row >= rows) return;
+  const int row = min(id / a.chunks, rows - 1), chunk = id - row * a.chunks;
   const bool draft = row >= a.B * a.n;
   const int k = draft ? row - a.B * a.n : row, per = draft ? a.n - 1 : a.n, b = k / per, i = k - b * per;
   const int nb = tokens_of(a, b);
-  if (i >= nb) return;
   // what a token without drafts of its own would have drawn from is not asked for
-  if (draft && !__any(lane > i && lane < nb && parent_of(a, b, lane) == i)) return;
+  const bool asked = chunk < a.chunks && i < nb && (!draft || __any(lane > i && lane < nb && parent_of(a, b, lane) == i));
   const T* p = row_of<T>(draft ? a.q : a.p, b, i);
   const int first = (chunk * U * 64 + lane) * E - shift_of(p);
   Piece<T> x[U];
+  if (asked) {
 #pragma unroll
-  for (int u = 0; u < U; ++u) x[u].load(p, first + u * 64 * E, a.V);
+    for (int u = 0; u < U; ++u) x[u].load(p, first + u * 64 * E, a.V);
+  }
+  if constexpr (!BEST) {
+    table[threadIdx.x] = entry;
+    __syncthreads();
+  }
+  if (!asked) return;
   float top = kNegInf;
   int place = INT_MAX;
 #pragma unroll
@@ -567,6 +571,7 @@ __global__ __launch_bounds__(kVerifyMassThreads) void verify_mass_kernel(VerifyA
   __shared__ RowSum rows[2][64];
   __shared__ double sums[kVerifyMaxRounds - 1];  // of the masses of the rounds before
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint64_t entry = kExp2Table[threadIdx.x & (kTable - 1)];  // on its way early
   const int k = blockIdx.x / groups, b = CHAIN ? k : k / (a.n - 1);
   const int chunk = NW * (blockIdx.x - k * groups) + w, nb = tokens_of(a, b);
   int node = CHAIN ? 0 : k - b * (a.n - 1);
@@ -583,7 +588,7 @@ __global__ __launch_bounds__(kVerifyMassThreads) void verify_mass_kernel(VerifyA
   };
   const uint64_t kids = __ballot(d.parent == node);
   if (!CHAIN && __builtin_popcountll(kids) <= round) return;
-  if (threadIdx.x < kTable) table[threadIdx.x] = kExp2Table[threadIdx.x];
+  if (threadIdx.x < kTable) table[threadIdx.x] = entry;
   __syncthreads();
   float lp = kNegInf, lq = kNegInf;
   if ((CHAIN || d.parent == node) && d.known(a)) {
@@ -644,6 +649,8 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(VerifyArgs a) {
     }
     return;
   }
+  uint64_t entry = 0;
+  if constexpr (!BEST) entry = kExp2Table[threadIdx.x & (kTable - 1)];  // on its way early
   // every wave holds the drafts and takes the same steps
   const Draft d(a, b, nb, lane);
   float lp = kNegInf, lq = kNegInf;
@@ -652,7 +659,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(VerifyArgs a) {
       lp = value_of(row_of<T>(a.p, b, d.parent)[d.token]);
       if constexpr (DRAFT) lq = value_of(row_of<T>(a.q, b, d.parent)[d.token]);
     }
-    if (threadIdx.x < kTable) table[threadIdx.x] = kExp2Table[threadIdx.x];
+    if (threadIdx.x < kTable) table[threadIdx.x] = entry;
     __syncthreads();
     // the masses that draft i's rejection leaves: of the token behind which it was
     // drafted and the number of its siblings before it (nothing, where it was not asked)
