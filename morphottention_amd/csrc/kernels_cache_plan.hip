@@ -11,7 +11,8 @@
 //   page j that is taken comes from  free[count + back - 1 - j],
 // so pages that are given back and taken again are the same ones in the same order.
 //
-// Bound by its launch and its chain: lengths, two scans, pages, table, slots.
+// Bound by its launch and its chain: lengths, two scans, pages, table, slots (64
+// sequences of 12 new tokens 3.8 us, 512 of 2000 7.0 + 3.8).
 #include "common.h"
 #include "internal.h"
 
