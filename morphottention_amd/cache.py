@@ -288,8 +288,9 @@ def _same(a: list[int], b: list[int], most: int) -> int:
 def _groups(rows: list[list[int]], full: list[int]) -> list[tuple[list[int], int]]:
     """Groups of rows with common first pages, and how many: those that spare the
     most pages (a group of k with c common ones spares (k - 1) c), of which a row
-    is in one. full: the pages of each that may be shared."""
-    def best(mine: list[int], depth: int) -> tuple[int, list[tuple[list[int], int]]]:
+    is in one. full: the pages of each that may be shared. Of forks of forks it looks
+    at 16 generations."""
+    def best(mine: list[int], depth: int, more: int) -> tuple[int, list[tuple[list[int], int]]]:
         by_page: dict[int, list[int]] = {}
         for b in mine:
             if full[b] > depth:
@@ -299,12 +300,12 @@ def _groups(rows: list[list[int]], full: list[int]) -> list[tuple[list[int], int
             if len(k) < 2:
                 continue
             common = min(_same(rows[k[0]], rows[b], full[b]) for b in k)
-            deeper, inner = best(k, common)
+            deeper, inner = best(k, common, more - 1) if more else (0, [])
             here = (len(k) - 1) * common
             spared += max(here, deeper)
             found += inner if deeper > here else [(k, common)]
         return spared, found
-    return best(list(range(len(rows))), 0)[1]
+    return best(list(range(len(rows))), 0, 16)[1]
 
 
 # What changes the tokens of a sequence gives it a new stamp. They rise and are

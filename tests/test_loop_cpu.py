@@ -263,6 +263,16 @@ def test_groups_spare_the_most_pages():
     assert cache_module._groups([[1, 2], [1, 2]], [2, 1]) == [([0, 1], 1)]  # the other's second page is not full
 
 
+def test_groups_of_forks_of_forks():
+    """Each row a fork of the one before, a page longer: as deep as there are rows."""
+    rows = [list(range(min(i + 1, 1499))) + [10000 + 2000 * i + j for j in range(3)] for i in range(1500)]
+    groups = cache_module._groups(rows, [len(r) for r in rows])
+    members = [b for k, _ in groups for b in k]
+    assert groups and len(set(members)) == len(members)
+    for k, common in groups:
+        assert len(k) > 1 and common > 0 and all(rows[b][:common] == rows[k[0]][:common] for b in k)
+
+
 def test_shared_prefix_of():
     s = ma.SharedPrefix.of([[3, 0], [2]], [5, 1], 4)
     assert s.members.tolist() == [3, 0, 2] and s.starts.tolist() == [0, 2, 3] and s.group.tolist() == [0, -1, 1, 0]
