@@ -46,6 +46,21 @@ struct PlanNote {
 };
 constexpr int kPlanHeader = 16;  // bytes before the notes: the pages to take from
 
+// Sum over the lanes of a wave up to this one, by register moves. What a wave's 64
+// sequences hold or lack stays below 2^31: 2^25 pages each at most.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ unsigned add_moved(unsigned x) {
+  return x + (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ unsigned wave_upto(unsigned x) {
+  x = add_moved<0x111, 0xf>(x);     // row_shr 1, 2, 4, 8
+  x = add_moved<0x112, 0xf>(x);
+  x = add_moved<0x114, 0xf>(x);
+  x = add_moved<0x118, 0xf>(x);
+  x = add_moved<0x142, 0xa>(x);     // row_bcast 15: of rows 0 and 2 to 1 and 3
+  return add_moved<0x143, 0xc>(x);  // row_bcast 31: of row 1 to 2 and 3
+}
+
 // Which of N runs, whose ends are `upto`, item j lies in.
 template <int N>
 __device__ __forceinline__ int run_of(const int64_t* upto, int64_t j) {
@@ -77,12 +92,8 @@ __global__ __launch_bounds__(N) void cache_plan_kernel(CachePlanArgs a) {
   const int64_t room = a.room, count = min(max((int64_t)a.free_count[0], (int64_t)0), room);
   // sums of a tile's pages over the sequences before and with this one, and all
   auto scan = [&](int64_t& back, int64_t& lack, int64_t& backs, int64_t& lacks) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int64_t x = __shfl_up(back, o), y = __shfl_up(lack, o);
-      back += lane >= o ? x : 0;
-      lack += lane >= o ? y : 0;
-    }
+    back = wave_upto((unsigned)back);
+    lack = wave_upto((unsigned)lack);
     __syncthreads();
     if (lane == 63) {
       back_sums[w] = back;
@@ -90,7 +101,7 @@ __global__ __launch_bounds__(N) void cache_plan_kernel(CachePlanArgs a) {
     }
     __syncthreads();
     backs = lacks = 0;
-#pragma unroll 4
+#pragma unroll
     for (int k = 0; k < NW; ++k) {
       if (k == w) {
         back += backs;

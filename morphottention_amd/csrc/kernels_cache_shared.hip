@@ -14,7 +14,7 @@
 // 5.1 TB/s: reading the keys. 64 of 8192, m16, 15.6 + 4.2; four groups of 12 of 4096 and
 // 16 alone, m32, 15.0 + 4.5: the launch, the first keys' latency and the last pieces.
 // 16 trees of 48 drafts behind 4096, H32 m64, 57 + 5.6: VALU and MFMA work (three
-// quarters of a SIMD's cycles) of the two waves a SIMD that LDS has room for.
+// quarters of a SIMD's cycles), which its waves, three at most, overlap only in part.
 #include "cache_attn.h"
 #include "common.h"
 #include "internal.h"

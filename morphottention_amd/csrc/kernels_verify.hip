@@ -12,7 +12,7 @@
 //
 // The results are whole numbers that depend on which side of a border a sum of
 // up to millions of terms falls, so weights and sums are in 64 bits: the order of
-// the terms then moves a border by 2^-48 or so, and the same inputs give the same
+// the terms then moves a border by 2^-45 or so, and the same inputs give the same
 // tokens as any other 64-bit evaluation. (In 32 bits one of a thousand sampled
 // tokens is another one.)
 //
