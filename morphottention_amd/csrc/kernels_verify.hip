@@ -822,6 +822,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_kernel(VerifyArgs a) {
   if (!(DRAFT && fresh)) {
     own_masses();
   } else if (from) {
+    __syncthreads();  // a token before may have left its masses here, which a wave behind still sums
 #pragma unroll 1
     for (int c = threadIdx.x; c < a.chunks; c += NT) masses[c] = from[c];
     __syncthreads();

@@ -115,6 +115,32 @@ def test_many_siblings_are_all_turned_down():
     assert d.check()[1] == [1] * 6
 
 
+@pytest.mark.parametrize("V", [3000, 50001])
+@pytest.mark.parametrize("rest", [1, 3])
+def test_a_late_sibling_is_kept_and_those_behind_it_turned_down(V, rest):
+    """The root's first drafts are turned down one after another, more than the chip has
+    summed remainders for, a later one is kept, and behind it drafts are turned down
+    again: the remainders of both tokens pass through the same shared memory."""
+    B, last = 16, 8
+    n = 1 + last + 6 + rest
+    d = Drafts(B, n, V, torch.float32, tree=True, seed=V + rest)
+    g = torch.Generator().manual_seed(V)
+    kept = [last + b % 6 for b in range(B)]  # the eighth draft of the root or a later one
+    d.parents = [[-1] + [0] * (last + 6) + [k] * rest for k in kept]
+    d.tree = torch.tensor([_bits(p) for p in d.parents], dtype=torch.int64)
+    d.draft = torch.randn((B, n - 1, V), generator=g)
+    d.logits = torch.randn((B, n, V), generator=g)
+    order = d.logits.argsort(-1)
+    for b, k in enumerate(kept):
+        d.uniform[b, 1:] = 0.999
+        d.tokens[b] = order[b, 0, :n]  # the target's least likely ones
+        d.tokens[b, last + 7:] = order[b, k, :rest]
+        d.tokens[b, k] = 7 + b  # likely in the target, hardly drawn: what is left of it outlasts the drafts before
+        d.logits[b, 0, 7 + b], d.draft[b, 0, 7 + b], d.uniform[b, k] = 9.0, -9.0, 0.0
+    for _ in range(3):
+        assert d.check()[0] == [[0, k] + [-1] * (n - 2) for k in kept]
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("n", [1, 5, 33])
 def test_the_best_token_decides(dtype, n):
