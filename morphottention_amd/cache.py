@@ -420,9 +420,12 @@ class MorphoCache:
             raise RuntimeError(f"sequence {seq} is in a loop, which has to be closed first")
         return seq
 
+    def _full(self, count: int, more: int = 0) -> None:
+        raise RuntimeError(f"the cache is full: {count} pages needed, {len(self._free) + more} of {self.num_pages} free")
+
     def _take(self, count: int) -> list[int]:
         if count > len(self._free):
-            raise RuntimeError(f"the cache is full: {count} pages needed, {len(self._free)} of {self.num_pages} free")
+            self._full(count)
         got = [self._free.pop() for _ in range(count)]
         for p in got:
             self._uses[p] = 1
@@ -712,13 +715,18 @@ class MorphoLoop:
         P = cache.page_size
         # a page that is not full belongs to its sequence alone from here on
         cache._own([(s, l, l + 1) for s, l in zip(seqs, lens) if l % P])
+        cache._shrink()
+        # what other steps claimed comes back: they are not good any more, whatever follows
+        claimed = [p for s, l in zip(seqs, lens) for p in cache._pages[s][-(-l // P) :]]
+        if pages is not None and pages > len(cache._free) + len(claimed):
+            cache._full(pages, len(claimed))
         for s, l in zip(seqs, lens):
             cache._cut(s, l)
+            cache._stamp[s] = next(_stamps)
         cache._grown.difference_update(seqs)
         width = -(-room // P)
         rows = [cache._pages[s] for s in seqs]
         need = sum(width - len(r) for r in rows)
-        cache._shrink()
         self._free = cache._take(min(need, len(cache._free)) if pages is None else pages)
         try:
             self.cache, self.seqs, self.n, self.room = cache, seqs, n, room
@@ -733,8 +741,6 @@ class MorphoLoop:
         except BaseException:
             cache._drop(self._free)
             raise
-        for s in seqs:
-            cache._stamp[s] = next(_stamps)  # steps that were made before are not good any more
         cache._away.update(seqs)
         self._last: CacheStep | None = None
         self._open = True

@@ -457,3 +457,47 @@ def test_loops_leave_the_cache_as_it_was_when_they_cannot_start(plain):
     with c.loop([a, b], 1, 41) as loop:
         assert loop.free_count.tolist() == [0]
     assert c.free_pages == 1 and len(c.pages(a)) == 2
+
+
+def test_a_loop_that_cannot_start_leaves_no_step_with_pages_of_others(plain, monkeypatch):
+    """A step that was made before still owns its pages after the failure, or is refused."""
+    c = ma.MorphoCache(6, 1, 16, 32, page_size=32)
+    a, b = c.new(), c.new()
+    step = c.step([a], 64)
+    for pages in (7, 100):
+        with pytest.raises(RuntimeError, match=f"{pages} pages needed, 6 of 6 free"):
+            c.loop([a], 1, 200, pages=pages)
+    other = c.step([b], 64)
+    assert not set(step.table[0].tolist()) & set(other.table[0].tolist())
+    c.commit(step)
+    assert c.length(a) == 64 and len(c.pages(a)) == 2
+
+    late = c.step([a], 64)
+    ints = c._ints
+
+    def fails(rows):
+        if rows == [64]:  # the lengths, after tables are built
+            raise RuntimeError("out of memory")
+        return ints(rows)
+    with monkeypatch.context() as m, pytest.raises(RuntimeError, match="out of memory"):
+        m.setattr(c, "_ints", fails)
+        c.loop([a], 1, 128)
+    assert c.free_pages == 2 and c.length(a) == 64
+    again = c.step([b], 128)  # takes what the failed loop and the step had
+    assert len(set(again.table[0].tolist())) == 4
+    with pytest.raises(RuntimeError, match="changed"):
+        c.commit(late)
+    with pytest.raises(RuntimeError, match="changed"):
+        c._check(late, torch.zeros(1, 64, 32))
+    assert c.length(a) == 64 and len(c.pages(a)) == 2
+
+
+def test_a_loop_takes_what_its_sequences_had_claimed(plain):
+    c = ma.MorphoCache(6, 1, 16, 32, page_size=32)
+    a = c.new()
+    step = c.step([a], 160)
+    with c.loop([a], 1, 200, pages=6) as loop:
+        assert loop.free_count.tolist() == [6]
+    with pytest.raises(RuntimeError, match="changed"):
+        c.commit(step)
+    assert c.free_pages == 6
