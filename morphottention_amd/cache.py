@@ -737,7 +737,7 @@ class MorphoLoop:
             # room for every page that may come back
             self.free_pages = cache._ints(self._free + [-1] * (sum(len(r) for r in rows) + 1))
             self.free_count = cache._ints([len(self._free)])
-            self._none = cache._ints([0] * len(seqs))
+            self._none, self._all = cache._ints([0] * len(seqs)), cache._ints([n] * len(seqs))
         except BaseException:
             cache._drop(self._free)
             raise
@@ -762,6 +762,11 @@ class MorphoLoop:
         A step whose tokens are not accepted before the next one leaves none."""
         if not self._open:
             raise RuntimeError("the loop is closed")
+        if new_lens is not None and (new_lens.shape != self.lens.shape or new_lens.dtype != torch.int32):
+            raise ValueError(f"new_lens must be int32 [{len(self.seqs)}] (got {new_lens.dtype} {tuple(new_lens.shape)})")
+        if self.room % self.cache.page_size:  # the table ends behind it
+            news = self._all if new_lens is None else torch.clamp(new_lens, 0, self.n)
+            new_lens = torch.where(self.lens + news <= self.room, news, self._none)
         granted, slots = morpho_cache_plan(self.table, self.held, self.lens, self.free_pages, self.free_count, self.n,
                                            new_lens=new_lens, page_size=self.cache.page_size)
         self.slots = slots

@@ -501,3 +501,35 @@ def test_a_loop_takes_what_its_sequences_had_claimed(plain):
     with pytest.raises(RuntimeError, match="changed"):
         c.commit(step)
     assert c.free_pages == 6
+
+
+@pytest.mark.parametrize("room", [32, 40, 41, 44, 63, 64])
+def test_no_sequence_of_a_loop_gets_more_tokens_than_its_room(plain, room):
+    """Also where its last page has places behind it: all of a step's new tokens, or none."""
+    c = ma.MorphoCache(12, 1, 16, 32, page_size=32)
+    a, b = c.new(), c.new()
+    c.commit(c.step([b], 3))
+    n, want = 5, [0, 3]
+    with c.loop([a, b], n, room) as loop:
+        for news in [None] * 14 + [[9, -3], [2, 1], [1, 1], [1, 2], [1, 1], [1, 1], [1, 1]]:
+            step = loop.step(None if news is None else torch.tensor(news, dtype=torch.int32))
+            asked = [n, n] if news is None else [min(max(k, 0), n) for k in news]
+            got = [k if have + k <= room else 0 for k, have in zip(asked, want)]
+            assert step.new_lens.tolist() == got
+            for b_, k in enumerate(got):
+                assert (loop.slots[b_, :k] >= 0).all() and (loop.slots[b_, k:] == -1).all()
+            loop.accept(step)
+            want = [have + k for have, k in zip(want, got)]
+            assert loop.lens.tolist() == want
+        assert want[0] <= room and want[1] <= room and max(want) > room - 5
+    assert c.length(a) == want[0] and c.length(b) == want[1]
+
+
+@pytest.mark.parametrize("room", [40, 64])
+def test_a_loops_counts_are_one_for_each_sequence(plain, room):
+    c = ma.MorphoCache(6, 1, 16, 32, page_size=32)
+    with c.loop([c.new(), c.new()], 5, room) as loop:
+        for bad in (torch.ones(1, dtype=torch.int32), torch.ones((1, 2), dtype=torch.int32), torch.ones(2, dtype=torch.int64)):
+            with pytest.raises(ValueError, match="new_lens"):
+                loop.step(bad)
+        assert loop.step(torch.tensor([1, 5], dtype=torch.int32)).new_lens.tolist() == [1, 5]
