@@ -208,7 +208,7 @@ def morpho_cache_attention(phi: torch.Tensor, gate_q: torch.Tensor, gate_k: torc
         raise ValueError("mask_diag with a tree: leave a draft's own bit out instead")
     refuse_grad(phi, gate_q, gate_k)
     if shared is not None:
-        if min(shared.max_prefix or 1, shared.max_rest or 1) <= 0:
+        if any(hint is not None and hint <= 0 for hint in (shared.max_prefix, shared.max_rest)):
             raise ValueError("max_prefix and max_rest must be positive")
         if phi.shape[1] <= _MOST_SHARED:
             out, lse = ops.cache_shared_attention(phi, gate_q, gate_k, codes, values, table, lens, new_lens, tree,

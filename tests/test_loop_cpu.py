@@ -533,3 +533,10 @@ def test_a_loops_counts_are_one_for_each_sequence(plain, room):
             with pytest.raises(ValueError, match="new_lens"):
                 loop.step(bad)
         assert loop.step(torch.tensor([1, 5], dtype=torch.int32)).new_lens.tolist() == [1, 5]
+
+
+@pytest.mark.parametrize("hints", [{"max_prefix": 0}, {"max_rest": 0}, {"max_rest": -5}, {"max_prefix": 64, "max_rest": 0}])
+def test_hints_that_are_not_positive(hints):
+    t = torch.zeros(1)
+    with pytest.raises(ValueError, match="positive"):
+        ma.morpho_cache_attention(t, t, t, t, t, t, t, shared=ma.SharedPrefix(t, t, t, t, **hints))
