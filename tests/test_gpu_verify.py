@@ -371,3 +371,9 @@ def test_another_stream_and_gradients():
     logits = d.logits.float().to(DEV).requires_grad_(True)  # whole numbers have no gradients
     got = ma.morpho_verify_drafts(logits, d.tokens.to(DEV), d.uniform.to(DEV), draft_logits=d.draft.float().to(DEV))
     assert tuple(t.tolist() for t in got) == want and not got[2].requires_grad
+
+
+@pytest.mark.parametrize("drawn", [False, True])
+def test_a_large_tree_of_16_bit_logits(drawn):
+    kept = Drafts(4, 64, 12345, torch.float16, tree=True, drawn=drawn, ragged=True, temperature=1.3, seed=12409).check()[1]
+    assert max(kept) >= 1
