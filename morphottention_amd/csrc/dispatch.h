@@ -426,7 +426,9 @@ inline CacheSharedPlan cache_shared_plan(int B, int H, int n, int members, int g
   // functions apart and shared, with what is spared: B16 n1 1024 common tokens (39 MB)
   // 10.8, 11.9, 2048 (79) 15.9, 11.9; B64 512 (83) 12.0, 12.5, 1024 (165) 16.1, 13.5; B2
   // 32768 m32 (101) 35, 22; trees of 48, H32 m64: B8 1024 (59) 23.5, 26, 4096 (235) 63,
-  // 46; B16 n20 1024 (39) 17.4, 16.8; all H16 m16 dv64 unless said.
+  // 46; B16 n20 1024 (39) 17.4, 16.8; all H16 m16 dv64 unless said. The host knows the
+  // longest prefix only: of groups of different lengths, or without a hint, less is
+  // spared than this says.
   p.apart = (int64_t)(members - groups) * max_prefix * H * (M + DV) * 2 < (int64_t)64 << 20;
   const int64_t rows = (int64_t)members * n, mean = (rows + groups - 1) / groups;
   // 32 rows a wave where there are many read the keys half as often from L2, with half

@@ -12,7 +12,7 @@
 // so pages that are given back and taken again are the same ones in the same order.
 //
 // Bound by its launch and its chain: lengths, two scans, pages, table, slots (64
-// sequences of 12 new tokens 3.5 us, 512 of 2000 6.2 + 3.8).
+// sequences of 12 new tokens 3.4 us, 512 of 2000 6.0 + 3.8).
 #include "common.h"
 #include "internal.h"
 

@@ -10,10 +10,11 @@
 // all of its prefix (whole pages of tokens before it), whatever the mask says
 // about the new tokens: no masks here.
 //
-// Measured (kernel + join): 32 sequences of 65536 common tokens, H16 m32 dv64, 43 + 5.4 us,
-// 5.1 TB/s: reading the keys. 64 of 8192, m16, 15.6 + 4.2; four groups of 12 of 4096 and
-// 16 alone, m32, 15.0 + 4.5: the launch, the first keys' latency and the last pieces.
-// 16 trees of 48 drafts behind 4096, H32 m64, 57 + 5.6: VALU and MFMA work (three
+// Measured (kernel + join): 32 sequences of 65536 common tokens, H16 m32 dv64, 43 + 5.3 us,
+// 5.1 TB/s: reading the keys. 64 of 8192, m16, 15.7 + 4.2; four groups of 12 of 4096 and
+// 16 alone, m32, 14.6 + 4.6: the launch, the first keys' latency and the last pieces.
+// The 64 with chains of 5 29.4 + 5.1, of 16 68 + 5.6 (matrix work 18).
+// 16 trees of 48 drafts behind 4096, H32 m64, 58 + 5.6: VALU and MFMA work (three
 // quarters of a SIMD's cycles), which its waves, three at most, overlap only in part.
 #include "cache_attn.h"
 #include "common.h"

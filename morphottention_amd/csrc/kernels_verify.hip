@@ -12,9 +12,12 @@
 //
 // The results are whole numbers that depend on which side of a border a sum of
 // up to millions of terms falls, so weights and sums are in 64 bits: the order of
-// the terms then moves a border by 2^-45 or so, and the same inputs give the same
-// tokens as any other 64-bit evaluation. (In 32 bits one of a thousand sampled
-// tokens is another one.)
+// the terms then moves a border by 2^-45 or so of the row's whole, and the same
+// inputs give the same tokens as any other 64-bit evaluation but for numbers that
+// close to a border. (In 32 bits one of a thousand sampled tokens is another one.)
+// Behind drafts that were turned down r is a difference (of a p and c q, or of p and
+// the drafts), so its borders move by that over what is left of the whole; that
+// little is left is as rare as it is little.
 //
 // 1. verify_stats_kernel: of every row's chunks the largest logit and the sum of
 //    the weights below it (the only pass over all rows).
@@ -25,12 +28,15 @@
 // A chunk is what one wave takes at a time, 64 U pieces of 16 bytes. Small, since
 // the last step draws from one on a single CU.
 //
-// Measured (kernels, step 1 + 2 + 3): one chain of 5 over 32000 tokens 3.2 + 5.0 + 7.6
-// us, 64 of 6 over 128000 (180 MB) 52 + 16 + 12, 16 trees of 48 over 50001, not drawn,
-// 11.4 + 8.4, 8 drawn of 24 over 32001 11.5 + 6 x 7.9 + 22, 32 of 8 over 65536 at
-// temperature 0 10.4 + 3.8 (34 MB). Step 1 is bound by the weights' instructions (3.5 TB/s),
-// the others by chains of loads and decisions on a cold instruction cache: a workgroup
-// of 1024 threads, whose waves all decide, is a third slower in step 3 than one of 512.
+// Measured (kernels, step 1 + 2 + 3): one chain of 5 over 32000 tokens 3.2 + 5.1 + 7.7
+// us, 64 of 6 over 128000 (180 MB) 54 + 16 + 12, 16 trees of 48 over 50001, not drawn,
+// full (77 MB) 25.5 + 9.4, ragged (17 MB) 11.1 + 8.6, 8 drawn of 24 over 32001 11.7 +
+// 6 x 7.9 + 22, 32 of 8 over 65536 at temperature 0 11.0 + 4.0 (34 MB). Step 1 is bound by the
+// weights' instructions where its rows fill the chip (3.4 TB/s; the full trees 3.0); of the
+// ragged trees' 11.1 us those are 4, the rest is the launch and the waves of the rows that
+// are padding, three of four, each with its table and barrier. Steps 2 and 3 are chains
+// of loads and decisions on a cold instruction cache: a workgroup of 1024 threads, whose
+// waves all decide, is a third slower in step 3 than one of 512.
 #include <limits.h>
 
 #include "common.h"
@@ -40,8 +46,10 @@ namespace morpho {
 
 namespace {
 
-// The bits of 2^(i / 256) less i 2^44, so that adding n 2^44 with n = 256 e + i gives
-// those of 2^(n / 256).
+// Powers of two by a table and a short polynomial, the way of P. T. P. Tang's
+// table-driven exponential (ACM Transactions on Mathematical Software 15, 1989). An
+// entry is the double next to 2^(i / 256), less i 2^44, so that adding n 2^44 with
+// n = 256 e + i gives the bits of 2^(n / 256).
 constexpr int kTable = 256;
 __constant__ uint64_t kExp2Table[kTable] = {
     0x3ff0000000000000, 0x3feffb1afa5abcbf, 0x3feff63da9fb3335, 0x3feff168143b0281, 0x3fefec9a3e778061, 0x3fefe7d42e11bbcc,
@@ -89,8 +97,8 @@ __constant__ uint64_t kExp2Table[kTable] = {
     0x3fefe7c1819e90d8, 0x3fefedba3692d514, 0x3feff3c22b8f71f1, 0x3feff9d96b2a23d9};
 
 // 2^((n + r) / 256), |r| <= 1/2, n >= -256000: 2^(n / 256) from the table and
-// 2^(r / 256) by a polynomial of degree 3 through its Chebyshev nodes (2^-45 off at
-// most). A table of 64 takes a degree more, and two instructions where the low byte of
+// 2^(r / 256) by the cubic that meets it at the four Chebyshev nodes cos((2 k + 1) pi / 8) / 2
+// (computed in 60 decimal digits, then rounded; 2^-45 off at most). A table of 64 takes a degree more, and two instructions where the low byte of
 // n is the index.
 __device__ __forceinline__ double exp2_256(const uint64_t* table, int n, double r) {
   double y = 0x1.c6b0902b5a0abp-29;
@@ -474,8 +482,9 @@ struct Rest {
     if constexpr (DRAFT) r = fma(-aq, q(lq), r);
     return fmax(r, 0.0);
   }
-  // The mass of a chunk, by a wave: a loop, since what a small launch waits for is its
-  // code (unrolled: x us).
+  // The mass of a chunk, by a wave: a loop with one pair of pieces ahead. Unrolled it
+  // takes all 256 registers and spills: 64 chains of 6 over 128000 16.2 -> 44.6 us for
+  // the masses and 12 -> 20 in the last kernel (one chain of 5 over 32000 alike).
   template <class T, int U>
   __device__ __forceinline__ double mass(PiecePair<T> x, const T* prow, const T* qrow, int first, int V) const {
     double sum = 0.0;

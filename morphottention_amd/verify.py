@@ -34,7 +34,8 @@ def morpho_verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, uniform: to
     r(t)``, and is then the token at hand; else r becomes ``max(r / Z - q, 0)`` and Z
     its sum. When none is left, the next token is the first one whose running sum
     of r passes ``uniform Z``. All sums are in 64 bits: the same inputs give the same
-    tokens as any other 64-bit evaluation.
+    tokens as any other 64-bit evaluation, up to rounding at a border (2^-45 or so,
+    over the part of the row that the drafts turned down have left).
 
     :param logits: the target's ``[B, n, vocab]``, ``n <= 64``, float16, bfloat16 or
         float32; row i is the one behind token i. Contiguous along the vocabulary, of

@@ -540,3 +540,28 @@ def test_hints_that_are_not_positive(hints):
     t = torch.zeros(1)
     with pytest.raises(ValueError, match="positive"):
         ma.morpho_cache_attention(t, t, t, t, t, t, t, shared=ma.SharedPrefix(t, t, t, t, **hints))
+
+
+def test_powers_of_the_verification():
+    """Its table holds the doubles next to 2^(i / 256), less i 2^44, and its cubic is 2^(r / 256)
+    to 2^-45 for |r| <= 1/2."""
+    import math
+    import re
+    import struct
+    from decimal import Decimal, localcontext
+    with open(f"{ROOT}/morphottention_amd/csrc/kernels_verify.hip") as f:
+        src = f.read()
+    table = [int(x, 16) for x in re.findall(r"0x[0-9a-f]{16}", src[src.index("kExp2Table[kTable] = {"):src.index("};")])]
+    cubic = [float.fromhex(x) for x in re.findall(r"0x1\.[0-9a-f]{13}p-\d+", src[src.index("double exp2_256("):])[:4]]
+    assert len(table) == 256
+    with localcontext() as c:
+        c.prec = 60
+        ln2 = Decimal(2).ln()
+        for i, entry in enumerate(table):
+            bits = struct.unpack("<Q", struct.pack("<d", float((ln2 * i / 256).exp())))[0]
+            assert bits - (i << 44) == entry, i
+        for k in range(-200, 201):
+            r, y = Decimal(k) / 400, Decimal(0)
+            for a in cubic:
+                y = y * r + Decimal(a)
+            assert abs(y / (ln2 * r / 256).exp() - 1) <= Decimal(math.ldexp(1, -45)), k
